@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI declared in include/mg_gemm.h.
+"""ctypes binding of the C ABI declared in include/mg_gemm.h and
+include/mg_attention.h.
 
 The product path has exactly one implementation: the sm_100a kernels in
 libmg_gemm.so. If the library is missing or cannot load, every entry point
@@ -100,6 +101,11 @@ SIGNATURES = {
     "mg_device_status": (ctypes.c_int, [_I32P, _I32]),
     "mg_launch_count": (ctypes.c_uint64, []),
     "mg_version": (ctypes.c_char_p, []),
+    # include/mg_attention.h: descriptors are passed as packed bytes (transformer.py)
+    "mg_attention": (ctypes.c_int, [ctypes.c_char_p, _P, _P, _P, _P, _P, _P]),
+    "mg_attention_backward": (ctypes.c_int, [ctypes.c_char_p, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "mg_rotary": (ctypes.c_int, [ctypes.c_char_p, _P, _P, _P, _P, _P]),
+    "mg_paged_attention": (ctypes.c_int, [ctypes.c_char_p, _P, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 

@@ -11,16 +11,23 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libmg_gemm.so")
-SOURCES = [os.path.join(PKG, "csrc", "mg_gemm.cu")]
-DEPS = SOURCES + [
-    os.path.join(PKG, "csrc", "mg_gemm_kernel.cuh"),
-    os.path.join(PKG, "csrc", "mg_ptx.cuh"),
-    os.path.join(ROOT, "include", "mg_gemm.h"),
-]
+CSRC = os.path.join(PKG, "csrc")
+OBJ = os.path.join(PKG, "_build")
+INCLUDE = os.path.join(ROOT, "include")
+# translation unit -> what it includes
+UNITS = {
+    "mg_gemm.cu": ["mg_gemm_kernel.cuh", "mg_ptx.cuh", "mg_host.h", "mg_plan.h"],
+    "mg_attention.cu": ["mg_attention_common.cuh", "mg_attention_simt.cuh", "mg_rotary.cuh", "mg_paged.cuh",
+                        "mg_ptx.cuh", "mg_host.h"],
+}
+SOURCES = [os.path.join(CSRC, u) for u in UNITS]
+HEADERS = [os.path.join(INCLUDE, h) for h in ("mg_gemm.h", "mg_attention.h")]
+DEPS = SOURCES + sorted({os.path.join(CSRC, h) for hs in UNITS.values() for h in hs}) + HEADERS
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -37,15 +44,28 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(p) <= t for p in DEPS if os.path.exists(p))
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and up_to_date():
-        return LIB
-    cmd = [nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
-           "-I" + os.path.join(ROOT, "include"), "-o", LIB, *SOURCES]
+def _object(unit: str, force: bool, verbose: bool) -> str:
+    """Compiles one translation unit if it, or what it includes, is newer."""
+    obj = os.path.join(OBJ, unit.replace(".cu", ".o"))
+    needs = [os.path.join(CSRC, f) for f in [unit] + UNITS[unit]] + HEADERS
+    if not force and os.path.exists(obj) and all(os.path.getmtime(p) <= os.path.getmtime(obj) for p in needs):
+        return obj
+    cmd = [nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-I" + INCLUDE, "-c", "-o", obj,
+           os.path.join(CSRC, unit)]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd))
     subprocess.run(cmd, check=True)
+    return obj
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    if not force and up_to_date():
+        return LIB
+    os.makedirs(OBJ, exist_ok=True)
+    with ThreadPoolExecutor(len(UNITS)) as pool:
+        objs = list(pool.map(lambda u: _object(u, force, verbose), UNITS))
+    subprocess.run([nvcc(), *ARCH, "-Xcompiler", "-fPIC", "-shared", "-o", LIB, *objs], check=True)
     return LIB
 
 

@@ -1,0 +1,334 @@
+// mg_attention.cu -- host side and C ABI of the attention operators: checks of
+// arguments, choice of kernel, scratch, launches.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "mg_attention.h"
+#include "mg_host.h"
+#include "mg_attention_simt.cuh"
+#include "mg_paged.cuh"
+#include "mg_rotary.cuh"
+
+using mg::host::Device;
+using mg::host::fail;
+using mg::host::Range;
+using mg::host::Scratch;
+
+namespace {
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+size_t elem_size(int dtype) { return dtype == MG_F32 ? 4 : 2; }
+
+mg_status launched(const char* what)
+{
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return fail(MG_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
+    mg::host::count_launch();
+    return MG_OK;
+}
+
+#define MG_TRY(call)                     \
+    do {                                 \
+        const mg_status s_ = (call);     \
+        if (s_ != MG_OK) return s_;      \
+    } while (0)
+
+// ---------------------------------------------------------------- attention
+mg_status check_attention(const mg_attention_desc* d, const char* who)
+{
+    if (!d) return fail(MG_ERR_INVALID, "%s: descriptor is NULL", who);
+    if (d->dtype != MG_F32 && d->dtype != MG_BF16)
+        return fail(MG_ERR_INVALID, "%s: dtype %d is neither MG_F32 nor MG_BF16", who, d->dtype);
+    if (d->batch < 0 || d->heads < 1 || d->kv_heads < 1 || d->q_len < 0 || d->k_len < 0)
+        return fail(MG_ERR_INVALID, "%s: batch %d, heads %d, kv_heads %d, q_len %d, k_len %d out of range", who,
+                    d->batch, d->heads, d->kv_heads, d->q_len, d->k_len);
+    if (d->heads % d->kv_heads)
+        return fail(MG_ERR_INVALID, "%s: heads %d is not a multiple of kv_heads %d", who, d->heads, d->kv_heads);
+    if (d->head_dim < 1 || d->head_dim > MG_MAX_HEAD_DIM)
+        return fail(MG_ERR_UNSUPPORTED, "%s: head_dim %d is outside 1..%d", who, d->head_dim, MG_MAX_HEAD_DIM);
+    if (!std::isfinite(d->scale)) return fail(MG_ERR_INVALID, "%s: scale is not finite", who);
+    if (!(d->cap >= 0.f) || !std::isfinite(d->cap))
+        return fail(MG_ERR_INVALID, "%s: cap must be 0 (none) or a positive number", who);
+    if (d->prefix && !d->causal) return fail(MG_ERR_INVALID, "%s: a prefix needs causal", who);
+    if ((int64_t)d->q_len + d->k_len >= (1ll << 30)) return fail(MG_ERR_UNSUPPORTED, "%s: rows are too long", who);
+    const int64_t rows = (int64_t)d->batch * d->heads * std::max(ceil_div(d->q_len, 32), ceil_div(d->k_len, 32));
+    if (rows >= (1ll << 31) - 1) return fail(MG_ERR_UNSUPPORTED, "%s: batch * heads * rows is too large", who);
+    return MG_OK;
+}
+
+mg::AttnParams attention_params(const mg_attention_desc* d)
+{
+    mg::AttnParams p = {};
+    p.B = d->batch, p.H = d->heads, p.Hkv = d->kv_heads, p.Lq = d->q_len, p.Lk = d->k_len, p.D = d->head_dim;
+    p.causal = d->causal != 0;
+    p.scale = d->scale, p.cap = d->cap;
+    // a dim of one element may carry any stride
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = d->q_stride[i], p.ks[i] = d->k_stride[i], p.vs[i] = d->v_stride[i], p.os[i] = d->out_stride[i];
+        p.dos[i] = d->dout_stride[i], p.dqs[i] = d->dq_stride[i];
+        p.dks[i] = d->dk_stride[i], p.dvs[i] = d->dv_stride[i];
+        const int qn = i == 0 ? d->batch : i == 1 ? d->heads : d->q_len;
+        const int kn = i == 0 ? d->batch : i == 1 ? d->kv_heads : d->k_len;
+        if (qn == 1) p.qs[i] = p.os[i] = p.dos[i] = p.dqs[i] = 0;
+        if (kn == 1) p.ks[i] = p.vs[i] = p.dks[i] = p.dvs[i] = 0;
+    }
+    p.slopes = d->slopes, p.docs = d->documents, p.prefix = d->prefix;
+    return p;
+}
+
+template <typename K>
+mg_status simt_launch(K kernel, int blocks, int rows_in_smem, int tiles33, const mg::AttnParams& p, cudaStream_t st,
+                      const char* what)
+{
+    const size_t smem = sizeof(float) * ((size_t)rows_in_smem * mg::kSimtTile * (p.D + 1) +
+                                         (size_t)tiles33 * mg::kSimtTile * 33);
+    MG_HOST_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kernel<<<blocks, mg::kSimtThreads, smem, st>>>(p);
+    return launched(what);
+}
+
+template <typename T>
+mg_status forward_simt(const mg::AttnParams& p, cudaStream_t st)
+{
+    return simt_launch(mg::attn_simt_forward<T>, p.B * p.H * ceil_div(p.Lq, mg::kSimtTile), 3, 1, p, st,
+                       "mg_attention");
+}
+
+template <typename T>
+mg_status backward_simt(const mg::AttnParams& p, cudaStream_t st)
+{
+    const char* who = "mg_attention_backward";
+    if (p.Lq > 0) {
+        mg::attn_delta_kernel<T><<<ceil_div((int64_t)p.B * p.H * p.Lq, 8), 256, 0, st>>>(p);
+        MG_TRY(launched(who));
+        MG_TRY(simt_launch(mg::attn_simt_backward_dq<T>, p.B * p.H * ceil_div(p.Lq, mg::kSimtTile), 4, 1, p, st, who));
+    }
+    if (p.Lk > 0)
+        MG_TRY(simt_launch(mg::attn_simt_backward_dkv<T>, p.B * p.Hkv * ceil_div(p.Lk, mg::kSimtTile), 4, 2, p, st,
+                           who));
+    return MG_OK;
+}
+
+// Whether rows at `ptr` with these strides start on multiples of `vec` elements.
+bool aligned(const void* ptr, const int64_t* strides, int n, size_t elem, int vec)
+{
+    if (reinterpret_cast<uintptr_t>(ptr) % (elem * vec)) return false;
+    for (int i = 0; i < n; ++i)
+        if (strides[i] % vec) return false;
+    return true;
+}
+
+// ---------------------------------------------------------------- paged
+// Splits: enough blocks to fill the GPU several times over, so that requests of
+// uneven lengths even out, but no chunk shorter than 128 keys.
+template <typename T>
+mg_status launch_paged(mg::PagedParams& p, int longest, const Device& dev, Scratch& ws, cudaStream_t st,
+                       const char* who)
+{
+    const int group = p.H / p.Hkv, packs = ceil_div(group, mg::kPagedHeads);
+    const int64_t heads = (int64_t)p.B * p.Hkv * packs;
+    const int64_t want = std::max<int64_t>(1, (int64_t)dev.sm_count * 8 / heads);
+    const int most = std::max(1, ceil_div(longest, 128));
+    int splits = (int)std::min<int64_t>(want, most);
+    p.chunk = std::max(1, ceil_div(longest, splits));
+    p.splits = splits = std::max(1, ceil_div(longest, p.chunk));
+    if (heads * splits >= (1ll << 31) - 1) return fail(MG_ERR_UNSUPPORTED, "%s: batch is too large", who);
+    if (splits > 1) {
+        const size_t rows = (size_t)p.B * p.H * splits;
+        p.part = static_cast<float*>(ws.get(rows * p.D * sizeof(float)));
+        p.stat = static_cast<float2*>(ws.get(rows * sizeof(float2)));
+        if (!p.part || !p.stat) return fail(MG_ERR_ALLOC, "%s: no scratch for %zu chunks", who, rows);
+    }
+    mg::paged_simt_kernel<T><<<(int)(heads * splits), mg::kPagedThreads, 0, st>>>(p);
+    MG_TRY(launched(who));
+    if (splits > 1) {
+        mg::paged_join_kernel<T><<<ceil_div((int64_t)p.B * p.H, mg::kPagedThreads / 32), mg::kPagedThreads, 0, st>>>(p);
+        MG_TRY(launched(who));
+    }
+    return MG_OK;
+}
+
+// ---------------------------------------------------------------- rotary
+template <typename T, int VEC>
+mg_status launch_rotary(mg::RotaryParams& p, const Device& dev, cudaStream_t st)
+{
+    p.units = p.pairs / VEC;
+    p.tail_units = (p.D - 2 * p.pairs) / VEC;
+    const int heads = p.H + p.Hkv;
+    const int64_t tokens = (int64_t)p.B * p.L, per_head = tokens * (p.units + p.tail_units);
+    // One set of sines serves several heads where there is work enough to fill
+    // the GPU (a few blocks an SM) all the same.
+    p.heads_per_thread = 1;
+    while (p.heads_per_thread < 8 && per_head * ceil_div(heads, 2 * p.heads_per_thread) >= (int64_t)dev.sm_count * 1024)
+        p.heads_per_thread *= 2;
+    p.groups = ceil_div(heads, p.heads_per_thread);
+    p.total = per_head * p.groups;
+    if (p.total == 0) return MG_OK;
+    if ((p.total + 127) / 128 >= (1ll << 31)) return fail(MG_ERR_UNSUPPORTED, "mg_rotary: too many elements");
+    mg::rotary_kernel<T, VEC><<<(unsigned)((p.total + 127) / 128), 128, 0, st>>>(p);
+    return launched("mg_rotary");
+}
+
+}  // namespace
+
+extern "C" {
+
+mg_status mg_attention(const mg_attention_desc* d, void* out, float* lse, const void* q, const void* k,
+                       const void* v, void* stream)
+{
+    Range range("mg_attention");
+    MG_TRY(check_attention(d, "mg_attention"));
+    if (d->batch == 0 || d->q_len == 0) return MG_OK;
+    if (!out || !lse || !q || (d->k_len > 0 && (!k || !v)))
+        return fail(MG_ERR_INVALID, "mg_attention: a tensor is NULL");
+    Device dev;
+    MG_TRY(mg::host::device(&dev));
+    mg::AttnParams p = attention_params(d);
+    p.out = out, p.lse = lse, p.q = q, p.k = k, p.v = v;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (d->q_len == 1) {
+        // One query: its row of keys is split over the GPU, as a paged cache of
+        // one page per batch would be. Its position is the last key's, so that
+        // causal and prefix masks hide nothing.
+        mg::PagedParams g = {};
+        g.B = p.B, g.H = p.H, g.Hkv = p.Hkv, g.D = p.D;
+        g.scale = p.scale, g.cap = p.cap, g.slopes = p.slopes;
+        g.length = p.Lk, g.docs = p.docs;
+        g.qs[0] = p.qs[0], g.qs[1] = p.qs[1], g.os[0] = p.os[0], g.os[1] = p.os[1];
+        g.ks[0] = p.ks[0], g.ks[1] = p.ks[2], g.ks[2] = p.ks[1];
+        g.vs[0] = p.vs[0], g.vs[1] = p.vs[2], g.vs[2] = p.vs[1];
+        g.q = q, g.k = const_cast<void*>(k), g.v = const_cast<void*>(v), g.out = out, g.lse = lse;
+        g.status = dev.status;
+        Scratch ws(dev, stream);
+        return d->dtype == MG_F32 ? launch_paged<float>(g, p.Lk, dev, ws, st, "mg_attention")
+                                  : launch_paged<__nv_bfloat16>(g, p.Lk, dev, ws, st, "mg_attention");
+    }
+    return d->dtype == MG_F32 ? forward_simt<float>(p, st) : forward_simt<__nv_bfloat16>(p, st);
+}
+
+mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, void* dv, const void* dout,
+                                const void* q, const void* k, const void* v, const void* out, const float* lse,
+                                void* stream)
+{
+    Range range("mg_attention_backward");
+    MG_TRY(check_attention(d, "mg_attention_backward"));
+    if (d->batch == 0 || (d->q_len == 0 && d->k_len == 0)) return MG_OK;
+    if ((d->q_len > 0 && (!dq || !dout || !q || !out || !lse)) || (d->k_len > 0 && (!dk || !dv || !k || !v)))
+        return fail(MG_ERR_INVALID, "mg_attention_backward: a tensor is NULL");
+    Device dev;
+    MG_TRY(mg::host::device(&dev));
+    mg::AttnParams p = attention_params(d);
+    p.q = q, p.k = k, p.v = v, p.out = const_cast<void*>(out), p.dout = dout, p.lse = const_cast<float*>(lse);
+    p.dq = dq, p.dk = dk, p.dv = dv;
+    Scratch ws(dev, stream);
+    if (d->q_len > 0) {
+        p.delta = static_cast<float*>(ws.get(sizeof(float) * d->batch * d->heads * (size_t)d->q_len));
+        if (!p.delta) return fail(MG_ERR_ALLOC, "mg_attention_backward: no scratch for the row sums");
+    }
+    cudaStream_t st = (cudaStream_t)stream;
+    return d->dtype == MG_F32 ? backward_simt<float>(p, st) : backward_simt<__nv_bfloat16>(p, st);
+}
+
+mg_status mg_rotary(const mg_rotary_desc* d, void* out_q, void* out_k, const void* q, const void* k, void* stream)
+{
+    Range range("mg_rotary");
+    if (!d) return fail(MG_ERR_INVALID, "mg_rotary: descriptor is NULL");
+    if (d->dtype != MG_F32 && d->dtype != MG_BF16)
+        return fail(MG_ERR_INVALID, "mg_rotary: dtype %d is neither MG_F32 nor MG_BF16", d->dtype);
+    if (d->batch < 0 || d->heads < 0 || d->kv_heads < 0 || d->len < 0 || d->head_dim < 1)
+        return fail(MG_ERR_INVALID, "mg_rotary: batch %d, heads %d, kv_heads %d, len %d, head_dim %d out of range",
+                    d->batch, d->heads, d->kv_heads, d->len, d->head_dim);
+    if (d->pairs < 0 || d->pairs > d->head_dim / 2)
+        return fail(MG_ERR_INVALID, "mg_rotary: %d pairs do not fit a head of %d", d->pairs, d->head_dim);
+    if (!std::isfinite(d->magnitude)) return fail(MG_ERR_INVALID, "mg_rotary: magnitude is not finite");
+    const int kvh = k ? d->kv_heads : 0;
+    if (d->batch == 0 || d->len == 0 || d->heads + kvh == 0) return MG_OK;
+    if ((d->heads > 0 && (!q || !out_q)) || (kvh > 0 && !out_k))
+        return fail(MG_ERR_INVALID, "mg_rotary: a tensor is NULL");
+    if (d->pairs > 0 && (!d->positions || !d->frequencies))
+        return fail(MG_ERR_INVALID, "mg_rotary: positions and frequencies are needed");
+    Device dev;
+    MG_TRY(mg::host::device(&dev));
+    mg::RotaryParams p = {};
+    p.B = d->batch, p.H = d->heads, p.Hkv = kvh, p.L = d->len, p.D = d->head_dim, p.pairs = d->pairs;
+    p.interleaved = d->interleaved != 0, p.inverse = d->inverse != 0, p.magnitude = d->magnitude;
+    // a dim of one element may carry any stride
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = d->q_stride[i], p.ks[i] = d->k_stride[i];
+        p.oqs[i] = d->out_q_stride[i], p.oks[i] = d->out_k_stride[i];
+        const int n = i == 0 ? d->batch : d->len;   // a dim of one element may carry any stride
+        if (i == 1 ? d->heads == 1 : n == 1) p.qs[i] = p.oqs[i] = 0;
+        if (i == 1 ? kvh == 1 : n == 1) p.ks[i] = p.oks[i] = 0;
+    }
+    p.pos_stride = d->position_stride, p.positions = d->positions, p.frequencies = d->frequencies;
+    p.q = q, p.k = k, p.oq = out_q, p.ok = out_k;
+    // The widest vector that every row, the pairs and the rest of the head allow.
+    const size_t e = elem_size(d->dtype);
+    int vec = (int)(16 / e);
+    while (vec > 1) {
+        bool ok = p.pairs % vec == 0 && (p.D - 2 * p.pairs) % vec == 0;
+        if (p.H) ok = ok && aligned(q, p.qs, 3, e, vec) && aligned(out_q, p.oqs, 3, e, vec);
+        if (kvh) ok = ok && aligned(k, p.ks, 3, e, vec) && aligned(out_k, p.oks, 3, e, vec);
+        if (ok) break;
+        vec /= 2;
+    }
+    cudaStream_t st = (cudaStream_t)stream;
+    using bf16 = __nv_bfloat16;
+    if (d->dtype == MG_F32)
+        return vec == 4 ? launch_rotary<float, 4>(p, dev, st)
+             : vec == 2 ? launch_rotary<float, 2>(p, dev, st) : launch_rotary<float, 1>(p, dev, st);
+    return vec == 8 ? launch_rotary<bf16, 8>(p, dev, st) : vec == 4 ? launch_rotary<bf16, 4>(p, dev, st)
+         : vec == 2 ? launch_rotary<bf16, 2>(p, dev, st) : launch_rotary<bf16, 1>(p, dev, st);
+}
+
+mg_status mg_paged_attention(const mg_paged_desc* d, void* out, float* lse, const void* q, void* k_pages,
+                             void* v_pages, const void* k_new, const void* v_new, void* stream)
+{
+    Range range("mg_paged_attention");
+    const char* who = "mg_paged_attention";
+    if (!d) return fail(MG_ERR_INVALID, "%s: descriptor is NULL", who);
+    if (d->dtype != MG_F32 && d->dtype != MG_BF16)
+        return fail(MG_ERR_INVALID, "%s: dtype %d is neither MG_F32 nor MG_BF16", who, d->dtype);
+    if (d->batch < 0 || d->heads < 1 || d->kv_heads < 1 || d->page_size < 1 || d->pages < 0 || d->table_width < 0)
+        return fail(MG_ERR_INVALID,
+                    "%s: batch %d, heads %d, kv_heads %d, page_size %d, pages %d, table_width %d out of range", who,
+                    d->batch, d->heads, d->kv_heads, d->page_size, d->pages, d->table_width);
+    if (d->heads % d->kv_heads)
+        return fail(MG_ERR_INVALID, "%s: heads %d is not a multiple of kv_heads %d", who, d->heads, d->kv_heads);
+    if (d->head_dim < 1 || d->head_dim > MG_MAX_HEAD_DIM)
+        return fail(MG_ERR_UNSUPPORTED, "%s: head_dim %d is outside 1..%d", who, d->head_dim, MG_MAX_HEAD_DIM);
+    if (!std::isfinite(d->scale)) return fail(MG_ERR_INVALID, "%s: scale is not finite", who);
+    if (!(d->cap >= 0.f) || !std::isfinite(d->cap))
+        return fail(MG_ERR_INVALID, "%s: cap must be 0 (none) or a positive number", who);
+    if ((k_new == nullptr) != (v_new == nullptr))
+        return fail(MG_ERR_INVALID, "%s: k_new and v_new come together", who);
+    if (d->batch == 0) return MG_OK;
+    const int64_t longest = (int64_t)d->table_width * d->page_size;
+    if (longest >= (1ll << 30)) return fail(MG_ERR_UNSUPPORTED, "%s: the block table is too wide", who);
+    if (!out || !lse || !q || !d->lengths || (longest > 0 && (!k_pages || !v_pages || !d->block_table)))
+        return fail(MG_ERR_INVALID, "%s: a tensor is NULL", who);
+    Device dev;
+    MG_TRY(mg::host::device(&dev));
+    mg::PagedParams p = {};
+    p.B = d->batch, p.H = d->heads, p.Hkv = d->kv_heads, p.D = d->head_dim;
+    p.page = d->page_size, p.pages = d->pages, p.width = d->table_width;
+    p.scale = d->scale, p.cap = d->cap;
+    for (int i = 0; i < 3; ++i) p.ks[i] = d->k_stride[i], p.vs[i] = d->v_stride[i];
+    for (int i = 0; i < 2; ++i) {
+        p.qs[i] = d->q_stride[i], p.os[i] = d->out_stride[i];
+        p.kns[i] = d->k_new_stride[i], p.vns[i] = d->v_new_stride[i];
+    }
+    p.table_stride = d->table_stride, p.slopes = d->slopes, p.table = d->block_table, p.lengths = d->lengths;
+    p.q = q, p.k = k_pages, p.v = v_pages, p.k_new = k_new, p.v_new = v_new, p.out = out, p.lse = lse;
+    p.status = dev.status;
+    Scratch ws(dev, stream);
+    cudaStream_t st = (cudaStream_t)stream;
+    return d->dtype == MG_F32 ? launch_paged<float>(p, (int)longest, dev, ws, st, who)
+                              : launch_paged<__nv_bfloat16>(p, (int)longest, dev, ws, st, who);
+}
+
+}  // extern "C"

@@ -1,0 +1,67 @@
+// mg_attention_common.cuh -- what the attention kernels share: parameters, the
+// rule which keys a query sees, and the score's curve.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+#include <stdint.h>
+
+namespace mg {
+
+struct AttnParams {
+    int B, H, Hkv, Lq, Lk, D;
+    int causal;
+    float scale, cap;
+    int64_t qs[3], ks[3], vs[3], os[3];          // batch, head, row
+    int64_t dos[3], dqs[3], dks[3], dvs[3];
+    const float* slopes;
+    const int32_t* docs;
+    const int32_t* prefix;
+    const void *q, *k, *v, *dout;
+    void *out, *dq, *dk, *dv;
+    float* lse;
+    float* delta;
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Position of query i, and its document id: -1 for a query that has none.
+__device__ __forceinline__ int query_pos(const AttnParams& p, int i) { return i + p.Lk - p.Lq; }
+
+__device__ __forceinline__ int doc_at(const AttnParams& p, int b, int pos)
+{
+    return pos >= 0 && pos < p.Lk ? __ldg(p.docs + (int64_t)b * p.Lk + pos) : -1;
+}
+
+// Whether the query at position qpos (document qdoc) sees key j (document kdoc).
+__device__ __forceinline__ bool sees(const AttnParams& p, int qpos, int qdoc, int j, int kdoc, int prefix)
+{
+    return (!p.causal || j <= qpos || j < prefix) && (p.docs == nullptr || (qdoc >= 0 && qdoc == kdoc));
+}
+
+// tanh(x) = 1 - 2 / (1 + exp(2x)), from both ends right for any x; the
+// absolute error is that of one fp32 rounding near 1, which is what a score
+// of up to `cap` can hold anyway. Used by the 32-bit kernels.
+__device__ __forceinline__ float tanh_full(float x) { return tanhf(x); }
+
+// The score of one pair from the scaled product t: capped and biased. `bend`
+// receives tanh(t / cap) (0 without a cap).
+__device__ __forceinline__ float score(float t, float cap, float slope, int dist, float& bend)
+{
+    bend = 0.f;
+    if (cap > 0.f) {
+        bend = tanh_full(t / cap);
+        t = cap * bend;
+    }
+    return t - slope * (float)(dist < 0 ? -dist : dist);
+}
+
+}  // namespace mg

@@ -23,6 +23,7 @@
 
 #include "mg_gemm.h"
 #include "mg_gemm_kernel.cuh"
+#include "mg_host.h"
 
 namespace {
 
@@ -1778,3 +1779,67 @@ uint64_t mg_launch_count(void) { return g_launches.load(); }
 const char* mg_version(void) { return "mg_gemm 0.1.0 (sm_100a tcgen05 tf32 / 3xtf32)"; }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------- shared with the other translation units
+namespace mg {
+namespace host {
+
+mg_status fail(mg_status s, const char* fmt, ...)
+{
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return ::fail(s, "%s", buf);
+}
+
+mg_status device(Device* out)
+{
+    DeviceState* d = nullptr;
+    const mg_status s = device_state(&d);
+    if (s != MG_OK) return s;
+    out->ordinal = (int)(d - g_dev);
+    out->sm_count = d->sm_count;
+    out->max_smem = d->max_smem;
+    out->status = d->status;
+    out->pool = d->pool;
+    return MG_OK;
+}
+
+void count_launch() { g_launches.fetch_add(1); }
+
+Scratch::~Scratch()
+{
+    for (int i = 0; i < n_; ++i) {
+        if (g_free) g_free(ptrs_[i], stream_, g_alloc_ctx);
+        else cudaFreeAsync(ptrs_[i], (cudaStream_t)stream_);
+    }
+}
+
+void* Scratch::get(size_t bytes)
+{
+    if (n_ == 8) return nullptr;
+    void* p = nullptr;
+    if (g_alloc) p = g_alloc(bytes, stream_, g_alloc_ctx);
+    else if (cudaMallocFromPoolAsync(&p, bytes, pool_, (cudaStream_t)stream_) != cudaSuccess) p = nullptr;
+    if (p) ptrs_[n_++] = p;
+    return p;
+}
+
+mg_status encode_bf16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                      const uint32_t* box)
+{
+    cuuint64_t d[5], st[4];
+    cuuint32_t b[5], one[5] = {1, 1, 1, 1, 1};
+    for (int i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i];
+    for (int i = 0; i + 1 < rank; ++i) st[i] = strides[i];
+    const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), d,
+                                st, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return ::fail(MG_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+    return MG_OK;
+}
+
+}  // namespace host
+}  // namespace mg

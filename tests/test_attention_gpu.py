@@ -1,0 +1,312 @@
+"""attention and attention_backward against the definition in 64 bits: types,
+shared heads, head sizes, lengths from one token on, strided views, caps, biases,
+documents, prefixes, rows that see nothing, padding that holds NaN; determinism,
+other streams, captured graphs, offsets beyond 32 bits."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import macrograd_b200 as mg  # noqa: E402
+from attention_reference import Reference, within  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+SIZES = [  # B, H, Hkv, Lq, Lk, D
+    (1, 1, 1, 1, 1, 8),
+    (2, 4, 2, 1, 257, 64),
+    (3, 2, 1, 5, 7, 16),
+    (1, 2, 1, 17, 17, 40),
+    (1, 3, 3, 33, 70, 33),
+    (2, 2, 2, 64, 64, 64),
+    (2, 3, 3, 128, 128, 64),
+    (1, 4, 2, 129, 255, 128),
+    (1, 2, 2, 200, 100, 64),
+    (1, 6, 2, 257, 513, 96),
+    (1, 2, 1, 640, 640, 128),
+    (2, 1, 1, 385, 385, 80),
+    (1, 5, 1, 128, 384, 128),
+]
+MASKS = ["full", "causal", "cap", "slopes", "documents", "prefix", "all"]
+
+
+def make(size, mask, dtype, seed=0, strided=True):
+    B, H, Hkv, Lq, Lk, D = size
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    gain = 3.0 if mask in ("cap", "all") else 1.0
+
+    def heads(n, L, gain=1.0):
+        if strided:
+            return (torch.randn((B, L, n, D), generator=g, device="cuda") * gain).to(dtype).transpose(1, 2)
+        return (torch.randn((B, n, L, D), generator=g, device="cuda") * gain).to(dtype)
+
+    q, k, v, dout = heads(H, Lq, gain), heads(Hkv, Lk), heads(Hkv, Lk), heads(H, Lq)
+    kw = dict(causal=mask != "full")
+    if mask in ("cap", "all"):
+        kw["cap"] = 10.0
+    if mask in ("slopes", "all"):
+        kw["slopes"] = torch.tensor([2.0 ** (-1 - h) for h in range(H)], device="cuda")
+    if mask in ("documents", "all"):
+        ids = torch.zeros((B, Lk), dtype=torch.int32)
+        for b in range(B):
+            cuts = sorted(int(x) for x in torch.randint(0, Lk + 1, (3,), generator=torch.Generator().manual_seed(b)))
+            for i, c in enumerate(cuts):
+                ids[b, c:] = 5 - i           # ids fall along the row
+            ids[b, Lk - Lk // 9:] = -1       # padding at the end
+        kw["documents"] = ids.cuda()
+    if mask in ("prefix", "all"):
+        kw["prefix"] = torch.tensor([Lk * (2 * b + 1) // (3 * B) for b in range(B)], dtype=torch.int32, device="cuda")
+    return q, k, v, dout, kw
+
+
+def compare(q, k, v, dout, kw):
+    out, lse = mg.attention(q, k, v, **kw)
+    ref = Reference(q, k, v, dout, **kw)
+    within(out, ref.out, ref.out_tol, "out")
+    within(lse, ref.lse, ref.lse_tol, "lse")
+    dq, dk, dv = mg.attention_backward(dout, q, k, v, out, lse, **kw)
+    within(dv, ref.dv, ref.dv_tol, "dv")
+    within(dq, ref.dq, ref.dq_tol, "dq")
+    within(dk, ref.dk, ref.dk_tol, "dk")
+    assert out.stride() == torch.empty_like(q).stride()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_attention_and_gradients(size, mask, dtype):
+    compare(*make(size, mask, dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_long_rows(dtype):
+    """Several rows of tiles, an odd length, shared heads, documents shorter and longer than a tile."""
+    q, k, v, dout, kw = make((1, 4, 2, 1537, 1537, 128), "causal", dtype, 3)
+    ids = torch.repeat_interleave(torch.arange(6), torch.tensor([1, 130, 700, 5, 601, 100])).int()[None].cuda()
+    kw["documents"] = ids.contiguous()
+    compare(q, k, v, dout, kw)
+
+
+@pytest.mark.parametrize("layout", ["packed", "unaligned", "wide"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_views(layout, dtype):
+    """q, k, v as slices of one buffer; rows that do not start on 16 bytes; rows much wider than a head."""
+    B, H, L, D = 2, 3, 150, 64
+    g = torch.Generator(device="cuda").manual_seed(7)
+    if layout == "packed":
+        qkv = torch.randn((B, L, 3, H, D), generator=g, device="cuda").to(dtype)
+        q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
+    else:
+        pad = 1 if layout == "unaligned" else 448
+        q, k, v = (torch.randn((B, H, L, D + pad), generator=g, device="cuda").to(dtype)[..., pad:] for _ in range(3))
+    dout = torch.randn((B, L, H, D), generator=g, device="cuda").to(dtype).transpose(1, 2)
+    compare(q, k, v, dout, dict(causal=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 33])
+def test_padding_may_hold_anything(dtype, D):
+    """NaN and infinity in the keys, values, queries and upstream gradients of padding reach nothing."""
+    L = 300
+    q, k, v, dout, _ = make((2, 2, 1, L, L, D), "causal", dtype, 11, strided=False)
+    ids = torch.zeros((2, L), dtype=torch.int32, device="cuda")
+    ids[0, 200:] = -1
+    ids[1, 100:140] = -1     # padding in the middle of a row
+    ids[1, 140:] = 4
+    for t in (q, k, v, dout):
+        pad = (ids < 0)[:, None, :, None].expand_as(t)
+        t[pad] = float("nan")
+        t[0, :, 250] = float("inf")
+    kw = dict(causal=True, documents=ids)
+    compare(q, k, v, dout, kw)
+    out, lse = mg.attention(q, k, v, **kw)
+    assert (out[0, :, 200:] == 0).all() and torch.isneginf(lse[0, :, 200:]).all()
+    dq, dk, dv = mg.attention_backward(dout, q, k, v, out, lse, **kw)
+    for t in (dq, dk, dv):
+        assert (t[0, :, 200:] == 0).all() and (t[1, :, 100:140] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_rows_that_see_nothing(dtype):
+    """More queries than keys: the first queries stand before every key."""
+    q, k, v, dout, kw = make((1, 2, 1, 150, 20, 64), "causal", dtype, 5)
+    out, lse = mg.attention(q, k, v, **kw)
+    assert (out[:, :, :130] == 0).all() and torch.isneginf(lse[:, :, :130]).all()
+    compare(q, k, v, dout, kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("Lq", [1, 9])
+def test_no_keys(dtype, Lq):
+    q = torch.randn((2, 2, Lq, 64), device="cuda").to(dtype)
+    k = torch.empty((2, 1, 0, 64), device="cuda", dtype=dtype)
+    out, lse = mg.attention(q, k, k)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    dq, dk, dv = mg.attention_backward(q, q, k, k, out, lse)
+    assert (dq == 0).all() and dk.numel() == dv.numel() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_no_queries(dtype):
+    q = torch.empty((2, 2, 0, 64), device="cuda", dtype=dtype)
+    k = torch.randn((2, 1, 130, 64), device="cuda").to(dtype)
+    out, lse = mg.attention(q, k, k)
+    dq, dk, dv = mg.attention_backward(q, q, k, k, out, lse)
+    assert out.numel() == dq.numel() == 0 and (dk == 0).all() and (dv == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_large_scores(dtype, cap):
+    """Scores of several hundred: the running maximum moves far, sums stay finite."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k = (torch.randn((1, 2, 400, 64), generator=g, device="cuda").mul(8).to(dtype) for _ in range(2))
+    v, dout = (torch.randn((1, 2, 400, 64), generator=g, device="cuda").to(dtype) for _ in range(2))
+    k[:, :, 300:] *= 4       # the maximum comes late
+    compare(q, k, v, dout, dict(causal=False, cap=cap))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_same_inputs_same_bits(dtype):
+    q, k, v, dout, kw = make((1, 4, 1, 300, 300, 64), "all", dtype, 4)
+    first = mg.attention(q, k, v, **kw)
+    grads = mg.attention_backward(dout, q, k, v, *first, **kw)
+    for _ in range(3):
+        again = mg.attention(q, k, v, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+        assert all(torch.equal(a, b) for a, b in zip(grads, mg.attention_backward(dout, q, k, v, *again, **kw)))
+
+
+def test_scale_is_the_callers():
+    q, k, v, dout, kw = make((1, 2, 2, 100, 100, 64), "causal", torch.float32, 8)
+    compare(q, k, v, dout, dict(kw, scale=0.3))
+    compare(q, k, v, dout, dict(kw, scale=-0.05))
+
+
+def test_out_and_its_neighbours():
+    """out given as a view: its rows are written, what lies around them stays."""
+    q, k, v, _, kw = make((2, 3, 3, 150, 150, 64), "causal", torch.bfloat16, 9)
+    room = torch.full((2, 170, 5, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+    out = room[:, 10:160, 1:4].transpose(1, 2)
+    got, _ = mg.attention(q, k, v, out=out, **kw)
+    assert got is out
+    assert torch.equal(out, mg.attention(q, k, v, **kw)[0])
+    rest = torch.ones_like(room, dtype=torch.bool)
+    rest[:, 10:160, 1:4] = False
+    assert (room[rest] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("Lq", [1, 140])
+def test_captured_and_replayed_with_other_inputs(dtype, Lq):
+    size = (2, 2, 1, Lq, 300, 64)
+    q, k, v, dout, kw = make(size, "all", dtype, 20)
+    mg.attention_backward(dout, q, k, v, *mg.attention(q, k, v, **kw), **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = mg.attention(q, k, v, **kw)
+        grads = mg.attention_backward(dout, q, k, v, out, lse, **kw)
+    for seed in (21, 22):
+        q2, k2, v2, dout2, _ = make(size, "all", dtype, seed)
+        for a, b in ((q, q2), (k, k2), (v, v2), (dout, dout2)):
+            a.copy_(b)
+        kw["documents"].copy_(kw["documents"].roll(seed - 20, 1))
+        kw["prefix"].add_(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = mg.attention(q, k, v, **kw)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        for a, b in zip(grads, mg.attention_backward(dout, q, k, v, *want, **kw)):
+            assert torch.equal(a, b)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams do not share scratch."""
+    sets = [make((1, 8, 2, 700, 700, 64), "all", torch.bfloat16, 30 + i) for i in range(2)]
+    want = []
+    for q, k, v, dout, kw in sets:
+        f = mg.attention(q, k, v, **kw)
+        want.append(f + mg.attention_backward(dout, q, k, v, *f, **kw))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, (q, k, v, dout, kw) in enumerate(sets):
+            f = mg.attention(q, k, v, stream=streams[i], **kw)
+            got[i].append(f + mg.attention_backward(dout, q, k, v, *f, stream=streams[i], **kw))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
+
+
+@pytest.mark.parametrize("Lq", [1, 130])
+def test_offsets_beyond_32_bits(Lq):
+    """Batches and heads more than 2^32 bytes and 2^31 elements apart."""
+    far = (1 << 31) + 4096
+    buf = torch.zeros(far + 300 * 64 * 4, dtype=torch.bfloat16, device="cuda")
+    k = torch.as_strided(buf, (2, 2, 200, 64), (far, 200 * 64, 64, 1))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k.copy_(torch.randn((2, 2, 200, 64), generator=g, device="cuda"))
+    q = torch.randn((2, 2, Lq, 64), generator=g, device="cuda").bfloat16()
+    dout = torch.randn((2, 2, Lq, 64), generator=g, device="cuda").bfloat16()
+    kw = dict(causal=True)
+    out, lse = mg.attention(q, k, k, **kw)
+    ref = Reference(q, k, k, dout, **kw)
+    within(out, ref.out, ref.out_tol, "out")
+    within(lse, ref.lse, ref.lse_tol, "lse")
+    dq, dk, dv = mg.attention_backward(dout, q, k, k, out, lse, **kw)
+    within(dq, ref.dq, ref.dq_tol, "dq")
+    within(dk, ref.dk, ref.dk_tol, "dk")
+    within(dv, ref.dv, ref.dv_tol, "dv")
+
+
+@pytest.mark.parametrize("kw", [dict(causal=True), dict(causal=False, cap=4.0)], ids=["causal", "cap"])
+def test_gradients_against_differences(kw):
+    """Central differences of the forward call itself, in fp32: step h = 2^-6 leaves h^2 / 6 of the third derivative
+    (below 2^-13 for these O(1) functions summed over 60 outputs) and 2^-24 * |loss| / h of rounding."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v, dout = (torch.randn((1, 1, 6, 10), generator=g, device="cuda") for _ in range(4))
+    out, lse = mg.attention(q, k, v, **kw)
+    grads = mg.attention_backward(dout, q, k, v, out, lse, **kw)
+    h = 2.0 ** -6
+    loss = lambda: float((mg.attention(q, k, v, **kw)[0].double() * dout.double()).sum())  # noqa: E731
+    for t, grad in zip((q, k, v), grads):
+        flat = t.view(-1)
+        for i in range(0, 60, 7):
+            x = float(flat[i])
+            flat[i] = x + h
+            up = loss()
+            flat[i] = x - h
+            down = loss()
+            flat[i] = x
+            assert abs((up - down) / (2 * h) - float(grad.view(-1)[i])) < 2e-3
+
+
+def test_refusals():
+    t = lambda *s, **k: torch.zeros(s, device="cuda", **k)  # noqa: E731
+    q, kv = t(1, 4, 8, 64), t(1, 2, 8, 64)
+    bad = [
+        (lambda: mg.attention(q.cpu(), kv, kv), "CUDA tensor"),
+        (lambda: mg.attention(q.half(), kv.half(), kv.half()), "float32 or bfloat16"),
+        (lambda: mg.attention(q, kv.bfloat16(), kv.bfloat16()), "as the others"),
+        (lambda: mg.attention(q[0], kv, kv), "4 dims"),
+        (lambda: mg.attention(q, t(1, 3, 8, 64), t(1, 3, 8, 64)), "multiple"),
+        (lambda: mg.attention(q, t(1, 2, 8, 32), t(1, 2, 8, 32)), "Found shapes"),
+        (lambda: mg.attention(q, kv, t(1, 2, 9, 64)), "Found shapes"),
+        (lambda: mg.attention(q.transpose(2, 3).contiguous().transpose(2, 3), kv, kv), "contiguous in its last dim"),
+        (lambda: mg.attention(t(1, 4, 8, 136), t(1, 2, 8, 136), t(1, 2, 8, 136)), "head_dim"),
+        (lambda: mg.attention(q, kv, kv, cap=-1.0), "cap"),
+        (lambda: mg.attention(q, kv, kv, scale=math.inf), "finite"),
+        (lambda: mg.attention(q, kv, kv, slopes=t(2)), "slopes"),
+        (lambda: mg.attention(q, kv, kv, documents=t(1, 8)), "documents"),
+        (lambda: mg.attention(q, kv, kv, causal=False, prefix=t(1, dtype=torch.int32)), "prefix"),
+        (lambda: mg.attention(q, kv, kv, out=t(1, 4, 8, 32)), "out"),
+        (lambda: mg.attention(q, kv, kv, out=t(1, 1, 8, 64).expand(1, 4, 8, 64)), "overlap"),
+        (lambda: mg.attention_backward(q, q, kv, kv, q, t(1, 4, 9)), "lse"),
+        (lambda: mg.attention_backward(t(1, 4, 9, 64), q, kv, kv, q, t(1, 4, 8)), "dout"),
+    ]
+    for call, fragment in bad:
+        with pytest.raises(mg.MacrogradError, match=fragment):
+            call()
