@@ -9,6 +9,7 @@
 #include "mg_attention.h"
 #include "mg_host.h"
 #include "mg_attention_simt.cuh"
+#include "mg_attention_tc.cuh"
 #include "mg_paged.cuh"
 #include "mg_rotary.cuh"
 
@@ -122,6 +123,92 @@ bool aligned(const void* ptr, const int64_t* strides, int n, size_t elem, int ve
     return true;
 }
 
+// ---------------------------------------------------------------- tensor cores
+// The tensor-core kernels read 16-bit tensors through TMA (rows on 16-byte
+// boundaries) and store 16-byte vectors; a scale of 0 would turn their masked
+// scores (-inf) into NaN. Everything else runs on the CUDA cores.
+bool tc_serves(const mg_attention_desc* d, const mg::AttnParams& p, std::initializer_list<const void*> rows_q,
+               std::initializer_list<const void*> rows_k)
+{
+    if (d->dtype != MG_BF16 || d->head_dim % 8 || d->scale == 0.f) return false;
+    if (!std::isfinite(1.f / d->scale)) return false;
+    for (const void* x : rows_q)
+        if (reinterpret_cast<uintptr_t>(x) % 16) return false;
+    for (const void* x : rows_k)
+        if (reinterpret_cast<uintptr_t>(x) % 16) return false;
+    for (int i = 0; i < 3; ++i)
+        for (int64_t s : {p.qs[i], p.ks[i], p.vs[i], p.os[i], p.dos[i], p.dqs[i], p.dks[i], p.dvs[i]})
+            if (s % 8 || s < 0 || s >= (1ll << 38)) return false;
+    const bool rows_repeat = (p.Lq > 1 && (p.qs[2] == 0 || (p.dout && p.dos[2] == 0))) ||
+                             (p.Lk > 1 && (p.ks[2] == 0 || p.vs[2] == 0));
+    return !rows_repeat;
+}
+
+// Map of [batch][heads][rows][D] for boxes of `box_rows` rows of 64 elements.
+mg_status tc_map(CUtensorMap* map, int* head_step, int* batch_step, const void* base, const int64_t* stride, int D,
+                 int rows, int heads, int batch, int box_rows)
+{
+    *head_step = stride[1] != 0;
+    *batch_step = stride[0] != 0;
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)rows, *head_step ? (uint64_t)heads : 1,
+                              *batch_step ? (uint64_t)batch : 1};
+    const uint64_t any = (uint64_t)(D + 7) / 8 * 16;      // of a dim of one element
+    uint64_t st[3];
+    for (int i = 0; i < 3; ++i) st[i] = stride[2 - i] ? (uint64_t)stride[2 - i] * 2 : any;
+    const uint32_t box[4] = {64, (uint32_t)box_rows, 1, 1};
+    return mg::host::encode_bf16(map, base, 4, dims, st, box);
+}
+
+mg_status tc_params(mg::TcAttnParams* t, const mg::AttnParams& p, const Device& dev, Scratch& ws, cudaStream_t st,
+                    const char* who)
+{
+    t->a = p;
+    t->scale = std::fabs(p.scale);
+    t->idesc_s = mg::idesc_bf16(128, 128, false, false, p.scale < 0.f);
+    t->status = dev.status;
+    if (p.docs) {
+        const int64_t tiles = (int64_t)p.B * ceil_div(p.Lk, 128);
+        int2* dt = static_cast<int2*>(ws.get(std::max<int64_t>(1, tiles) * sizeof(int2)));
+        if (!dt) return fail(MG_ERR_ALLOC, "%s: no scratch for the documents' tiles", who);
+        t->doc_tiles = dt;
+        if (tiles) {
+            mg::attn_doc_tiles_kernel<<<ceil_div(tiles, 4), 128, 0, st>>>(p.docs, dt, p.B, p.Lk);
+            MG_TRY(launched(who));
+        }
+    }
+    return MG_OK;
+}
+
+template <int DP, bool kCap, bool kBias>
+mg_status launch_tc_forward(const mg::TcAttnParams& t, cudaStream_t st)
+{
+    const auto kernel = mg::attn_tc_forward<DP, kCap, kBias>;
+    constexpr size_t smem = mg::tc_forward_smem<DP>();
+    MG_HOST_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kernel<<<ceil_div(t.a.Lq, 128) * t.a.B * t.a.H, mg::kTcFwdThreads, smem, st>>>(t);
+    return launched("mg_attention");
+}
+
+template <int DP>
+mg_status launch_tc_forward(const mg::TcAttnParams& t, cudaStream_t st)
+{
+    const bool cap = t.a.cap > 0.f, bias = t.a.slopes != nullptr;
+    return cap ? (bias ? launch_tc_forward<DP, true, true>(t, st) : launch_tc_forward<DP, true, false>(t, st))
+               : (bias ? launch_tc_forward<DP, false, true>(t, st) : launch_tc_forward<DP, false, false>(t, st));
+}
+
+mg_status forward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
+{
+    mg::TcAttnParams t = {};
+    Scratch ws(dev, stream);
+    cudaStream_t st = (cudaStream_t)stream;
+    MG_TRY(tc_params(&t, p, dev, ws, st, "mg_attention"));
+    MG_TRY(tc_map(&t.q, &t.head_step[0], &t.batch_step[0], p.q, p.qs, p.D, p.Lq, p.H, p.B, 128));
+    MG_TRY(tc_map(&t.k, &t.head_step[1], &t.batch_step[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 128));
+    MG_TRY(tc_map(&t.v, &t.head_step[2], &t.batch_step[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 128));
+    return p.D <= 64 ? launch_tc_forward<64>(t, st) : launch_tc_forward<128>(t, st);
+}
+
 // ---------------------------------------------------------------- paged
 // Splits: enough blocks to fill the GPU several times over, so that requests of
 // uneven lengths even out, but no chunk shorter than 128 keys.
@@ -207,6 +294,7 @@ mg_status mg_attention(const mg_attention_desc* d, void* out, float* lse, const 
         return d->dtype == MG_F32 ? launch_paged<float>(g, p.Lk, dev, ws, st, "mg_attention")
                                   : launch_paged<__nv_bfloat16>(g, p.Lk, dev, ws, st, "mg_attention");
     }
+    if (p.Lk > 0 && tc_serves(d, p, {q, out}, {k, v})) return forward_tc(p, dev, stream);
     return d->dtype == MG_F32 ? forward_simt<float>(p, st) : forward_simt<__nv_bfloat16>(p, st);
 }
 

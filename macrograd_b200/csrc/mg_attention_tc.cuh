@@ -1,0 +1,481 @@
+// mg_attention_tc.cuh -- attention of 16-bit tensors on the 5th-generation
+// tensor cores.
+//
+// Forward: one block per 128 queries of one head; two blocks share an SM. Per
+// tile of 128 keys
+//     S = Q K^T        (tcgen05, Q and K in shared memory, S in tensor memory)
+//     P = exp2(S - m)  (four warps; thread i owns query i: no shuffles)
+//     O += P V         (tcgen05, P from tensor memory, written over S)
+// with the running maximum m of each query in a register. O stays in tensor
+// memory; it is rescaled only when a row's maximum has grown by more than 2^8
+// since it was last used (P is then at most 2^8, exact in bf16's range, and the
+// division by the row sum at the end takes the factor out).
+//
+// Why this shape: the exponentials bound the kernel (16 a clock and SM: 1024
+// clocks a tile, as much as both products together at head_dim 128), so the
+// tensor core has to work on one tile while the exponentials of another are
+// taken. Two blocks an SM with one tile each do that without any hand-off
+// between them; each needs half of the tensor memory (128 columns S, 64 or 128
+// columns O) and one buffer for K and for V, refilled by TMA as soon as its
+// product is done.
+#pragma once
+
+#include "mg_attention_common.cuh"
+#include "mg_tc16.cuh"
+
+namespace mg {
+
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLn2 = 0.693147180559945309f;
+
+// ---------------------------------------------------------------- documents
+// Per 128 positions of a row: the smallest and the largest document id, ids
+// below 0 (padding) counted as -1. One warp each.
+__global__ void attn_doc_tiles_kernel(const int32_t* __restrict__ docs, int2* __restrict__ tiles, int B, int Lk)
+{
+    const int per = (Lk + 127) / 128;
+    const int64_t t = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    if (t >= (int64_t)B * per) return;
+    const int b = (int)(t / per), j0 = (int)(t % per) * 128, lane = threadIdx.x % 32;
+    int lo = INT_MAX, hi = -1;
+    for (int j = j0 + lane; j < min(Lk, j0 + 128); j += 32) {
+        const int d = max(-1, __ldg(docs + (int64_t)b * Lk + j));
+        lo = min(lo, d);
+        hi = max(hi, d);
+    }
+    lo = __reduce_min_sync(~0u, lo);
+    hi = __reduce_max_sync(~0u, hi);
+    if (lane == 0) tiles[t] = make_int2(lo, hi);
+}
+
+// ---------------------------------------------------------------- arithmetic
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// tanh(x) for |x| <= 1: x times a polynomial in x^2 (least maximum of the
+// relative error over [0, 1], fitted by reweighted least squares: 1.4e-7 with
+// its fp32 evaluation), two values at a time.
+__device__ __forceinline__ uint64_t tanh_small2(uint64_t x)
+{
+    const uint64_t u = mul2(x, x);
+    uint64_t r = pack2(0.001041021547280252f, 0.001041021547280252f);
+    r = fma2(r, u, pack2(-0.00620337575674057f, -0.00620337575674057f));
+    r = fma2(r, u, pack2(0.02028997614979744f, 0.02028997614979744f));
+    r = fma2(r, u, pack2(-0.05345702916383743f, -0.05345702916383743f));
+    r = fma2(r, u, pack2(0.13325203955173492f, 0.13325203955173492f));
+    r = fma2(r, u, pack2(-0.33332839608192444f, -0.33332839608192444f));
+    r = fma2(r, u, pack2(0.9999999403953552f, 0.9999999403953552f));
+    return mul2(r, x);
+}
+// tanh(x) for any x: 1 - 2 / (1 + exp(2x)); its error is absolute, some 2^-23.
+__device__ __forceinline__ float tanh_any(float x) { return fmaf(-2.f, rcp(1.f + ex2(x * (2.f * kLog2e))), 1.f); }
+
+// s[i] <- cap2 * tanh(s[i] * pre) for N values. The polynomial serves where no
+// value of the warp leaves [-1, 1] (scores well below the cap, the usual case:
+// 4 issue slots a value instead of 16 of the exponential unit).
+template <int N>
+__device__ __forceinline__ void cap_scores(float (&s)[N], float pre, float cap2)
+{
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(s[i]));
+    if (__any_sync(~0u, top * fabsf(pre) > 1.f)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = cap2 * tanh_any(s[i] * pre);
+    } else {
+        const uint64_t a = pack2(pre, pre), c = pack2(cap2, cap2);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) unpack2(mul2(c, tanh_small2(mul2(a, pack2(s[i], s[i + 1])))), s[i], s[i + 1]);
+    }
+}
+
+// ---------------------------------------------------------------- parameters
+struct TcAttnParams {
+    CUtensorMap q, k, v, dout;   // {D, rows, heads, batch}, boxes of 64 x 128 rows
+    AttnParams a;
+    const int2* doc_tiles;       // [B][ceil(Lk / 128)], with documents
+    int head_step[4], batch_step[4];   // of q, k, v, dout: 0 where the dim is broadcast (stride 0)
+    uint32_t idesc_s;            // of S = Q K^T: A negated where the scale is negative
+    float scale;                 // |scale|
+    int* status;
+};
+
+struct TcState {
+    uint64_t q_full, k_full, v_full, s_full, p_full, o_full, drain;
+    uint32_t tmem;
+    int failed;
+    int range[2];                // tiles of keys that some query of the block sees
+    int qdoc[2];                 // documents of its queries
+    int qpad;
+    int loads[2];                // tiles of K and of V that were asked for
+    alignas(16) int kdoc[4][128];    // documents of the keys, a copy a warp (read as int4)
+};
+
+__device__ __forceinline__ void tc_report(int* status, int where)
+{
+    if (atomicCAS(status, 0, 5 /* MG_ERR_TIMEOUT */) == 0) status[1] = where;
+}
+
+// One 128-row tile, DP columns: DP / 64 boxes.
+template <int DP>
+__device__ __forceinline__ void tc_load_tile(const CUtensorMap* map, uint32_t bar, uint32_t dst, int rows, int row,
+                                             int head, int batch)
+{
+    mbar_arrive_expect_tx(bar, (uint32_t)rows * DP * 2u);
+#pragma unroll
+    for (int c = 0; c < DP; c += 64)
+        tma_load(map, bar, dst + (uint32_t)(c / 64) * rows * 128u, 4, c, row, head, batch, 0);
+}
+
+// Zeroes the rows of padding (documents below 0, or no position at all) of a
+// tile that has landed: a product with weight 0 then adds 0 whatever they held. Whole warp.
+template <int DP>
+__device__ __forceinline__ void tc_clear_padding(uint32_t tile, int rows, const int32_t* docs, int pos0, int Lk, int lane)
+{
+    for (int r = lane; r < rows; r += 32) {
+        const int pos = pos0 + r;
+        if (pos >= 0 && pos < Lk && __ldg(docs + pos) >= 0) continue;
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + (uint32_t)c * rows * 128u +
+                                                                             (uint32_t)r * 128u + x * 16u),
+                             "r"(0)
+                             : "memory");
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
+constexpr int kTcFwdThreads = 192;
+
+template <int DP>
+constexpr size_t tc_forward_smem() { return 3 * 128 * DP * 2 + 1024; }
+
+template <int DP, bool kCap, bool kBias>
+__global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid_constant__ TcAttnParams tp)
+{
+    extern __shared__ uint8_t dyn[];
+    __shared__ TcState st;
+    const AttnParams& p = tp.a;
+    const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
+    const uint32_t sQ = base, sK = base + 128 * DP * 2, sV = sK + 128 * DP * 2;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    // blocks with the most keys first
+    const int heads = p.B * p.H, qtiles = (p.Lq + 127) / 128;
+    const int qt = qtiles - 1 - blockIdx.x / heads, bh = blockIdx.x % heads;
+    const int h = bh % p.H, b = bh / p.H, kv = h / (p.H / p.Hkv);
+    const int q0 = qt * 128, shift = p.Lk - p.Lq;
+    const int32_t* docs = p.docs ? p.docs + (int64_t)b * p.Lk : nullptr;
+    const int prefix = p.prefix ? __ldg(p.prefix + b) : 0;
+    const int qlast = min(q0 + 127, p.Lq - 1) + shift;
+
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&st.q_full), 1);
+        mbar_init(smem_u32(&st.k_full), 1);
+        mbar_init(smem_u32(&st.v_full), 1);
+        mbar_init(smem_u32(&st.s_full), 1);
+        mbar_init(smem_u32(&st.p_full), 4);
+        mbar_init(smem_u32(&st.o_full), 1);
+        mbar_init(smem_u32(&st.drain), 1);
+        mbar_fence_init();
+        st.failed = 0;
+        st.range[0] = INT_MAX;
+        st.range[1] = 0;
+        st.qdoc[0] = INT_MAX;
+        st.qdoc[1] = -1;
+        st.qpad = 0;
+        st.loads[0] = st.loads[1] = 0;
+    }
+    if (warp == 5) {
+        tmem_alloc(smem_u32(&st.tmem), 256);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // Tiles [t0, t1) hold every key that a query of this block sees.
+    const int kend = !p.causal ? p.Lk : max(0, min(p.Lk, max(qlast + 1, prefix)));
+    int t0 = 0, t1 = (kend + 127) / 128;
+    if (docs) {
+        for (int i = threadIdx.x; i < 128; i += kTcFwdThreads) {
+            if (q0 + i >= p.Lq) continue;
+            const int d = doc_at(p, b, q0 + i + shift);
+            if (d >= 0) {
+                atomicMin(&st.qdoc[0], d);
+                atomicMax(&st.qdoc[1], d);
+            } else {
+                st.qpad = 1;
+            }
+        }
+        __syncthreads();
+        for (int t = threadIdx.x; t < t1; t += kTcFwdThreads) {
+            const int2 r = __ldg(tp.doc_tiles + (int64_t)b * ((p.Lk + 127) / 128) + t);
+            if (r.x <= st.qdoc[1] && r.y >= st.qdoc[0]) {
+                atomicMin(&st.range[0], t);
+                atomicMax(&st.range[1], t + 1);
+            }
+        }
+        __syncthreads();
+        t0 = min(st.range[0], st.range[1]);
+        t1 = st.range[1];
+    }
+    const int n = max(0, t1 - t0);
+    const uint32_t tS = st.tmem, tO = st.tmem + 128;
+    volatile int* failed = &st.failed;
+
+    if (warp == 4) {
+        // ------------------------------------------------ loads
+        if (lane == 0 && n > 0) {
+            const int hk = kv * tp.head_step[1], bk = b * tp.batch_step[1];
+            const int hv = kv * tp.head_step[2], bv = b * tp.batch_step[2];
+            tc_load_tile<DP>(&tp.q, smem_u32(&st.q_full), sQ, 128, q0, h * tp.head_step[0], b * tp.batch_step[0]);
+            for (int j = 0; j < n; ++j) {
+                if (j > 0 && !tc_wait(smem_u32(&st.s_full), (j - 1) & 1, failed)) break;
+                tc_load_tile<DP>(&tp.k, smem_u32(&st.k_full), sK, 128, (t0 + j) * 128, hk, bk);
+                st.loads[0] = j + 1;
+                if (j > 0 && !tc_wait(smem_u32(&st.o_full), (j - 1) & 1, failed)) break;
+                tc_load_tile<DP>(&tp.v, smem_u32(&st.v_full), sV, 128, (t0 + j) * 128, hv, bv);
+                st.loads[1] = j + 1;
+            }
+        }
+    } else if (warp == 5) {
+        // ------------------------------------------------ products
+        constexpr uint32_t idesc_o = idesc_bf16(128, DP, false, true);
+        bool ok = n == 0 || tc_wait(smem_u32(&st.q_full), 0, failed);
+        for (int j = 0; j <= n && n > 0; ++j) {
+            if (j > 0) {      // O += P(j-1) V(j-1)
+                ok = ok && tc_wait(smem_u32(&st.v_full), (j - 1) & 1, failed);
+                ok = __all_sync(~0u, ok);
+                if (!ok) break;
+                if (docs && __ldg(&tp.doc_tiles[(int64_t)b * ((p.Lk + 127) / 128) + t0 + j - 1]).x < 0)
+                    tc_clear_padding<DP>(sV, 128, docs, (t0 + j - 1) * 128, p.Lk, lane);
+                ok = __all_sync(~0u, tc_wait(smem_u32(&st.p_full), (j - 1) & 1, failed));
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        tc_mma_f16_ta(tO, tS + 8 * k, desc_mn_major(sV, 128, k), idesc_o, j > 1 || k > 0);
+                    tc_commit(smem_u32(&st.o_full));
+                }
+                __syncwarp();
+            }
+            if (j < n) {      // S = Q K(j)^T
+                ok = __all_sync(~0u, ok && tc_wait(smem_u32(&st.k_full), j & 1, failed));
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k)
+                        tc_mma_f16(tS, desc_k_major(sQ, 128, k), desc_k_major(sK, 128, k), tp.idesc_s, k > 0);
+                    tc_commit(smem_u32(&st.s_full));
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) {
+            if (lane == 0) {
+                tc_report(tp.status, 201);
+                tc_commit(smem_u32(&st.drain));
+                tc_drain(smem_u32(&st.drain), 0);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ------------------------------------------------ softmax
+        const int row = q0 + threadIdx.x, qpos = row + shift;
+        const uint32_t lanes = (uint32_t)warp << 21;      // this warp's 32 lanes of tensor memory
+        const int qdoc = docs ? doc_at(p, b, qpos) : 0;
+        const bool one_doc = !docs || (st.qdoc[0] == st.qdoc[1] && !st.qpad && q0 + 127 < p.Lq);
+        // keys before `upto` are seen as far as causal and prefix go
+        const int upto = qdoc < 0 ? 0 : !p.causal ? p.Lk : min(p.Lk, max(qpos + 1, prefix));
+        // scores are kept in units whose multiple by `mul` is the power of two
+        const float mul = kCap ? 1.f : tp.scale * kLog2e;
+        const float slope = kBias ? __ldg(p.slopes + h) * (kCap ? kLog2e : 1.f / tp.scale) : 0.f;
+        float m = -CUDART_INF_F;     // maximum in use, in units of the raw values; base2 = m * mul
+        uint64_t sum2 = pack2(0.f, 0.f);
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            const int k0 = (t0 + j) * 128;
+            // whether any of the tile's pairs is masked (same for all threads)
+            bool full = k0 + 128 <= p.Lk && (!p.causal || k0 + 127 <= q0 + shift || k0 + 128 <= prefix);
+            if (docs) {
+                const int2 r = __ldg(tp.doc_tiles + (int64_t)b * ((p.Lk + 127) / 128) + t0 + j);
+                full = full && one_doc && r.x == r.y && r.x == st.qdoc[0];
+                if (!full) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 128; i += 32) st.kdoc[warp][i + lane] = doc_at(p, b, k0 + i + lane);
+                    __syncwarp();
+                }
+            }
+            ok = __all_sync(~0u, tc_wait(smem_u32(&st.s_full), j & 1, failed));
+            if (!ok) break;
+            tc_fence_after();
+            float s[128];
+            tmem_ld_x128(tS + lanes, s);
+            if (kCap) cap_scores(s, tp.scale / p.cap, p.cap * kLog2e);
+            if (kBias) {
+                const float far = (float)(qpos - k0);
+#pragma unroll
+                for (int c = 0; c < 128; ++c) s[c] = fmaf(-slope, fabsf(far - (float)c), s[c]);
+            }
+            if (!full) {
+                const int lim = upto - k0;
+                if (docs) {
+                    const int4* kd = reinterpret_cast<const int4*>(st.kdoc[warp]);
+#pragma unroll
+                    for (int c = 0; c < 128; c += 4) {
+                        const int4 d = kd[c / 4];
+                        s[c] = c < lim && d.x == qdoc ? s[c] : -CUDART_INF_F;
+                        s[c + 1] = c + 1 < lim && d.y == qdoc ? s[c + 1] : -CUDART_INF_F;
+                        s[c + 2] = c + 2 < lim && d.z == qdoc ? s[c + 2] : -CUDART_INF_F;
+                        s[c + 3] = c + 3 < lim && d.w == qdoc ? s[c + 3] : -CUDART_INF_F;
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 128; ++c) s[c] = c < lim ? s[c] : -CUDART_INF_F;
+                }
+            }
+            float top = fmaxf(s[0], s[1]);
+#pragma unroll
+            for (int c = 2; c < 128; c += 2) top = fmaxf(top, fmaxf(s[c], s[c + 1]));
+            // rescale O and the sum where the maximum has outgrown the one in use
+            const bool grown = m == -CUDART_INF_F ? top > m : (top - m) * mul > 8.f;
+            if (j > 0) {
+                ok = __all_sync(~0u, tc_wait(smem_u32(&st.o_full), (j - 1) & 1, failed));
+                if (!ok) break;
+            }
+            if (__any_sync(~0u, grown)) {
+                const float mn = grown ? top : m;
+                if (j > 0) {
+                    tc_fence_after();
+                    const float f = m == -CUDART_INF_F ? 0.f : ex2((m - mn) * mul);
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 32) {
+                        float o[32];
+                        uint32_t w[32];
+                        tmem_ld_x32(tO + lanes + c, o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * f);
+                        tmem_st_x32(tO + lanes + c, w);
+                    }
+                    sum2 = mul2(sum2, pack2(f, f));
+                }
+                m = mn;
+            }
+            const float base2 = m == -CUDART_INF_F ? 0.f : m * mul;
+            const uint64_t mul_2 = pack2(mul, mul), base_2 = pack2(-base2, -base2);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t w[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    float x, y;
+                    unpack2(fma2(pack2(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]), mul_2, base_2), x, y);
+                    x = ex2(x);
+                    y = ex2(y);
+                    sum2 = add2(sum2, pack2(x, y));
+                    w[i] = bf16x2(x, y);
+                }
+                tmem_st_x32(tS + lanes + 32 * half, w);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&st.p_full));
+        }
+        if (ok && n > 0) ok = __all_sync(~0u, tc_wait(smem_u32(&st.o_full), (n - 1) & 1, failed));
+        if (ok) {
+            tc_fence_after();
+            float la, lb;
+            unpack2(sum2, la, lb);
+            const float l = la + lb, inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+            const bool store = row < p.Lq;
+            __nv_bfloat16* out = (__nv_bfloat16*)p.out + b * p.os[0] + h * p.os[1] + (int64_t)row * p.os[2];
+#pragma unroll 1
+            for (int c = 0; c < p.D; c += 32) {
+                float o[32];
+                if (n > 0) {
+                    tmem_ld_x32(tO + lanes + c, o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0.f;
+                }
+                if (!store) continue;
+                const int left = p.D - c;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    const uint4 w = make_uint4(bf16x2(o[i] * inv, o[i + 1] * inv), bf16x2(o[i + 2] * inv, o[i + 3] * inv),
+                                               bf16x2(o[i + 4] * inv, o[i + 5] * inv),
+                                               bf16x2(o[i + 6] * inv, o[i + 7] * inv));
+                    if (i + 8 <= left) *reinterpret_cast<uint4*>(out + c + i) = w;
+                }
+            }
+            if (store)
+                p.lse[((int64_t)b * p.H + h) * p.Lq + row] =
+                    l == 0.f ? -CUDART_INF_F : ((m == -CUDART_INF_F ? 0.f : m * mul) + log2f(l)) * kLn2;
+        }
+        if (!ok && lane == 0) tc_report(tp.status, 202);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (st.failed && threadIdx.x == 0 && n > 0) {     // copies that nobody waited for
+        tc_drain(smem_u32(&st.q_full), 0);
+        if (st.loads[0]) tc_drain(smem_u32(&st.k_full), (st.loads[0] - 1) & 1);
+        if (st.loads[1]) tc_drain(smem_u32(&st.v_full), (st.loads[1] - 1) & 1);
+    }
+    if (warp == 5) tmem_dealloc(st.tmem, 256);
+}
+
+}  // namespace mg
