@@ -10,6 +10,7 @@
 #include "mg_host.h"
 #include "mg_attention_simt.cuh"
 #include "mg_attention_tc.cuh"
+#include "mg_attention_tc_bwd.cuh"
 #include "mg_paged.cuh"
 #include "mg_rotary.cuh"
 
@@ -209,6 +210,60 @@ mg_status forward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     return p.D <= 64 ? launch_tc_forward<64>(t, st) : launch_tc_forward<128>(t, st);
 }
 
+template <int DP, bool kKeys, bool kCap, bool kBias>
+mg_status launch_tc_backward(const mg::TcBwdParams& t, cudaStream_t st)
+{
+    const auto kernel = mg::attn_tc_backward<DP, kKeys, kCap, kBias>;
+    constexpr size_t smem = mg::tc_backward_smem<DP>();
+    MG_HOST_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int blocks = kKeys ? ceil_div(t.a.Lk, 128) * t.a.B * t.a.Hkv : ceil_div(t.a.Lq, 128) * t.a.B * t.a.H;
+    kernel<<<blocks, mg::kTcBwdThreads, smem, st>>>(t);
+    return launched("mg_attention_backward");
+}
+
+template <int DP, bool kKeys>
+mg_status launch_tc_backward(const mg::TcBwdParams& t, cudaStream_t st)
+{
+    const bool cap = t.a.cap > 0.f, bias = t.a.slopes != nullptr;
+    return cap ? (bias ? launch_tc_backward<DP, kKeys, true, true>(t, st)
+                       : launch_tc_backward<DP, kKeys, true, false>(t, st))
+               : (bias ? launch_tc_backward<DP, kKeys, false, true>(t, st)
+                       : launch_tc_backward<DP, kKeys, false, false>(t, st));
+}
+
+mg_status backward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
+{
+    const char* who = "mg_attention_backward";
+    mg::TcAttnParams f = {};
+    mg::TcBwdParams t = {};
+    Scratch ws(dev, stream);
+    cudaStream_t st = (cudaStream_t)stream;
+    MG_TRY(tc_params(&f, p, dev, ws, st, who));
+    t.a = p, t.doc_tiles = f.doc_tiles, t.scale = f.scale, t.status = f.status;
+    t.idesc_s = mg::idesc_bf16(128, 64, false, false, p.scale < 0.f);
+    t.Lp = ceil_div(p.Lq, 128) * 128;
+    const int64_t rows = (int64_t)p.B * p.H * t.Lp;
+    float* stats = static_cast<float*>(ws.get(2 * rows * sizeof(float)));
+    if (!stats) return fail(MG_ERR_ALLOC, "%s: no scratch for the row sums", who);
+    t.lse2 = stats, t.delta = stats + rows;
+    mg::attn_tc_stats_kernel<<<ceil_div(rows, 16), 256, 0, st>>>(p, t.Lp, stats, stats + rows);
+    MG_TRY(launched(who));
+    int* hs = t.head_step;
+    int* bs = t.batch_step;
+    // the keys resident: dK, dV
+    MG_TRY(tc_map(&t.x0, &hs[1], &bs[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 128));
+    MG_TRY(tc_map(&t.x1, &hs[2], &bs[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 128));
+    MG_TRY(tc_map(&t.y0, &hs[0], &bs[0], p.q, p.qs, p.D, p.Lq, p.H, p.B, 64));
+    MG_TRY(tc_map(&t.y1, &hs[3], &bs[3], p.dout, p.dos, p.D, p.Lq, p.H, p.B, 64));
+    MG_TRY((p.D <= 64 ? launch_tc_backward<64, true>(t, st) : launch_tc_backward<128, true>(t, st)));
+    // the queries resident: dQ
+    MG_TRY(tc_map(&t.x0, &hs[0], &bs[0], p.q, p.qs, p.D, p.Lq, p.H, p.B, 128));
+    MG_TRY(tc_map(&t.x1, &hs[3], &bs[3], p.dout, p.dos, p.D, p.Lq, p.H, p.B, 128));
+    MG_TRY(tc_map(&t.y0, &hs[1], &bs[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 64));
+    MG_TRY(tc_map(&t.y1, &hs[2], &bs[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 64));
+    return p.D <= 64 ? launch_tc_backward<64, false>(t, st) : launch_tc_backward<128, false>(t, st);
+}
+
 // ---------------------------------------------------------------- paged
 // Splits: enough blocks to fill the GPU several times over, so that requests of
 // uneven lengths even out, but no chunk shorter than 128 keys.
@@ -312,6 +367,8 @@ mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, 
     mg::AttnParams p = attention_params(d);
     p.q = q, p.k = k, p.v = v, p.out = const_cast<void*>(out), p.dout = dout, p.lse = const_cast<float*>(lse);
     p.dq = dq, p.dk = dk, p.dv = dv;
+    if (d->q_len > 0 && d->k_len > 0 && tc_serves(d, p, {q, out, dout, dq}, {k, v, dk, dv}))
+        return backward_tc(p, dev, stream);
     Scratch ws(dev, stream);
     if (d->q_len > 0) {
         p.delta = static_cast<float*>(ws.get(sizeof(float) * d->batch * d->heads * (size_t)d->q_len));

@@ -1,0 +1,442 @@
+// mg_attention_tc_bwd.cuh -- gradients of attention of 16-bit tensors on the
+// 5th-generation tensor cores.
+//
+// One kernel in two forms. A block keeps 128 rows of two tensors X0, X1 in shared
+// memory and streams tiles of 64 rows of two others, Y0, Y1:
+//     S = X0 Y0^T,  dP = X1 Y1^T            (tensor memory, fp32)
+//     P = exp2(S - lse),  dS = P * (dP - delta) * curve
+//     acc += dS Y0   (and acc' += P Y1)     (P, dS from tensor memory, bf16)
+// With the queries resident (X = q, dout; Y = k, v) acc is dQ. With the keys
+// resident (X = k, v; Y = q, dout) S and dP are transposed, acc is dK and acc' is
+// dV, summed over the query heads that share the key-value head. So no gradient
+// is added to by two blocks: no atomics, and the same bits every time, for 7
+// products instead of the 5 of a single kernel that would add dQ up atomically.
+// P and dS go back to tensor memory over S and dP, as the A operand of the
+// second pair of products: they never pass through shared memory.
+//
+// Two warpgroups take the tiles in turn, each with S and dP columns of its own,
+// so that while one works on the exponentials of tile i the tensor core runs S,
+// dP of tile i + 1 and the accumulations of tile i - 1. Tensor memory at head_dim
+// 128: 2 x (64 + 64) + 128 + 128 = all 512 columns, hence one block an SM.
+#pragma once
+
+#include "mg_attention_tc.cuh"
+
+namespace mg {
+
+constexpr int kTcBwdThreads = 320;       // two warpgroups, loads, products
+constexpr int kTcBwdStages = 4;
+
+struct TcBwdParams {
+    CUtensorMap x0, x1, y0, y1;          // boxes of 64 x 128 rows (x), 64 x 64 rows (y)
+    AttnParams a;
+    const int2* doc_tiles;
+    const float* lse2;                   // [B * H][Lp] lse * log2(e); +inf where no key is seen
+    const float* delta;                  // [B * H][Lp]
+    int Lp;                              // q_len rounded up to 128
+    int head_step[4], batch_step[4];     // of q, k, v, dout
+    uint32_t idesc_s;
+    float scale;                         // |scale|
+    int* status;
+};
+
+// lse2 and delta of each row, padded with rows whose P is 0. 16 lanes to a row of
+// up to 128 elements, 8 each.
+__global__ void attn_tc_stats_kernel(const __grid_constant__ AttnParams p, int Lp, float* __restrict__ lse2,
+                                     float* __restrict__ delta)
+{
+    const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 16;
+    if (row >= (int64_t)p.B * p.H * Lp) return;      // whole 16-lane groups, and Lp is even: whole warps
+    const int part = threadIdx.x % 16, i = (int)(row % Lp);
+    const int64_t bh = row / Lp;
+    const int h = (int)(bh % p.H), b = (int)(bh / p.H);
+    float s = 0.f, l = CUDART_INF_F;
+    if (i < p.Lq) {
+        const float lse = p.lse[bh * p.Lq + i];
+        if (lse != -CUDART_INF_F) {
+            l = lse * kLog2e;
+            if (part * 8 < p.D) {
+                const uint4 o = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.out + b * p.os[0] + h * p.os[1] +
+                                                                (int64_t)i * p.os[2] + part * 8);
+                const uint4 g = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.dout + b * p.dos[0] +
+                                                                h * p.dos[1] + (int64_t)i * p.dos[2] + part * 8);
+                const __nv_bfloat162* ov = reinterpret_cast<const __nv_bfloat162*>(&o);
+                const __nv_bfloat162* gv = reinterpret_cast<const __nv_bfloat162*>(&g);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 x = __bfloat1622float2(ov[k]), y = __bfloat1622float2(gv[k]);
+                    s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 8; o; o /= 2) s += __shfl_xor_sync(~0u, s, o);
+    if (part == 0) {
+        lse2[row] = l;
+        delta[row] = s;
+    }
+}
+
+struct TcBwdState {
+    uint64_t x_full, y_full[kTcBwdStages], y_empty[kTcBwdStages], s_full[2], p_full[2], acc_full, drain;
+    uint32_t tmem;
+    int failed;
+    int range[2];
+    int loads;                           // stages that were asked for
+    alignas(16) int doc[8][64];          // documents of the streamed rows, a copy a warp
+    alignas(16) float lse2[kTcBwdStages][64];
+    alignas(16) float delta[kTcBwdStages][64];
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t bar, uint32_t dst, const void* src, uint32_t bytes)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+// The one document that positions [pos, pos + n) have in common by the tiles of
+// 128, or -1 (some padding, several documents, positions outside the row).
+__device__ __forceinline__ int common_doc(const int2* tiles, int pos, int n, int Lk)
+{
+    if (pos < 0 || pos + n > Lk) return -1;
+    const int2 a = __ldg(tiles + (pos >> 7)), b = __ldg(tiles + ((pos + n - 1) >> 7));
+    return a.x == a.y && b.x == b.y && a.x == b.x ? a.x : -1;
+}
+
+// Whether a document of positions [pos, pos + n) can be one of `want`'s range.
+__device__ __forceinline__ bool docs_meet(const int2* tiles, int pos, int n, int Lk, int2 want)
+{
+    const int p0 = max(pos, 0), p1 = min(pos + n, Lk);
+    for (int t = p0 >> 7; t * 128 < p1; ++t) {
+        const int2 r = __ldg(tiles + t);
+        if (r.y >= 0 && want.y >= 0 && max(r.x, 0) <= want.y && r.y >= max(want.x, 0)) return true;
+    }
+    return false;
+}
+
+template <int DP>
+constexpr size_t tc_backward_smem() { return (2 * 128 + kTcBwdStages * 2 * 64) * DP * 2 + 1024; }
+
+template <int DP, bool kKeys, bool kCap, bool kBias>
+__global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __grid_constant__ TcBwdParams tp)
+{
+    extern __shared__ uint8_t dyn[];
+    __shared__ TcBwdState st;
+    const AttnParams& p = tp.a;
+    constexpr uint32_t kX = 128 * DP * 2, kY = 64 * DP * 2;
+    const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
+    const uint32_t sX0 = base, sX1 = base + kX, sY = base + 2 * kX;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    // blocks with the most tiles first: the first keys, the last queries
+    const int nhead = kKeys ? p.Hkv : p.H, xrows = kKeys ? p.Lk : p.Lq, yrows = kKeys ? p.Lq : p.Lk;
+    const int xtiles = (xrows + 127) / 128, bh = blockIdx.x % (p.B * nhead), rank = blockIdx.x / (p.B * nhead);
+    const int x0 = (kKeys ? rank : xtiles - 1 - rank) * 128;
+    const int xh = bh % nhead, b = bh / nhead, group = p.H / p.Hkv;
+    const int shift = p.Lk - p.Lq;
+    const int32_t* docs = p.docs ? p.docs + (int64_t)b * p.Lk : nullptr;
+    const int2* dt = p.docs ? tp.doc_tiles + (int64_t)b * ((p.Lk + 127) / 128) : nullptr;
+    const int prefix = p.prefix ? __ldg(p.prefix + b) : 0;
+    const int xpos = kKeys ? x0 : x0 + shift;            // position of the first resident row
+
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&st.x_full), 1);
+        for (int i = 0; i < kTcBwdStages; ++i) {
+            mbar_init(smem_u32(&st.y_full[i]), 1);
+            mbar_init(smem_u32(&st.y_empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&st.s_full[i]), 1);
+            mbar_init(smem_u32(&st.p_full[i]), 4);
+        }
+        mbar_init(smem_u32(&st.acc_full), 1);
+        mbar_init(smem_u32(&st.drain), 1);
+        mbar_fence_init();
+        st.failed = 0;
+        st.loads = 0;
+        st.range[0] = INT_MAX;
+        st.range[1] = 0;
+    }
+    if (warp == 9) {
+        tmem_alloc(smem_u32(&st.tmem), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // Tiles [t0, t1) of 64 streamed rows that meet the resident rows in some pair.
+    int t0 = 0, t1;
+    if (kKeys) {
+        if (p.causal && x0 >= prefix) t0 = min(max(0, x0 - shift), p.Lq) / 64;
+        t1 = (p.Lq + 63) / 64;
+    } else {
+        const int last = min(x0 + 127, p.Lq - 1) + shift;
+        t1 = ((!p.causal ? p.Lk : max(0, min(p.Lk, max(last + 1, prefix)))) + 63) / 64;
+    }
+    if (docs) {
+        int2 mine = make_int2(INT_MAX, -1);
+        for (int t = max(xpos, 0) >> 7; t * 128 < min(xpos + 128, p.Lk); ++t) {
+            const int2 r = __ldg(dt + t);
+            if (r.y >= 0) mine = make_int2(min(mine.x, max(r.x, 0)), max(mine.y, r.y));
+        }
+        for (int t = t0 + threadIdx.x; t < t1; t += kTcBwdThreads) {
+            if (!docs_meet(dt, t * 64 + (kKeys ? shift : 0), 64, p.Lk, mine)) continue;
+            atomicMin(&st.range[0], t);
+            atomicMax(&st.range[1], t + 1);
+        }
+        __syncthreads();
+        t0 = min(st.range[0], st.range[1]);
+        t1 = st.range[1];
+    }
+    const int tiles = max(0, t1 - t0), n = kKeys ? tiles * group : tiles;
+    const uint32_t tA = st.tmem + 256, tB = tA + DP;     // accumulators: dS Y0, P Y1
+    volatile int* failed = &st.failed;
+    // columns of step i's S (and P) and dP (and dS)
+    const auto tS = [&](int i) { return st.tmem + 128 * (i & 1); };
+    const auto sY0 = [&](int i) { return sY + (uint32_t)(i % kTcBwdStages) * 2 * kY; };
+
+    if (warp == 8) {
+        // ------------------------------------------------ loads
+        if (lane == 0 && n > 0) {
+            constexpr int X0 = kKeys ? 1 : 0, X1 = kKeys ? 2 : 3, Y0 = kKeys ? 0 : 1, Y1 = kKeys ? 3 : 2;
+            const uint32_t xb = smem_u32(&st.x_full);
+            mbar_arrive_expect_tx(xb, 2 * kX);
+            for (int c = 0; c < DP; c += 64) {
+                tma_load(&tp.x0, xb, sX0 + c / 64 * 128 * 128, 4, c, x0, xh * tp.head_step[X0], b * tp.batch_step[X0], 0);
+                tma_load(&tp.x1, xb, sX1 + c / 64 * 128 * 128, 4, c, x0, xh * tp.head_step[X1], b * tp.batch_step[X1], 0);
+            }
+            for (int i = 0; i < n; ++i) {
+                const int s = i % kTcBwdStages;
+                if (i >= kTcBwdStages && !tc_wait(smem_u32(&st.y_empty[s]), (i / kTcBwdStages - 1) & 1, failed)) break;
+                const int yh = kKeys ? xh * group + i / tiles : xh / group, y0 = (t0 + (kKeys ? i % tiles : i)) * 64;
+                const uint32_t yb = smem_u32(&st.y_full[s]);
+                mbar_arrive_expect_tx(yb, 2 * kY + (kKeys ? 512u : 0u));
+                for (int c = 0; c < DP; c += 64) {
+                    tma_load(&tp.y0, yb, sY0(i) + c / 64 * 64 * 128, 4, c, y0, yh * tp.head_step[Y0],
+                             b * tp.batch_step[Y0], 0);
+                    tma_load(&tp.y1, yb, sY0(i) + kY + c / 64 * 64 * 128, 4, c, y0, yh * tp.head_step[Y1],
+                             b * tp.batch_step[Y1], 0);
+                }
+                if (kKeys) {
+                    const int64_t at = ((int64_t)b * p.H + yh) * tp.Lp + y0;
+                    bulk_load(yb, smem_u32(st.lse2[s]), tp.lse2 + at, 256);
+                    bulk_load(yb, smem_u32(st.delta[s]), tp.delta + at, 256);
+                }
+                st.loads = i + 1;
+            }
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------ products
+        constexpr uint32_t idesc_dp = idesc_bf16(128, 64, false, false), idesc_acc = idesc_bf16(128, DP, false, true);
+        bool ok = n == 0 || __all_sync(~0u, tc_wait(smem_u32(&st.x_full), 0, failed));
+        for (int i = 0; i <= n && n > 0 && ok; ++i) {
+            if (i < n) {
+                const int s = i % kTcBwdStages;
+                ok = __all_sync(~0u, tc_wait(smem_u32(&st.y_full[s]), (i / kTcBwdStages) & 1, failed));
+                if (!ok) break;
+                if (docs) {
+                    const int y0 = (t0 + (kKeys ? i % tiles : i)) * 64, pos = y0 + (kKeys ? shift : 0);
+                    bool pad = pos < 0 || pos + 64 > p.Lk;
+                    if (!pad) pad = __ldg(dt + (pos >> 7)).x < 0 || __ldg(dt + ((pos + 63) >> 7)).x < 0;
+                    if (pad) {
+                        tc_clear_padding<DP>(sY0(i), 64, docs, pos, p.Lk, lane);
+                        tc_clear_padding<DP>(sY0(i) + kY, 64, docs, pos, p.Lk, lane);
+                    }
+                }
+                tc_fence_after();
+                if (lane == 0) {
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k)
+                        tc_mma_f16(tS(i), desc_k_major(sX0, 128, k), desc_k_major(sY0(i), 64, k), tp.idesc_s, k > 0);
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k)
+                        tc_mma_f16(tS(i) + 64, desc_k_major(sX1, 128, k), desc_k_major(sY0(i) + kY, 64, k), idesc_dp,
+                                   k > 0);
+                    tc_commit(smem_u32(&st.s_full[i & 1]));
+                }
+                __syncwarp();
+            }
+            if (i > 0) {
+                const int j = i - 1;
+                ok = __all_sync(~0u, tc_wait(smem_u32(&st.p_full[j & 1]), (j >> 1) & 1, failed));
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    if (kKeys) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            tc_mma_f16_ta(tB, tS(j) + 8 * k, desc_mn_major(sY0(j) + kY, 64, k), idesc_acc,
+                                          j > 0 || k > 0);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tc_mma_f16_ta(tA, tS(j) + 64 + 8 * k, desc_mn_major(sY0(j), 64, k), idesc_acc, j > 0 || k > 0);
+                    tc_commit(smem_u32(&st.y_empty[j % kTcBwdStages]));
+                    if (i == n) tc_commit(smem_u32(&st.acc_full));
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) {
+            if (lane == 0) {
+                tc_report(tp.status, 211);
+                tc_commit(smem_u32(&st.drain));
+                tc_drain(smem_u32(&st.drain), 0);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ------------------------------------------------ P and dS
+        const int wg = warp / 4, r = threadIdx.x % 128;          // this thread's resident row
+        const uint32_t lanes = (uint32_t)(warp % 4) << 21;
+        const int pos = xpos + r;
+        const int rdoc = docs ? (x0 + r < xrows ? doc_at(p, b, pos) : -1) : 0;
+        const int common = docs ? (x0 + 128 <= xrows ? common_doc(dt, xpos, 128, p.Lk) : -1) : 0;
+        const float mul = kCap ? p.cap * kLog2e : tp.scale * kLog2e;
+        float lse2 = 0.f, delta = 0.f;
+        if (!kKeys) {
+            const int64_t at = ((int64_t)b * p.H + xh) * tp.Lp + x0 + r;
+            lse2 = tp.lse2[at];
+            delta = tp.delta[at];
+        }
+        bool ok = true;
+        for (int i = wg; i < n; i += 2) {
+            const int h = kKeys ? xh * group + i / tiles : xh;
+            const int y0 = (t0 + (kKeys ? i % tiles : i)) * 64, ypos = y0 + (kKeys ? shift : 0);
+            const int s = i % kTcBwdStages;
+            const float slope = kBias ? __ldg(p.slopes + h) * kLog2e : 0.f;
+            // this row's streamed rows [lo, hi) as far as causal, prefix and the ends go
+            int lo = 0, hi = 64;
+            bool full;
+            if (kKeys) {
+                if (p.causal && pos >= prefix) lo = max(0, pos - ypos);
+                full = !p.causal || ypos >= xpos + 127 || xpos + 128 <= prefix;
+            } else {
+                hi = (!p.causal ? p.Lk : min(p.Lk, max(pos + 1, prefix))) - ypos;
+                full = ypos + 64 <= p.Lk && (!p.causal || ypos + 63 <= xpos || ypos + 64 <= prefix);
+            }
+            if (docs) {
+                if (rdoc < 0) hi = 0;
+                full = full && common >= 0 && (!kKeys || y0 + 64 <= p.Lq) && common_doc(dt, ypos, 64, p.Lk) == common;
+                if (!full) {
+                    __syncwarp();
+                    st.doc[warp][lane] = doc_at(p, b, ypos + lane);
+                    st.doc[warp][lane + 32] = doc_at(p, b, ypos + lane + 32);
+                    __syncwarp();
+                }
+            }
+            ok = __all_sync(~0u, tc_wait(smem_u32(&st.s_full[wg]), (i >> 1) & 1, failed) &&
+                                     (!kKeys || tc_wait(smem_u32(&st.y_full[s]), (i / kTcBwdStages) & 1, failed)));
+            if (!ok) break;
+            tc_fence_after();
+            float v[64];
+            tmem_ld_x64(tS(i) + lanes, v);
+            if (kCap) cap_scores(v, tp.scale / p.cap, 1.f);      // tanh of the score over the cap
+            uint32_t w[32];
+            const float far = (float)(pos - ypos);
+#pragma unroll
+            for (int c = 0; c < 64; c += 4) {
+                float4 l4;
+                if (kKeys) l4 = *reinterpret_cast<const float4*>(&st.lse2[s][c]);
+                const float ls[4] = {kKeys ? l4.x : lse2, kKeys ? l4.y : lse2, kKeys ? l4.z : lse2, kKeys ? l4.w : lse2};
+                float e[4];
+#pragma unroll
+                for (int k = 0; k < 4; k += 2) {
+                    float nl0 = -ls[k], nl1 = -ls[k + 1];
+                    if (kBias) {
+                        nl0 = fmaf(-slope, fabsf(far - (float)(c + k)), nl0);
+                        nl1 = fmaf(-slope, fabsf(far - (float)(c + k + 1)), nl1);
+                    }
+                    unpack2(fma2(pack2(v[c + k], v[c + k + 1]), pack2(mul, mul), pack2(nl0, nl1)), e[k], e[k + 1]);
+                    e[k] = ex2(e[k]);
+                    e[k + 1] = ex2(e[k + 1]);
+                }
+                if (!full) {
+                    const int4 d4 = docs ? *reinterpret_cast<const int4*>(&st.doc[warp][c]) : make_int4(0, 0, 0, 0);
+                    const int ds[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const bool seen = c + k >= lo && c + k < hi && ds[k] == rdoc;
+                        e[k] = seen ? e[k] : 0.f;
+                        if (kCap) v[c + k] = seen ? v[c + k] : 0.f;
+                    }
+                }
+                if (kKeys) {
+                    w[c / 2] = bf16x2(e[0], e[1]);
+                    w[c / 2 + 1] = bf16x2(e[2], e[3]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[c + k] = kCap ? e[k] * fmaf(-v[c + k], v[c + k], 1.f) : e[k];
+            }
+            if (kKeys) tmem_st_x32(tS(i) + lanes, w);
+            float g[64];
+            tmem_ld_x64(tS(i) + 64 + lanes, g);
+#pragma unroll
+            for (int c = 0; c < 64; c += 4) {
+                float4 d4;
+                if (kKeys) d4 = *reinterpret_cast<const float4*>(&st.delta[s][c]);
+                const float ds[4] = {kKeys ? d4.x : delta, kKeys ? d4.y : delta, kKeys ? d4.z : delta,
+                                     kKeys ? d4.w : delta};
+                float e[4];
+#pragma unroll
+                for (int k = 0; k < 4; k += 2)
+                    unpack2(mul2(pack2(v[c + k], v[c + k + 1]),
+                                 add2(pack2(g[c + k], g[c + k + 1]), pack2(-ds[k], -ds[k + 1]))),
+                            e[k], e[k + 1]);
+                if (!full) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) e[k] = v[c + k] == 0.f ? 0.f : e[k];
+                }
+                w[c / 2] = bf16x2(e[0], e[1]);
+                w[c / 2 + 1] = bf16x2(e[2], e[3]);
+            }
+            tmem_st_x32(tS(i) + 64 + lanes, w);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&st.p_full[wg]));
+        }
+        if (ok && n > 0) ok = __all_sync(~0u, tc_wait(smem_u32(&st.acc_full), 0, failed));
+        if (ok) {
+            tc_fence_after();
+            // with the keys: one warpgroup stores dK, the other dV; with the queries: half of dQ each
+            const bool is_dv = kKeys && wg == 1;
+            const int64_t* os = kKeys ? (is_dv ? p.dvs : p.dks) : p.dqs;
+            __nv_bfloat16* out = (__nv_bfloat16*)(kKeys ? (is_dv ? p.dv : p.dk) : p.dq) + b * os[0] + xh * os[1] +
+                                 (int64_t)(x0 + r) * os[2];
+            const float f = is_dv ? 1.f : p.scale;
+            const int c0 = kKeys ? 0 : wg * (DP / 2), c1 = min(p.D, kKeys ? DP : c0 + DP / 2);
+#pragma unroll 1
+            for (int c = c0; c < c1; c += 32) {
+                float o[32];
+                if (n > 0) {
+                    tmem_ld_x32((is_dv ? tB : tA) + lanes + c, o);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = 0.f;
+                }
+                if (x0 + r >= xrows) continue;
+#pragma unroll
+                for (int k = 0; k < 32; k += 8)
+                    if (c + k + 8 <= c1)
+                        *reinterpret_cast<uint4*>(out + c + k) =
+                            make_uint4(bf16x2(o[k] * f, o[k + 1] * f), bf16x2(o[k + 2] * f, o[k + 3] * f),
+                                       bf16x2(o[k + 4] * f, o[k + 5] * f), bf16x2(o[k + 6] * f, o[k + 7] * f));
+            }
+        }
+        if (!ok && lane == 0) tc_report(tp.status, 212);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (st.failed && threadIdx.x == 0 && n > 0) {        // copies that nobody waited for
+        tc_drain(smem_u32(&st.x_full), 0);
+        for (int i = max(0, st.loads - kTcBwdStages); i < st.loads; ++i)
+            tc_drain(smem_u32(&st.y_full[i % kTcBwdStages]), (i / kTcBwdStages) & 1);
+    }
+    if (warp == 9) tmem_dealloc(st.tmem, 512);
+}
+
+}  // namespace mg
