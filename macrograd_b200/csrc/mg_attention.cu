@@ -265,13 +265,26 @@ mg_status backward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
 }
 
 // ---------------------------------------------------------------- paged
+template <typename T, int DP>
+mg_status launch_paged_kernel(const mg::PagedParams& p, int blocks, cudaStream_t st)
+{
+    constexpr size_t smem = mg::paged_smem<T, DP>();
+    MG_HOST_TRY(cudaFuncSetAttribute(mg::paged_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    mg::paged_kernel<T, DP><<<blocks, mg::kPagedThreads, smem, st>>>(p);
+    return MG_OK;
+}
+
 // Splits: enough blocks to fill the GPU several times over, so that requests of
 // uneven lengths even out, but no chunk shorter than 128 keys.
 template <typename T>
 mg_status launch_paged(mg::PagedParams& p, int longest, const Device& dev, Scratch& ws, cudaStream_t st,
                        const char* who)
 {
-    const int group = p.H / p.Hkv, packs = ceil_div(group, mg::kPagedHeads);
+    const int vec = 16 / (int)sizeof(T);
+    bool stream = p.D % vec == 0 && aligned(p.k, p.ks, 3, sizeof(T), vec) && aligned(p.v, p.vs, 3, sizeof(T), vec);
+    if (p.k_new) stream = stream && aligned(p.k_new, p.kns, 2, sizeof(T), vec) &&
+                          aligned(p.v_new, p.vns, 2, sizeof(T), vec);
+    const int group = p.H / p.Hkv, packs = ceil_div(group, stream ? mg::paged_pack<T>() : mg::kPagedHeads);
     const int64_t heads = (int64_t)p.B * p.Hkv * packs;
     const int64_t want = std::max<int64_t>(1, (int64_t)dev.sm_count * 8 / heads);
     const int most = std::max(1, ceil_div(longest, 128));
@@ -285,7 +298,9 @@ mg_status launch_paged(mg::PagedParams& p, int longest, const Device& dev, Scrat
         p.stat = static_cast<float2*>(ws.get(rows * sizeof(float2)));
         if (!p.part || !p.stat) return fail(MG_ERR_ALLOC, "%s: no scratch for %zu chunks", who, rows);
     }
-    mg::paged_simt_kernel<T><<<(int)(heads * splits), mg::kPagedThreads, 0, st>>>(p);
+    const int blocks = (int)(heads * splits);
+    if (!stream) mg::paged_simt_kernel<T><<<blocks, mg::kPagedThreads, 0, st>>>(p);
+    else MG_TRY((p.D <= 64 ? launch_paged_kernel<T, 64>(p, blocks, st) : launch_paged_kernel<T, 128>(p, blocks, st)));
     MG_TRY(launched(who));
     if (splits > 1) {
         mg::paged_join_kernel<T><<<ceil_div((int64_t)p.B * p.H, mg::kPagedThreads / 32), mg::kPagedThreads, 0, st>>>(p);

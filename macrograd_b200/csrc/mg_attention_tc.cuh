@@ -116,6 +116,13 @@ __device__ __forceinline__ uint64_t tanh_small2(uint64_t x)
 // tanh(x) for any x: 1 - 2 / (1 + exp(2x)); its error is absolute, some 2^-23.
 __device__ __forceinline__ float tanh_any(float x) { return fmaf(-2.f, rcp(1.f + ex2(x * (2.f * kLog2e))), 1.f); }
 
+__device__ __forceinline__ float tanh_fast(float x)
+{
+    float small, other;
+    unpack2(tanh_small2(pack2(x, x)), small, other);
+    return fabsf(x) <= 1.f ? small : tanh_any(x);
+}
+
 // s[i] <- cap2 * tanh(s[i] * pre) for N values. The polynomial serves where no
 // value of the warp leaves [-1, 1] (scores well below the cap, the usual case:
 // 4 issue slots a value instead of 16 of the exponential unit).

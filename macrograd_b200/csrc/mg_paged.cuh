@@ -1,6 +1,9 @@
 // mg_paged.cuh -- attention of one new token per request over a paged cache,
 // split over the cache's length and joined.
 //
+// Two forms. paged_kernel streams the cache through shared memory (rows on
+// 16-byte boundaries); paged_simt_kernel takes any strides.
+//
 // One block reads `chunk` keys of one key-value head of one request, once, for
 // all query heads that share it (in groups of kPagedHeads), and leaves per query
 // head the maximum m, the sum l = sum exp(s - m) and the sum of exp(s - m) v. A
@@ -9,7 +12,7 @@
 // The bound is the cache's bytes.
 #pragma once
 
-#include "mg_attention_common.cuh"
+#include "mg_attention_tc.cuh"
 
 namespace mg {
 
@@ -66,6 +69,38 @@ __device__ __forceinline__ bool paged_row(const PagedParams& p, int b, int j, in
     page = __ldg(p.table + b * p.table_stride + n);
     row = j - n * p.page;
     return page >= 0 && page < p.pages;
+}
+
+__device__ __forceinline__ float4 lds4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float2 lds2(uint32_t addr)
+{
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
+    return v;
+}
+
+// What one warp does with a finished chunk of one query head: the result where
+// the request has no other chunk, else its part of the join. M: natural log.
+template <typename T, typename F>
+__device__ __forceinline__ void paged_store(const PagedParams& p, int b, int h, int split, float M, float L, int lane,
+                                            F&& acc)
+{
+    const int64_t row = (int64_t)b * p.H + h;
+    const float inv = L > 0.f ? 1.f / L : L;           // 0: no key; NaN stays
+    for (int d = lane; d < p.D; d += 32) {
+        const float a = acc(d);
+        if (p.splits == 1) ((T*)p.out)[b * p.os[0] + h * p.os[1] + d] = from_f32<T>(a * inv);
+        else p.part[(row * p.splits + split) * p.D + d] = a;
+    }
+    if (lane == 0) {
+        if (p.splits == 1) p.lse[row] = L == 0.f ? -CUDART_INF_F : M + logf(L);
+        else p.stat[row * p.splits + split] = make_float2(M, L);
+    }
 }
 
 // Simple form: a warp per key, lanes over the head's elements.
@@ -166,19 +201,401 @@ __global__ void __launch_bounds__(kPagedThreads) paged_simt_kernel(const __grid_
             f[w] = expf(sm_m[w][g] - base);
             L += f[w] * sm_l[w][g];
         }
-        const int64_t row = (int64_t)b * p.H + h0 + g;
-        const float inv = L > 0.f ? 1.f / L : 0.f;
-        for (int d = lane; d < p.D; d += 32) {
+        paged_store<T>(p, b, h0 + g, split, M, L, lane, [&](int d) {
             float a = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) a = fmaf(f[w], sm_acc[w][g][d], a);
-            if (p.splits == 1) ((T*)p.out)[b * p.os[0] + (h0 + g) * p.os[1] + d] = from_f32<T>(a * inv);
-            else p.part[(row * p.splits + split) * p.D + d] = a;
+            return a;
+        });
+    }
+}
+
+// ---------------------------------------------------------------- streaming form
+// Each warp walks tiles of 16 keys of its block's chunk (every fourth tile) and
+// keeps kPagedStages of them in flight into shared memory by 16-byte
+// asynchronous copies, so that the loads of the next tiles run under the
+// arithmetic of this one and no warp waits for another: a block of 4 warps has
+// up to 4 * 2 * 16 * D elements of keys and values on the way. A row's 16-byte
+// pieces are permuted by its number (piece ^ (row & 7)), so that reading one
+// piece of 8 rows meets 8 different groups of banks. What a page table entry or
+// a document hides is filled with zeros instead of being loaded, and masked.
+//
+// bf16: the query heads of the key-value head are the 16 rows of m16n8k16
+// products (S = Q K^T, O += P V; P in the layout that S leaves it in): with
+// one to sixteen heads to a key-value head the loads bound the kernel, not the
+// arithmetic, so the warp-level instruction is enough here. fp32: a lane has one key (half of the head
+// each in two lanes) for the scores and D / 32 elements of the output.
+constexpr int kPagedStages = 3;
+constexpr int kPagedTile = 16;
+constexpr int kPagedWarps = kPagedThreads / 32;
+
+template <typename T>
+__host__ __device__ constexpr int paged_pack() { return sizeof(T) == 2 ? 16 : kPagedHeads; }    // query heads of a block
+
+template <typename T, int DP>
+constexpr size_t paged_smem()
+{
+    const size_t ring = (size_t)kPagedWarps * kPagedStages * 2 * kPagedTile * DP * sizeof(T);
+    const size_t join = (size_t)kPagedWarps * paged_pack<T>() * DP * sizeof(float);
+    return ring > join ? ring : join;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// What a warp keeps of its keys: bf16.
+template <typename T, int DP>
+struct PagedAcc {
+    uint32_t q[DP / 16][4];      // A operand: rows g and g + 8, elements 2t, 2t + 1 (+ 8) of each 16
+    float o[DP / 8][4];
+    float m[2], l[2], slope[2];  // heads g and g + 8; l of this lane's keys alone
+    __device__ __forceinline__ void init(const PagedParams& p, int b, int h0, int nh, int lane, const float*)
+    {
+        const int g = lane / 4, t = lane % 4;
+        const T* q0 = (const T*)p.q + b * p.qs[0] + (h0 + g) * p.qs[1];
+        const T* q1 = q0 + 8 * p.qs[1];
+        const auto two = [&](const T* x, bool head, int d) {
+            __nv_bfloat162 v;
+            v.x = head && d < p.D ? x[d] : __float2bfloat16(0.f);
+            v.y = head && d + 1 < p.D ? x[d + 1] : __float2bfloat16(0.f);
+            return *reinterpret_cast<uint32_t*>(&v);
+        };
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            q[k][0] = two(q0, g < nh, 16 * k + 2 * t);
+            q[k][1] = two(q1, g + 8 < nh, 16 * k + 2 * t);
+            q[k][2] = two(q0, g < nh, 16 * k + 2 * t + 8);
+            q[k][3] = two(q1, g + 8 < nh, 16 * k + 2 * t + 8);
         }
-        if (lane == 0) {
-            if (p.splits == 1) p.lse[row] = L > 0.f ? M + logf(L) : -CUDART_INF_F;
-            else p.stat[row * p.splits + split] = make_float2(M, L);
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            m[i] = -CUDART_INF_F;
+            l[i] = 0.f;
+            slope[i] = p.slopes && g + 8 * i < nh ? __ldg(p.slopes + h0 + g + 8 * i) * kLog2e : 0.f;
         }
+    }
+    // Tile of 16 keys at sk, sv; key i is seen where bit i of `seen` is set and stands `back - i` before the query.
+    __device__ __forceinline__ void tile(const PagedParams& p, uint32_t sk, uint32_t sv, uint32_t seen, int back, int nh,
+                                         int lane)
+    {
+        const int t = lane % 4;
+        float s[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            // matrices: keys 0-7 of both halves of the 16 elements, then keys 8-15
+            const int row = (lane & 7) + (lane >> 4) * 8, piece = 2 * k + ((lane >> 3) & 1);
+            uint32_t b[4];
+            ldmatrix4(b, sk + row * (DP * 2) + ((piece ^ (row & 7)) << 4));
+            mma16816(s[0], q[k], b[0], b[1]);
+            mma16816(s[1], q[k], b[2], b[3]);
+        }
+        const float mul = p.scale * kLog2e, cap2 = p.cap * kLog2e, pre = p.cap > 0.f ? p.scale / p.cap : 0.f;
+        float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = 8 * n + 2 * t + (i & 1);
+                float x = s[n][i] * mul;
+                if (p.cap > 0.f) x = cap2 * tanh_fast(s[n][i] * pre);
+                x = fmaf(-slope[i >> 1], (float)(back - key), x);
+                x = (seen >> key) & 1 ? x : -CUDART_INF_F;
+                s[n][i] = x;
+                top[i >> 1] = fmaxf(top[i >> 1], x);
+            }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 1));
+            top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 2));
+        }
+        // the maximum in use follows once it is 2^8 behind (or there was none)
+        const bool up0 = m[0] == -CUDART_INF_F ? top[0] > m[0] : top[0] - m[0] > 8.f;
+        const bool up1 = m[1] == -CUDART_INF_F ? top[1] > m[1] : top[1] - m[1] > 8.f;
+        if (__any_sync(~0u, up0 || up1)) {
+            const float n0 = up0 ? top[0] : m[0], n1 = up1 ? top[1] : m[1];
+            const float f0 = up0 ? ex2(m[0] - n0) : 1.f, f1 = up1 ? ex2(m[1] - n1) : 1.f;
+            m[0] = n0, m[1] = n1;
+            l[0] *= f0, l[1] *= f1;
+#pragma unroll
+            for (int i = 0; i < DP / 8; ++i) o[i][0] *= f0, o[i][1] *= f0, o[i][2] *= f1, o[i][3] *= f1;
+        }
+        const float b0 = m[0] == -CUDART_INF_F ? 0.f : m[0], b1 = m[1] == -CUDART_INF_F ? 0.f : m[1];
+        uint32_t a[4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const float e0 = ex2(s[n][0] - b0), e1 = ex2(s[n][1] - b0);
+            const float e2 = ex2(s[n][2] - b1), e3 = ex2(s[n][3] - b1);
+            l[0] += e0 + e1;
+            l[1] += e2 + e3;
+            const __nv_bfloat162 x = __floats2bfloat162_rn(e0, e1), y = __floats2bfloat162_rn(e2, e3);
+            a[2 * n] = *reinterpret_cast<const uint32_t*>(&x);
+            a[2 * n + 1] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            // matrices: keys 0-7 and 8-15 of 8 elements, then of the next 8
+            const int row = lane & 15, piece = 2 * k + (lane >> 4);
+            uint32_t b[4];
+            ldmatrix4_trans(b, sv + row * (DP * 2) + ((piece ^ (row & 7)) << 4));
+            mma16816(o[2 * k], a, b[0], b[1]);
+            mma16816(o[2 * k + 1], a, b[2], b[3]);
+        }
+    }
+    __device__ __forceinline__ void finish(float* sm_m, float* sm_l, float* sm_o, int nh, int lane)
+    {
+        const int g = lane / 4, t = lane % 4;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            l[i] += __shfl_xor_sync(~0u, l[i], 1);
+            l[i] += __shfl_xor_sync(~0u, l[i], 2);
+            if (t == 0) sm_m[g + 8 * i] = m[i], sm_l[g + 8 * i] = l[i];
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+            float2* lo = reinterpret_cast<float2*>(sm_o + g * DP + 8 * i + 2 * t);
+            float2* hi = reinterpret_cast<float2*>(sm_o + (g + 8) * DP + 8 * i + 2 * t);
+            *lo = make_float2(o[i][0], o[i][1]);
+            *hi = make_float2(o[i][2], o[i][3]);
+        }
+    }
+};
+
+// fp32.
+template <int DP>
+struct PagedAcc<float, DP> {
+    static constexpr int kPer = DP / 32;
+    const float* q;              // [heads][DP] in shared memory
+    float o[kPagedHeads][kPer], m[kPagedHeads], l[kPagedHeads], slope[kPagedHeads];
+    __device__ __forceinline__ void init(const PagedParams& p, int, int h0, int nh, int, const float* sq)
+    {
+        q = sq;
+#pragma unroll
+        for (int g = 0; g < kPagedHeads; ++g) {
+            m[g] = -CUDART_INF_F;
+            l[g] = 0.f;
+            slope[g] = p.slopes && g < nh ? __ldg(p.slopes + h0 + g) * kLog2e : 0.f;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) o[g][i] = 0.f;
+        }
+    }
+    __device__ __forceinline__ void tile(const PagedParams& p, uint32_t sk, uint32_t sv, uint32_t seen, int back, int nh,
+                                         int lane)
+    {
+        const int key = lane & 15, half = lane >> 4;
+        float s[kPagedHeads];
+#pragma unroll
+        for (int g = 0; g < kPagedHeads; ++g) s[g] = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < DP / 8; ++i) {
+            const int piece = half * (DP / 8) + i;
+            const float4 k4 = lds4(sk + key * (DP * 4) + ((piece ^ (key & 7)) << 4));
+#pragma unroll
+            for (int g = 0; g < kPagedHeads; ++g) {
+                if (g >= nh) break;
+                const float4 q4 = *reinterpret_cast<const float4*>(q + g * DP + 4 * piece);
+                s[g] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[g]))));
+            }
+        }
+        const float mul = p.scale * kLog2e;
+#pragma unroll
+        for (int g = 0; g < kPagedHeads; ++g) {
+            if (g >= nh) break;
+            float x = s[g] + __shfl_xor_sync(~0u, s[g], 16);
+            x = p.cap > 0.f ? p.cap * kLog2e * tanhf(x * p.scale / p.cap) : x * mul;
+            x = fmaf(-slope[g], (float)(back - key), x);
+            x = (seen >> key) & 1 ? x : -CUDART_INF_F;
+            float top = x;
+#pragma unroll
+            for (int w = 8; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
+            if (m[g] == -CUDART_INF_F ? top > m[g] : top - m[g] > 8.f) {     // the same for the whole warp
+                const float f = ex2(m[g] - top);
+                m[g] = top;
+                l[g] *= f;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) o[g][i] *= f;
+            }
+            s[g] = ex2(x - (m[g] == -CUDART_INF_F ? 0.f : m[g]));
+            l[g] += half ? 0.f : s[g];
+        }
+#pragma unroll 4
+        for (int r = 0; r < kPagedTile; ++r) {
+            float v[kPer];
+            const uint32_t row = sv + r * (DP * 4);
+            if (kPer == 4) {
+                const float4 x = lds4(row + ((lane ^ (r & 7)) << 4));
+                v[0] = x.x, v[1] = x.y, v[kPer - 2] = x.z, v[kPer - 1] = x.w;
+            } else {
+                const float2 x = lds2(row + (((lane >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8);
+                v[0] = x.x, v[1] = x.y;
+            }
+#pragma unroll
+            for (int g = 0; g < kPagedHeads; ++g) {
+                if (g >= nh) break;
+                const float e = __shfl_sync(~0u, s[g], r);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) o[g][i] = fmaf(e, v[i], o[g][i]);
+            }
+        }
+    }
+    __device__ __forceinline__ void finish(float* sm_m, float* sm_l, float* sm_o, int nh, int lane)
+    {
+#pragma unroll
+        for (int g = 0; g < kPagedHeads; ++g) {
+            if (g >= nh) break;
+            for (int w = 8; w; w /= 2) l[g] += __shfl_xor_sync(~0u, l[g], w);
+            if (lane == 0) sm_m[g] = m[g], sm_l[g] = l[g];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) sm_o[g * DP + lane * kPer + i] = o[g][i];
+        }
+    }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_constant__ PagedParams p)
+{
+    constexpr int kPack = paged_pack<T>(), kPieces = DP * (int)sizeof(T) / 16;
+    constexpr uint32_t kTileBytes = kPagedTile * DP * sizeof(T);
+    extern __shared__ __align__(128) uint8_t paged_dyn[];
+    __shared__ float sm_m[kPagedWarps][16], sm_l[kPagedWarps][16];
+    __shared__ __align__(16) float sq[sizeof(T) == 4 ? kPagedHeads * DP : 4];
+    __shared__ uint32_t sm_seen[kPagedWarps][kPagedStages];
+
+    const int split = blockIdx.x % p.splits, bh = blockIdx.x / p.splits;
+    const int groups = p.H / p.Hkv, packs = (groups + kPack - 1) / kPack;
+    const int pack = bh % packs, kv = bh / packs % p.Hkv, b = bh / packs / p.Hkv;
+    const int len = paged_length(p, b);
+    if (threadIdx.x == 0 && split == 0 && p.lengths && __ldg(p.lengths + b) != len) paged_report(p, kPagedBadLength);
+    const int j0 = split * p.chunk, j1 = min(len, j0 + p.chunk);
+    if (j0 >= j1 && split > 0) return;      // a chunk beyond the request's keys is not joined
+    const int h0 = kv * groups + pack * kPack, nh = min(kPack, groups - pack * kPack);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(paged_dyn) + warp * kPagedStages * 2 * kTileBytes;
+    const int qdoc = p.docs && len > 0 ? __ldg(p.docs + (int64_t)b * p.length + len - 1) : 0;
+
+    // Tile n of this warp: keys j0 + (4 n + warp) * 16 and on. Lanes i and i + 16 find the rows of key i.
+    const auto issue = [&](int n) {
+        const int j = j0 + (n * kPagedWarps + warp) * kPagedTile + (lane & 15);
+        bool live = j < j1;
+        const T *kr = (const T*)p.k, *vr = (const T*)p.v;
+        bool fresh = false;
+        T *kc = nullptr, *vc = nullptr;
+        if (live) {
+            int page, row;
+            if (!paged_row(p, b, j, page, row)) {
+                paged_report(p, kPagedBadPage);
+                live = false;
+            } else if (p.docs && (qdoc < 0 || __ldg(p.docs + (int64_t)b * p.length + j) != qdoc)) {
+                live = false;
+            } else {
+                kr = kc = (T*)p.k + page * p.ks[0] + row * p.ks[1] + kv * p.ks[2];
+                vr = vc = (T*)p.v + page * p.vs[0] + row * p.vs[1] + kv * p.vs[2];
+                fresh = p.k_new != nullptr && j == len - 1;
+                if (fresh) {
+                    kr = (const T*)p.k_new + b * p.kns[0] + kv * p.kns[1];
+                    vr = (const T*)p.v_new + b * p.vns[0] + kv * p.vns[1];
+                }
+            }
+        }
+        const uint32_t seen = __ballot_sync(~0u, live);
+        if (lane == 0) sm_seen[warp][n % kPagedStages] = seen & 0xFFFFu;
+        const uint32_t dst = ring + (n % kPagedStages) * 2 * kTileBytes;
+#pragma unroll
+        for (int i = 0; i < kPagedTile * kPieces / 32; ++i) {
+            const int r = (i * 32 + lane) / kPieces, c = (i * 32 + lane) % kPieces;
+            const T* ks = (const T*)__shfl_sync(~0u, (unsigned long long)kr, r);
+            const T* vs = (const T*)__shfl_sync(~0u, (unsigned long long)vr, r);
+            const int e = c * (16 / (int)sizeof(T));
+            const bool in = (seen >> r & 1) && e < p.D;
+            const uint32_t at = dst + r * (DP * (int)sizeof(T)) + ((c ^ (r & 7)) << 4);
+            copy16(at, ks + (in ? e : 0), in);
+            copy16(at + kTileBytes, vs + (in ? e : 0), in);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        // the token's own key and value go to the cache (lanes 0-15 the key, 16-31 the value)
+        const uint32_t new_row = __ballot_sync(~0u, fresh) & 0xFFFFu;
+        if (new_row && pack == 0) {
+            const int r = __ffs(new_row) - 1;
+            const bool is_v = lane >= 16;
+            const T* src = (const T*)__shfl_sync(~0u, (unsigned long long)(is_v ? vr : kr), r + (lane & 16));
+            T* out = (T*)__shfl_sync(~0u, (unsigned long long)(is_v ? vc : kc), r + (lane & 16));
+            for (int e = (lane & 15) * (16 / (int)sizeof(T)); e < p.D; e += 16 * (16 / (int)sizeof(T)))
+                *reinterpret_cast<uint4*>(out + e) = *reinterpret_cast<const uint4*>(src + e);
+        }
+    };
+    const int tiles = max(0, (j1 - j0 + kPagedTile - 1) / kPagedTile);
+    const int mine = tiles > warp ? (tiles - warp + kPagedWarps - 1) / kPagedWarps : 0;
+#pragma unroll
+    for (int n = 0; n < kPagedStages - 1; ++n) {
+        if (n < mine) issue(n);
+        else asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    if (sizeof(T) == 4) {
+        for (int i = threadIdx.x; i < nh * DP; i += kPagedThreads) {
+            const int g = i / DP, d = i % DP;
+            sq[i] = d < p.D ? to_f32(((const T*)p.q)[b * p.qs[0] + (h0 + g) * p.qs[1] + d]) : 0.f;
+        }
+        __syncthreads();
+    }
+    PagedAcc<T, DP> acc;
+    acc.init(p, b, h0, nh, lane, sq);
+    for (int n = 0; n < mine; ++n) {
+        __syncwarp();
+        if (n + kPagedStages - 1 < mine) issue(n + kPagedStages - 1);
+        else asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(kPagedStages - 1) : "memory");
+        __syncwarp();
+        const uint32_t at = ring + (n % kPagedStages) * 2 * kTileBytes;
+        acc.tile(p, at, at + kTileBytes, sm_seen[warp][n % kPagedStages],
+                 len - 1 - (j0 + (n * kPagedWarps + warp) * kPagedTile), nh, lane);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();                        // the rings become the join's buffer
+    float* so = reinterpret_cast<float*>(paged_dyn);
+    acc.finish(sm_m[warp], sm_l[warp], so + warp * kPack * DP, nh, lane);
+    __syncthreads();
+    for (int g = warp; g < nh; g += kPagedWarps) {
+        float M = -CUDART_INF_F, L = 0.f, f[kPagedWarps];
+#pragma unroll
+        for (int w = 0; w < kPagedWarps; ++w) M = fmaxf(M, sm_m[w][g]);
+        const float base = M == -CUDART_INF_F ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < kPagedWarps; ++w) {
+            f[w] = ex2(sm_m[w][g] - base);
+            L = fmaf(f[w], sm_l[w][g], L);
+        }
+        paged_store<T>(p, b, h0 + g, split, M * kLn2, L, lane, [&](int d) {
+            float a = 0.f;
+#pragma unroll
+            for (int w = 0; w < kPagedWarps; ++w) a = fmaf(f[w], so[(w * kPack + g) * DP + d], a);
+            return a;
+        });
     }
 }
 
@@ -201,14 +618,14 @@ __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const __grid_
     for (int s = lane; s < n; s += 32) L += expf(st[s].x - base) * st[s].y;
 #pragma unroll
     for (int o = 16; o; o /= 2) L += __shfl_xor_sync(~0u, L, o);
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = L > 0.f ? 1.f / L : L;           // 0: no key; NaN stays
     T* out = (T*)p.out + b * p.os[0] + h * p.os[1];
     for (int d = lane; d < p.D; d += 32) {
         float a = 0.f;
         for (int s = 0; s < n; ++s) a = fmaf(expf(st[s].x - base), p.part[(row * p.splits + s) * p.D + d], a);
         out[d] = from_f32<T>(a * inv);
     }
-    if (lane == 0) p.lse[row] = L > 0.f ? M + logf(L) : -CUDART_INF_F;
+    if (lane == 0) p.lse[row] = L == 0.f ? -CUDART_INF_F : M + logf(L);
 }
 
 }  // namespace mg
