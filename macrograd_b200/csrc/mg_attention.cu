@@ -11,6 +11,7 @@
 #include "mg_attention_simt.cuh"
 #include "mg_attention_tc.cuh"
 #include "mg_attention_tc_bwd.cuh"
+#include "mg_attention_tc32.cuh"
 #include "mg_paged.cuh"
 #include "mg_rotary.cuh"
 
@@ -125,21 +126,22 @@ bool aligned(const void* ptr, const int64_t* strides, int n, size_t elem, int ve
 }
 
 // ---------------------------------------------------------------- tensor cores
-// The tensor-core kernels read 16-bit tensors through TMA (rows on 16-byte
-// boundaries) and store 16-byte vectors; a scale of 0 would turn their masked
-// scores (-inf) into NaN. Everything else runs on the CUDA cores.
+// The tensor-core kernels read and store rows of whole 16-byte vectors, 16-bit
+// tensors through TMA; a scale of 0 would turn their masked scores (-inf) into
+// NaN. Everything else runs on the CUDA cores.
 bool tc_serves(const mg_attention_desc* d, const mg::AttnParams& p, std::initializer_list<const void*> rows_q,
                std::initializer_list<const void*> rows_k)
 {
-    if (d->dtype != MG_BF16 || d->head_dim % 8 || d->scale == 0.f) return false;
-    if (!std::isfinite(1.f / d->scale)) return false;
+    if (d->head_dim % 8 || d->scale == 0.f || !std::isfinite(1.f / d->scale)) return false;
+    const int vec = d->dtype == MG_BF16 ? 8 : 4;
     for (const void* x : rows_q)
         if (reinterpret_cast<uintptr_t>(x) % 16) return false;
     for (const void* x : rows_k)
         if (reinterpret_cast<uintptr_t>(x) % 16) return false;
     for (int i = 0; i < 3; ++i)
         for (int64_t s : {p.qs[i], p.ks[i], p.vs[i], p.os[i], p.dos[i], p.dqs[i], p.dks[i], p.dvs[i]})
-            if (s % 8 || s < 0 || s >= (1ll << 38)) return false;
+            if (s % vec || s < 0 || s >= (1ll << 38)) return false;
+    if (d->dtype == MG_F32) return true;
     const bool rows_repeat = (p.Lq > 1 && (p.qs[2] == 0 || (p.dout && p.dos[2] == 0))) ||
                              (p.Lk > 1 && (p.ks[2] == 0 || p.vs[2] == 0));
     return !rows_repeat;
@@ -264,6 +266,34 @@ mg_status backward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     return p.D <= 64 ? launch_tc_backward<64, false>(t, st) : launch_tc_backward<128, false>(t, st);
 }
 
+template <int DP, bool kCap, bool kBias>
+mg_status launch_tc32_forward(const mg::Tc32Params& t, cudaStream_t st)
+{
+    const auto kernel = mg::attn_tc32_forward<DP, kCap, kBias>;
+    constexpr size_t smem = mg::tc32_forward_smem<DP>();
+    MG_HOST_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kernel<<<ceil_div(t.a.Lq, 128 * mg::tc32_nq<DP>()) * t.a.B * t.a.H, mg::tc32_threads<DP>(), smem, st>>>(t);
+    return launched("mg_attention");
+}
+
+template <int DP>
+mg_status launch_tc32_forward(const mg::Tc32Params& t, cudaStream_t st)
+{
+    const bool cap = t.a.cap > 0.f, bias = t.a.slopes != nullptr;
+    return cap ? (bias ? launch_tc32_forward<DP, true, true>(t, st) : launch_tc32_forward<DP, true, false>(t, st))
+               : (bias ? launch_tc32_forward<DP, false, true>(t, st) : launch_tc32_forward<DP, false, false>(t, st));
+}
+
+mg_status forward_tc32(const mg::AttnParams& p, const Device& dev, void* stream)
+{
+    mg::TcAttnParams f = {};
+    Scratch ws(dev, stream);
+    cudaStream_t st = (cudaStream_t)stream;
+    MG_TRY(tc_params(&f, p, dev, ws, st, "mg_attention"));
+    mg::Tc32Params t = {p, f.doc_tiles, mg::idesc_bf16(128, 64, false, false, p.scale < 0.f), f.scale, f.status};
+    return p.D <= 64 ? launch_tc32_forward<64>(t, st) : launch_tc32_forward<128>(t, st);
+}
+
 // ---------------------------------------------------------------- paged
 template <typename T, int DP>
 mg_status launch_paged_kernel(const mg::PagedParams& p, int blocks, cudaStream_t st)
@@ -364,7 +394,8 @@ mg_status mg_attention(const mg_attention_desc* d, void* out, float* lse, const 
         return d->dtype == MG_F32 ? launch_paged<float>(g, p.Lk, dev, ws, st, "mg_attention")
                                   : launch_paged<__nv_bfloat16>(g, p.Lk, dev, ws, st, "mg_attention");
     }
-    if (p.Lk > 0 && tc_serves(d, p, {q, out}, {k, v})) return forward_tc(p, dev, stream);
+    if (p.Lk > 0 && tc_serves(d, p, {q, out}, {k, v}))
+        return d->dtype == MG_F32 ? forward_tc32(p, dev, stream) : forward_tc(p, dev, stream);
     return d->dtype == MG_F32 ? forward_simt<float>(p, st) : forward_simt<__nv_bfloat16>(p, st);
 }
 
@@ -382,7 +413,7 @@ mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, 
     mg::AttnParams p = attention_params(d);
     p.q = q, p.k = k, p.v = v, p.out = const_cast<void*>(out), p.dout = dout, p.lse = const_cast<float*>(lse);
     p.dq = dq, p.dk = dk, p.dv = dv;
-    if (d->q_len > 0 && d->k_len > 0 && tc_serves(d, p, {q, out, dout, dq}, {k, v, dk, dv}))
+    if (d->dtype == MG_BF16 && d->q_len > 0 && d->k_len > 0 && tc_serves(d, p, {q, out, dout, dq}, {k, v, dk, dv}))
         return backward_tc(p, dev, stream);
     Scratch ws(dev, stream);
     if (d->q_len > 0) {

@@ -96,26 +96,6 @@ __device__ __forceinline__ void bulk_load(uint32_t bar, uint32_t dst, const void
                  : "memory");
 }
 
-// The one document that positions [pos, pos + n) have in common by the tiles of
-// 128, or -1 (some padding, several documents, positions outside the row).
-__device__ __forceinline__ int common_doc(const int2* tiles, int pos, int n, int Lk)
-{
-    if (pos < 0 || pos + n > Lk) return -1;
-    const int2 a = __ldg(tiles + (pos >> 7)), b = __ldg(tiles + ((pos + n - 1) >> 7));
-    return a.x == a.y && b.x == b.y && a.x == b.x ? a.x : -1;
-}
-
-// Whether a document of positions [pos, pos + n) can be one of `want`'s range.
-__device__ __forceinline__ bool docs_meet(const int2* tiles, int pos, int n, int Lk, int2 want)
-{
-    const int p0 = max(pos, 0), p1 = min(pos + n, Lk);
-    for (int t = p0 >> 7; t * 128 < p1; ++t) {
-        const int2 r = __ldg(tiles + t);
-        if (r.y >= 0 && want.y >= 0 && max(r.x, 0) <= want.y && r.y >= max(want.x, 0)) return true;
-    }
-    return false;
-}
-
 template <int DP>
 constexpr size_t tc_backward_smem() { return (2 * 128 + kTcBwdStages * 2 * 64) * DP * 2 + 1024; }
 
