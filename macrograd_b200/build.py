@@ -23,7 +23,7 @@ INCLUDE = os.path.join(ROOT, "include")
 UNITS = {
     "mg_gemm.cu": ["mg_gemm_kernel.cuh", "mg_ptx.cuh", "mg_host.h", "mg_plan.h"],
     "mg_attention.cu": ["mg_attention_common.cuh", "mg_attention_simt.cuh", "mg_attention_tc.cuh", "mg_attention_tc_bwd.cuh",
-                        "mg_attention_tc32.cuh",
+                        "mg_attention_tc32.cuh", "mg_attention_tc32_bwd.cuh",
                         "mg_tc16.cuh",
                         "mg_rotary.cuh", "mg_paged.cuh", "mg_ptx.cuh", "mg_host.h"],
 }

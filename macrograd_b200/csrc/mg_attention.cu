@@ -12,6 +12,7 @@
 #include "mg_attention_tc.cuh"
 #include "mg_attention_tc_bwd.cuh"
 #include "mg_attention_tc32.cuh"
+#include "mg_attention_tc32_bwd.cuh"
 #include "mg_paged.cuh"
 #include "mg_rotary.cuh"
 
@@ -248,7 +249,7 @@ mg_status backward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     float* stats = static_cast<float*>(ws.get(2 * rows * sizeof(float)));
     if (!stats) return fail(MG_ERR_ALLOC, "%s: no scratch for the row sums", who);
     t.lse2 = stats, t.delta = stats + rows;
-    mg::attn_tc_stats_kernel<<<ceil_div(rows, 16), 256, 0, st>>>(p, t.Lp, stats, stats + rows);
+    mg::attn_tc_stats_kernel<__nv_bfloat16><<<ceil_div(rows, 16), 256, 0, st>>>(p, t.Lp, stats, stats + rows);
     MG_TRY(launched(who));
     int* hs = t.head_step;
     int* bs = t.batch_step;
@@ -292,6 +293,44 @@ mg_status forward_tc32(const mg::AttnParams& p, const Device& dev, void* stream)
     MG_TRY(tc_params(&f, p, dev, ws, st, "mg_attention"));
     mg::Tc32Params t = {p, f.doc_tiles, mg::idesc_bf16(128, 64, false, false, p.scale < 0.f), f.scale, f.status};
     return p.D <= 64 ? launch_tc32_forward<64>(t, st) : launch_tc32_forward<128>(t, st);
+}
+
+template <bool kKeys, bool kCap, bool kBias>
+mg_status launch_tc32_backward(const mg::Tc32BwdParams& t, cudaStream_t st)
+{
+    const auto kernel = mg::attn_tc32_backward<kKeys, kCap, kBias>;
+    MG_HOST_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)mg::kTc32BwdSmem));
+    const int blocks = kKeys ? ceil_div(t.a.Lk, 128) * t.a.B * t.a.Hkv : ceil_div(t.a.Lq, 128) * t.a.B * t.a.H;
+    kernel<<<blocks, mg::kTc32BwdThreads, mg::kTc32BwdSmem, st>>>(t);
+    return launched("mg_attention_backward");
+}
+
+template <bool kKeys>
+mg_status launch_tc32_backward(const mg::Tc32BwdParams& t, cudaStream_t st)
+{
+    const bool cap = t.a.cap > 0.f, bias = t.a.slopes != nullptr;
+    return cap ? (bias ? launch_tc32_backward<kKeys, true, true>(t, st) : launch_tc32_backward<kKeys, true, false>(t, st))
+               : (bias ? launch_tc32_backward<kKeys, false, true>(t, st)
+                       : launch_tc32_backward<kKeys, false, false>(t, st));
+}
+
+mg_status backward_tc32(const mg::AttnParams& p, const Device& dev, void* stream)
+{
+    const char* who = "mg_attention_backward";
+    mg::TcAttnParams f = {};
+    Scratch ws(dev, stream);
+    cudaStream_t st = (cudaStream_t)stream;
+    MG_TRY(tc_params(&f, p, dev, ws, st, who));
+    const int Lp = ceil_div(p.Lq, 128) * 128;
+    const int64_t rows = (int64_t)p.B * p.H * Lp;
+    float* stats = static_cast<float*>(ws.get(2 * rows * sizeof(float)));
+    if (!stats) return fail(MG_ERR_ALLOC, "%s: no scratch for the row sums", who);
+    mg::attn_tc_stats_kernel<float><<<ceil_div(rows, 16), 256, 0, st>>>(p, Lp, stats, stats + rows);
+    MG_TRY(launched(who));
+    const mg::Tc32BwdParams t = {p,        f.doc_tiles, stats, stats + rows, Lp, mg::idesc_bf16(128, 64, false, false, p.scale < 0.f),
+                                 f.scale, f.status};
+    MG_TRY(launch_tc32_backward<true>(t, st));
+    return launch_tc32_backward<false>(t, st);
 }
 
 // ---------------------------------------------------------------- paged
@@ -413,8 +452,11 @@ mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, 
     mg::AttnParams p = attention_params(d);
     p.q = q, p.k = k, p.v = v, p.out = const_cast<void*>(out), p.dout = dout, p.lse = const_cast<float*>(lse);
     p.dq = dq, p.dk = dk, p.dv = dv;
-    if (d->dtype == MG_BF16 && d->q_len > 0 && d->k_len > 0 && tc_serves(d, p, {q, out, dout, dq}, {k, v, dk, dv}))
-        return backward_tc(p, dev, stream);
+    if (d->q_len > 0 && d->k_len > 0 && tc_serves(d, p, {q, out, dout, dq}, {k, v, dk, dv})) {
+        if (d->dtype == MG_BF16) return backward_tc(p, dev, stream);
+        // the pieces of longer fp32 heads do not fit the shared memory
+        if (d->head_dim <= 64) return backward_tc32(p, dev, stream);
+    }
     Scratch ws(dev, stream);
     if (d->q_len > 0) {
         p.delta = static_cast<float*>(ws.get(sizeof(float) * d->batch * d->heads * (size_t)d->q_len));

@@ -1,0 +1,355 @@
+// mg_attention_tc32_bwd.cuh -- gradients of attention of fp32 tensors with heads of
+// up to 64 elements on the 5th-generation tensor cores at fp32 accuracy.
+//
+// The two forms of mg_attention_tc_bwd.cuh (queries resident: dQ; keys resident:
+// dK, dV), with every product made of the six of mg_attention_tc32.cuh. The pieces of
+// 128 resident rows and of two stages of 64 streamed rows of two tensors fill the
+// shared memory (96 + 96 KB). Two warpgroups share a tile: warpgroup g has
+// columns [32 g, 32 g + 32) of S and dP, writes the pieces of its part of P and dS
+// to tensor memory, and adds its share of each tile's accumulators up in registers. The tensor
+// core runs S and dP of the next tile while the exponentials of this one are taken.
+#pragma once
+
+#include "mg_attention_tc32.cuh"
+#include "mg_attention_tc_bwd.cuh"
+
+namespace mg {
+
+struct Tc32BwdParams {
+    AttnParams a;
+    const int2* doc_tiles;
+    const float* lse2;           // as TcBwdParams
+    const float* delta;
+    int Lp;
+    uint32_t idesc_s;
+    float scale;                 // |scale|
+    int* status;
+};
+
+struct Tc32BwdState {
+    uint64_t x_full, y_full[2], y_empty[2], s_full, s_free, p_full, acc_full, drain;
+    uint32_t tmem;
+    int failed;
+    int range[2];
+    alignas(16) int doc[8][32];
+    alignas(16) float lse2[2][64];
+    alignas(16) float delta[2][64];
+};
+
+constexpr int kTc32BwdThreads = 384;     // two warpgroups, three warps that load, one that issues
+constexpr size_t kTc32BwdSmem = (size_t)(2 * 128 + 2 * 2 * 64) * 64 * 6 + 1024;
+
+template <bool kKeys, bool kCap, bool kBias>
+__global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const __grid_constant__ Tc32BwdParams tp)
+{
+    constexpr int DP = 64;
+    constexpr uint32_t kPieceX = 128 * DP * 2, kPieceY = 64 * DP * 2;
+    extern __shared__ uint8_t dyn[];
+    __shared__ Tc32BwdState st;
+    const AttnParams& p = tp.a;
+    const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
+    const uint32_t sX0 = base, sX1 = base + 3 * kPieceX, sY = base + 6 * kPieceX;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    const int nhead = kKeys ? p.Hkv : p.H, xrows = kKeys ? p.Lk : p.Lq, yrows = kKeys ? p.Lq : p.Lk;
+    const int xtiles = (xrows + 127) / 128, bh = blockIdx.x % (p.B * nhead), rank = blockIdx.x / (p.B * nhead);
+    const int x0 = (kKeys ? rank : xtiles - 1 - rank) * 128;
+    const int xh = bh % nhead, b = bh / nhead, group = p.H / p.Hkv;
+    const int shift = p.Lk - p.Lq;
+    const int32_t* docs = p.docs ? p.docs + (int64_t)b * p.Lk : nullptr;
+    const int2* dt = p.docs ? tp.doc_tiles + (int64_t)b * ((p.Lk + 127) / 128) : nullptr;
+    const int prefix = p.prefix ? __ldg(p.prefix + b) : 0;
+    const int xpos = kKeys ? x0 : x0 + shift;
+
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&st.x_full), 8);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&st.y_full[i]), kTc32LoadWarps);
+            mbar_init(smem_u32(&st.y_empty[i]), 1);
+        }
+        mbar_init(smem_u32(&st.s_full), 1);
+        mbar_init(smem_u32(&st.s_free), 8);
+        mbar_init(smem_u32(&st.p_full), 8);
+        mbar_init(smem_u32(&st.acc_full), 1);
+        mbar_init(smem_u32(&st.drain), 1);
+        mbar_fence_init();
+        st.failed = 0;
+        st.range[0] = INT_MAX;
+        st.range[1] = 0;
+    }
+    if (warp == 11) {
+        tmem_alloc(smem_u32(&st.tmem), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    int t0, t1;
+    stream_range<kKeys>(p, docs, dt, prefix, x0, xpos, shift, st.range, t0, t1);
+    const int tiles = max(0, t1 - t0), n = kKeys ? tiles * group : tiles;
+    const uint32_t tm = st.tmem, tS = tm, tdP = tm + 64, tP = tm + 128, tdS = tm + 224, tA = tm + 320, tB = tm + 384;
+    volatile int* failed = &st.failed;
+    const auto sY0 = [&](int i) { return sY + (uint32_t)(i & 1) * 6 * kPieceY; };
+
+    if (warp >= 8 && warp < 11) {
+        // ------------------------------------------------ loads and splits of the streamed rows
+        constexpr int kLoaders = kTc32LoadWarps * 32, kItems = (64 * (DP / 8) + kLoaders - 1) / kLoaders;
+        const int tid = threadIdx.x - 256;
+        const int64_t* s0 = kKeys ? p.qs : p.ks;
+        const int64_t* s1 = kKeys ? p.dos : p.vs;
+        bool ok = true;
+        for (int i = 0; i < n && ok; ++i) {
+            const int yh = kKeys ? xh * group + i / tiles : xh / group, y0 = (t0 + (kKeys ? i % tiles : i)) * 64;
+            const float* a = (const float*)(kKeys ? p.q : p.k) + b * s0[0] + yh * s0[1];
+            const float* c = (const float*)(kKeys ? p.dout : p.v) + b * s1[0] + yh * s1[1];
+            float4 x[kItems][2], y[kItems][2];
+#pragma unroll
+            for (int k = 0; k < kItems; ++k) {
+                const int item = k * kLoaders + tid, r = item / 8, e = item % 8 * 8, row = y0 + r;
+                const bool live = r < 64 && row < yrows && e < p.D &&
+                                  (!docs || doc_at(p, b, row + (kKeys ? shift : 0)) >= 0);
+                tc32_fetch(x[k], a + (int64_t)row * s0[2] + e, live);
+                tc32_fetch(y[k], c + (int64_t)row * s1[2] + e, live);
+            }
+            float stat = 0.f;
+            if (kKeys && tid < 64) stat = tp.lse2[((int64_t)b * p.H + yh) * tp.Lp + y0 + tid];
+            float stat2 = 0.f;
+            if (kKeys && tid < 64) stat2 = tp.delta[((int64_t)b * p.H + yh) * tp.Lp + y0 + tid];
+            if (i >= 2) ok = __all_sync(~0u, tc_wait(smem_u32(&st.y_empty[i & 1]), (i / 2 - 1) & 1, failed));
+            if (!ok) break;
+#pragma unroll
+            for (int k = 0; k < kItems; ++k) {
+                const int item = k * kLoaders + tid, r = item / 8, e = item % 8;
+                if (r >= 64) continue;
+                tc32_put(sY0(i), 64, kPieceY, r, e, x[k]);
+                tc32_put(sY0(i) + 3 * kPieceY, 64, kPieceY, r, e, y[k]);
+            }
+            if (kKeys && tid < 64) {
+                st.lse2[i & 1][tid] = stat;
+                st.delta[i & 1][tid] = stat2;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&st.y_full[i & 1]));
+        }
+    } else if (warp == 11) {
+        // ------------------------------------------------ products
+        constexpr uint32_t idesc_dp = idesc_bf16(128, 64, false, false), idesc_acc = idesc_bf16(128, DP, false, true);
+        bool ok = true;
+        for (int i = 0; i <= n && n > 0 && ok; ++i) {
+            if (i < n) {
+                ok = tc_wait(smem_u32(&st.y_full[i & 1]), (i >> 1) & 1, failed) &&
+                     (i > 0 ? tc_wait(smem_u32(&st.s_free), (i - 1) & 1, failed)
+                            : tc_wait(smem_u32(&st.x_full), 0, failed));
+                ok = __all_sync(~0u, ok);
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+#pragma unroll
+                    for (int x = 0; x < 6; ++x)
+#pragma unroll
+                        for (int k = 0; k < DP / 16; ++k)
+                            tc_mma_f16(tS, desc_k_major(sX0 + kPieceA[x] * kPieceX, 128, k),
+                                       desc_k_major(sY0(i) + kPieceB[x] * kPieceY, 64, k), tp.idesc_s, x + k > 0);
+#pragma unroll
+                    for (int x = 0; x < 6; ++x)
+#pragma unroll
+                        for (int k = 0; k < DP / 16; ++k)
+                            tc_mma_f16(tdP, desc_k_major(sX1 + kPieceA[x] * kPieceX, 128, k),
+                                       desc_k_major(sY0(i) + (3 + kPieceB[x]) * kPieceY, 64, k), idesc_dp, x + k > 0);
+                    tc_commit(smem_u32(&st.s_full));
+                }
+                __syncwarp();
+            }
+            if (i > 0) {
+                const int j = i - 1;
+                ok = __all_sync(~0u, tc_wait(smem_u32(&st.p_full), j & 1, failed));
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    if (kKeys) {
+#pragma unroll
+                        for (int x = 0; x < 6; ++x)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                tc_mma_f16_ta(tB, tP + kPieceA[x] * 32 + 8 * k,
+                                              desc_mn_major(sY0(j) + (3 + kPieceB[x]) * kPieceY, 64, k), idesc_acc,
+                                              x + k > 0);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 6; ++x)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            tc_mma_f16_ta(tA, tdS + kPieceA[x] * 32 + 8 * k,
+                                          desc_mn_major(sY0(j) + kPieceB[x] * kPieceY, 64, k), idesc_acc, x + k > 0);
+                    tc_commit(smem_u32(&st.acc_full));
+                    tc_commit(smem_u32(&st.y_empty[j & 1]));
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) {
+            if (lane == 0) {
+                tc_report(tp.status, 231);
+                tc_commit(smem_u32(&st.drain));
+                tc_drain(smem_u32(&st.drain), 0);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ------------------------------------------------ P and dS
+        const int wg = warp / 4, r = threadIdx.x % 128, col = 32 * wg;    // resident row, first column
+        const uint32_t lanes = (uint32_t)(warp % 4) << 21;
+        const int pos = xpos + r;
+        bool ok = true;
+        if (n > 0) {
+            const int64_t* s = kKeys ? (wg ? p.vs : p.ks) : (wg ? p.dos : p.qs);
+            const float* src = (const float*)(kKeys ? (wg ? p.v : p.k) : (wg ? p.dout : p.q)) + b * s[0] + xh * s[1];
+#pragma unroll 4
+            for (int i = 0; i < DP / 8; ++i) {
+                const int item = i * 128 + r, row = x0 + item / 8, e = item % 8;
+                float4 x[2];
+                tc32_fetch(x, src + (int64_t)row * s[2] + e * 8,
+                           row < xrows && e * 8 < p.D && (!docs || doc_at(p, b, row + (kKeys ? 0 : shift)) >= 0));
+                tc32_put(wg ? sX1 : sX0, 128, kPieceX, item / 8, e, x);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&st.x_full));
+        }
+        const int rdoc = docs ? (x0 + r < xrows ? doc_at(p, b, pos) : -1) : 0;
+        const int common = docs ? (x0 + 128 <= xrows ? common_doc(dt, xpos, 128, p.Lk) : -1) : 0;
+        const float mul = kCap ? p.cap * kLog2e : tp.scale * kLog2e, pre = kCap ? tp.scale / p.cap : 0.f;
+        float lse2 = 0.f, delta = 0.f;
+        if (!kKeys) {
+            const int64_t at = ((int64_t)b * p.H + xh) * tp.Lp + x0 + r;
+            lse2 = tp.lse2[at];
+            delta = tp.delta[at];
+        }
+        // this thread's accumulators: dK (warpgroup 0) or dV (1), or half of dQ
+        constexpr int kAcc = kKeys ? 64 : 32;
+        const uint32_t tAcc = (kKeys ? (wg ? tB : tA) : tA + col) + lanes;
+        float o[kAcc];
+#pragma unroll
+        for (int i = 0; i < kAcc; ++i) o[i] = 0.f;
+        const auto add_up = [&]() {
+#pragma unroll
+            for (int c = 0; c < kAcc; c += 32) {
+                float x[32];
+                tmem_ld_x32(tAcc + c, x);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[c + k] += x[k];
+            }
+        };
+        for (int i = 0; i < n; ++i) {
+            const int h = kKeys ? xh * group + i / tiles : xh;
+            const int y0 = (t0 + (kKeys ? i % tiles : i)) * 64, ypos = y0 + (kKeys ? shift : 0);
+            const float slope = kBias ? __ldg(p.slopes + h) * kLog2e : 0.f;
+            int lo = 0, hi = 64;
+            bool full;
+            if (kKeys) {
+                if (p.causal && pos >= prefix) lo = max(0, pos - ypos);
+                full = !p.causal || ypos >= xpos + 127 || xpos + 128 <= prefix;
+            } else {
+                hi = (!p.causal ? p.Lk : min(p.Lk, max(pos + 1, prefix))) - ypos;
+                full = ypos + 64 <= p.Lk && (!p.causal || ypos + 63 <= xpos || ypos + 64 <= prefix);
+            }
+            if (docs) {
+                if (rdoc < 0) hi = 0;
+                full = full && common >= 0 && (!kKeys || y0 + 64 <= p.Lq) && common_doc(dt, ypos, 64, p.Lk) == common;
+                if (!full) {
+                    __syncwarp();
+                    st.doc[warp][lane] = doc_at(p, b, ypos + col + lane);
+                    __syncwarp();
+                }
+            }
+            ok = __all_sync(~0u, tc_wait(smem_u32(&st.s_full), i & 1, failed) &&
+                                     (!kKeys || tc_wait(smem_u32(&st.y_full[i & 1]), (i >> 1) & 1, failed)));
+            if (!ok) break;
+            tc_fence_after();
+            float v[32], g[32];
+            tmem_ld_x32(tS + lanes + col, v);
+            tmem_ld_x32(tdP + lanes + col, g);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&st.s_free));
+            if (i > 0) {
+                ok = __all_sync(~0u, tc_wait(smem_u32(&st.acc_full), (i - 1) & 1, failed));
+                if (!ok) break;
+                tc_fence_after();
+                add_up();
+            }
+            if (kCap) cap_scores32(v, pre, 1.f);
+            const float far = (float)(pos - ypos - col);
+            uint32_t w[3][16];
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+                float e[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float nl = -(kKeys ? st.lse2[i & 1][col + c + k] : lse2);
+                    if (kBias) nl = fmaf(-slope, fabsf(far - (float)(c + k)), nl);
+                    e[k] = ex2(fmaf(v[c + k], mul, nl));
+                    bool seen = true;
+                    if (!full) {
+                        seen = col + c + k >= lo && col + c + k < hi;
+                        if (docs) seen = seen && st.doc[warp][c + k] == rdoc;
+                        e[k] = seen ? e[k] : 0.f;
+                    }
+                    const float curve = kCap ? fmaf(-v[c + k], v[c + k], 1.f) : 1.f;
+                    const float d = e[k] * curve * (g[c + k] - (kKeys ? st.delta[i & 1][col + c + k] : delta));
+                    g[c + k] = seen ? d : 0.f;
+                }
+                if (kKeys) {
+                    uint32_t pc[3];
+                    split3(e[0], e[1], pc);
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) w[k][c / 2] = pc[k];
+                }
+            }
+            if (kKeys) {
+#pragma unroll
+                for (int k = 0; k < 3; ++k) tmem_st_x16(tP + lanes + 32 * k + col / 2, w[k]);
+            }
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+                uint32_t pc[3];
+                split3(g[c], g[c + 1], pc);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) w[k][c / 2] = pc[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 3; ++k) tmem_st_x16(tdS + lanes + 32 * k + col / 2, w[k]);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&st.p_full));
+        }
+        if (ok && n > 0) {
+            ok = __all_sync(~0u, tc_wait(smem_u32(&st.acc_full), (n - 1) & 1, failed));
+            if (ok) {
+                tc_fence_after();
+                add_up();
+            }
+        }
+        if (ok && x0 + r < xrows) {
+            const bool is_dv = kKeys && wg == 1;
+            const int64_t* os = kKeys ? (is_dv ? p.dvs : p.dks) : p.dqs;
+            float* out = (float*)(kKeys ? (is_dv ? p.dv : p.dk) : p.dq) + b * os[0] + xh * os[1] +
+                         (int64_t)(x0 + r) * os[2] + (kKeys ? 0 : col);
+            const float f = is_dv ? 1.f : p.scale;
+            const int cols = p.D - (kKeys ? 0 : col);
+#pragma unroll
+            for (int c = 0; c < kAcc; c += 4)
+                if (c < cols)
+                    *reinterpret_cast<float4*>(out + c) = make_float4(o[c] * f, o[c + 1] * f, o[c + 2] * f, o[c + 3] * f);
+        }
+        if (!ok && lane == 0) tc_report(tp.status, 232);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 11) tmem_dealloc(st.tmem, 512);
+}
+
+}  // namespace mg

@@ -42,6 +42,23 @@ struct TcBwdParams {
 
 // lse2 and delta of each row, padded with rows whose P is 0. 16 lanes to a row of
 // up to 128 elements, 8 each.
+__device__ __forceinline__ void load8(const __nv_bfloat16* x, float (&v)[8])
+{
+    const uint4 w = *reinterpret_cast<const uint4*>(x);
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 f = __bfloat1622float2(h[k]);
+        v[2 * k] = f.x, v[2 * k + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void load8(const float* x, float (&v)[8])
+{
+    const float4 a = *reinterpret_cast<const float4*>(x), b = *reinterpret_cast<const float4*>(x + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+
+template <typename T>
 __global__ void attn_tc_stats_kernel(const __grid_constant__ AttnParams p, int Lp, float* __restrict__ lse2,
                                      float* __restrict__ delta)
 {
@@ -56,17 +73,11 @@ __global__ void attn_tc_stats_kernel(const __grid_constant__ AttnParams p, int L
         if (lse != -CUDART_INF_F) {
             l = lse * kLog2e;
             if (part * 8 < p.D) {
-                const uint4 o = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.out + b * p.os[0] + h * p.os[1] +
-                                                                (int64_t)i * p.os[2] + part * 8);
-                const uint4 g = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.dout + b * p.dos[0] +
-                                                                h * p.dos[1] + (int64_t)i * p.dos[2] + part * 8);
-                const __nv_bfloat162* ov = reinterpret_cast<const __nv_bfloat162*>(&o);
-                const __nv_bfloat162* gv = reinterpret_cast<const __nv_bfloat162*>(&g);
+                float o[8], g[8];
+                load8((const T*)p.out + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2] + part * 8, o);
+                load8((const T*)p.dout + b * p.dos[0] + h * p.dos[1] + (int64_t)i * p.dos[2] + part * 8, g);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float2 x = __bfloat1622float2(ov[k]), y = __bfloat1622float2(gv[k]);
-                    s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
-                }
+                for (int k = 0; k < 8; ++k) s = fmaf(o[k], g[k], s);
             }
         }
     }
@@ -94,6 +105,36 @@ __device__ __forceinline__ void bulk_load(uint32_t bar, uint32_t dst, const void
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                  "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
+}
+
+// Tiles [t0, t1) of 64 streamed rows that meet the 128 resident rows from x0 (at
+// position xpos) in some pair. All threads; `range` is {INT_MAX, 0} in shared memory.
+template <bool kKeys>
+__device__ __forceinline__ void stream_range(const AttnParams& p, const int32_t* docs, const int2* dt, int prefix,
+                                             int x0, int xpos, int shift, int* range, int& t0, int& t1)
+{
+    t0 = 0;
+    if (kKeys) {
+        if (p.causal && x0 >= prefix) t0 = min(max(0, x0 - shift), p.Lq) / 64;
+        t1 = (p.Lq + 63) / 64;
+    } else {
+        const int last = min(x0 + 127, p.Lq - 1) + shift;
+        t1 = ((!p.causal ? p.Lk : max(0, min(p.Lk, max(last + 1, prefix)))) + 63) / 64;
+    }
+    if (!docs) return;
+    int2 mine = make_int2(INT_MAX, -1);
+    for (int t = max(xpos, 0) >> 7; t * 128 < min(xpos + 128, p.Lk); ++t) {
+        const int2 r = __ldg(dt + t);
+        if (r.y >= 0) mine = make_int2(min(mine.x, max(r.x, 0)), max(mine.y, r.y));
+    }
+    for (int t = t0 + threadIdx.x; t < t1; t += blockDim.x) {
+        if (!docs_meet(dt, t * 64 + (kKeys ? shift : 0), 64, p.Lk, mine)) continue;
+        atomicMin(&range[0], t);
+        atomicMax(&range[1], t + 1);
+    }
+    __syncthreads();
+    t0 = min(range[0], range[1]);
+    t1 = range[1];
 }
 
 template <int DP>
@@ -146,30 +187,8 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    // Tiles [t0, t1) of 64 streamed rows that meet the resident rows in some pair.
-    int t0 = 0, t1;
-    if (kKeys) {
-        if (p.causal && x0 >= prefix) t0 = min(max(0, x0 - shift), p.Lq) / 64;
-        t1 = (p.Lq + 63) / 64;
-    } else {
-        const int last = min(x0 + 127, p.Lq - 1) + shift;
-        t1 = ((!p.causal ? p.Lk : max(0, min(p.Lk, max(last + 1, prefix)))) + 63) / 64;
-    }
-    if (docs) {
-        int2 mine = make_int2(INT_MAX, -1);
-        for (int t = max(xpos, 0) >> 7; t * 128 < min(xpos + 128, p.Lk); ++t) {
-            const int2 r = __ldg(dt + t);
-            if (r.y >= 0) mine = make_int2(min(mine.x, max(r.x, 0)), max(mine.y, r.y));
-        }
-        for (int t = t0 + threadIdx.x; t < t1; t += kTcBwdThreads) {
-            if (!docs_meet(dt, t * 64 + (kKeys ? shift : 0), 64, p.Lk, mine)) continue;
-            atomicMin(&st.range[0], t);
-            atomicMax(&st.range[1], t + 1);
-        }
-        __syncthreads();
-        t0 = min(st.range[0], st.range[1]);
-        t1 = st.range[1];
-    }
+    int t0, t1;
+    stream_range<kKeys>(p, docs, dt, prefix, x0, xpos, shift, st.range, t0, t1);
     const int tiles = max(0, t1 - t0), n = kKeys ? tiles * group : tiles;
     const uint32_t tA = st.tmem + 256, tB = tA + DP;     // accumulators: dS Y0, P Y1
     volatile int* failed = &st.failed;
