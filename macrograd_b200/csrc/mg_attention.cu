@@ -170,6 +170,14 @@ mg_status tc_params(mg::TcAttnParams* t, const mg::AttnParams& p, const Device& 
     t->scale = std::fabs(p.scale);
     t->idesc_s = mg::idesc_bf16(128, 128, false, false, p.scale < 0.f);
     t->status = dev.status;
+    if (p.cap > 0.f) {
+        const double pre = t->scale / p.cap, c[4] = {0.999999463558197, -0.33326318860054016, 0.13190296292304993,
+                                                     -0.04440222308039665};
+        t->curve.pre = (float)pre;
+        t->curve.bound = pre > 1e-5 && pre < 1e4 ? (float)(0.5 / pre) : 0.f;
+        double power = pre;
+        for (int i = 0; i < 4; ++i, power *= pre * pre) t->curve.tc[i] = (float)(c[i] * power);
+    }
     if (p.docs) {
         const int64_t tiles = (int64_t)p.B * ceil_div(p.Lk, 128);
         int2* dt = static_cast<int2*>(ws.get(std::max<int64_t>(1, tiles) * sizeof(int2)));
@@ -242,7 +250,7 @@ mg_status backward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     Scratch ws(dev, stream);
     cudaStream_t st = (cudaStream_t)stream;
     MG_TRY(tc_params(&f, p, dev, ws, st, who));
-    t.a = p, t.doc_tiles = f.doc_tiles, t.scale = f.scale, t.status = f.status;
+    t.a = p, t.doc_tiles = f.doc_tiles, t.scale = f.scale, t.curve = f.curve, t.status = f.status;
     t.idesc_s = mg::idesc_bf16(128, 64, false, false, p.scale < 0.f);
     t.Lp = ceil_div(p.Lq, 128) * 128;
     const int64_t rows = (int64_t)p.B * p.H * t.Lp;

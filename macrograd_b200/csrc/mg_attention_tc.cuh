@@ -68,6 +68,34 @@ __device__ __forceinline__ bool docs_meet(const int2* tiles, int pos, int n, int
     return false;
 }
 
+// The span of the documents of positions [pos, pos + n), by the tiles of 128: {0, -1} if there is none.
+__device__ __forceinline__ int2 docs_of(const int2* tiles, int pos, int n, int Lk)
+{
+    int2 m = make_int2(INT_MAX, -1);
+    const int p1 = min(pos + n, Lk);
+    for (int t = max(pos, 0) >> 7; t * 128 < p1; ++t) {
+        const int2 r = __ldg(tiles + t);
+        if (r.y >= 0) m = make_int2(min(m.x, max(r.x, 0)), max(m.y, r.y));
+    }
+    return m;
+}
+
+// Narrows tiles [t0, t1) of `step` positions (the first at position pos0) to the
+// span of those whose documents meet `want`. Whole warp, the same in every warp.
+__device__ __forceinline__ void narrow_to_docs(const int2* tiles, int Lk, int pos0, int step, int2 want, int& t0, int& t1)
+{
+    const int lane = threadIdx.x % 32;
+    int lo = INT_MAX, hi = 0;
+    for (int t = t0 + lane; t < t1; t += 32)
+        if (docs_meet(tiles, pos0 + t * step, step, Lk, want)) {
+            lo = min(lo, t);
+            hi = t + 1;
+        }
+    lo = __reduce_min_sync(~0u, lo);
+    t1 = __reduce_max_sync(~0u, hi);
+    t0 = min(lo, t1);
+}
+
 // ---------------------------------------------------------------- arithmetic
 __device__ __forceinline__ float ex2(float x)
 {
@@ -80,6 +108,37 @@ __device__ __forceinline__ float rcp(float x)
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// The largest of three, and of three magnitudes (NaN where all are, or is skipped).
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c)
+{
+    float r;
+    asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// The largest of N values (of their magnitudes): four chains, two values a step.
+template <int N, bool kAbs>
+__device__ __forceinline__ float max_of(const float (&s)[N])
+{
+    float t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = kAbs ? fabsf(s[i]) : s[i];
+#pragma unroll
+    for (int i = 4; i + 8 <= N; i += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            t[k] = kAbs ? max3_abs(t[k], s[i + 2 * k], s[i + 2 * k + 1]) : max3(t[k], s[i + 2 * k], s[i + 2 * k + 1]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)      // N is a multiple of 8: four are left
+        t[k] = kAbs ? fmaxf(t[k], fabsf(s[N - 4 + k])) : fmaxf(t[k], s[N - 4 + k]);
+    return fmaxf(max3(t[0], t[1], t[2]), t[3]);
 }
 
 // Two fp32 operations in one instruction.
@@ -143,22 +202,37 @@ __device__ __forceinline__ float tanh_fast(float x)
     return fabsf(x) <= 1.f ? small : tanh_any(x);
 }
 
-// s[i] <- cap2 * tanh(s[i] * pre) for N values. The polynomial serves where no
-// value of the warp leaves [-1, 1] (scores well below the cap, the usual case:
-// 4 issue slots a value instead of 16 of the exponential unit).
+// tanh(x) for |x| <= 1/2 with four terms (fitted as above: 6e-7), from the
+// unscaled score: x = s * pre, tc[k] = pre^(2k + 1) times the coefficient.
+struct CapCurve {
+    float tc[4];
+    float bound;        // |s| up to this: |x| <= 1/2; 0 where a coefficient would leave fp32's range
+    float pre;          // |scale| / cap
+};
+
+// s[i] <- tanh(s[i] * pre). What bounds this is the fp32 pipe: the four-term form
+// is 5 operations a score, where the warp's scores are all below half the cap
+// (the usual case); with scores up to the cap it is 9, and beyond it an
+// exponential and a reciprocal.
 template <int N>
-__device__ __forceinline__ void cap_scores(float (&s)[N], float pre, float cap2)
+__device__ __forceinline__ void cap_scores(float (&s)[N], const CapCurve& cc)
 {
-    float top = 0.f;
+    const float top = max_of<N, true>(s);
+    if (!__any_sync(~0u, !(top <= cc.bound))) {
+        const uint64_t c0 = pack2(cc.tc[0], cc.tc[0]), c1 = pack2(cc.tc[1], cc.tc[1]), c2 = pack2(cc.tc[2], cc.tc[2]),
+                       c3 = pack2(cc.tc[3], cc.tc[3]);
 #pragma unroll
-    for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(s[i]));
-    if (__any_sync(~0u, top * fabsf(pre) > 1.f)) {
+        for (int i = 0; i < N; i += 2) {
+            const uint64_t x = pack2(s[i], s[i + 1]), u = mul2(x, x);
+            unpack2(mul2(x, fma2(u, fma2(u, fma2(u, c3, c2), c1), c0)), s[i], s[i + 1]);
+        }
+    } else if (!__any_sync(~0u, !(top * cc.pre <= 1.f))) {
+        const uint64_t a = pack2(cc.pre, cc.pre);
 #pragma unroll
-        for (int i = 0; i < N; ++i) s[i] = cap2 * tanh_any(s[i] * pre);
+        for (int i = 0; i < N; i += 2) unpack2(tanh_small2(mul2(a, pack2(s[i], s[i + 1]))), s[i], s[i + 1]);
     } else {
-        const uint64_t a = pack2(pre, pre), c = pack2(cap2, cap2);
 #pragma unroll
-        for (int i = 0; i < N; i += 2) unpack2(mul2(c, tanh_small2(mul2(a, pack2(s[i], s[i + 1])))), s[i], s[i + 1]);
+        for (int i = 0; i < N; ++i) s[i] = tanh_any(s[i] * cc.pre);
     }
 }
 
@@ -170,18 +244,17 @@ struct TcAttnParams {
     int head_step[4], batch_step[4];   // of q, k, v, dout: 0 where the dim is broadcast (stride 0)
     uint32_t idesc_s;            // of S = Q K^T: A negated where the scale is negative
     float scale;                 // |scale|
+    CapCurve curve;
     int* status;
 };
 
 struct TcState {
-    uint64_t q_full, k_full, v_full, s_full, p_full, o_full, drain;
+    uint64_t q_full, k_full, v_full, s_full, s_free, p_full[2], o_full, pair[4], drain;
     uint32_t tmem;
     int failed;
-    int range[2];                // tiles of keys that some query of the block sees
-    int qdoc[2];                 // documents of its queries
-    int qpad;
     int loads[2];                // tiles of K and of V that were asked for
-    alignas(16) int kdoc[4][128];    // documents of the keys, a copy a warp (read as int4)
+    float top[2][2][128];        // [tile parity][half][query] maximum of half a row; at the end its sum
+    alignas(16) int kdoc[8][64];     // documents of the keys, a copy a warp (read as int4)
 };
 
 __device__ __forceinline__ void tc_report(int* status, int where)
@@ -221,7 +294,7 @@ __device__ __forceinline__ void tc_clear_padding(uint32_t tile, int rows, const 
     __syncwarp();
 }
 
-constexpr int kTcFwdThreads = 192;
+constexpr int kTcFwdThreads = 320;       // eight warps of exponentials, loads, products
 
 template <int DP>
 constexpr size_t tc_forward_smem() { return 3 * 128 * DP * 2 + 1024; }
@@ -234,7 +307,7 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
     const AttnParams& p = tp.a;
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
     const uint32_t sQ = base, sK = base + 128 * DP * 2, sV = sK + 128 * DP * 2;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;   // uniform: so are the roles
 
     // blocks with the most keys first
     const int heads = p.B * p.H, qtiles = (p.Lq + 127) / 128;
@@ -250,56 +323,37 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
         mbar_init(smem_u32(&st.k_full), 1);
         mbar_init(smem_u32(&st.v_full), 1);
         mbar_init(smem_u32(&st.s_full), 1);
-        mbar_init(smem_u32(&st.p_full), 4);
+        mbar_init(smem_u32(&st.s_free), 8);
+        mbar_init(smem_u32(&st.p_full[0]), 8);
+        mbar_init(smem_u32(&st.p_full[1]), 4);
         mbar_init(smem_u32(&st.o_full), 1);
+        for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&st.pair[i]), 2);
         mbar_init(smem_u32(&st.drain), 1);
         mbar_fence_init();
         st.failed = 0;
-        st.range[0] = INT_MAX;
-        st.range[1] = 0;
-        st.qdoc[0] = INT_MAX;
-        st.qdoc[1] = -1;
-        st.qpad = 0;
         st.loads[0] = st.loads[1] = 0;
     }
-    if (warp == 5) {
+    if (warp == 9) {
         tmem_alloc(smem_u32(&st.tmem), 256);
         tmem_relinquish();
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
     // Tiles [t0, t1) hold every key that a query of this block sees.
     const int kend = !p.causal ? p.Lk : max(0, min(p.Lk, max(qlast + 1, prefix)));
     int t0 = 0, t1 = (kend + 127) / 128;
-    if (docs) {
-        for (int i = threadIdx.x; i < 128; i += kTcFwdThreads) {
-            if (q0 + i >= p.Lq) continue;
-            const int d = doc_at(p, b, q0 + i + shift);
-            if (d >= 0) {
-                atomicMin(&st.qdoc[0], d);
-                atomicMax(&st.qdoc[1], d);
-            } else {
-                st.qpad = 1;
-            }
-        }
-        __syncthreads();
-        for (int t = threadIdx.x; t < t1; t += kTcFwdThreads) {
-            const int2 r = __ldg(tp.doc_tiles + (int64_t)b * ((p.Lk + 127) / 128) + t);
-            if (r.x <= st.qdoc[1] && r.y >= st.qdoc[0]) {
-                atomicMin(&st.range[0], t);
-                atomicMax(&st.range[1], t + 1);
-            }
-        }
-        __syncthreads();
-        t0 = min(st.range[0], st.range[1]);
-        t1 = st.range[1];
-    }
+    const int2* dt = docs ? tp.doc_tiles + (int64_t)b * ((p.Lk + 127) / 128) : nullptr;
+    if (docs) narrow_to_docs(dt, p.Lk, 0, 128, docs_of(dt, q0 + shift, 128, p.Lk), t0, t1);
     const int n = max(0, t1 - t0);
-    const uint32_t tS = st.tmem, tO = st.tmem + 128;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // Scores in columns 0-127. With heads of up to 64 there is room for P beside
+    // them, and the next scores are computed while this tile's exponentials are
+    // taken; with longer heads P lies over the scores.
+    constexpr bool kBeside = DP == 64;
+    const uint32_t tS = st.tmem, tP = tS + (kBeside ? 128 : 0), tO = tS + (kBeside ? 192 : 128);
     volatile int* failed = &st.failed;
 
-    if (warp == 4) {
+    if (warp == 8) {
         // ------------------------------------------------ loads
         if (lane == 0 && n > 0) {
             const int hk = kv * tp.head_step[1], bk = b * tp.batch_step[1];
@@ -314,94 +368,104 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
                 st.loads[1] = j + 1;
             }
         }
-    } else if (warp == 5) {
+    } else if (warp == 9) {
         // ------------------------------------------------ products
         constexpr uint32_t idesc_o = idesc_bf16(128, DP, false, true);
-        bool ok = n == 0 || tc_wait(smem_u32(&st.q_full), 0, failed);
-        for (int j = 0; j <= n && n > 0; ++j) {
-            if (j > 0) {      // O += P(j-1) V(j-1)
-                ok = ok && tc_wait(smem_u32(&st.v_full), (j - 1) & 1, failed);
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
-                if (docs && __ldg(&tp.doc_tiles[(int64_t)b * ((p.Lk + 127) / 128) + t0 + j - 1]).x < 0)
-                    tc_clear_padding<DP>(sV, 128, docs, (t0 + j - 1) * 128, p.Lk, lane);
-                ok = __all_sync(~0u, tc_wait(smem_u32(&st.p_full), (j - 1) & 1, failed));
-                if (!ok) break;
-                tc_fence_after();
-                if (lane == 0) {
+        bool ok = n == 0 || __all_sync(~0u, tc_wait(smem_u32(&st.q_full), 0, failed));
+        const auto scores_of = [&](int j) {       // S = Q K(j)^T
+            ok = ok && tc_wait(smem_u32(&st.k_full), j & 1, failed) &&
+                 (!kBeside || j == 0 || tc_wait(smem_u32(&st.s_free), (j - 1) & 1, failed));
+            ok = __all_sync(~0u, ok);
+            if (!ok) return;
+            tc_fence_after();
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        tc_mma_f16_ta(tO, tS + 8 * k, desc_mn_major(sV, 128, k), idesc_o, j > 1 || k > 0);
-                    tc_commit(smem_u32(&st.o_full));
-                }
-                __syncwarp();
-            }
-            if (j < n) {      // S = Q K(j)^T
-                ok = __all_sync(~0u, ok && tc_wait(smem_u32(&st.k_full), j & 1, failed));
-                if (!ok) break;
-                tc_fence_after();
-                if (lane == 0) {
+            for (int k = 0; k < DP / 16; ++k)
+                tc_mma_f16(tS, desc_k_major(sQ, 128, k), desc_k_major(sK, 128, k), tp.idesc_s, k > 0);
+            tc_commit_warp(smem_u32(&st.s_full));
+        };
+        const auto output_of = [&](int j) {       // O += P V(j), half of the keys at a time
+            ok = __all_sync(~0u, ok && tc_wait(smem_u32(&st.v_full), j & 1, failed));
+            if (!ok) return;
+            if (docs && __ldg(&dt[t0 + j]).x < 0) tc_clear_padding<DP>(sV, 128, docs, (t0 + j) * 128, p.Lk, lane);
 #pragma unroll
-                    for (int k = 0; k < DP / 16; ++k)
-                        tc_mma_f16(tS, desc_k_major(sQ, 128, k), desc_k_major(sK, 128, k), tp.idesc_s, k > 0);
-                    tc_commit(smem_u32(&st.s_full));
-                }
-                __syncwarp();
+            for (int half = 0; half < 2; ++half) {
+                ok = __all_sync(~0u, ok && tc_wait(smem_u32(&st.p_full[half]), j & 1, failed));
+                if (!ok) return;
+                tc_fence_after();
+#pragma unroll
+                for (int k = 4 * half; k < 4 * half + 4; ++k)
+                    tc_mma_f16_ta(tO, tP + 8 * k, desc_mn_major(sV, 128, k), idesc_o, j > 0 || k > 0);
+                if (half) tc_commit_warp(smem_u32(&st.o_full));
             }
+        };
+        for (int j = 0; j <= n && n > 0 && ok; ++j) {
+            if (kBeside && j < n) scores_of(j);
+            if (ok && j > 0) output_of(j - 1);
+            if (!kBeside && ok && j < n) scores_of(j);
         }
         if (!ok) {
+            __syncwarp();
+            tc_commit_warp(smem_u32(&st.drain));
             if (lane == 0) {
                 tc_report(tp.status, 201);
-                tc_commit(smem_u32(&st.drain));
                 tc_drain(smem_u32(&st.drain), 0);
             }
             __syncwarp();
         }
     } else {
         // ------------------------------------------------ softmax
-        const int row = q0 + threadIdx.x, qpos = row + shift;
-        const uint32_t lanes = (uint32_t)warp << 21;      // this warp's 32 lanes of tensor memory
+        // Warps w and w + 4 have the same 32 queries, each half of the keys.
+        const int half = warp / 4, r = threadIdx.x % 128, row = q0 + r, qpos = row + shift;
+        const uint32_t lanes = (uint32_t)(warp % 4) << 21;      // this warp's 32 lanes of tensor memory
+        const uint32_t pair = smem_u32(&st.pair[warp % 4]);     // where the two warps meet
         const int qdoc = docs ? doc_at(p, b, qpos) : 0;
-        const bool one_doc = !docs || (st.qdoc[0] == st.qdoc[1] && !st.qpad && q0 + 127 < p.Lq);
+        const int common = docs ? (q0 + 128 <= p.Lq ? common_doc(dt, q0 + shift, 128, p.Lk) : -1) : 0;
         // keys before `upto` are seen as far as causal and prefix go
         const int upto = qdoc < 0 ? 0 : !p.causal ? p.Lk : min(p.Lk, max(qpos + 1, prefix));
         // scores are kept in units whose multiple by `mul` is the power of two
-        const float mul = kCap ? 1.f : tp.scale * kLog2e;
-        const float slope = kBias ? __ldg(p.slopes + h) * (kCap ? kLog2e : 1.f / tp.scale) : 0.f;
-        float m = -CUDART_INF_F;     // maximum in use, in units of the raw values; base2 = m * mul
-        uint64_t sum2 = pack2(0.f, 0.f);
+        const float mul = kCap ? p.cap * kLog2e : tp.scale * kLog2e;
+        const float slope = kBias ? __ldg(p.slopes + h) / (kCap ? p.cap : tp.scale) : 0.f;
+        float m = -CUDART_INF_F;     // maximum in use; the power of two is m * mul
+        uint64_t sum[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = pack2(0.f, 0.f);
         bool ok = true;
         for (int j = 0; j < n; ++j) {
-            const int k0 = (t0 + j) * 128;
-            // whether any of the tile's pairs is masked (same for all threads)
-            bool full = k0 + 128 <= p.Lk && (!p.causal || k0 + 127 <= q0 + shift || k0 + 128 <= prefix);
+            const int k0 = (t0 + j) * 128 + 64 * half;
+            // whether any of the half tile's pairs is masked (same for all threads of the half)
+            bool full = k0 + 64 <= p.Lk && (!p.causal || k0 + 63 <= q0 + shift || k0 + 64 <= prefix);
             if (docs) {
-                const int2 r = __ldg(tp.doc_tiles + (int64_t)b * ((p.Lk + 127) / 128) + t0 + j);
-                full = full && one_doc && r.x == r.y && r.x == st.qdoc[0];
+                const int2 d = __ldg(dt + t0 + j);
+                full = full && common >= 0 && d.x == d.y && d.x == common;
                 if (!full) {
                     __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 128; i += 32) st.kdoc[warp][i + lane] = doc_at(p, b, k0 + i + lane);
+                    st.kdoc[warp][lane] = doc_at(p, b, k0 + lane);
+                    st.kdoc[warp][lane + 32] = doc_at(p, b, k0 + 32 + lane);
                     __syncwarp();
                 }
             }
             ok = __all_sync(~0u, tc_wait(smem_u32(&st.s_full), j & 1, failed));
             if (!ok) break;
             tc_fence_after();
-            float s[128];
-            tmem_ld_x128(tS + lanes, s);
-            if (kCap) cap_scores(s, tp.scale / p.cap, p.cap * kLog2e);
+            float s[64];
+            tmem_ld_x64(tS + lanes + 64 * half, s);
+            if (kBeside) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&st.s_free));
+            }
+            if (kCap) cap_scores(s, tp.curve);
             if (kBias) {
                 const float far = (float)(qpos - k0);
 #pragma unroll
-                for (int c = 0; c < 128; ++c) s[c] = fmaf(-slope, fabsf(far - (float)c), s[c]);
+                for (int c = 0; c < 64; ++c) s[c] = fmaf(-slope, fabsf(far - (float)c), s[c]);
             }
             if (!full) {
                 const int lim = upto - k0;
                 if (docs) {
                     const int4* kd = reinterpret_cast<const int4*>(st.kdoc[warp]);
 #pragma unroll
-                    for (int c = 0; c < 128; c += 4) {
+                    for (int c = 0; c < 64; c += 4) {
                         const int4 d = kd[c / 4];
                         s[c] = c < lim && d.x == qdoc ? s[c] : -CUDART_INF_F;
                         s[c + 1] = c + 1 < lim && d.y == qdoc ? s[c + 1] : -CUDART_INF_F;
@@ -410,67 +474,82 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
                     }
                 } else {
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) s[c] = c < lim ? s[c] : -CUDART_INF_F;
+                    for (int c = 0; c < 64; ++c) s[c] = c < lim ? s[c] : -CUDART_INF_F;
                 }
             }
-            float top = fmaxf(s[0], s[1]);
-#pragma unroll
-            for (int c = 2; c < 128; c += 2) top = fmaxf(top, fmaxf(s[c], s[c + 1]));
+            // the row's maximum; past this barrier both halves have their scores in registers
+            const float mine = max_of<64, false>(s);
+            st.top[j & 1][half][r] = mine;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pair);
+            ok = __all_sync(~0u, (j == 0 || tc_wait(smem_u32(&st.o_full), (j - 1) & 1, failed)) &&
+                                     tc_wait(pair, j & 1, failed));
+            if (!ok) break;
+            const float top = fmaxf(mine, st.top[j & 1][half ^ 1][r]);
             // rescale O and the sum where the maximum has outgrown the one in use
             const bool grown = m == -CUDART_INF_F ? top > m : (top - m) * mul > 8.f;
-            if (j > 0) {
-                ok = __all_sync(~0u, tc_wait(smem_u32(&st.o_full), (j - 1) & 1, failed));
-                if (!ok) break;
-            }
             if (__any_sync(~0u, grown)) {
                 const float mn = grown ? top : m;
                 if (j > 0) {
                     tc_fence_after();
                     const float f = m == -CUDART_INF_F ? 0.f : ex2((m - mn) * mul);
 #pragma unroll 1
-                    for (int c = 0; c < DP; c += 32) {
-                        float o[32];
-                        uint32_t w[32];
-                        tmem_ld_x32(tO + lanes + c, o);
+                    for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 16) {
+                        float o[16];
+                        uint32_t w[16];
+                        tmem_ld_x16(tO + lanes + c, o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * f);
-                        tmem_st_x32(tO + lanes + c, w);
+                        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * f);
+                        tmem_st_x16(tO + lanes + c, w);
                     }
-                    sum2 = mul2(sum2, pack2(f, f));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] = mul2(sum[i], pack2(f, f));
+                    tmem_wait_st();
                 }
                 m = mn;
+            }
+            if (half) {              // O may be added to as far as this half goes
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&st.p_full[0]));
             }
             const float base2 = m == -CUDART_INF_F ? 0.f : m * mul;
             const uint64_t mul_2 = pack2(mul, mul), base_2 = pack2(-base2, -base2);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t w[32];
+            for (int c = 0; c < 64; c += 32) {
+                uint32_t w[16];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
+                for (int i = 0; i < 16; ++i) {
                     float x, y;
-                    unpack2(fma2(pack2(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]), mul_2, base_2), x, y);
+                    unpack2(fma2(pack2(s[c + 2 * i], s[c + 2 * i + 1]), mul_2, base_2), x, y);
                     x = ex2(x);
                     y = ex2(y);
-                    sum2 = add2(sum2, pack2(x, y));
+                    sum[i % 4] = add2(sum[i % 4], pack2(x, y));
                     w[i] = bf16x2(x, y);
                 }
-                tmem_st_x32(tS + lanes + 32 * half, w);
+                tmem_st_x16(tP + lanes + 32 * half + c / 2, w);
             }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&st.p_full));
+            if (lane == 0) mbar_arrive(smem_u32(&st.p_full[half]));
         }
-        if (ok && n > 0) ok = __all_sync(~0u, tc_wait(smem_u32(&st.o_full), (n - 1) & 1, failed));
+        float l, lb;
+        unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l, lb);
+        st.top[n & 1][half][r] = l + lb;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pair);
+        ok = ok && (n == 0 || tc_wait(smem_u32(&st.o_full), (n - 1) & 1, failed)) && tc_wait(pair, n & 1, failed);
+        ok = __all_sync(~0u, ok);
         if (ok) {
             tc_fence_after();
-            float la, lb;
-            unpack2(sum2, la, lb);
-            const float l = la + lb, inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+            l = st.top[n & 1][0][r] + st.top[n & 1][1][r];
+            const float inv = l > 0.f ? 1.f / l : l;       // 0: no key; NaN stays
             const bool store = row < p.Lq;
             __nv_bfloat16* out = (__nv_bfloat16*)p.out + b * p.os[0] + h * p.os[1] + (int64_t)row * p.os[2];
+            const int c1 = min(p.D, (half + 1) * (DP / 2));
 #pragma unroll 1
-            for (int c = 0; c < p.D; c += 32) {
+            for (int c = half * (DP / 2); c < c1; c += 32) {
                 float o[32];
                 if (n > 0) {
                     tmem_ld_x32(tO + lanes + c, o);
@@ -479,16 +558,14 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
                     for (int i = 0; i < 32; ++i) o[i] = 0.f;
                 }
                 if (!store) continue;
-                const int left = p.D - c;
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    const uint4 w = make_uint4(bf16x2(o[i] * inv, o[i + 1] * inv), bf16x2(o[i + 2] * inv, o[i + 3] * inv),
-                                               bf16x2(o[i + 4] * inv, o[i + 5] * inv),
-                                               bf16x2(o[i + 6] * inv, o[i + 7] * inv));
-                    if (i + 8 <= left) *reinterpret_cast<uint4*>(out + c + i) = w;
-                }
+                for (int i = 0; i < 32; i += 8)
+                    if (c + i + 8 <= c1)
+                        *reinterpret_cast<uint4*>(out + c + i) =
+                            make_uint4(bf16x2(o[i] * inv, o[i + 1] * inv), bf16x2(o[i + 2] * inv, o[i + 3] * inv),
+                                       bf16x2(o[i + 4] * inv, o[i + 5] * inv), bf16x2(o[i + 6] * inv, o[i + 7] * inv));
             }
-            if (store)
+            if (store && half == 0)
                 p.lse[((int64_t)b * p.H + h) * p.Lq + row] =
                     l == 0.f ? -CUDART_INF_F : ((m == -CUDART_INF_F ? 0.f : m * mul) + log2f(l)) * kLn2;
         }
@@ -502,7 +579,7 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
         if (st.loads[0]) tc_drain(smem_u32(&st.k_full), (st.loads[0] - 1) & 1);
         if (st.loads[1]) tc_drain(smem_u32(&st.v_full), (st.loads[1] - 1) & 1);
     }
-    if (warp == 5) tmem_dealloc(st.tmem, 256);
+    if (warp == 9) tmem_dealloc(st.tmem, 256);
 }
 
 }  // namespace mg

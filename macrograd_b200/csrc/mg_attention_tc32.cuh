@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(DP == 64 ? 384 : 256, 1) attn_tc32_forward(con
     const AttnParams& p = tp.a;
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
     const uint32_t sQ = base, sKV = base + NQ * 3 * kPieceQ;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;   // uniform: so are the roles
     constexpr int kLoadWarp = NQ * 4, kMmaWarp = NQ * 4 + kTc32LoadWarps;
 
     const int heads = p.B * p.H, blocks = (p.Lq + NQ * 128 - 1) / (NQ * 128);
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(DP == 64 ? 384 : 256, 1) attn_tc32_forward(con
             ok = __all_sync(~0u, ok);
             if (!ok) return;
             tc_fence_after();
-            if (lane == 0) {
+            {
                 const uint32_t q = sQ + t * 3 * kPieceQ;
 #pragma unroll
                 for (int x = 0; x < 6; ++x)
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(DP == 64 ? 384 : 256, 1) attn_tc32_forward(con
                     for (int k = 0; k < DP / 16; ++k)
                         tc_mma_f16(st.tmem + t * 256, desc_k_major(q + kPieceA[x] * kPieceQ, 128, k),
                                    desc_k_major(sK(j) + kPieceB[x] * kPieceK, 64, k), tp.idesc_s, x + k > 0);
-                tc_commit(smem_u32(&st.s_full[t]));
+                tc_commit_warp(smem_u32(&st.s_full[t]));
             }
             __syncwarp();
         };
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(DP == 64 ? 384 : 256, 1) attn_tc32_forward(con
             ok = __all_sync(~0u, ok && tc_wait(smem_u32(&st.p_full[t]), (j - first) & 1, failed));
             if (!ok) return;
             tc_fence_after();
-            if (lane == 0) {
+            {
                 const uint32_t tP = st.tmem + t * 256 + 64;
 #pragma unroll
                 for (int x = 0; x < 6; ++x)
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(DP == 64 ? 384 : 256, 1) attn_tc32_forward(con
                     for (int k = 0; k < 4; ++k)
                         tc_mma_f16_ta(tP + 96, tP + kPieceA[x] * 32 + 8 * k,
                                       desc_mn_major(sV(j) + kPieceB[x] * kPieceK, 64, k), idesc_o, x + k > 0);
-                tc_commit(smem_u32(&st.o_full[t]));
+                tc_commit_warp(smem_u32(&st.o_full[t]));
             }
             __syncwarp();
         };
@@ -288,14 +288,15 @@ __global__ void __launch_bounds__(DP == 64 ? 384 : 256, 1) attn_tc32_forward(con
                 if (kStages > 1 && j < n) scores_of(t, j);
                 if (ok && j > 0) output_of(t, j - 1);
             }
-            if (ok && j > 0 && lane == 0) tc_commit(smem_u32(&st.kv_empty[(j - 1) % kStages]));
+            if (ok && j > 0) tc_commit_warp(smem_u32(&st.kv_empty[(j - 1) % kStages]));
             __syncwarp();
             if (kStages == 1 && ok && j < n) scores_of(0, j);
         }
         if (!ok) {
+            __syncwarp();
+            tc_commit_warp(smem_u32(&st.drain));
             if (lane == 0) {
                 tc_report(tp.status, 221);
-                tc_commit(smem_u32(&st.drain));
                 tc_drain(smem_u32(&st.drain), 0);
             }
             __syncwarp();

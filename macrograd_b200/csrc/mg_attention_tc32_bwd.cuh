@@ -30,7 +30,6 @@ struct Tc32BwdState {
     uint64_t x_full, y_full[2], y_empty[2], s_full, s_free, p_full, acc_full, drain;
     uint32_t tmem;
     int failed;
-    int range[2];
     alignas(16) int doc[8][32];
     alignas(16) float lse2[2][64];
     alignas(16) float delta[2][64];
@@ -49,7 +48,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
     const AttnParams& p = tp.a;
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
     const uint32_t sX0 = base, sX1 = base + 3 * kPieceX, sY = base + 6 * kPieceX;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;   // uniform: so are the roles
 
     const int nhead = kKeys ? p.Hkv : p.H, xrows = kKeys ? p.Lk : p.Lq, yrows = kKeys ? p.Lq : p.Lk;
     const int xtiles = (xrows + 127) / 128, bh = blockIdx.x % (p.B * nhead), rank = blockIdx.x / (p.B * nhead);
@@ -74,18 +73,16 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
         mbar_init(smem_u32(&st.drain), 1);
         mbar_fence_init();
         st.failed = 0;
-        st.range[0] = INT_MAX;
-        st.range[1] = 0;
     }
     if (warp == 11) {
         tmem_alloc(smem_u32(&st.tmem), 512);
         tmem_relinquish();
     }
+    int t0, t1;
+    stream_range<kKeys>(p, docs, dt, prefix, x0, xpos, shift, t0, t1);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    int t0, t1;
-    stream_range<kKeys>(p, docs, dt, prefix, x0, xpos, shift, st.range, t0, t1);
     const int tiles = max(0, t1 - t0), n = kKeys ? tiles * group : tiles;
     const uint32_t tm = st.tmem, tS = tm, tdP = tm + 64, tP = tm + 128, tdS = tm + 224, tA = tm + 320, tB = tm + 384;
     volatile int* failed = &st.failed;
@@ -144,7 +141,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                 ok = __all_sync(~0u, ok);
                 if (!ok) break;
                 tc_fence_after();
-                if (lane == 0) {
+                {
 #pragma unroll
                     for (int x = 0; x < 6; ++x)
 #pragma unroll
@@ -157,7 +154,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                         for (int k = 0; k < DP / 16; ++k)
                             tc_mma_f16(tdP, desc_k_major(sX1 + kPieceA[x] * kPieceX, 128, k),
                                        desc_k_major(sY0(i) + (3 + kPieceB[x]) * kPieceY, 64, k), idesc_dp, x + k > 0);
-                    tc_commit(smem_u32(&st.s_full));
+                    tc_commit_warp(smem_u32(&st.s_full));
                 }
                 __syncwarp();
             }
@@ -166,7 +163,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                 ok = __all_sync(~0u, tc_wait(smem_u32(&st.p_full), j & 1, failed));
                 if (!ok) break;
                 tc_fence_after();
-                if (lane == 0) {
+                {
                     if (kKeys) {
 #pragma unroll
                         for (int x = 0; x < 6; ++x)
@@ -182,16 +179,17 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                         for (int k = 0; k < 4; ++k)
                             tc_mma_f16_ta(tA, tdS + kPieceA[x] * 32 + 8 * k,
                                           desc_mn_major(sY0(j) + kPieceB[x] * kPieceY, 64, k), idesc_acc, x + k > 0);
-                    tc_commit(smem_u32(&st.acc_full));
-                    tc_commit(smem_u32(&st.y_empty[j & 1]));
+                    tc_commit_warp(smem_u32(&st.acc_full));
+                    tc_commit_warp(smem_u32(&st.y_empty[j & 1]));
                 }
                 __syncwarp();
             }
         }
         if (!ok) {
+            __syncwarp();
+            tc_commit_warp(smem_u32(&st.drain));
             if (lane == 0) {
                 tc_report(tp.status, 231);
-                tc_commit(smem_u32(&st.drain));
                 tc_drain(smem_u32(&st.drain), 0);
             }
             __syncwarp();

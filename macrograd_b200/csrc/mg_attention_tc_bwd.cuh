@@ -37,6 +37,7 @@ struct TcBwdParams {
     int head_step[4], batch_step[4];     // of q, k, v, dout
     uint32_t idesc_s;
     float scale;                         // |scale|
+    CapCurve curve;
     int* status;
 };
 
@@ -93,7 +94,6 @@ struct TcBwdState {
     uint64_t x_full, y_full[kTcBwdStages], y_empty[kTcBwdStages], s_full[2], p_full[2], acc_full, drain;
     uint32_t tmem;
     int failed;
-    int range[2];
     int loads;                           // stages that were asked for
     alignas(16) int doc[8][64];          // documents of the streamed rows, a copy a warp
     alignas(16) float lse2[kTcBwdStages][64];
@@ -108,10 +108,10 @@ __device__ __forceinline__ void bulk_load(uint32_t bar, uint32_t dst, const void
 }
 
 // Tiles [t0, t1) of 64 streamed rows that meet the 128 resident rows from x0 (at
-// position xpos) in some pair. All threads; `range` is {INT_MAX, 0} in shared memory.
+// position xpos) in some pair. Whole warps.
 template <bool kKeys>
 __device__ __forceinline__ void stream_range(const AttnParams& p, const int32_t* docs, const int2* dt, int prefix,
-                                             int x0, int xpos, int shift, int* range, int& t0, int& t1)
+                                             int x0, int xpos, int shift, int& t0, int& t1)
 {
     t0 = 0;
     if (kKeys) {
@@ -121,20 +121,7 @@ __device__ __forceinline__ void stream_range(const AttnParams& p, const int32_t*
         const int last = min(x0 + 127, p.Lq - 1) + shift;
         t1 = ((!p.causal ? p.Lk : max(0, min(p.Lk, max(last + 1, prefix)))) + 63) / 64;
     }
-    if (!docs) return;
-    int2 mine = make_int2(INT_MAX, -1);
-    for (int t = max(xpos, 0) >> 7; t * 128 < min(xpos + 128, p.Lk); ++t) {
-        const int2 r = __ldg(dt + t);
-        if (r.y >= 0) mine = make_int2(min(mine.x, max(r.x, 0)), max(mine.y, r.y));
-    }
-    for (int t = t0 + threadIdx.x; t < t1; t += blockDim.x) {
-        if (!docs_meet(dt, t * 64 + (kKeys ? shift : 0), 64, p.Lk, mine)) continue;
-        atomicMin(&range[0], t);
-        atomicMax(&range[1], t + 1);
-    }
-    __syncthreads();
-    t0 = min(range[0], range[1]);
-    t1 = range[1];
+    if (docs) narrow_to_docs(dt, p.Lk, kKeys ? shift : 0, 64, docs_of(dt, xpos, 128, p.Lk), t0, t1);
 }
 
 template <int DP>
@@ -149,7 +136,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
     constexpr uint32_t kX = 128 * DP * 2, kY = 64 * DP * 2;
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
     const uint32_t sX0 = base, sX1 = base + kX, sY = base + 2 * kX;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;   // uniform: so are the roles
 
     // blocks with the most tiles first: the first keys, the last queries
     const int nhead = kKeys ? p.Hkv : p.H, xrows = kKeys ? p.Lk : p.Lq, yrows = kKeys ? p.Lq : p.Lk;
@@ -177,18 +164,16 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
         mbar_fence_init();
         st.failed = 0;
         st.loads = 0;
-        st.range[0] = INT_MAX;
-        st.range[1] = 0;
     }
     if (warp == 9) {
         tmem_alloc(smem_u32(&st.tmem), 512);
         tmem_relinquish();
     }
+    int t0, t1;
+    stream_range<kKeys>(p, docs, dt, prefix, x0, xpos, shift, t0, t1);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    int t0, t1;
-    stream_range<kKeys>(p, docs, dt, prefix, x0, xpos, shift, st.range, t0, t1);
     const int tiles = max(0, t1 - t0), n = kKeys ? tiles * group : tiles;
     const uint32_t tA = st.tmem + 256, tB = tA + DP;     // accumulators: dS Y0, P Y1
     volatile int* failed = &st.failed;
@@ -245,7 +230,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                     }
                 }
                 tc_fence_after();
-                if (lane == 0) {
+                {
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k)
                         tc_mma_f16(tS(i), desc_k_major(sX0, 128, k), desc_k_major(sY0(i), 64, k), tp.idesc_s, k > 0);
@@ -253,7 +238,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                     for (int k = 0; k < DP / 16; ++k)
                         tc_mma_f16(tS(i) + 64, desc_k_major(sX1, 128, k), desc_k_major(sY0(i) + kY, 64, k), idesc_dp,
                                    k > 0);
-                    tc_commit(smem_u32(&st.s_full[i & 1]));
+                    tc_commit_warp(smem_u32(&st.s_full[i & 1]));
                 }
                 __syncwarp();
             }
@@ -262,7 +247,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                 ok = __all_sync(~0u, tc_wait(smem_u32(&st.p_full[j & 1]), (j >> 1) & 1, failed));
                 if (!ok) break;
                 tc_fence_after();
-                if (lane == 0) {
+                {
                     if (kKeys) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
@@ -272,16 +257,17 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         tc_mma_f16_ta(tA, tS(j) + 64 + 8 * k, desc_mn_major(sY0(j), 64, k), idesc_acc, j > 0 || k > 0);
-                    tc_commit(smem_u32(&st.y_empty[j % kTcBwdStages]));
-                    if (i == n) tc_commit(smem_u32(&st.acc_full));
+                    tc_commit_warp(smem_u32(&st.y_empty[j % kTcBwdStages]));
+                    if (i == n) tc_commit_warp(smem_u32(&st.acc_full));
                 }
                 __syncwarp();
             }
         }
         if (!ok) {
+            __syncwarp();
+            tc_commit_warp(smem_u32(&st.drain));
             if (lane == 0) {
                 tc_report(tp.status, 211);
-                tc_commit(smem_u32(&st.drain));
                 tc_drain(smem_u32(&st.drain), 0);
             }
             __syncwarp();
@@ -332,7 +318,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             tc_fence_after();
             float v[64];
             tmem_ld_x64(tS(i) + lanes, v);
-            if (kCap) cap_scores(v, tp.scale / p.cap, 1.f);      // tanh of the score over the cap
+            if (kCap) cap_scores(v, tp.curve);      // tanh of the score over the cap
             uint32_t w[32];
             const float far = (float)(pos - ypos);
 #pragma unroll

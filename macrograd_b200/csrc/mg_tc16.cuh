@@ -15,13 +15,21 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool a_mn, bool 
            ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
+// Issue of products and commits: by the whole warp, of which elect.sync picks one
+// lane (always the same for a whole warp). The compiler then knows that one lane
+// issues; with a predicate of its own (lane == 0) it has to provide for several
+// and an instruction takes 66 (operands in shared memory) to 82 clocks (A in
+// tensor memory) to issue, whatever its size. Measured with elect.sync: 68 clocks for
+// M = N = 128, K = 16 (64 at the nominal rate), for N = 64 52 (both operands from
+// shared memory, whose bandwidth that is) and 36 (A in tensor memory).
 // D[tmem] (+)= A[smem] * B[smem]
 __device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
@@ -30,10 +38,34 @@ __device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t a, uint64_t b, u
 __device__ __forceinline__ void tc_mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Arrives once on `bar` when the products that the warp has issued are complete.
+__device__ __forceinline__ void tc_commit_warp(uint32_t bar)
+{
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+        : "memory");
+}
+
+// Thread i of the warp receives lane base + i, columns [col, col + 16); the wait is part of the statement.
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, float (&r)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(taddr)
         : "memory");
 }
 
@@ -169,12 +201,6 @@ __device__ __forceinline__ uint64_t desc_k_major(uint32_t tile, int rows, int k)
 __device__ __forceinline__ uint64_t desc_mn_major(uint32_t tile, int rows, int k)
 {
     return smem_desc(tile + (uint32_t)k * 2048u, (uint32_t)rows * 128u, 1024u, kLayoutSw128);
-}
-
-// Barriers 1..15 of bar.sync: a meeting of some of the block's warps.
-__device__ __forceinline__ void named_sync(int id, int threads)
-{
-    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 // Bounded wait: false if the phase did not complete within kTcWaitLimitNs, or
