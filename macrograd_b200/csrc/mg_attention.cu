@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 
@@ -32,6 +33,18 @@ mg_status launched(const char* what)
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return fail(MG_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
     mg::host::count_launch();
+    return MG_OK;
+}
+
+// Opts kernel K in to `smem` bytes of dynamic shared memory, once on each device.
+template <auto K>
+mg_status allow_smem(const Device& dev, size_t smem)
+{
+    static std::atomic<uint64_t> done{0};     // a bit a device; the library serves 64
+    const uint64_t bit = 1ull << dev.ordinal;
+    if (done.load(std::memory_order_acquire) & bit) return MG_OK;
+    MG_HOST_TRY(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    done.fetch_or(bit, std::memory_order_release);
     return MG_OK;
 }
 
@@ -163,6 +176,20 @@ mg_status tc_map(CUtensorMap* map, int* head_step, int* batch_step, const void* 
     return mg::host::encode_bf16(map, base, 4, dims, st, box);
 }
 
+// The terms of the capped score's curve for products of magnitude |scale| (see mg::CapCurve).
+mg::CapCurve cap_curve(float scale, float cap)
+{
+    mg::CapCurve cc = {};
+    if (!(cap > 0.f)) return cc;
+    const double pre = (double)scale / cap, c[4] = {0.999999463558197, -0.33326318860054016, 0.13190296292304993,
+                                                    -0.04440222308039665};
+    cc.pre = (float)pre;
+    cc.bound = pre > 1e-5 && pre < 1e4 ? (float)(0.5 / pre) : 0.f;
+    double power = pre;
+    for (int i = 0; i < 4; ++i, power *= pre * pre) cc.tc[i] = (float)(c[i] * power);
+    return cc;
+}
+
 mg_status tc_params(mg::TcAttnParams* t, const mg::AttnParams& p, const Device& dev, Scratch& ws, cudaStream_t st,
                     const char* who)
 {
@@ -170,14 +197,7 @@ mg_status tc_params(mg::TcAttnParams* t, const mg::AttnParams& p, const Device& 
     t->scale = std::fabs(p.scale);
     t->idesc_s = mg::idesc_bf16(128, 128, false, false, p.scale < 0.f);
     t->status = dev.status;
-    if (p.cap > 0.f) {
-        const double pre = t->scale / p.cap, c[4] = {0.999999463558197, -0.33326318860054016, 0.13190296292304993,
-                                                     -0.04440222308039665};
-        t->curve.pre = (float)pre;
-        t->curve.bound = pre > 1e-5 && pre < 1e4 ? (float)(0.5 / pre) : 0.f;
-        double power = pre;
-        for (int i = 0; i < 4; ++i, power *= pre * pre) t->curve.tc[i] = (float)(c[i] * power);
-    }
+    t->curve = cap_curve(t->scale, p.cap);
     if (p.docs) {
         const int64_t tiles = (int64_t)p.B * ceil_div(p.Lk, 128);
         int2* dt = static_cast<int2*>(ws.get(std::max<int64_t>(1, tiles) * sizeof(int2)));
@@ -192,21 +212,21 @@ mg_status tc_params(mg::TcAttnParams* t, const mg::AttnParams& p, const Device& 
 }
 
 template <int DP, bool kCap, bool kBias>
-mg_status launch_tc_forward(const mg::TcAttnParams& t, cudaStream_t st)
+mg_status launch_tc_forward(const mg::TcAttnParams& t, const Device& dev, cudaStream_t st)
 {
-    const auto kernel = mg::attn_tc_forward<DP, kCap, kBias>;
+    constexpr auto kernel = mg::attn_tc_forward<DP, kCap, kBias>;
     constexpr size_t smem = mg::tc_forward_smem<DP>();
-    MG_HOST_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    MG_TRY(allow_smem<kernel>(dev, smem));
     kernel<<<ceil_div(t.a.Lq, 128) * t.a.B * t.a.H, mg::kTcFwdThreads, smem, st>>>(t);
     return launched("mg_attention");
 }
 
 template <int DP>
-mg_status launch_tc_forward(const mg::TcAttnParams& t, cudaStream_t st)
+mg_status launch_tc_forward(const mg::TcAttnParams& t, const Device& dev, cudaStream_t st)
 {
     const bool cap = t.a.cap > 0.f, bias = t.a.slopes != nullptr;
-    return cap ? (bias ? launch_tc_forward<DP, true, true>(t, st) : launch_tc_forward<DP, true, false>(t, st))
-               : (bias ? launch_tc_forward<DP, false, true>(t, st) : launch_tc_forward<DP, false, false>(t, st));
+    return cap ? (bias ? launch_tc_forward<DP, true, true>(t, dev, st) : launch_tc_forward<DP, true, false>(t, dev, st))
+               : (bias ? launch_tc_forward<DP, false, true>(t, dev, st) : launch_tc_forward<DP, false, false>(t, dev, st));
 }
 
 mg_status forward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
@@ -218,28 +238,28 @@ mg_status forward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     MG_TRY(tc_map(&t.q, &t.head_step[0], &t.batch_step[0], p.q, p.qs, p.D, p.Lq, p.H, p.B, 128));
     MG_TRY(tc_map(&t.k, &t.head_step[1], &t.batch_step[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 128));
     MG_TRY(tc_map(&t.v, &t.head_step[2], &t.batch_step[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 128));
-    return p.D <= 64 ? launch_tc_forward<64>(t, st) : launch_tc_forward<128>(t, st);
+    return p.D <= 64 ? launch_tc_forward<64>(t, dev, st) : launch_tc_forward<128>(t, dev, st);
 }
 
 template <int DP, bool kKeys, bool kCap, bool kBias>
-mg_status launch_tc_backward(const mg::TcBwdParams& t, cudaStream_t st)
+mg_status launch_tc_backward(const mg::TcBwdParams& t, const Device& dev, cudaStream_t st)
 {
-    const auto kernel = mg::attn_tc_backward<DP, kKeys, kCap, kBias>;
+    constexpr auto kernel = mg::attn_tc_backward<DP, kKeys, kCap, kBias>;
     constexpr size_t smem = mg::tc_backward_smem<DP>();
-    MG_HOST_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    MG_TRY(allow_smem<kernel>(dev, smem));
     const int blocks = kKeys ? ceil_div(t.a.Lk, 128) * t.a.B * t.a.Hkv : ceil_div(t.a.Lq, 128) * t.a.B * t.a.H;
     kernel<<<blocks, mg::kTcBwdThreads, smem, st>>>(t);
     return launched("mg_attention_backward");
 }
 
 template <int DP, bool kKeys>
-mg_status launch_tc_backward(const mg::TcBwdParams& t, cudaStream_t st)
+mg_status launch_tc_backward(const mg::TcBwdParams& t, const Device& dev, cudaStream_t st)
 {
     const bool cap = t.a.cap > 0.f, bias = t.a.slopes != nullptr;
-    return cap ? (bias ? launch_tc_backward<DP, kKeys, true, true>(t, st)
-                       : launch_tc_backward<DP, kKeys, true, false>(t, st))
-               : (bias ? launch_tc_backward<DP, kKeys, false, true>(t, st)
-                       : launch_tc_backward<DP, kKeys, false, false>(t, st));
+    return cap ? (bias ? launch_tc_backward<DP, kKeys, true, true>(t, dev, st)
+                       : launch_tc_backward<DP, kKeys, true, false>(t, dev, st))
+               : (bias ? launch_tc_backward<DP, kKeys, false, true>(t, dev, st)
+                       : launch_tc_backward<DP, kKeys, false, false>(t, dev, st));
 }
 
 mg_status backward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
@@ -266,31 +286,31 @@ mg_status backward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     MG_TRY(tc_map(&t.x1, &hs[2], &bs[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 128));
     MG_TRY(tc_map(&t.y0, &hs[0], &bs[0], p.q, p.qs, p.D, p.Lq, p.H, p.B, 64));
     MG_TRY(tc_map(&t.y1, &hs[3], &bs[3], p.dout, p.dos, p.D, p.Lq, p.H, p.B, 64));
-    MG_TRY((p.D <= 64 ? launch_tc_backward<64, true>(t, st) : launch_tc_backward<128, true>(t, st)));
+    MG_TRY((p.D <= 64 ? launch_tc_backward<64, true>(t, dev, st) : launch_tc_backward<128, true>(t, dev, st)));
     // the queries resident: dQ
     MG_TRY(tc_map(&t.x0, &hs[0], &bs[0], p.q, p.qs, p.D, p.Lq, p.H, p.B, 128));
     MG_TRY(tc_map(&t.x1, &hs[3], &bs[3], p.dout, p.dos, p.D, p.Lq, p.H, p.B, 128));
     MG_TRY(tc_map(&t.y0, &hs[1], &bs[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 64));
     MG_TRY(tc_map(&t.y1, &hs[2], &bs[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 64));
-    return p.D <= 64 ? launch_tc_backward<64, false>(t, st) : launch_tc_backward<128, false>(t, st);
+    return p.D <= 64 ? launch_tc_backward<64, false>(t, dev, st) : launch_tc_backward<128, false>(t, dev, st);
 }
 
 template <int DP, bool kCap, bool kBias>
-mg_status launch_tc32_forward(const mg::Tc32Params& t, cudaStream_t st)
+mg_status launch_tc32_forward(const mg::Tc32Params& t, const Device& dev, cudaStream_t st)
 {
-    const auto kernel = mg::attn_tc32_forward<DP, kCap, kBias>;
+    constexpr auto kernel = mg::attn_tc32_forward<DP, kCap, kBias>;
     constexpr size_t smem = mg::tc32_forward_smem<DP>();
-    MG_HOST_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    MG_TRY(allow_smem<kernel>(dev, smem));
     kernel<<<ceil_div(t.a.Lq, 128 * mg::tc32_nq<DP>()) * t.a.B * t.a.H, mg::tc32_threads<DP>(), smem, st>>>(t);
     return launched("mg_attention");
 }
 
 template <int DP>
-mg_status launch_tc32_forward(const mg::Tc32Params& t, cudaStream_t st)
+mg_status launch_tc32_forward(const mg::Tc32Params& t, const Device& dev, cudaStream_t st)
 {
     const bool cap = t.a.cap > 0.f, bias = t.a.slopes != nullptr;
-    return cap ? (bias ? launch_tc32_forward<DP, true, true>(t, st) : launch_tc32_forward<DP, true, false>(t, st))
-               : (bias ? launch_tc32_forward<DP, false, true>(t, st) : launch_tc32_forward<DP, false, false>(t, st));
+    return cap ? (bias ? launch_tc32_forward<DP, true, true>(t, dev, st) : launch_tc32_forward<DP, true, false>(t, dev, st))
+               : (bias ? launch_tc32_forward<DP, false, true>(t, dev, st) : launch_tc32_forward<DP, false, false>(t, dev, st));
 }
 
 mg_status forward_tc32(const mg::AttnParams& p, const Device& dev, void* stream)
@@ -300,26 +320,26 @@ mg_status forward_tc32(const mg::AttnParams& p, const Device& dev, void* stream)
     cudaStream_t st = (cudaStream_t)stream;
     MG_TRY(tc_params(&f, p, dev, ws, st, "mg_attention"));
     mg::Tc32Params t = {p, f.doc_tiles, mg::idesc_bf16(128, 64, false, false, p.scale < 0.f), f.scale, f.status};
-    return p.D <= 64 ? launch_tc32_forward<64>(t, st) : launch_tc32_forward<128>(t, st);
+    return p.D <= 64 ? launch_tc32_forward<64>(t, dev, st) : launch_tc32_forward<128>(t, dev, st);
 }
 
 template <bool kKeys, bool kCap, bool kBias>
-mg_status launch_tc32_backward(const mg::Tc32BwdParams& t, cudaStream_t st)
+mg_status launch_tc32_backward(const mg::Tc32BwdParams& t, const Device& dev, cudaStream_t st)
 {
-    const auto kernel = mg::attn_tc32_backward<kKeys, kCap, kBias>;
-    MG_HOST_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)mg::kTc32BwdSmem));
+    constexpr auto kernel = mg::attn_tc32_backward<kKeys, kCap, kBias>;
+    MG_TRY(allow_smem<kernel>(dev, mg::kTc32BwdSmem));
     const int blocks = kKeys ? ceil_div(t.a.Lk, 128) * t.a.B * t.a.Hkv : ceil_div(t.a.Lq, 128) * t.a.B * t.a.H;
     kernel<<<blocks, mg::kTc32BwdThreads, mg::kTc32BwdSmem, st>>>(t);
     return launched("mg_attention_backward");
 }
 
 template <bool kKeys>
-mg_status launch_tc32_backward(const mg::Tc32BwdParams& t, cudaStream_t st)
+mg_status launch_tc32_backward(const mg::Tc32BwdParams& t, const Device& dev, cudaStream_t st)
 {
     const bool cap = t.a.cap > 0.f, bias = t.a.slopes != nullptr;
-    return cap ? (bias ? launch_tc32_backward<kKeys, true, true>(t, st) : launch_tc32_backward<kKeys, true, false>(t, st))
-               : (bias ? launch_tc32_backward<kKeys, false, true>(t, st)
-                       : launch_tc32_backward<kKeys, false, false>(t, st));
+    return cap ? (bias ? launch_tc32_backward<kKeys, true, true>(t, dev, st) : launch_tc32_backward<kKeys, true, false>(t, dev, st))
+               : (bias ? launch_tc32_backward<kKeys, false, true>(t, dev, st)
+                       : launch_tc32_backward<kKeys, false, false>(t, dev, st));
 }
 
 mg_status backward_tc32(const mg::AttnParams& p, const Device& dev, void* stream)
@@ -337,16 +357,16 @@ mg_status backward_tc32(const mg::AttnParams& p, const Device& dev, void* stream
     MG_TRY(launched(who));
     const mg::Tc32BwdParams t = {p,        f.doc_tiles, stats, stats + rows, Lp, mg::idesc_bf16(128, 64, false, false, p.scale < 0.f),
                                  f.scale, f.status};
-    MG_TRY(launch_tc32_backward<true>(t, st));
-    return launch_tc32_backward<false>(t, st);
+    MG_TRY(launch_tc32_backward<true>(t, dev, st));
+    return launch_tc32_backward<false>(t, dev, st);
 }
 
 // ---------------------------------------------------------------- paged
 template <typename T, int DP>
-mg_status launch_paged_kernel(const mg::PagedParams& p, int blocks, cudaStream_t st)
+mg_status launch_paged_kernel(const mg::PagedParams& p, const Device& dev, int blocks, cudaStream_t st)
 {
     constexpr size_t smem = mg::paged_smem<T, DP>();
-    MG_HOST_TRY(cudaFuncSetAttribute(mg::paged_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    MG_TRY((allow_smem<mg::paged_kernel<T, DP>>(dev, smem)));
     mg::paged_kernel<T, DP><<<blocks, mg::kPagedThreads, smem, st>>>(p);
     return MG_OK;
 }
@@ -363,24 +383,40 @@ mg_status launch_paged(mg::PagedParams& p, int longest, const Device& dev, Scrat
                           aligned(p.v_new, p.vns, 2, sizeof(T), vec);
     const int group = p.H / p.Hkv, packs = ceil_div(group, stream ? mg::paged_pack<T>() : mg::kPagedHeads);
     const int64_t heads = (int64_t)p.B * p.Hkv * packs;
-    const int64_t want = std::max<int64_t>(1, (int64_t)dev.sm_count * 8 / heads);
+    const int64_t want = std::max<int64_t>(1, (int64_t)dev.sm_count * 24 / heads);
     const int most = std::max(1, ceil_div(longest, 128));
     int splits = (int)std::min<int64_t>(want, most);
     p.chunk = std::max(1, ceil_div(longest, splits));
     p.splits = splits = std::max(1, ceil_div(longest, p.chunk));
     if (heads * splits >= (1ll << 31) - 1) return fail(MG_ERR_UNSUPPORTED, "%s: batch is too large", who);
+    p.curve = cap_curve(std::fabs(p.scale), p.cap);
+    p.page_shift = -1;
+    if (p.page > 0 && (p.page & (p.page - 1)) == 0)
+        for (p.page_shift = 0; (1 << p.page_shift) < p.page;) ++p.page_shift;
+    if ((int64_t)p.B * p.H >= (1ll << 31) - 1) return fail(MG_ERR_UNSUPPORTED, "%s: batch is too large", who);
     if (splits > 1) {
         const size_t rows = (size_t)p.B * p.H * splits;
-        p.part = static_cast<float*>(ws.get(rows * p.D * sizeof(float)));
-        p.stat = static_cast<float2*>(ws.get(rows * sizeof(float2)));
-        if (!p.part || !p.stat) return fail(MG_ERR_ALLOC, "%s: no scratch for %zu chunks", who, rows);
+        const size_t part = (rows * p.D * sizeof(float) + 15) / 16 * 16;
+        uint8_t* mem = static_cast<uint8_t*>(ws.get(part + rows * sizeof(float2)));
+        p.part = reinterpret_cast<float*>(mem);
+        p.stat = reinterpret_cast<float2*>(mem + part);
+        if (!mem) return fail(MG_ERR_ALLOC, "%s: no scratch for %zu chunks", who, rows);
     }
     const int blocks = (int)(heads * splits);
     if (!stream) mg::paged_simt_kernel<T><<<blocks, mg::kPagedThreads, 0, st>>>(p);
-    else MG_TRY((p.D <= 64 ? launch_paged_kernel<T, 64>(p, blocks, st) : launch_paged_kernel<T, 128>(p, blocks, st)));
+    else MG_TRY((p.D <= 64 ? launch_paged_kernel<T, 64>(p, dev, blocks, st) : launch_paged_kernel<T, 128>(p, dev, blocks, st)));
     MG_TRY(launched(who));
     if (splits > 1) {
-        mg::paged_join_kernel<T><<<ceil_div((int64_t)p.B * p.H, mg::kPagedThreads / 32), mg::kPagedThreads, 0, st>>>(p);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(p.B * p.H));
+        cfg.blockDim = dim3(mg::kJoinThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute early = {};
+        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &early;
+        cfg.numAttrs = 1;
+        MG_HOST_TRY(cudaLaunchKernelEx(&cfg, mg::paged_join_kernel<T>, p));
         MG_TRY(launched(who));
     }
     return MG_OK;

@@ -31,7 +31,9 @@ struct PagedParams {
     const void *k_new, *v_new;
     void* out;
     float* lse;
+    int page_shift;              // log2(page), or -1
     int chunk, splits;           // keys a block reads; blocks along the length
+    CapCurve curve;              // of the cap, with a cap
     float* part;                 // [B * H][splits][D] accumulators
     float2* stat;                // [B * H][splits] (m, l)
     int* status;
@@ -65,7 +67,7 @@ __device__ __forceinline__ bool paged_row(const PagedParams& p, int b, int j, in
         row = j;
         return true;
     }
-    const int n = j / p.page;
+    const int n = p.page_shift >= 0 ? j >> p.page_shift : j / p.page;
     page = __ldg(p.table + b * p.table_stride + n);
     row = j - n * p.page;
     return page >= 0 && page < p.pages;
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_simt_kernel(const __grid_
 // one to sixteen heads to a key-value head the loads bound the kernel, not the
 // arithmetic, so the warp-level instruction is enough here. fp32: a lane has one key (half of the head
 // each in two lanes) for the scores and D / 32 elements of the output.
-constexpr int kPagedStages = 3;
+constexpr int kPagedStages = 2;
 constexpr int kPagedTile = 16;
 constexpr int kPagedWarps = kPagedThreads / 32;
 
@@ -316,7 +318,16 @@ struct PagedAcc {
             mma16816(s[0], q[k], b[0], b[1]);
             mma16816(s[1], q[k], b[2], b[3]);
         }
-        const float mul = p.scale * kLog2e, cap2 = p.cap * kLog2e, pre = p.cap > 0.f ? p.scale / p.cap : 0.f;
+        float mul = p.scale * kLog2e;
+        if (p.cap > 0.f) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = p.scale < 0.f ? -s[i / 4][i % 4] : s[i / 4][i % 4];
+            cap_scores(x, p.curve);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = x[i];
+            mul = p.cap * kLog2e;
+        }
         float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -324,7 +335,6 @@ struct PagedAcc {
             for (int i = 0; i < 4; ++i) {
                 const int key = 8 * n + 2 * t + (i & 1);
                 float x = s[n][i] * mul;
-                if (p.cap > 0.f) x = cap2 * tanh_fast(s[n][i] * pre);
                 x = fmaf(-slope[i >> 1], (float)(back - key), x);
                 x = (seen >> key) & 1 ? x : -CUDART_INF_F;
                 s[n][i] = x;
@@ -387,12 +397,14 @@ struct PagedAcc {
     }
 };
 
-// fp32.
+// fp32. For the scores a lane has one key and half of the head; for the output it
+// has half of the keys (its half warp's eight) and every sixteenth piece of the head.
 template <int DP>
 struct PagedAcc<float, DP> {
-    static constexpr int kPer = DP / 32;
+    static constexpr int kPer = DP / 64;     // pieces of four elements a lane
     const float* q;              // [heads][DP] in shared memory
-    float o[kPagedHeads][kPer], m[kPagedHeads], l[kPagedHeads], slope[kPagedHeads];
+    float4 o[kPagedHeads][kPer];
+    float m[kPagedHeads], l[kPagedHeads], slope[kPagedHeads];
     __device__ __forceinline__ void init(const PagedParams& p, int, int h0, int nh, int, const float* sq)
     {
         q = sq;
@@ -402,7 +414,7 @@ struct PagedAcc<float, DP> {
             l[g] = 0.f;
             slope[g] = p.slopes && g < nh ? __ldg(p.slopes + h0 + g) * kLog2e : 0.f;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) o[g][i] = 0.f;
+            for (int i = 0; i < kPer; ++i) o[g][i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
     }
     __device__ __forceinline__ void tile(const PagedParams& p, uint32_t sk, uint32_t sv, uint32_t seen, int back, int nh,
@@ -412,7 +424,7 @@ struct PagedAcc<float, DP> {
         float s[kPagedHeads];
 #pragma unroll
         for (int g = 0; g < kPagedHeads; ++g) s[g] = 0.f;
-#pragma unroll 4
+#pragma unroll
         for (int i = 0; i < DP / 8; ++i) {
             const int piece = half * (DP / 8) + i;
             const float4 k4 = lds4(sk + key * (DP * 4) + ((piece ^ (key & 7)) << 4));
@@ -439,28 +451,26 @@ struct PagedAcc<float, DP> {
                 m[g] = top;
                 l[g] *= f;
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) o[g][i] *= f;
+                for (int i = 0; i < kPer; ++i) o[g][i].x *= f, o[g][i].y *= f, o[g][i].z *= f, o[g][i].w *= f;
             }
             s[g] = ex2(x - (m[g] == -CUDART_INF_F ? 0.f : m[g]));
             l[g] += half ? 0.f : s[g];
         }
-#pragma unroll 4
-        for (int r = 0; r < kPagedTile; ++r) {
-            float v[kPer];
-            const uint32_t row = sv + r * (DP * 4);
-            if (kPer == 4) {
-                const float4 x = lds4(row + ((lane ^ (r & 7)) << 4));
-                v[0] = x.x, v[1] = x.y, v[kPer - 2] = x.z, v[kPer - 1] = x.w;
-            } else {
-                const float2 x = lds2(row + (((lane >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8);
-                v[0] = x.x, v[1] = x.y;
-            }
+#pragma unroll
+        for (int r = 0; r < kPagedTile / 2; ++r) {
+            const int row = r + 8 * half;
+            float4 v[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) v[i] = lds4(sv + row * (DP * 4) + (((lane & 15) + 16 * i) ^ (row & 7)) * 16);
 #pragma unroll
             for (int g = 0; g < kPagedHeads; ++g) {
                 if (g >= nh) break;
-                const float e = __shfl_sync(~0u, s[g], r);
+                const float e = __shfl_sync(~0u, s[g], row);
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) o[g][i] = fmaf(e, v[i], o[g][i]);
+                for (int i = 0; i < kPer; ++i) {
+                    o[g][i].x = fmaf(e, v[i].x, o[g][i].x), o[g][i].y = fmaf(e, v[i].y, o[g][i].y);
+                    o[g][i].z = fmaf(e, v[i].z, o[g][i].z), o[g][i].w = fmaf(e, v[i].w, o[g][i].w);
+                }
             }
         }
     }
@@ -472,7 +482,12 @@ struct PagedAcc<float, DP> {
             for (int w = 8; w; w /= 2) l[g] += __shfl_xor_sync(~0u, l[g], w);
             if (lane == 0) sm_m[g] = m[g], sm_l[g] = l[g];
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) sm_o[g * DP + lane * kPer + i] = o[g][i];
+            for (int i = 0; i < kPer; ++i) {
+                float4 x = o[g][i];
+                x.x += __shfl_xor_sync(~0u, x.x, 16), x.y += __shfl_xor_sync(~0u, x.y, 16);
+                x.z += __shfl_xor_sync(~0u, x.z, 16), x.w += __shfl_xor_sync(~0u, x.w, 16);
+                if (lane < 16) *reinterpret_cast<float4*>(sm_o + g * DP + 4 * (lane + 16 * i)) = x;
+            }
         }
     }
 };
@@ -486,6 +501,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
     __shared__ float sm_m[kPagedWarps][16], sm_l[kPagedWarps][16];
     __shared__ __align__(16) float sq[sizeof(T) == 4 ? kPagedHeads * DP : 4];
     __shared__ uint32_t sm_seen[kPagedWarps][kPagedStages];
+    __shared__ ulonglong2 sm_rows[kPagedWarps][kPagedTile];
 
     const int split = blockIdx.x % p.splits, bh = blockIdx.x / p.splits;
     const int groups = p.H / p.Hkv, packs = (groups + kPack - 1) / kPack;
@@ -499,12 +515,11 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(paged_dyn) + warp * kPagedStages * 2 * kTileBytes;
     const int qdoc = p.docs && len > 0 ? __ldg(p.docs + (int64_t)b * p.length + len - 1) : 0;
 
-    // Tile n of this warp: keys j0 + (4 n + warp) * 16 and on. Lanes i and i + 16 find the rows of key i.
+    // Tile n of this warp: keys j0 + (4 n + warp) * 16 and on. Lanes 0-15 find the
+    // rows of a key each and leave them to the others in shared memory.
     const auto issue = [&](int n) {
-        const int j = j0 + (n * kPagedWarps + warp) * kPagedTile + (lane & 15);
-        bool live = j < j1;
-        const T *kr = (const T*)p.k, *vr = (const T*)p.v;
-        bool fresh = false;
+        const int j = j0 + (n * kPagedWarps + warp) * kPagedTile + lane;
+        bool live = lane < kPagedTile && j < j1;
         T *kc = nullptr, *vc = nullptr;
         if (live) {
             int page, row;
@@ -514,40 +529,45 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
             } else if (p.docs && (qdoc < 0 || __ldg(p.docs + (int64_t)b * p.length + j) != qdoc)) {
                 live = false;
             } else {
-                kr = kc = (T*)p.k + page * p.ks[0] + row * p.ks[1] + kv * p.ks[2];
-                vr = vc = (T*)p.v + page * p.vs[0] + row * p.vs[1] + kv * p.vs[2];
-                fresh = p.k_new != nullptr && j == len - 1;
-                if (fresh) {
-                    kr = (const T*)p.k_new + b * p.kns[0] + kv * p.kns[1];
-                    vr = (const T*)p.v_new + b * p.vns[0] + kv * p.vns[1];
-                }
+                kc = (T*)p.k + page * p.ks[0] + row * p.ks[1] + kv * p.ks[2];
+                vc = (T*)p.v + page * p.vs[0] + row * p.vs[1] + kv * p.vs[2];
             }
         }
+        ulonglong2* rows = sm_rows[warp];
+        __syncwarp();
+        if (lane < kPagedTile) rows[lane] = make_ulonglong2((unsigned long long)kc, (unsigned long long)vc);
         const uint32_t seen = __ballot_sync(~0u, live);
-        if (lane == 0) sm_seen[warp][n % kPagedStages] = seen & 0xFFFFu;
+        if (lane == 0) sm_seen[warp][n % kPagedStages] = seen;
+        // the token's own key and value go to the cache, and are read from where they came
+        const int last = len - 1 - (j0 + (n * kPagedWarps + warp) * kPagedTile);
+        if (p.k_new != nullptr && last >= 0 && last < kPagedTile && (seen >> last & 1)) {
+            __syncwarp();
+            const ulonglong2 at = rows[last];
+            const bool is_v = lane >= 16;
+            const T* src = is_v ? (const T*)p.v_new + b * p.vns[0] + kv * p.vns[1]
+                                : (const T*)p.k_new + b * p.kns[0] + kv * p.kns[1];
+            T* out = (T*)(is_v ? at.y : at.x);
+            __syncwarp();
+            if (pack == 0)
+                for (int e = (lane & 15) * (16 / (int)sizeof(T)); e < p.D; e += 16 * (16 / (int)sizeof(T)))
+                    *reinterpret_cast<uint4*>(out + e) = *reinterpret_cast<const uint4*>(src + e);
+            if (lane == last) rows[lane] = make_ulonglong2((unsigned long long)((const T*)p.k_new + b * p.kns[0] + kv * p.kns[1]),
+                                                           (unsigned long long)((const T*)p.v_new + b * p.vns[0] + kv * p.vns[1]));
+        }
+        __syncwarp();
         const uint32_t dst = ring + (n % kPagedStages) * 2 * kTileBytes;
+        constexpr int kStep = 32 / kPieces;              // rows a warp copies at a time
+        const int c = lane % kPieces, e = c * (16 / (int)sizeof(T));
 #pragma unroll
-        for (int i = 0; i < kPagedTile * kPieces / 32; ++i) {
-            const int r = (i * 32 + lane) / kPieces, c = (i * 32 + lane) % kPieces;
-            const T* ks = (const T*)__shfl_sync(~0u, (unsigned long long)kr, r);
-            const T* vs = (const T*)__shfl_sync(~0u, (unsigned long long)vr, r);
-            const int e = c * (16 / (int)sizeof(T));
-            const bool in = (seen >> r & 1) && e < p.D;
-            const uint32_t at = dst + r * (DP * (int)sizeof(T)) + ((c ^ (r & 7)) << 4);
-            copy16(at, ks + (in ? e : 0), in);
-            copy16(at + kTileBytes, vs + (in ? e : 0), in);
+        for (int i = 0; i < kPagedTile / kStep; ++i) {
+            const int r = lane / kPieces + i * kStep;
+            const ulonglong2 at = rows[r];
+            const bool in = at.x != 0 && e < p.D;
+            const uint32_t to = dst + r * (DP * (int)sizeof(T)) + ((c ^ (r & 7)) << 4);
+            copy16(to, (const T*)(in ? at.x : (unsigned long long)p.k) + (in ? e : 0), in);
+            copy16(to + kTileBytes, (const T*)(in ? at.y : (unsigned long long)p.v) + (in ? e : 0), in);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        // the token's own key and value go to the cache (lanes 0-15 the key, 16-31 the value)
-        const uint32_t new_row = __ballot_sync(~0u, fresh) & 0xFFFFu;
-        if (new_row && pack == 0) {
-            const int r = __ffs(new_row) - 1;
-            const bool is_v = lane >= 16;
-            const T* src = (const T*)__shfl_sync(~0u, (unsigned long long)(is_v ? vr : kr), r + (lane & 16));
-            T* out = (T*)__shfl_sync(~0u, (unsigned long long)(is_v ? vc : kc), r + (lane & 16));
-            for (int e = (lane & 15) * (16 / (int)sizeof(T)); e < p.D; e += 16 * (16 / (int)sizeof(T)))
-                *reinterpret_cast<uint4*>(out + e) = *reinterpret_cast<const uint4*>(src + e);
-        }
     };
     const int tiles = max(0, (j1 - j0 + kPagedTile - 1) / kPagedTile);
     const int mine = tiles > warp ? (tiles - warp + kPagedWarps - 1) / kPagedWarps : 0;
@@ -576,6 +596,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
                  len - 1 - (j0 + (n * kPagedWarps + warp) * kPagedTile), nh, lane);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __syncthreads();                        // the rings become the join's buffer
     float* so = reinterpret_cast<float*>(paged_dyn);
     acc.finish(sm_m[warp], sm_l[warp], so + warp * kPack * DP, nh, lane);
@@ -599,33 +620,79 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
     }
 }
 
-// Joins the chunks of one query head: one warp per head.
+// Joins the chunks of one query head: a block per head, D / 4 lanes to a chunk's
+// accumulators. Launched while the chunks are still being read (programmatic
+// dependent launch): it waits for them before it touches their results.
+constexpr int kJoinThreads = 512;
+
 template <typename T>
-__global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const __grid_constant__ PagedParams p)
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p)
 {
-    const int64_t row = (int64_t)blockIdx.x * (kPagedThreads / 32) + threadIdx.x / 32;
-    if (row >= (int64_t)p.B * p.H) return;
-    const int lane = threadIdx.x % 32;
+    __shared__ float weight[kJoinThreads], red[2][kJoinThreads / 32];
+    __shared__ float4 acc[kJoinThreads];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int b = (int)(row / p.H), h = (int)(row % p.H);
     const int n = max(1, (paged_length(p, b) + p.chunk - 1) / p.chunk);
     const float2* st = p.stat + row * p.splits;
     float M = -CUDART_INF_F;
-    for (int s = lane; s < n; s += 32) M = fmaxf(M, st[s].x);
+    for (int s = threadIdx.x; s < n; s += kJoinThreads) M = fmaxf(M, st[s].x);
 #pragma unroll
     for (int o = 16; o; o /= 2) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
+    if (lane == 0) red[0][warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) M = fmaxf(M, red[0][w]);
     const float base = M == -CUDART_INF_F ? 0.f : M;
+    // rows of accumulators are read as pieces of four elements where they allow it
+    const int width = p.D % 4 ? 1 : 4, lanes = (p.D + width - 1) / width, sets = max(1, kJoinThreads / lanes);
+    const int set = threadIdx.x / lanes, piece = threadIdx.x % lanes;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     float L = 0.f;
-    for (int s = lane; s < n; s += 32) L += expf(st[s].x - base) * st[s].y;
+    for (int s0 = 0; s0 < n; s0 += kJoinThreads) {
+        __syncthreads();
+        const int s = s0 + threadIdx.x;
+        float w = 0.f;
+        if (s < n) {
+            const float2 x = st[s];
+            w = expf(x.x - base);
+            L = fmaf(w, x.y, L);
+        }
+        weight[threadIdx.x] = w;
+        __syncthreads();
+        if (set < sets)
+#pragma unroll 4
+            for (int i = set; i < min(kJoinThreads, n - s0); i += sets) {
+                const float* src = p.part + (row * p.splits + s0 + i) * p.D + piece * width;
+                const float f = weight[i];
+                if (width == 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(src);
+                    a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
+                } else {
+                    a.x = fmaf(f, *src, a.x);
+                }
+            }
+    }
 #pragma unroll
     for (int o = 16; o; o /= 2) L += __shfl_xor_sync(~0u, L, o);
+    if (lane == 0) red[1][warp] = L;
+    acc[threadIdx.x] = a;
+    __syncthreads();
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) L += red[1][w];
     const float inv = L > 0.f ? 1.f / L : L;           // 0: no key; NaN stays
-    T* out = (T*)p.out + b * p.os[0] + h * p.os[1];
-    for (int d = lane; d < p.D; d += 32) {
-        float a = 0.f;
-        for (int s = 0; s < n; ++s) a = fmaf(expf(st[s].x - base), p.part[(row * p.splits + s) * p.D + d], a);
-        out[d] = from_f32<T>(a * inv);
+    if (set == 0) {
+        for (int i = 1; i < sets; ++i) {
+            const float4 v = acc[i * lanes + piece];
+            a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+        }
+        T* out = (T*)p.out + b * p.os[0] + h * p.os[1] + piece * width;
+        out[0] = from_f32<T>(a.x * inv);
+        if (width == 4) out[1] = from_f32<T>(a.y * inv), out[2] = from_f32<T>(a.z * inv), out[3] = from_f32<T>(a.w * inv);
     }
-    if (lane == 0) p.lse[row] = L == 0.f ? -CUDART_INF_F : M + logf(L);
+    if (threadIdx.x == 0) p.lse[row] = L == 0.f ? -CUDART_INF_F : M + logf(L);
 }
 
 }  // namespace mg

@@ -71,7 +71,7 @@ def _plain(t: torch.Tensor, name: str, shape, dtype: torch.dtype, device) -> Non
     """A contiguous CUDA tensor of exactly this shape and type."""
     if not isinstance(t, torch.Tensor) or t.device != device:
         _bad(f"{name} must be a tensor on {device}")
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+    if t.dtype != dtype or t.shape != shape:
         _bad(f"{name} must be {dtype} of shape {tuple(shape)}, found {t.dtype} of shape {tuple(t.shape)}")
     if not t.is_contiguous():
         _bad(f"{name} must be contiguous")
@@ -82,6 +82,8 @@ def _written(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
     _heads(t, name, like.dim(), like.dtype, like.device)
     if t.shape != like.shape:
         _bad(f"{name} must have shape {tuple(like.shape)}, found {tuple(t.shape)}")
+    if t.is_contiguous():
+        return
     spans = sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1)
     end = 1
     for st, n in spans:
@@ -97,30 +99,25 @@ def _number(x: float, name: str) -> float:
     return x
 
 
-class _On:
-    """Runs a call on `stream` (its device current, its allocations the stream's own), by default on the current
-    stream of the operands' device."""
+# The raw handle of the current stream, and the current device, without the
+# objects around them: a call's host time counts where one token is decoded.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_device = torch.cuda.current_device
 
-    __slots__ = ("ctx", "handle")
 
-    def __init__(self, device: torch.device, stream: Optional[torch.cuda.Stream]):
-        if stream is not None:
-            if torch.device(stream.device) != device:
-                _bad(f"operands (and stream) are on different devices: {device}, {stream.device}")
-            self.ctx = torch.cuda.stream(stream)
-            self.handle = stream.cuda_stream
-        else:
-            self.ctx = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-            self.handle = torch.cuda.current_stream(device).cuda_stream
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-        return self.handle
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+def _on(device: torch.device, stream: Optional[torch.cuda.Stream], call):
+    """call(stream handle) on `stream` (its device current, its allocations the stream's own), by default on the
+    current stream of the operands' device."""
+    if stream is None:
+        if _device() == device.index:
+            return call(_raw_stream(device.index))
+        with torch.cuda.device(device):
+            return call(_raw_stream(device.index))
+    if torch.device(stream.device) != device:
+        _bad(f"operands (and stream) are on different devices: {device}, {stream.device}")
+    with torch.cuda.stream(stream):
+        return call(stream.cuda_stream)
 
 
 def _at(t: Optional[torch.Tensor]) -> int:
@@ -180,14 +177,17 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     dev, lead, ptrs = _attention_args(q, k, v, scale, causal, cap, slopes, documents, prefix)
     if out is not None:
         _written(out, "out", q)
-    with _On(dev, stream) as st:
-        if out is None:
-            out = torch.empty_like(q)
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
-        desc = _ATTENTION.pack(*lead, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
-                               *_ZERO3, *_ZERO3, *_ZERO3, *_ZERO3, *ptrs)
-        check(lib.mg_attention(desc, out.data_ptr(), lse.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), st))
-    return out, lse
+
+    def call(st):
+        o = torch.empty_like(q) if out is None else out
+        H, Lq = lead[2], lead[4]
+        lse = torch.empty_strided(q.shape[:3], (H * Lq, Lq, 1), dtype=torch.float32, device=dev)
+        desc = _ATTENTION.pack(*lead, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3], *_ZERO3,
+                               *_ZERO3, *_ZERO3, *_ZERO3, *ptrs)
+        check(lib.mg_attention(desc, o.data_ptr(), lse.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), st))
+        return o, lse
+
+    return _on(dev, stream, call)
 
 
 def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
@@ -206,13 +206,16 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
         if t.shape != q.shape:
             _bad(f"{name} must have q's shape {tuple(q.shape)}, found {tuple(t.shape)}")
     _plain(lse, "lse", q.shape[:3], torch.float32, dev)
-    with _On(dev, stream) as st:
+
+    def call(st):
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         desc = _ATTENTION.pack(*lead, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
                                *dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], *ptrs)
         check(lib.mg_attention_backward(desc, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dout.data_ptr(),
                                         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), st))
-    return dq, dk, dv
+        return dq, dk, dv
+
+    return _on(dev, stream, call)
 
 
 # ------------------------------------------------------------------ rotary positions
@@ -276,17 +279,18 @@ def _rotary(q, k, positions, frequencies, interleaved, inverse, magnitude, out_q
     for x, y, name in ((q, out_q, "out_q"), (k, out_k, "out_k")):
         if x is not None and y is not None and x.data_ptr() == y.data_ptr() and x.stride() != y.stride():
             _bad(f"{name} starts where its input does but has other strides")
-    with _On(dev, stream) as st:
-        if out_q is None:
-            out_q = torch.empty_like(q)
-        if k is not None and out_k is None:
-            out_k = torch.empty_like(k)
+
+    def call(st):
+        oq = torch.empty_like(q) if out_q is None else out_q
+        ok = torch.empty_like(k) if k is not None and out_k is None else out_k
         desc = _ROTARY.pack(_DTYPES[dt], B, H, Hkv, L, D, pairs, 1 if interleaved else 0, 1 if inverse else 0,
-                            magnitude, *q.stride()[:3], *(k.stride()[:3] if Hkv else _ZERO3), *out_q.stride()[:3],
-                            *(out_k.stride()[:3] if Hkv else _ZERO3), 0 if shared else L, positions.data_ptr(),
+                            magnitude, *q.stride()[:3], *(k.stride()[:3] if Hkv else _ZERO3), *oq.stride()[:3],
+                            *(ok.stride()[:3] if Hkv else _ZERO3), 0 if shared else L, positions.data_ptr(),
                             frequencies.data_ptr())
-        check(lib.mg_rotary(desc, out_q.data_ptr(), _at(out_k), q.data_ptr(), _at(k), st))
-    return out_q, out_k
+        check(lib.mg_rotary(desc, oq.data_ptr(), _at(ok), q.data_ptr(), _at(k), st))
+        return oq, ok
+
+    return _on(dev, stream, call)
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor,
@@ -365,14 +369,16 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _written(v_pages, "v_pages", v_pages)
     if out is not None:
         _written(out, "out", q)
-    with _On(dev, stream) as st:
-        if out is None:
-            out = torch.empty_like(q)
-        lse = torch.empty((B, H), dtype=torch.float32, device=dev)
+
+    def call(st):
+        o = torch.empty_like(q) if out is None else out
+        lse = torch.empty_strided((B, H), (H, 1), dtype=torch.float32, device=dev)
         new = (*k_new.stride()[:2], *v_new.stride()[:2]) if k_new is not None else (0, 0, 0, 0)
-        desc = _PAGED.pack(_DTYPES[dt], B, H, Hkv, D, page, pages, width, scale, cap, *q.stride()[:2],
-                           *out.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3], *new, width,
-                           _at(slopes), block_table.data_ptr(), lengths.data_ptr())
-        check(lib.mg_paged_attention(desc, out.data_ptr(), lse.data_ptr(), q.data_ptr(), k_pages.data_ptr(),
+        desc = _PAGED.pack(_DTYPES[dt], B, H, Hkv, D, page, pages, width, scale, cap, *q.stride()[:2], *o.stride()[:2],
+                           *k_pages.stride()[:3], *v_pages.stride()[:3], *new, width, _at(slopes),
+                           block_table.data_ptr(), lengths.data_ptr())
+        check(lib.mg_paged_attention(desc, o.data_ptr(), lse.data_ptr(), q.data_ptr(), k_pages.data_ptr(),
                                      v_pages.data_ptr(), _at(k_new), _at(v_new), st))
-    return out, lse
+        return o, lse
+
+    return _on(dev, stream, call)
