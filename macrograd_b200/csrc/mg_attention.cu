@@ -301,7 +301,7 @@ mg_status launch_tc32_forward(const mg::Tc32Params& t, const Device& dev, cudaSt
     constexpr auto kernel = mg::attn_tc32_forward<DP, kCap, kBias>;
     constexpr size_t smem = mg::tc32_forward_smem<DP>();
     MG_TRY(allow_smem<kernel>(dev, smem));
-    kernel<<<ceil_div(t.a.Lq, 128 * mg::tc32_nq<DP>()) * t.a.B * t.a.H, mg::tc32_threads<DP>(), smem, st>>>(t);
+    kernel<<<ceil_div(t.a.Lq, 128) * t.a.B * t.a.H, mg::kTc32Threads, smem, st>>>(t);
     return launched("mg_attention");
 }
 
