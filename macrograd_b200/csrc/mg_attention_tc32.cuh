@@ -28,12 +28,13 @@ namespace mg {
 // Two numbers into their three pieces, the first in the lower half of each word.
 __device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[3])
 {
+    const uint64_t minus = pack2(-1.f, -1.f);
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-        w[i] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+        const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+        w[i] = __byte_perm(x, y, 0x7632);
         if (i == 2) break;
-        a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
-        b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+        unpack2(fma2(pack2(__uint_as_float(x & 0xFFFF0000u), __uint_as_float(y & 0xFFFF0000u)), minus, pack2(a, b)), a, b);
     }
 }
 
@@ -143,24 +144,26 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
 
     if (warp >= kLoadWarp && warp < kMmaWarp) {
         // ------------------------------------------------ loads and splits of keys and values
-        constexpr int kLoaders = kTc32LoadWarps * 32, kItems = (64 * (DP / 8) + kLoaders - 1) / kLoaders;
-        const int tid = threadIdx.x - kLoadWarp * 32;
-        const float* kp = (const float*)p.k + b * p.ks[0] + kv * p.ks[1];
-        const float* vp = (const float*)p.v + b * p.vs[0] + kv * p.vs[1];
+        // item i of a thread: 8 elements of row r0 + i * kRows, always the same columns
+        constexpr int kRows = kTc32LoadWarps * 32 / (DP / 8), kItems = (64 + kRows - 1) / kRows;
+        const int tid = threadIdx.x - kLoadWarp * 32, r0 = tid / (DP / 8), c = tid % (DP / 8);
+        const bool in = c * 8 < p.D;
+        const float* kp = (const float*)p.k + b * p.ks[0] + kv * p.ks[1] + c * 8;
+        const float* vp = (const float*)p.v + b * p.vs[0] + kv * p.vs[1] + c * 8;
         const auto fetch = [&](const float* src, int64_t stride, int j, float4 (&x)[kItems][2]) {
+            const int row0 = (t0 + j) * 64 + r0;
+            const float* at = src + row0 * stride;
 #pragma unroll
             for (int i = 0; i < kItems; ++i) {
-                const int item = i * kLoaders + tid, r = item / (DP / 8), c = item % (DP / 8), row = (t0 + j) * 64 + r;
-                const bool live = r < 64 && row < p.Lk && c * 8 < p.D && (!docs || __ldg(docs + row) >= 0);
-                tc32_fetch(x[i], src + (int64_t)row * stride + c * 8, live);
+                const int row = row0 + i * kRows;
+                const bool live = in && r0 + i * kRows < 64 && row < p.Lk && (!docs || __ldg(docs + row) >= 0);
+                tc32_fetch(x[i], at + i * kRows * stride, live);
             }
         };
         const auto put = [&](uint32_t tile, uint32_t full, const float4 (&x)[kItems][2]) {
 #pragma unroll
-            for (int i = 0; i < kItems; ++i) {
-                const int item = i * kLoaders + tid, r = item / (DP / 8), c = item % (DP / 8);
-                if (r < 64) tc32_put(tile, 64, kPieceK, r, c, x[i]);
-            }
+            for (int i = 0; i < kItems; ++i)
+                if (r0 + i * kRows < 64) tc32_put(tile, 64, kPieceK, r0 + i * kRows, c, x[i]);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(full);
@@ -246,9 +249,9 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
         const int qdoc = docs ? doc_at(p, b, qpos) : 0;
         const int common = docs ? (q0 + 128 <= p.Lq ? common_doc(dt, q0 + shift, 128, p.Lk) : -1) : 0;
         const int upto = qdoc < 0 ? 0 : !p.causal ? p.Lk : min(p.Lk, max(qpos + 1, prefix));
-        const float mul = kCap ? 1.f : tp.scale * kLog2e;
-        const float slope = kBias ? __ldg(p.slopes + h) * (kCap ? kLog2e : 1.f / tp.scale) : 0.f;
-        const float pre = kCap ? tp.scale / p.cap : 0.f, cap2 = p.cap * kLog2e;
+        // powers of two: a score's is s * mul - slope * distance
+        const float mul = kCap ? p.cap * kLog2e : tp.scale * kLog2e, pre = kCap ? tp.scale / p.cap : 0.f;
+        const float slope = kBias ? __ldg(p.slopes + h) * kLog2e : 0.f;
         // m: the maximum in use; f: what the output so far is to be multiplied by after the next tile's part is added
         float m = -CUDART_INF_F, l = 0.f, f = 1.f, o[DP];
 #pragma unroll
@@ -267,21 +270,32 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
             }
             const float far = (float)(qpos - k0);
             const int lim = upto - k0;
-            // columns [c0, c0 + 16) of the scores: capped, biased, masked
-            const auto scores = [&](int c0, float (&s)[16]) {
+            // columns [c0, c0 + 16): the powers of two less `base`, -inf where masked
+            const auto powers = [&](int c0, float base, float (&s)[16]) {
                 tmem_ld_x16(tS + c0, s);
-                if (kCap) cap_scores32(s, pre, cap2);
-                if (kBias) {
+                if (kCap) cap_scores32(s, pre, 1.f);
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) s[c] = fmaf(-slope, fabsf(far - (float)(c0 + c)), s[c]);
-                }
-                if (!full) {
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        bool seen = c0 + c < lim;
-                        if (docs) seen = seen && st.kdoc[warp][c0 + c] == qdoc;
-                        s[c] = seen ? s[c] : -CUDART_INF_F;
+                for (int c = 0; c < 16; c += 2) {
+                    float b0 = -base, b1 = -base;
+                    if (kBias) {
+                        b0 = fmaf(-slope, fabsf(far - (float)(c0 + c)), b0);
+                        b1 = fmaf(-slope, fabsf(far - (float)(c0 + c + 1)), b1);
                     }
+                    unpack2(fma2(pack2(s[c], s[c + 1]), pack2(mul, mul), pack2(b0, b1)), s[c], s[c + 1]);
+                }
+                if (full) return;
+                if (docs) {
+#pragma unroll
+                    for (int c = 0; c < 16; c += 4) {
+                        const int4 d = *reinterpret_cast<const int4*>(&st.kdoc[warp][c0 + c]);
+                        s[c] = c0 + c < lim && d.x == qdoc ? s[c] : -CUDART_INF_F;
+                        s[c + 1] = c0 + c + 1 < lim && d.y == qdoc ? s[c + 1] : -CUDART_INF_F;
+                        s[c + 2] = c0 + c + 2 < lim && d.z == qdoc ? s[c + 2] : -CUDART_INF_F;
+                        s[c + 3] = c0 + c + 3 < lim && d.w == qdoc ? s[c + 3] : -CUDART_INF_F;
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) s[c] = c0 + c < lim ? s[c] : -CUDART_INF_F;
                 }
             };
             ok = __all_sync(~0u, tc_wait(smem_u32(&st.s_full), i & 1, failed));
@@ -296,36 +310,39 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
                     float x[32];
                     tmem_ld_x32(tO + c0, x);
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) o[c0 + c] = (o[c0 + c] + x[c]) * f;
+                    for (int c = 0; c < 32; c += 2)
+                        unpack2(mul2(add2(pack2(o[c0 + c], o[c0 + c + 1]), pack2(x[c], x[c + 1])), pack2(f, f)), o[c0 + c],
+                                o[c0 + c + 1]);
                 }
                 f = 1.f;
             }
-            float top, sum;
+            float top;               // the tile's maximum, above the one in use
+            uint64_t sum;
             bool again = __any_sync(~0u, m == -CUDART_INF_F);
             if (again) {             // no maximum to go by yet
                 top = -CUDART_INF_F;
 #pragma unroll
                 for (int c0 = 0; c0 < 64; c0 += 16) {
                     float s[16];
-                    scores(c0, s);
+                    powers(c0, 0.f, s);
                     top = fmaxf(top, max_of<16, false>(s));
                 }
                 m = m == -CUDART_INF_F ? top : m;
             }
             do {
-                const float base2 = m == -CUDART_INF_F ? 0.f : m * mul;
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                const float base = m == -CUDART_INF_F ? 0.f : m;
+                uint64_t part[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
                 top = -CUDART_INF_F;
 #pragma unroll
                 for (int c0 = 0; c0 < 64; c0 += 16) {
                     float s[16];
-                    scores(c0, s);
+                    powers(c0, base, s);
                     top = fmaxf(top, max_of<16, false>(s));
                     uint32_t w[3][8];
 #pragma unroll
                     for (int c = 0; c < 16; c += 2) {
-                        const float x = ex2(fmaf(s[c], mul, -base2)), y = ex2(fmaf(s[c + 1], mul, -base2));
-                        part[c / 2 % 4] += x + y;
+                        const float x = ex2(s[c]), y = ex2(s[c + 1]);
+                        part[c / 2 % 2] = add2(part[c / 2 % 2], pack2(x, y));
                         uint32_t pc[3];
                         split3(x, y, pc);
 #pragma unroll
@@ -334,23 +351,27 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
 #pragma unroll
                     for (int k = 0; k < 3; ++k) tmem_st_x8(tP + 32 * k + c0 / 2, w[k]);
                 }
-                sum = (part[0] + part[1]) + (part[2] + part[3]);
+                sum = add2(part[0], part[1]);
                 // far above the maximum in use (or the first keys that the row sees): again with its own
-                const bool high = m == -CUDART_INF_F ? top > m : (top - m) * mul > 40.f;
+                const bool high = top > (m == -CUDART_INF_F ? -CUDART_INF_F : 40.f);
                 again = __any_sync(~0u, high);
                 if (again && high) {
-                    const float g = m == -CUDART_INF_F ? 0.f : ex2((m - top) * mul);
+                    const float g = m == -CUDART_INF_F ? 0.f : ex2(-top);
                     l *= g;
 #pragma unroll
                     for (int c = 0; c < DP; ++c) o[c] *= g;
-                    m = top;
+                    m = base + top;
                 }
             } while (again);
-            l += sum;
-            if ((top - m) * mul > 8.f) {
-                f = ex2((m - top) * mul);
+            {
+                float x, y;
+                unpack2(sum, x, y);
+                l += x + y;
+            }
+            if (top > 8.f) {
+                f = ex2(-top);
                 l *= f;
-                m = top;
+                m += top;
             }
             tmem_wait_st();
             tc_fence_before();
@@ -382,7 +403,7 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
             }
             if (row < p.Lq)
                 p.lse[((int64_t)b * p.H + h) * p.Lq + row] =
-                    l == 0.f ? -CUDART_INF_F : ((m == -CUDART_INF_F ? 0.f : m * mul) + log2f(l)) * kLn2;
+                    l == 0.f ? -CUDART_INF_F : ((m == -CUDART_INF_F ? 0.f : m) + log2f(l)) * kLn2;
         }
         if (!ok && lane == 0) tc_report(tp.status, 222);
     }
