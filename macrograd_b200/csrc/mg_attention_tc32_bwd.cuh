@@ -31,8 +31,8 @@ struct Tc32BwdState {
     uint32_t tmem;
     int failed;
     alignas(16) int doc[8][32];
-    alignas(16) float lse2[2][64];
-    alignas(16) float delta[2][64];
+    alignas(16) float lse2[2][64];       // negated
+    alignas(16) float delta[2][64];      // negated
 };
 
 constexpr int kTc32BwdThreads = 384;     // two warpgroups, three warps that load, one that issues
@@ -90,40 +90,45 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
 
     if (warp >= 8 && warp < 11) {
         // ------------------------------------------------ loads and splits of the streamed rows
-        constexpr int kLoaders = kTc32LoadWarps * 32, kItems = (64 * (DP / 8) + kLoaders - 1) / kLoaders;
-        const int tid = threadIdx.x - 256;
+        // item k of a thread: 8 elements of row r0 + 12 k of both tensors, always the same columns
+        constexpr int kRows = kTc32LoadWarps * 32 / (DP / 8), kItems = (64 + kRows - 1) / kRows;
+        const int tid = threadIdx.x - 256, r0 = tid / (DP / 8), c = tid % (DP / 8);
+        const bool in = c * 8 < p.D;
         const int64_t* s0 = kKeys ? p.qs : p.ks;
         const int64_t* s1 = kKeys ? p.dos : p.vs;
+        const float* src0 = (const float*)(kKeys ? p.q : p.k) + b * s0[0] + c * 8;
+        const float* src1 = (const float*)(kKeys ? p.dout : p.v) + b * s1[0] + c * 8;
+        const int64_t step0 = s0[2], step1 = s1[2];
         bool ok = true;
         for (int i = 0; i < n && ok; ++i) {
             const int yh = kKeys ? xh * group + i / tiles : xh / group, y0 = (t0 + (kKeys ? i % tiles : i)) * 64;
-            const float* a = (const float*)(kKeys ? p.q : p.k) + b * s0[0] + yh * s0[1];
-            const float* c = (const float*)(kKeys ? p.dout : p.v) + b * s1[0] + yh * s1[1];
+            const float* a0 = src0 + yh * s0[1] + (y0 + r0) * step0;
+            const float* a1 = src1 + yh * s1[1] + (y0 + r0) * step1;
             float4 x[kItems][2], y[kItems][2];
 #pragma unroll
             for (int k = 0; k < kItems; ++k) {
-                const int item = k * kLoaders + tid, r = item / 8, e = item % 8 * 8, row = y0 + r;
-                const bool live = r < 64 && row < yrows && e < p.D &&
+                const int row = y0 + r0 + k * kRows;
+                const bool live = in && r0 + k * kRows < 64 && row < yrows &&
                                   (!docs || doc_at(p, b, row + (kKeys ? shift : 0)) >= 0);
-                tc32_fetch(x[k], a + (int64_t)row * s0[2] + e, live);
-                tc32_fetch(y[k], c + (int64_t)row * s1[2] + e, live);
+                tc32_fetch(x[k], a0 + k * kRows * step0, live);
+                tc32_fetch(y[k], a1 + k * kRows * step1, live);
             }
-            float stat = 0.f;
-            if (kKeys && tid < 64) stat = tp.lse2[((int64_t)b * p.H + yh) * tp.Lp + y0 + tid];
-            float stat2 = 0.f;
-            if (kKeys && tid < 64) stat2 = tp.delta[((int64_t)b * p.H + yh) * tp.Lp + y0 + tid];
+            float lse2 = 0.f, delta = 0.f;
+            if (kKeys && tid < 64) {
+                lse2 = tp.lse2[((int64_t)b * p.H + yh) * tp.Lp + y0 + tid];
+                delta = tp.delta[((int64_t)b * p.H + yh) * tp.Lp + y0 + tid];
+            }
             if (i >= 2) ok = __all_sync(~0u, tc_wait(smem_u32(&st.y_empty[i & 1]), (i / 2 - 1) & 1, failed));
             if (!ok) break;
 #pragma unroll
             for (int k = 0; k < kItems; ++k) {
-                const int item = k * kLoaders + tid, r = item / 8, e = item % 8;
-                if (r >= 64) continue;
-                tc32_put(sY0(i), 64, kPieceY, r, e, x[k]);
-                tc32_put(sY0(i) + 3 * kPieceY, 64, kPieceY, r, e, y[k]);
+                if (r0 + k * kRows >= 64) continue;
+                tc32_put(sY0(i), 64, kPieceY, r0 + k * kRows, c, x[k]);
+                tc32_put(sY0(i) + 3 * kPieceY, 64, kPieceY, r0 + k * kRows, c, y[k]);
             }
             if (kKeys && tid < 64) {
-                st.lse2[i & 1][tid] = stat;
-                st.delta[i & 1][tid] = stat2;
+                st.lse2[i & 1][tid] = -lse2;
+                st.delta[i & 1][tid] = -delta;
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -203,14 +208,15 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
         if (n > 0) {
             const int64_t* s = kKeys ? (wg ? p.vs : p.ks) : (wg ? p.dos : p.qs);
             const float* src = (const float*)(kKeys ? (wg ? p.v : p.k) : (wg ? p.dout : p.q)) + b * s[0] + xh * s[1];
-#pragma unroll 4
+            float4 x[DP / 8][2];
+#pragma unroll
             for (int i = 0; i < DP / 8; ++i) {
-                const int item = i * 128 + r, row = x0 + item / 8, e = item % 8;
-                float4 x[2];
-                tc32_fetch(x, src + (int64_t)row * s[2] + e * 8,
+                const int row = x0 + r / 8 + 16 * i, e = r % 8;
+                tc32_fetch(x[i], src + row * s[2] + e * 8,
                            row < xrows && e * 8 < p.D && (!docs || doc_at(p, b, row + (kKeys ? 0 : shift)) >= 0));
-                tc32_put(wg ? sX1 : sX0, 128, kPieceX, item / 8, e, x);
             }
+#pragma unroll
+            for (int i = 0; i < DP / 8; ++i) tc32_put(wg ? sX1 : sX0, 128, kPieceX, r / 8 + 16 * i, r % 8, x[i]);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&st.x_full));
@@ -221,8 +227,8 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
         float lse2 = 0.f, delta = 0.f;
         if (!kKeys) {
             const int64_t at = ((int64_t)b * p.H + xh) * tp.Lp + x0 + r;
-            lse2 = tp.lse2[at];
-            delta = tp.delta[at];
+            lse2 = -tp.lse2[at];
+            delta = -tp.delta[at];
         }
         // this thread's accumulators: dK (warpgroup 0) or dV (1), or half of dQ
         constexpr int kAcc = kKeys ? 64 : 32;
@@ -236,7 +242,8 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                 float x[32];
                 tmem_ld_x32(tAcc + c, x);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[c + k] += x[k];
+                for (int k = 0; k < 32; k += 2)
+                    unpack2(add2(pack2(o[c + k], o[c + k + 1]), pack2(x[k], x[k + 1])), o[c + k], o[c + k + 1]);
             }
         };
         for (int i = 0; i < n; ++i) {
@@ -279,45 +286,93 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
             }
             if (kCap) cap_scores32(v, pre, 1.f);
             const float far = (float)(pos - ypos - col);
-            uint32_t w[3][16];
+            const uint64_t mul_2 = pack2(mul, mul);
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-                float e[2];
+            for (int c0 = 0; c0 < 32; c0 += 16) {
+                float e[16];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float nl = -(kKeys ? st.lse2[i & 1][col + c + k] : lse2);
-                    if (kBias) nl = fmaf(-slope, fabsf(far - (float)(c + k)), nl);
-                    e[k] = ex2(fmaf(v[c + k], mul, nl));
-                    bool seen = true;
-                    if (!full) {
-                        seen = col + c + k >= lo && col + c + k < hi;
-                        if (docs) seen = seen && st.doc[warp][c + k] == rdoc;
-                        e[k] = seen ? e[k] : 0.f;
+                for (int c = 0; c < 16; c += 4) {
+                    float nl[4] = {lse2, lse2, lse2, lse2};
+                    if (kKeys) {
+                        const float4 x = *reinterpret_cast<const float4*>(&st.lse2[i & 1][col + c0 + c]);
+                        nl[0] = x.x, nl[1] = x.y, nl[2] = x.z, nl[3] = x.w;
                     }
-                    const float curve = kCap ? fmaf(-v[c + k], v[c + k], 1.f) : 1.f;
-                    const float d = e[k] * curve * (g[c + k] - (kKeys ? st.delta[i & 1][col + c + k] : delta));
-                    g[c + k] = seen ? d : 0.f;
+                    if (kBias) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) nl[k] = fmaf(-slope, fabsf(far - (float)(c0 + c + k)), nl[k]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k += 2) {
+                        unpack2(fma2(pack2(v[c0 + c + k], v[c0 + c + k + 1]), mul_2, pack2(nl[k], nl[k + 1])), e[c + k],
+                                e[c + k + 1]);
+                        e[c + k] = ex2(e[c + k]);
+                        e[c + k + 1] = ex2(e[c + k + 1]);
+                    }
+                }
+                if (!full) {
+                    // a pair that is not seen: P = 0, and its dP does not count
+                    if (docs) {
+#pragma unroll
+                        for (int c = 0; c < 16; c += 4) {
+                            const int4 d = *reinterpret_cast<const int4*>(&st.doc[warp][c0 + c]);
+                            const int at = col + c0 + c;
+                            e[c] = at >= lo && at < hi && d.x == rdoc ? e[c] : 0.f;
+                            e[c + 1] = at + 1 >= lo && at + 1 < hi && d.y == rdoc ? e[c + 1] : 0.f;
+                            e[c + 2] = at + 2 >= lo && at + 2 < hi && d.z == rdoc ? e[c + 2] : 0.f;
+                            e[c + 3] = at + 3 >= lo && at + 3 < hi && d.w == rdoc ? e[c + 3] : 0.f;
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            const int at = col + c0 + c;
+                            e[c] = (kKeys ? at >= lo : at < hi) ? e[c] : 0.f;
+                        }
+                    }
                 }
                 if (kKeys) {
-                    uint32_t pc[3];
-                    split3(e[0], e[1], pc);
+                    uint32_t w[3][8];
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) w[k][c / 2] = pc[k];
+                    for (int c = 0; c < 16; c += 2) {
+                        uint32_t pc[3];
+                        split3(e[c], e[c + 1], pc);
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) w[k][c / 2] = pc[k];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) tmem_st_x8(tP + lanes + 32 * k + (col + c0) / 2, w[k]);
                 }
+                // dS = P * curve * (dP - delta)
+                uint32_t w[3][8];
+#pragma unroll
+                for (int c = 0; c < 16; c += 4) {
+                    float nd[4] = {delta, delta, delta, delta};
+                    if (kKeys) {
+                        const float4 x = *reinterpret_cast<const float4*>(&st.delta[i & 1][col + c0 + c]);
+                        nd[0] = x.x, nd[1] = x.y, nd[2] = x.z, nd[3] = x.w;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k += 2) {
+                        const int at = c0 + c + k;
+                        uint64_t q = pack2(e[c + k], e[c + k + 1]);
+                        if (kCap) {
+                            const uint64_t t = pack2(v[at], v[at + 1]);
+                            q = mul2(q, fma2(mul2(t, pack2(-1.f, -1.f)), t, pack2(1.f, 1.f)));
+                        }
+                        float x, y;
+                        unpack2(mul2(q, add2(pack2(g[at], g[at + 1]), pack2(nd[k], nd[k + 1]))), x, y);
+                        if (!full) {
+                            x = e[c + k] == 0.f ? 0.f : x;
+                            y = e[c + k + 1] == 0.f ? 0.f : y;
+                        }
+                        uint32_t pc[3];
+                        split3(x, y, pc);
+#pragma unroll
+                        for (int z = 0; z < 3; ++z) w[z][(c + k) / 2] = pc[z];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 3; ++k) tmem_st_x8(tdS + lanes + 32 * k + (col + c0) / 2, w[k]);
             }
-            if (kKeys) {
-#pragma unroll
-                for (int k = 0; k < 3; ++k) tmem_st_x16(tP + lanes + 32 * k + col / 2, w[k]);
-            }
-#pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-                uint32_t pc[3];
-                split3(g[c], g[c + 1], pc);
-#pragma unroll
-                for (int k = 0; k < 3; ++k) w[k][c / 2] = pc[k];
-            }
-#pragma unroll
-            for (int k = 0; k < 3; ++k) tmem_st_x16(tdS + lanes + 32 * k + col / 2, w[k]);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
