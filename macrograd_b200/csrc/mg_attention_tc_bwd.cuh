@@ -14,21 +14,24 @@
 // P and dS go back to tensor memory over S and dP, as the A operand of the
 // second pair of products: they never pass through shared memory.
 //
-// Two warpgroups take the tiles in turn, each with S and dP columns of its own, so
-// that the tensor core works for one while the other takes exponentials. P lies over
-// S and dS over dP, which are all the columns there are at head_dim 128 (2 x (64 +
-// 64) + 128 + 128 = 512, hence one block an SM), so a warpgroup's next S is issued
+// Two sets of eight warps take the tiles in turn, each with S and dP columns of its
+// own, so that the tensor core works for one while the other takes exponentials. In a
+// set two warps share 32 rows, 32 of the tile's columns each: the work is bound by
+// the latency of its instructions, which four warps a scheduler hide better than two (with
+// two, a tile took 3800 clocks of its set's time). P lies over S and dS over dP, which are all the columns there are at head_dim 128 (2 x (64 +
+// 64) + 128 + 128 = 512, hence one block an SM), so a set's next S is issued
 // as soon as its P has been multiplied (the queries resident: as soon as S is in
 // registers), under the dS of the same tile, and its next dP after its dS: it
 // finds both when it comes to them. Issued together, after dS, they cost each
-// warpgroup another 2700 clocks a tile, against 3200 of its own work.
+// set another 2700 clocks a tile.
 #pragma once
 
 #include "mg_attention_tc.cuh"
 
 namespace mg {
 
-constexpr int kTcBwdThreads = 320;       // two warpgroups, loads, products
+constexpr int kTcBwdThreads = 576;       // two sets of eight warps, loads, products
+constexpr int kTcBwdLoadWarp = 16, kTcBwdMmaWarp = 17;
 constexpr int kTcBwdStages = 4;
 
 struct TcBwdParams {
@@ -100,7 +103,7 @@ struct TcBwdState {
     uint32_t tmem;
     int failed;
     int loads;                           // stages that were asked for
-    alignas(16) int doc[8][64];          // documents of the streamed rows, a copy a warp
+    alignas(16) int doc[16][32];         // documents of a warp's streamed rows
     alignas(16) float lse2[kTcBwdStages][64];
     alignas(16) float delta[kTcBwdStages][64];
 };
@@ -163,8 +166,8 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&st.s_full[i]), 1);
             mbar_init(smem_u32(&st.dp_full[i]), 1);
-            mbar_init(smem_u32(&st.p_full[i]), 4);
-            mbar_init(smem_u32(&st.ds_full[i]), 4);
+            mbar_init(smem_u32(&st.p_full[i]), 8);
+            mbar_init(smem_u32(&st.ds_full[i]), 8);
         }
         mbar_init(smem_u32(&st.acc_full), 1);
         mbar_init(smem_u32(&st.drain), 1);
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
         st.failed = 0;
         st.loads = 0;
     }
-    if (warp == 9) {
+    if (warp == kTcBwdMmaWarp) {
         tmem_alloc(smem_u32(&st.tmem), 512);
         tmem_relinquish();
     }
@@ -184,11 +187,11 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
     const int tiles = max(0, t1 - t0), n = kKeys ? tiles * group : tiles;
     const uint32_t tA = st.tmem + 256, tB = tA + DP;     // accumulators: dS Y0, P Y1
     volatile int* failed = &st.failed;
-    // columns of step i's S (and P) and dP (and dS)
+    // columns of step i's S and dP; the 16-bit P and dS of columns [32 h, 32 h + 32) lie in the first 16 of these
     const auto tS = [&](int i) { return st.tmem + 128 * (i & 1); };
     const auto sY0 = [&](int i) { return sY + (uint32_t)(i % kTcBwdStages) * 2 * kY; };
 
-    if (warp == 8) {
+    if (warp == kTcBwdLoadWarp) {
         // ------------------------------------------------ loads
         if (lane == 0 && n > 0) {
             constexpr int X0 = kKeys ? 1 : 0, X1 = kKeys ? 2 : 3, Y0 = kKeys ? 0 : 1, Y1 = kKeys ? 3 : 2;
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                 st.loads = i + 1;
             }
         }
-    } else if (warp == 9) {
+    } else if (warp == kTcBwdMmaWarp) {
         // ------------------------------------------------ products
         constexpr uint32_t idesc_dp = idesc_bf16(128, 64, false, false), idesc_acc = idesc_bf16(128, DP, false, true);
         bool ok = n == 0 || __all_sync(~0u, tc_wait(smem_u32(&st.x_full), 0, failed));
@@ -259,7 +262,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             if (kKeys) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    tc_mma_f16_ta(tB, tS(i) + 8 * k, desc_mn_major(sY0(i) + kY, 64, k), idesc_acc, i > 0 || k > 0);
+                    tc_mma_f16_ta(tB, tS(i) + 8 * k + 16 * (k / 2), desc_mn_major(sY0(i) + kY, 64, k), idesc_acc, i > 0 || k > 0);
             }
             if (i + 2 < n) scores_of(i + 2);
             ok = __all_sync(~0u, ok && tc_wait(smem_u32(&st.ds_full[i & 1]), (i >> 1) & 1, failed));
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                tc_mma_f16_ta(tA, tS(i) + 64 + 8 * k, desc_mn_major(sY0(i), 64, k), idesc_acc, i > 0 || k > 0);
+                tc_mma_f16_ta(tA, tS(i) + 64 + 8 * k + 16 * (k / 2), desc_mn_major(sY0(i), 64, k), idesc_acc, i > 0 || k > 0);
             tc_commit_warp(smem_u32(&st.y_empty[i % kTcBwdStages]));
             if (i + 1 == n) tc_commit_warp(smem_u32(&st.acc_full));
             if (i + 2 < n) dp_of(i + 2);
@@ -283,7 +286,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
         }
     } else {
         // ------------------------------------------------ P and dS
-        const int wg = warp / 4, r = threadIdx.x % 128;          // this thread's resident row
+        const int set = warp / 8, col = 32 * (warp / 4 % 2), r = threadIdx.x % 128;   // resident row, first column
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;
         const int pos = xpos + r;
         const int rdoc = docs ? (x0 + r < xrows ? doc_at(p, b, pos) : -1) : 0;
@@ -296,7 +299,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             delta = tp.delta[at];
         }
         bool ok = true;
-        for (int i = wg; i < n; i += 2) {
+        for (int i = set; i < n; i += 2) {
             const int h = kKeys ? xh * group + i / tiles : xh;
             const int y0 = (t0 + (kKeys ? i % tiles : i)) * 64, ypos = y0 + (kKeys ? shift : 0);
             const int s = i % kTcBwdStages;
@@ -316,48 +319,52 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                 full = full && common >= 0 && (!kKeys || y0 + 64 <= p.Lq) && common_doc(dt, ypos, 64, p.Lk) == common;
                 if (!full) {
                     __syncwarp();
-                    st.doc[warp][lane] = doc_at(p, b, ypos + lane);
-                    st.doc[warp][lane + 32] = doc_at(p, b, ypos + lane + 32);
+                    st.doc[warp][lane] = doc_at(p, b, ypos + col + lane);
                     __syncwarp();
                 }
             }
-            ok = __all_sync(~0u, tc_wait(smem_u32(&st.s_full[wg]), (i >> 1) & 1, failed) &&
+            ok = __all_sync(~0u, tc_wait(smem_u32(&st.s_full[set]), (i >> 1) & 1, failed) &&
                                      (!kKeys || tc_wait(smem_u32(&st.y_full[s]), (i / kTcBwdStages) & 1, failed)));
             if (!ok) break;
             tc_fence_after();
-            float v[64];
-            tmem_ld_x64(tS(i) + lanes, v);
+            float v[32];
+            tmem_ld_x32(tS(i) + lanes + col, v);
             if (!kKeys) {                         // S may be overwritten
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&st.p_full[wg]));
+                if (lane == 0) mbar_arrive(smem_u32(&st.p_full[set]));
             }
             if (kCap) cap_scores(v, tp.curve);      // tanh of the score over the cap
-            uint32_t w[32];
-            const float far = (float)(pos - ypos);
+            uint32_t w[16];
+            const float far = (float)(pos - ypos - col);
+            const uint64_t mul_2 = pack2(mul, mul);
 #pragma unroll
-            for (int c = 0; c < 64; c += 4) {
-                float4 l4;
-                if (kKeys) l4 = *reinterpret_cast<const float4*>(&st.lse2[s][c]);
-                const float ls[4] = {kKeys ? l4.x : lse2, kKeys ? l4.y : lse2, kKeys ? l4.z : lse2, kKeys ? l4.w : lse2};
+            for (int c = 0; c < 32; c += 4) {
+                float nl[4] = {-lse2, -lse2, -lse2, -lse2};
+                if (kKeys) {
+                    const float4 x = *reinterpret_cast<const float4*>(&st.lse2[s][col + c]);
+                    nl[0] = -x.x, nl[1] = -x.y, nl[2] = -x.z, nl[3] = -x.w;
+                }
+                if (kBias) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) nl[k] = fmaf(-slope, fabsf(far - (float)(c + k)), nl[k]);
+                }
                 float e[4];
 #pragma unroll
                 for (int k = 0; k < 4; k += 2) {
-                    float nl0 = -ls[k], nl1 = -ls[k + 1];
-                    if (kBias) {
-                        nl0 = fmaf(-slope, fabsf(far - (float)(c + k)), nl0);
-                        nl1 = fmaf(-slope, fabsf(far - (float)(c + k + 1)), nl1);
-                    }
-                    unpack2(fma2(pack2(v[c + k], v[c + k + 1]), pack2(mul, mul), pack2(nl0, nl1)), e[k], e[k + 1]);
+                    unpack2(fma2(pack2(v[c + k], v[c + k + 1]), mul_2, pack2(nl[k], nl[k + 1])), e[k], e[k + 1]);
                     e[k] = ex2(e[k]);
                     e[k + 1] = ex2(e[k + 1]);
                 }
                 if (!full) {
-                    const int4 d4 = docs ? *reinterpret_cast<const int4*>(&st.doc[warp][c]) : make_int4(0, 0, 0, 0);
-                    const int ds[4] = {d4.x, d4.y, d4.z, d4.w};
+                    int d[4] = {rdoc, rdoc, rdoc, rdoc};
+                    if (docs) {
+                        const int4 x = *reinterpret_cast<const int4*>(&st.doc[warp][c]);
+                        d[0] = x.x, d[1] = x.y, d[2] = x.z, d[3] = x.w;
+                    }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const bool seen = c + k >= lo && c + k < hi && ds[k] == rdoc;
+                        const bool seen = col + c + k >= lo && col + c + k < hi && d[k] == rdoc;
                         e[k] = seen ? e[k] : 0.f;
                         if (kCap) v[c + k] = seen ? v[c + k] : 0.f;
                     }
@@ -367,31 +374,39 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                     w[c / 2 + 1] = bf16x2(e[2], e[3]);
                 }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[c + k] = kCap ? e[k] * fmaf(-v[c + k], v[c + k], 1.f) : e[k];
+                for (int k = 0; k < 4; k += 2) {
+                    uint64_t q = pack2(e[k], e[k + 1]);
+                    if (kCap) {
+                        const uint64_t t = pack2(v[c + k], v[c + k + 1]);
+                        q = mul2(q, fma2(mul2(t, pack2(-1.f, -1.f)), t, pack2(1.f, 1.f)));
+                    }
+                    unpack2(q, v[c + k], v[c + k + 1]);
+                }
             }
             if (kKeys) {
-                tmem_st_x32(tS(i) + lanes, w);
+                tmem_st_x16(tS(i) + lanes + col, w);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&st.p_full[wg]));
+                if (lane == 0) mbar_arrive(smem_u32(&st.p_full[set]));
             }
-            ok = __all_sync(~0u, tc_wait(smem_u32(&st.dp_full[wg]), (i >> 1) & 1, failed));
+            ok = __all_sync(~0u, tc_wait(smem_u32(&st.dp_full[set]), (i >> 1) & 1, failed));
             if (!ok) break;
             tc_fence_after();
-            float g[64];
-            tmem_ld_x64(tS(i) + 64 + lanes, g);
+            float g[32];
+            tmem_ld_x32(tS(i) + 64 + lanes + col, g);
 #pragma unroll
-            for (int c = 0; c < 64; c += 4) {
-                float4 d4;
-                if (kKeys) d4 = *reinterpret_cast<const float4*>(&st.delta[s][c]);
-                const float ds[4] = {kKeys ? d4.x : delta, kKeys ? d4.y : delta, kKeys ? d4.z : delta,
-                                     kKeys ? d4.w : delta};
+            for (int c = 0; c < 32; c += 4) {
+                float nd[4] = {-delta, -delta, -delta, -delta};
+                if (kKeys) {
+                    const float4 x = *reinterpret_cast<const float4*>(&st.delta[s][col + c]);
+                    nd[0] = -x.x, nd[1] = -x.y, nd[2] = -x.z, nd[3] = -x.w;
+                }
                 float e[4];
 #pragma unroll
                 for (int k = 0; k < 4; k += 2)
                     unpack2(mul2(pack2(v[c + k], v[c + k + 1]),
-                                 add2(pack2(g[c + k], g[c + k + 1]), pack2(-ds[k], -ds[k + 1]))),
+                                 add2(pack2(g[c + k], g[c + k + 1]), pack2(nd[k], nd[k + 1]))),
                             e[k], e[k + 1]);
                 if (!full) {
 #pragma unroll
@@ -400,34 +415,35 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                 w[c / 2] = bf16x2(e[0], e[1]);
                 w[c / 2 + 1] = bf16x2(e[2], e[3]);
             }
-            tmem_st_x32(tS(i) + 64 + lanes, w);
+            tmem_st_x16(tS(i) + 64 + lanes + col, w);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&st.ds_full[wg]));
+            if (lane == 0) mbar_arrive(smem_u32(&st.ds_full[set]));
         }
         if (ok && n > 0) ok = __all_sync(~0u, tc_wait(smem_u32(&st.acc_full), 0, failed));
         if (ok) {
             tc_fence_after();
-            // with the keys: one warpgroup stores dK, the other dV; with the queries: half of dQ each
-            const bool is_dv = kKeys && wg == 1;
+            // with the keys: half of dK or of dV to each four warps; with the queries: a quarter of dQ
+            const int quarter = warp / 4;
+            const bool is_dv = kKeys && quarter >= 2;
             const int64_t* os = kKeys ? (is_dv ? p.dvs : p.dks) : p.dqs;
             __nv_bfloat16* out = (__nv_bfloat16*)(kKeys ? (is_dv ? p.dv : p.dk) : p.dq) + b * os[0] + xh * os[1] +
                                  (int64_t)(x0 + r) * os[2];
             const float f = is_dv ? 1.f : p.scale;
-            const int c0 = kKeys ? 0 : wg * (DP / 2), c1 = min(p.D, kKeys ? DP : c0 + DP / 2);
+            const int c0 = kKeys ? quarter % 2 * (DP / 2) : quarter * (DP / 4), c1 = min(p.D, c0 + DP / (kKeys ? 2 : 4));
 #pragma unroll 1
-            for (int c = c0; c < c1; c += 32) {
-                float o[32];
+            for (int c = c0; c < c1; c += 16) {
+                float o[16];
                 if (n > 0) {
-                    tmem_ld_x32((is_dv ? tB : tA) + lanes + c, o);
+                    tmem_ld_x16((is_dv ? tB : tA) + lanes + c, o);
                 } else {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = 0.f;
+                    for (int k = 0; k < 16; ++k) o[k] = 0.f;
                 }
                 if (x0 + r >= xrows) continue;
 #pragma unroll
-                for (int k = 0; k < 32; k += 8)
+                for (int k = 0; k < 16; k += 8)
                     if (c + k + 8 <= c1)
                         *reinterpret_cast<uint4*>(out + c + k) =
                             make_uint4(bf16x2(o[k] * f, o[k + 1] * f), bf16x2(o[k + 2] * f, o[k + 3] * f),
@@ -444,7 +460,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
         for (int i = max(0, st.loads - kTcBwdStages); i < st.loads; ++i)
             tc_drain(smem_u32(&st.y_full[i % kTcBwdStages]), (i / kTcBwdStages) & 1);
     }
-    if (warp == 9) tmem_dealloc(st.tmem, 512);
+    if (warp == kTcBwdMmaWarp) tmem_dealloc(st.tmem, 512);
 }
 
 }  // namespace mg
