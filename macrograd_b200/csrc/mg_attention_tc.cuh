@@ -236,6 +236,31 @@ __device__ __forceinline__ void cap_scores(float (&s)[N], const CapCurve& cc)
     }
 }
 
+// ---------------------------------------------------------------- masks
+// Masks are words, bit i for column i of 32: tests of single bits of a word cost
+// one instruction to several columns, comparisons of positions and documents two to
+// three to each (the masked tiles were bound by them).
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
+// got[w] bit i: whether theirs[w] of lane i is this thread's document `mine` (below 0:
+// none is). One round for each document among the warp's own. Whole warp.
+template <int W>
+__device__ __forceinline__ void same_document(int mine, const int (&theirs)[W], uint32_t (&got)[W])
+{
+#pragma unroll
+    for (int w = 0; w < W; ++w) got[w] = 0;
+    uint32_t todo = __ballot_sync(~0u, mine >= 0);
+    while (todo) {
+        const int v = __shfl_sync(~0u, mine, __ffs(todo) - 1);
+        todo &= ~__ballot_sync(~0u, mine == v);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const uint32_t m = __ballot_sync(~0u, theirs[w] == v);
+            if (mine == v) got[w] = m;
+        }
+    }
+}
+
 // ---------------------------------------------------------------- parameters
 struct TcAttnParams {
     CUtensorMap q, k, v, dout;   // {D, rows, heads, batch}, boxes of 64 x 128 rows
@@ -254,7 +279,6 @@ struct TcState {
     int failed;
     int loads[2];                // tiles of K and of V that were asked for
     float top[2][2][128];        // [tile parity][half][query] maximum of half a row; at the end its sum
-    alignas(16) int kdoc[8][64];     // documents of the keys, a copy a warp (read as int4)
 };
 
 __device__ __forceinline__ void tc_report(int* status, int where)
@@ -430,20 +454,28 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] = pack2(0.f, 0.f);
         bool ok = true;
+        // documents of a tile's keys (this lane's two) and their span, a tile ahead
+        int kdoc[2] = {-1, -1};
+        int2 span = make_int2(0, 0);
+        const auto look_up = [&](int j) {
+            const int k0 = (t0 + j) * 128 + 64 * half;
+            span = __ldg(dt + t0 + j);
+            kdoc[0] = doc_at(p, b, k0 + lane);
+            kdoc[1] = doc_at(p, b, k0 + 32 + lane);
+        };
+        if (docs && n > 0) look_up(0);
         for (int j = 0; j < n; ++j) {
             const int k0 = (t0 + j) * 128 + 64 * half;
             // whether any of the half tile's pairs is masked (same for all threads of the half)
             bool full = k0 + 64 <= p.Lk && (!p.causal || k0 + 63 <= q0 + shift || k0 + 64 <= prefix);
-            if (docs) {
-                const int2 d = __ldg(dt + t0 + j);
-                full = full && common >= 0 && d.x == d.y && d.x == common;
-                if (!full) {
-                    __syncwarp();
-                    st.kdoc[warp][lane] = doc_at(p, b, k0 + lane);
-                    st.kdoc[warp][lane + 32] = doc_at(p, b, k0 + 32 + lane);
-                    __syncwarp();
-                }
+            if (docs) full = full && common >= 0 && span.x == span.y && span.x == common;
+            uint32_t seen[2] = {~0u, ~0u};
+            if (!full) {
+                if (docs) same_document(qdoc, kdoc, seen);
+                seen[0] &= bits_below(upto - k0);
+                seen[1] &= bits_below(upto - k0 - 32);
             }
+            if (docs && j + 1 < n) look_up(j + 1);
             ok = __all_sync(~0u, tc_wait(smem_u32(&st.s_full), j & 1, failed));
             if (!ok) break;
             tc_fence_after();
@@ -461,21 +493,8 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
                 for (int c = 0; c < 64; ++c) s[c] = fmaf(-slope, fabsf(far - (float)c), s[c]);
             }
             if (!full) {
-                const int lim = upto - k0;
-                if (docs) {
-                    const int4* kd = reinterpret_cast<const int4*>(st.kdoc[warp]);
 #pragma unroll
-                    for (int c = 0; c < 64; c += 4) {
-                        const int4 d = kd[c / 4];
-                        s[c] = c < lim && d.x == qdoc ? s[c] : -CUDART_INF_F;
-                        s[c + 1] = c + 1 < lim && d.y == qdoc ? s[c + 1] : -CUDART_INF_F;
-                        s[c + 2] = c + 2 < lim && d.z == qdoc ? s[c + 2] : -CUDART_INF_F;
-                        s[c + 3] = c + 3 < lim && d.w == qdoc ? s[c + 3] : -CUDART_INF_F;
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 64; ++c) s[c] = c < lim ? s[c] : -CUDART_INF_F;
-                }
+                for (int c = 0; c < 64; ++c) s[c] = seen[c / 32] >> (c % 32) & 1 ? s[c] : -CUDART_INF_F;
             }
             // the row's maximum; past this barrier both halves have their scores in registers
             const float mine = max_of<64, false>(s);

@@ -88,7 +88,6 @@ struct Tc32State {
     uint64_t q_full, k_full, v_full, s_full, p_full, o_full, drain;
     uint32_t tmem;
     int failed;
-    alignas(16) int kdoc[4][64];
 };
 
 // Four warps of exponentials, three that load, one that issues.
@@ -259,17 +258,17 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
         for (int i = 0; i < n; ++i) {
             const int k0 = (t0 + i) * 64;
             bool full = k0 + 64 <= p.Lk && (!p.causal || k0 + 63 <= q0 + shift || k0 + 64 <= prefix);
-            if (docs) {
-                full = full && common >= 0 && common_doc(dt, k0, 64, p.Lk) == common;
-                if (!full) {
-                    __syncwarp();
-                    st.kdoc[warp][lane] = doc_at(p, b, k0 + lane);
-                    st.kdoc[warp][lane + 32] = doc_at(p, b, k0 + 32 + lane);
-                    __syncwarp();
+            if (docs) full = full && common >= 0 && common_doc(dt, k0, 64, p.Lk) == common;
+            uint32_t seen[2] = {~0u, ~0u};
+            if (!full) {
+                if (docs) {
+                    const int kdoc[2] = {doc_at(p, b, k0 + lane), doc_at(p, b, k0 + 32 + lane)};
+                    same_document(qdoc, kdoc, seen);
                 }
+                seen[0] &= bits_below(upto - k0);
+                seen[1] &= bits_below(upto - k0 - 32);
             }
             const float far = (float)(qpos - k0);
-            const int lim = upto - k0;
             // columns [c0, c0 + 16): the powers of two less `base`, -inf where masked
             const auto powers = [&](int c0, float base, float (&s)[16]) {
                 tmem_ld_x16(tS + c0, s);
@@ -284,19 +283,8 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
                     unpack2(fma2(pack2(s[c], s[c + 1]), pack2(mul, mul), pack2(b0, b1)), s[c], s[c + 1]);
                 }
                 if (full) return;
-                if (docs) {
 #pragma unroll
-                    for (int c = 0; c < 16; c += 4) {
-                        const int4 d = *reinterpret_cast<const int4*>(&st.kdoc[warp][c0 + c]);
-                        s[c] = c0 + c < lim && d.x == qdoc ? s[c] : -CUDART_INF_F;
-                        s[c + 1] = c0 + c + 1 < lim && d.y == qdoc ? s[c + 1] : -CUDART_INF_F;
-                        s[c + 2] = c0 + c + 2 < lim && d.z == qdoc ? s[c + 2] : -CUDART_INF_F;
-                        s[c + 3] = c0 + c + 3 < lim && d.w == qdoc ? s[c + 3] : -CUDART_INF_F;
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) s[c] = c0 + c < lim ? s[c] : -CUDART_INF_F;
-                }
+                for (int c = 0; c < 16; ++c) s[c] = seen[c0 / 32] >> (c0 % 32 + c) & 1 ? s[c] : -CUDART_INF_F;
             };
             ok = __all_sync(~0u, tc_wait(smem_u32(&st.s_full), i & 1, failed));
             if (!ok) break;

@@ -30,7 +30,6 @@ struct Tc32BwdState {
     uint64_t x_full, y_full[2], y_empty[2], s_full, s_free, p_full, acc_full, drain;
     uint32_t tmem;
     int failed;
-    alignas(16) int doc[8][32];
     alignas(16) float lse2[2][64];       // negated
     alignas(16) float delta[2][64];      // negated
 };
@@ -246,28 +245,24 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                     unpack2(add2(pack2(o[c + k], o[c + k + 1]), pack2(x[k], x[k + 1])), o[c + k], o[c + k + 1]);
             }
         };
+        // this lane's document of a tile's streamed rows, a tile ahead
+        const auto y_of = [&](int i) { return (t0 + (kKeys ? i % tiles : i)) * 64; };
+        int ydoc[1] = {docs && n > 0 ? doc_at(p, b, y_of(0) + (kKeys ? shift : 0) + col + lane) : -1};
         for (int i = 0; i < n; ++i) {
             const int h = kKeys ? xh * group + i / tiles : xh;
-            const int y0 = (t0 + (kKeys ? i % tiles : i)) * 64, ypos = y0 + (kKeys ? shift : 0);
+            const int y0 = y_of(i), ypos = y0 + (kKeys ? shift : 0);
             const float slope = kBias ? __ldg(p.slopes + h) * kLog2e : 0.f;
-            int lo = 0, hi = 64;
             bool full;
-            if (kKeys) {
-                if (p.causal && pos >= prefix) lo = max(0, pos - ypos);
-                full = !p.causal || ypos >= xpos + 127 || xpos + 128 <= prefix;
-            } else {
-                hi = (!p.causal ? p.Lk : min(p.Lk, max(pos + 1, prefix))) - ypos;
-                full = ypos + 64 <= p.Lk && (!p.causal || ypos + 63 <= xpos || ypos + 64 <= prefix);
+            uint32_t seen[1] = {~0u};
+            if (kKeys) full = !p.causal || ypos >= xpos + 127 || xpos + 128 <= prefix;
+            else full = ypos + 64 <= p.Lk && (!p.causal || ypos + 63 <= xpos || ypos + 64 <= prefix);
+            if (docs) full = full && common >= 0 && (!kKeys || y0 + 64 <= p.Lq) && common_doc(dt, ypos, 64, p.Lk) == common;
+            if (!full) {
+                if (docs) same_document(rdoc, ydoc, seen);
+                if (!kKeys) seen[0] &= bits_below((!p.causal ? p.Lk : min(p.Lk, max(pos + 1, prefix))) - ypos - col);
+                else if (p.causal && pos >= prefix) seen[0] &= ~bits_below(pos - ypos - col);
             }
-            if (docs) {
-                if (rdoc < 0) hi = 0;
-                full = full && common >= 0 && (!kKeys || y0 + 64 <= p.Lq) && common_doc(dt, ypos, 64, p.Lk) == common;
-                if (!full) {
-                    __syncwarp();
-                    st.doc[warp][lane] = doc_at(p, b, ypos + col + lane);
-                    __syncwarp();
-                }
-            }
+            if (docs && i + 1 < n) ydoc[0] = doc_at(p, b, y_of(i + 1) + (kKeys ? shift : 0) + col + lane);
             ok = __all_sync(~0u, tc_wait(smem_u32(&st.s_full), i & 1, failed) &&
                                      (!kKeys || tc_wait(smem_u32(&st.y_full[i & 1]), (i >> 1) & 1, failed)));
             if (!ok) break;
@@ -311,23 +306,8 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                 }
                 if (!full) {
                     // a pair that is not seen: P = 0, and its dP does not count
-                    if (docs) {
 #pragma unroll
-                        for (int c = 0; c < 16; c += 4) {
-                            const int4 d = *reinterpret_cast<const int4*>(&st.doc[warp][c0 + c]);
-                            const int at = col + c0 + c;
-                            e[c] = at >= lo && at < hi && d.x == rdoc ? e[c] : 0.f;
-                            e[c + 1] = at + 1 >= lo && at + 1 < hi && d.y == rdoc ? e[c + 1] : 0.f;
-                            e[c + 2] = at + 2 >= lo && at + 2 < hi && d.z == rdoc ? e[c + 2] : 0.f;
-                            e[c + 3] = at + 3 >= lo && at + 3 < hi && d.w == rdoc ? e[c + 3] : 0.f;
-                        }
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) {
-                            const int at = col + c0 + c;
-                            e[c] = (kKeys ? at >= lo : at < hi) ? e[c] : 0.f;
-                        }
-                    }
+                    for (int c = 0; c < 16; ++c) e[c] = seen[0] >> (c0 + c) & 1 ? e[c] : 0.f;
                 }
                 if (kKeys) {
                     uint32_t w[3][8];

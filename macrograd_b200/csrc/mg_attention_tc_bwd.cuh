@@ -103,7 +103,6 @@ struct TcBwdState {
     uint32_t tmem;
     int failed;
     int loads;                           // stages that were asked for
-    alignas(16) int doc[16][32];         // documents of a warp's streamed rows
     alignas(16) float lse2[kTcBwdStages][64];
     alignas(16) float delta[kTcBwdStages][64];
 };
@@ -299,30 +298,25 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             delta = tp.delta[at];
         }
         bool ok = true;
+        // this lane's document of a tile's streamed rows, a tile of the set ahead
+        const auto y_of = [&](int i) { return (t0 + (kKeys ? i % tiles : i)) * 64; };
+        int ydoc[1] = {docs && set < n ? doc_at(p, b, y_of(set) + (kKeys ? shift : 0) + col + lane) : -1};
         for (int i = set; i < n; i += 2) {
             const int h = kKeys ? xh * group + i / tiles : xh;
-            const int y0 = (t0 + (kKeys ? i % tiles : i)) * 64, ypos = y0 + (kKeys ? shift : 0);
+            const int y0 = y_of(i), ypos = y0 + (kKeys ? shift : 0);
             const int s = i % kTcBwdStages;
             const float slope = kBias ? __ldg(p.slopes + h) * kLog2e : 0.f;
-            // this row's streamed rows [lo, hi) as far as causal, prefix and the ends go
-            int lo = 0, hi = 64;
             bool full;
-            if (kKeys) {
-                if (p.causal && pos >= prefix) lo = max(0, pos - ypos);
-                full = !p.causal || ypos >= xpos + 127 || xpos + 128 <= prefix;
-            } else {
-                hi = (!p.causal ? p.Lk : min(p.Lk, max(pos + 1, prefix))) - ypos;
-                full = ypos + 64 <= p.Lk && (!p.causal || ypos + 63 <= xpos || ypos + 64 <= prefix);
+            uint32_t seen[1] = {~0u};
+            if (kKeys) full = !p.causal || ypos >= xpos + 127 || xpos + 128 <= prefix;
+            else full = ypos + 64 <= p.Lk && (!p.causal || ypos + 63 <= xpos || ypos + 64 <= prefix);
+            if (docs) full = full && common >= 0 && (!kKeys || y0 + 64 <= p.Lq) && common_doc(dt, ypos, 64, p.Lk) == common;
+            if (!full) {
+                if (docs) same_document(rdoc, ydoc, seen);
+                if (!kKeys) seen[0] &= bits_below((!p.causal ? p.Lk : min(p.Lk, max(pos + 1, prefix))) - ypos - col);
+                else if (p.causal && pos >= prefix) seen[0] &= ~bits_below(pos - ypos - col);
             }
-            if (docs) {
-                if (rdoc < 0) hi = 0;
-                full = full && common >= 0 && (!kKeys || y0 + 64 <= p.Lq) && common_doc(dt, ypos, 64, p.Lk) == common;
-                if (!full) {
-                    __syncwarp();
-                    st.doc[warp][lane] = doc_at(p, b, ypos + col + lane);
-                    __syncwarp();
-                }
-            }
+            if (docs && i + 2 < n) ydoc[0] = doc_at(p, b, y_of(i + 2) + (kKeys ? shift : 0) + col + lane);
             ok = __all_sync(~0u, tc_wait(smem_u32(&st.s_full[set]), (i >> 1) & 1, failed) &&
                                      (!kKeys || tc_wait(smem_u32(&st.y_full[s]), (i / kTcBwdStages) & 1, failed)));
             if (!ok) break;
@@ -357,16 +351,11 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                     e[k + 1] = ex2(e[k + 1]);
                 }
                 if (!full) {
-                    int d[4] = {rdoc, rdoc, rdoc, rdoc};
-                    if (docs) {
-                        const int4 x = *reinterpret_cast<const int4*>(&st.doc[warp][c]);
-                        d[0] = x.x, d[1] = x.y, d[2] = x.z, d[3] = x.w;
-                    }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const bool seen = col + c + k >= lo && col + c + k < hi && d[k] == rdoc;
-                        e[k] = seen ? e[k] : 0.f;
-                        if (kCap) v[c + k] = seen ? v[c + k] : 0.f;
+                        const bool in = seen[0] >> (c + k) & 1;
+                        e[k] = in ? e[k] : 0.f;
+                        if (kCap) v[c + k] = in ? v[c + k] : 0.f;
                     }
                 }
                 if (kKeys) {
