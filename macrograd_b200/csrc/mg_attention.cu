@@ -428,18 +428,17 @@ mg_status launch_rotary(mg::RotaryParams& p, const Device& dev, cudaStream_t st)
 {
     p.units = p.pairs / VEC;
     p.tail_units = (p.D - 2 * p.pairs) / VEC;
-    const int heads = p.H + p.Hkv;
-    const int64_t tokens = (int64_t)p.B * p.L, per_head = tokens * (p.units + p.tail_units);
-    // One set of sines serves several heads where there is work enough to fill
-    // the GPU (a few blocks an SM) all the same.
-    p.heads_per_thread = 1;
-    while (p.heads_per_thread < 8 && per_head * ceil_div(heads, 2 * p.heads_per_thread) >= (int64_t)dev.sm_count * 1024)
-        p.heads_per_thread *= 2;
-    p.groups = ceil_div(heads, p.heads_per_thread);
-    p.total = per_head * p.groups;
-    if (p.total == 0) return MG_OK;
-    if ((p.total + 127) / 128 >= (1ll << 31)) return fail(MG_ERR_UNSUPPORTED, "mg_rotary: too many elements");
-    mg::rotary_kernel<T, VEC><<<(unsigned)((p.total + 127) / 128), 128, 0, st>>>(p);
+    // Tokens of a block: enough that each thread has a pair's sines to compute and
+    // a few items to turn, but blocks for the whole GPU where there are few tokens.
+    const int64_t tokens = (int64_t)p.B * p.L, items = (int64_t)(p.H + p.Hkv) * (p.units + p.tail_units);
+    int64_t per_block = std::max<int64_t>(1, std::min<int64_t>(std::min(mg::kRotaryTokens, mg::kRotaryThreads / std::max(1, p.pairs)),
+                                                               tokens / (4 * dev.sm_count)));
+    while (per_block > 1 && per_block * items > 8 * mg::kRotaryThreads) --per_block;
+    p.tokens = (int)per_block;
+    const int64_t blocks = (tokens + per_block - 1) / per_block;
+    if (tokens + per_block >= (1ll << 31)) return fail(MG_ERR_UNSUPPORTED, "mg_rotary: too many tokens for one call");
+    const size_t smem = (size_t)2 * per_block * p.pairs * sizeof(float);
+    mg::rotary_kernel<T, VEC><<<(unsigned)blocks, mg::kRotaryThreads, smem, st>>>(p);
     return launched("mg_rotary");
 }
 
@@ -521,6 +520,8 @@ mg_status mg_rotary(const mg_rotary_desc* d, void* out_q, void* out_k, const voi
                     d->batch, d->heads, d->kv_heads, d->len, d->head_dim);
     if (d->pairs < 0 || d->pairs > d->head_dim / 2)
         return fail(MG_ERR_INVALID, "mg_rotary: %d pairs do not fit a head of %d", d->pairs, d->head_dim);
+    if (d->pairs > mg::kRotaryMaxPairs)
+        return fail(MG_ERR_UNSUPPORTED, "mg_rotary: %d pairs, %d at most", d->pairs, mg::kRotaryMaxPairs);
     if (!std::isfinite(d->magnitude)) return fail(MG_ERR_INVALID, "mg_rotary: magnitude is not finite");
     const int kvh = k ? d->kv_heads : 0;
     if (d->batch == 0 || d->len == 0 || d->heads + kvh == 0) return MG_OK;
