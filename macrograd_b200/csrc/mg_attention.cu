@@ -323,23 +323,24 @@ mg_status forward_tc32(const mg::AttnParams& p, const Device& dev, void* stream)
     return p.D <= 64 ? launch_tc32_forward<64>(t, dev, st) : launch_tc32_forward<128>(t, dev, st);
 }
 
-template <bool kKeys, bool kCap, bool kBias>
+template <int DP, bool kKeys, int kTake, bool kCap, bool kBias>
 mg_status launch_tc32_backward(const mg::Tc32BwdParams& t, const Device& dev, cudaStream_t st)
 {
-    constexpr auto kernel = mg::attn_tc32_backward<kKeys, kCap, kBias>;
+    constexpr auto kernel = mg::attn_tc32_backward<DP, kKeys, kTake, kCap, kBias>;
     MG_TRY(allow_smem<kernel>(dev, mg::kTc32BwdSmem));
     const int blocks = kKeys ? ceil_div(t.a.Lk, 128) * t.a.B * t.a.Hkv : ceil_div(t.a.Lq, 128) * t.a.B * t.a.H;
     kernel<<<blocks, mg::kTc32BwdThreads, mg::kTc32BwdSmem, st>>>(t);
     return launched("mg_attention_backward");
 }
 
-template <bool kKeys>
+template <int DP, bool kKeys, int kTake>
 mg_status launch_tc32_backward(const mg::Tc32BwdParams& t, const Device& dev, cudaStream_t st)
 {
     const bool cap = t.a.cap > 0.f, bias = t.a.slopes != nullptr;
-    return cap ? (bias ? launch_tc32_backward<kKeys, true, true>(t, dev, st) : launch_tc32_backward<kKeys, true, false>(t, dev, st))
-               : (bias ? launch_tc32_backward<kKeys, false, true>(t, dev, st)
-                       : launch_tc32_backward<kKeys, false, false>(t, dev, st));
+    return cap ? (bias ? launch_tc32_backward<DP, kKeys, kTake, true, true>(t, dev, st)
+                       : launch_tc32_backward<DP, kKeys, kTake, true, false>(t, dev, st))
+               : (bias ? launch_tc32_backward<DP, kKeys, kTake, false, true>(t, dev, st)
+                       : launch_tc32_backward<DP, kKeys, kTake, false, false>(t, dev, st));
 }
 
 mg_status backward_tc32(const mg::AttnParams& p, const Device& dev, void* stream)
@@ -355,10 +356,15 @@ mg_status backward_tc32(const mg::AttnParams& p, const Device& dev, void* stream
     if (!stats) return fail(MG_ERR_ALLOC, "%s: no scratch for the row sums", who);
     mg::attn_tc_stats_kernel<float><<<ceil_div(rows, 16), 256, 0, st>>>(p, Lp, stats, stats + rows);
     MG_TRY(launched(who));
-    const mg::Tc32BwdParams t = {p,        f.doc_tiles, stats, stats + rows, Lp, mg::idesc_bf16(128, 64, false, false, p.scale < 0.f),
-                                 f.scale, f.status};
-    MG_TRY(launch_tc32_backward<true>(t, dev, st));
-    return launch_tc32_backward<false>(t, dev, st);
+    mg::Tc32BwdParams t = {p, f.doc_tiles, stats, stats + rows, Lp, 0, f.scale, f.status};
+    t.idesc_s = mg::idesc_bf16(128, p.D <= 64 ? 64 : 32, false, false, p.scale < 0.f);
+    if (p.D <= 64) {
+        MG_TRY((launch_tc32_backward<64, true, mg::kTakeBoth>(t, dev, st)));
+        return launch_tc32_backward<64, false, mg::kTakeDs>(t, dev, st);
+    }
+    MG_TRY((launch_tc32_backward<128, true, mg::kTakeDs>(t, dev, st)));
+    MG_TRY((launch_tc32_backward<128, true, mg::kTakeP>(t, dev, st)));
+    return launch_tc32_backward<128, false, mg::kTakeDs>(t, dev, st);
 }
 
 // ---------------------------------------------------------------- paged
@@ -495,11 +501,8 @@ mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, 
     mg::AttnParams p = attention_params(d);
     p.q = q, p.k = k, p.v = v, p.out = const_cast<void*>(out), p.dout = dout, p.lse = const_cast<float*>(lse);
     p.dq = dq, p.dk = dk, p.dv = dv;
-    if (d->q_len > 0 && d->k_len > 0 && tc_serves(d, p, {q, out, dout, dq}, {k, v, dk, dv})) {
-        if (d->dtype == MG_BF16) return backward_tc(p, dev, stream);
-        // the pieces of longer fp32 heads do not fit the shared memory
-        if (d->head_dim <= 64) return backward_tc32(p, dev, stream);
-    }
+    if (d->q_len > 0 && d->k_len > 0 && tc_serves(d, p, {q, out, dout, dq}, {k, v, dk, dv}))
+        return d->dtype == MG_BF16 ? backward_tc(p, dev, stream) : backward_tc32(p, dev, stream);
     Scratch ws(dev, stream);
     if (d->q_len > 0) {
         p.delta = static_cast<float*>(ws.get(sizeof(float) * d->batch * d->heads * (size_t)d->q_len));

@@ -1,13 +1,18 @@
-// mg_attention_tc32_bwd.cuh -- gradients of attention of fp32 tensors with heads of
-// up to 64 elements on the 5th-generation tensor cores at fp32 accuracy.
+// mg_attention_tc32_bwd.cuh -- gradients of attention of fp32 tensors on the
+// 5th-generation tensor cores at fp32 accuracy.
 //
 // The two forms of mg_attention_tc_bwd.cuh (queries resident: dQ; keys resident:
-// dK, dV), with every product made of the six of mg_attention_tc32.cuh. The pieces of
-// 128 resident rows and of two stages of 64 streamed rows of two tensors fill the
-// shared memory (96 + 96 KB). Two warpgroups share a tile: warpgroup g has
-// columns [32 g, 32 g + 32) of S and dP, writes the pieces of its part of P and dS
-// to tensor memory, and adds its share of each tile's accumulators up in registers. The tensor
-// core runs S and dP of the next tile while the exponentials of this one are taken.
+// dK, dV), with every product made of the six of mg_attention_tc32.cuh. Two
+// warpgroups share a tile of kN streamed rows: warpgroup g has half of the columns of S and
+// dP, writes the pieces of its part of P and dS to tensor memory, and adds its
+// share of each tile's accumulators up in registers. The tensor core runs S and dP of
+// the next tile while the exponentials of this one are taken.
+//
+// Heads of up to 64: the pieces of 128 resident rows and of two stages of kN = 64
+// streamed rows of two tensors fill the shared memory (96 + 96 KB).
+// Heads of up to 128: X0's pieces lie in tensor memory (3 x 64 columns, the A operand
+// of S), kN = 32, and one accumulator of 128 columns is all that is left, so dK and
+// dV take a launch each (8 products in all instead of 7).
 #pragma once
 
 #include "mg_attention_tc32.cuh"
@@ -26,6 +31,9 @@ struct Tc32BwdParams {
     int* status;
 };
 
+// What a launch accumulates: dS Y0 (dQ or dK), P Y1 (dV), or both.
+enum : int { kTakeBoth = 0, kTakeDs = 1, kTakeP = 2 };
+
 struct Tc32BwdState {
     uint64_t x_full, y_full[2], y_empty[2], s_full, s_free, p_full, acc_full, drain;
     uint32_t tmem;
@@ -36,17 +44,22 @@ struct Tc32BwdState {
 
 constexpr int kTc32BwdThreads = 384;     // two warpgroups, three warps that load, one that issues
 constexpr size_t kTc32BwdSmem = (size_t)(2 * 128 + 2 * 2 * 64) * 64 * 6 + 1024;
+static_assert(kTc32BwdSmem == (size_t)(128 + 2 * 2 * 32) * 128 * 6 + 1024, "both head sizes take the same");
 
-template <bool kKeys, bool kCap, bool kBias>
+template <int DP, bool kKeys, int kTake, bool kCap, bool kBias>
 __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const __grid_constant__ Tc32BwdParams tp)
 {
-    constexpr int DP = 64;
-    constexpr uint32_t kPieceX = 128 * DP * 2, kPieceY = 64 * DP * 2;
+    constexpr bool kXt = DP == 128;                  // X0 in tensor memory
+    constexpr int kN = kXt ? 32 : 64;                // streamed rows of a tile
+    constexpr int kCols = kN / 2;                    // of them, a thread's
+    static_assert(kTake != kTakeBoth || (kKeys && !kXt), "two accumulators: keys resident, heads of up to 64");
+    static_assert(kTake != kTakeP || kKeys, "dV needs the keys resident");
+    constexpr uint32_t kPieceX = 128 * DP * 2, kPieceY = kN * DP * 2;
     extern __shared__ uint8_t dyn[];
     __shared__ Tc32BwdState st;
     const AttnParams& p = tp.a;
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
-    const uint32_t sX0 = base, sX1 = base + 3 * kPieceX, sY = base + 6 * kPieceX;
+    const uint32_t sX0 = base, sX1 = base + (kXt ? 0 : 3 * kPieceX), sY = sX1 + 3 * kPieceX;
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;   // uniform: so are the roles
 
     const int nhead = kKeys ? p.Hkv : p.H, xrows = kKeys ? p.Lk : p.Lq, yrows = kKeys ? p.Lq : p.Lk;
@@ -79,18 +92,21 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
     }
     int t0, t1;
     stream_range<kKeys>(p, docs, dt, prefix, x0, xpos, shift, t0, t1);
+    t0 *= 64 / kN, t1 *= 64 / kN;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const int tiles = max(0, t1 - t0), n = kKeys ? tiles * group : tiles;
-    const uint32_t tm = st.tmem, tS = tm, tdP = tm + 64, tP = tm + 128, tdS = tm + 224, tA = tm + 320, tB = tm + 384;
+    // columns: X0's pieces, S, dP, the pieces of P and of dS, the accumulators
+    const uint32_t tX = st.tmem, tS = tX + (kXt ? 192 : 0), tdP = tS + kN, tP = tdP + kN;
+    const uint32_t tdS = tP + (kXt ? 0 : 96), tA = st.tmem + (kXt ? 384 : 320), tB = tA + (kXt ? 0 : 64);
     volatile int* failed = &st.failed;
     const auto sY0 = [&](int i) { return sY + (uint32_t)(i & 1) * 6 * kPieceY; };
 
     if (warp >= 8 && warp < 11) {
         // ------------------------------------------------ loads and splits of the streamed rows
         // item k of a thread: 8 elements of row r0 + 12 k of both tensors, always the same columns
-        constexpr int kRows = kTc32LoadWarps * 32 / (DP / 8), kItems = (64 + kRows - 1) / kRows;
+        constexpr int kRows = kTc32LoadWarps * 32 / (DP / 8), kItems = (kN + kRows - 1) / kRows;
         const int tid = threadIdx.x - 256, r0 = tid / (DP / 8), c = tid % (DP / 8);
         const bool in = c * 8 < p.D;
         const int64_t* s0 = kKeys ? p.qs : p.ks;
@@ -100,20 +116,20 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
         const int64_t step0 = s0[2], step1 = s1[2];
         bool ok = true;
         for (int i = 0; i < n && ok; ++i) {
-            const int yh = kKeys ? xh * group + i / tiles : xh / group, y0 = (t0 + (kKeys ? i % tiles : i)) * 64;
+            const int yh = kKeys ? xh * group + i / tiles : xh / group, y0 = (t0 + (kKeys ? i % tiles : i)) * kN;
             const float* a0 = src0 + yh * s0[1] + (y0 + r0) * step0;
             const float* a1 = src1 + yh * s1[1] + (y0 + r0) * step1;
             float4 x[kItems][2], y[kItems][2];
 #pragma unroll
             for (int k = 0; k < kItems; ++k) {
                 const int row = y0 + r0 + k * kRows;
-                const bool live = in && r0 + k * kRows < 64 && row < yrows &&
+                const bool live = in && r0 + k * kRows < kN && row < yrows &&
                                   (!docs || doc_at(p, b, row + (kKeys ? shift : 0)) >= 0);
                 tc32_fetch(x[k], a0 + k * kRows * step0, live);
                 tc32_fetch(y[k], a1 + k * kRows * step1, live);
             }
             float lse2 = 0.f, delta = 0.f;
-            if (kKeys && tid < 64) {
+            if (kKeys && tid < kN) {
                 lse2 = tp.lse2[((int64_t)b * p.H + yh) * tp.Lp + y0 + tid];
                 delta = tp.delta[((int64_t)b * p.H + yh) * tp.Lp + y0 + tid];
             }
@@ -121,11 +137,11 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
             if (!ok) break;
 #pragma unroll
             for (int k = 0; k < kItems; ++k) {
-                if (r0 + k * kRows >= 64) continue;
-                tc32_put(sY0(i), 64, kPieceY, r0 + k * kRows, c, x[k]);
-                tc32_put(sY0(i) + 3 * kPieceY, 64, kPieceY, r0 + k * kRows, c, y[k]);
+                if (r0 + k * kRows >= kN) continue;
+                tc32_put(sY0(i), kN, kPieceY, r0 + k * kRows, c, x[k]);
+                tc32_put(sY0(i) + 3 * kPieceY, kN, kPieceY, r0 + k * kRows, c, y[k]);
             }
-            if (kKeys && tid < 64) {
+            if (kKeys && tid < kN) {
                 st.lse2[i & 1][tid] = -lse2;
                 st.delta[i & 1][tid] = -delta;
             }
@@ -135,7 +151,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
         }
     } else if (warp == 11) {
         // ------------------------------------------------ products
-        constexpr uint32_t idesc_dp = idesc_bf16(128, 64, false, false), idesc_acc = idesc_bf16(128, DP, false, true);
+        constexpr uint32_t idesc_dp = idesc_bf16(128, kN, false, false), idesc_acc = idesc_bf16(128, DP, false, true);
         bool ok = true;
         for (int i = 0; i <= n && n > 0 && ok; ++i) {
             if (i < n) {
@@ -145,48 +161,48 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                 ok = __all_sync(~0u, ok);
                 if (!ok) break;
                 tc_fence_after();
-                {
 #pragma unroll
-                    for (int x = 0; x < 6; ++x)
+                for (int x = 0; x < 6; ++x)
 #pragma unroll
-                        for (int k = 0; k < DP / 16; ++k)
-                            tc_mma_f16(tS, desc_k_major(sX0 + kPieceA[x] * kPieceX, 128, k),
-                                       desc_k_major(sY0(i) + kPieceB[x] * kPieceY, 64, k), tp.idesc_s, x + k > 0);
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint64_t y = desc_k_major(sY0(i) + kPieceB[x] * kPieceY, kN, k);
+                        if constexpr (kXt) tc_mma_f16_ta(tS, tX + kPieceA[x] * 64 + 8 * k, y, tp.idesc_s, x + k > 0);
+                        else tc_mma_f16(tS, desc_k_major(sX0 + kPieceA[x] * kPieceX, 128, k), y, tp.idesc_s, x + k > 0);
+                    }
+                if constexpr (kTake != kTakeP) {
 #pragma unroll
                     for (int x = 0; x < 6; ++x)
 #pragma unroll
                         for (int k = 0; k < DP / 16; ++k)
                             tc_mma_f16(tdP, desc_k_major(sX1 + kPieceA[x] * kPieceX, 128, k),
-                                       desc_k_major(sY0(i) + (3 + kPieceB[x]) * kPieceY, 64, k), idesc_dp, x + k > 0);
-                    tc_commit_warp(smem_u32(&st.s_full));
+                                       desc_k_major(sY0(i) + (3 + kPieceB[x]) * kPieceY, kN, k), idesc_dp, x + k > 0);
                 }
-                __syncwarp();
+                tc_commit_warp(smem_u32(&st.s_full));
             }
             if (i > 0) {
                 const int j = i - 1;
                 ok = __all_sync(~0u, tc_wait(smem_u32(&st.p_full), j & 1, failed));
                 if (!ok) break;
                 tc_fence_after();
-                {
-                    if (kKeys) {
-#pragma unroll
-                        for (int x = 0; x < 6; ++x)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                tc_mma_f16_ta(tB, tP + kPieceA[x] * 32 + 8 * k,
-                                              desc_mn_major(sY0(j) + (3 + kPieceB[x]) * kPieceY, 64, k), idesc_acc,
-                                              x + k > 0);
-                    }
+                if constexpr (kTake != kTakeDs) {
 #pragma unroll
                     for (int x = 0; x < 6; ++x)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            tc_mma_f16_ta(tA, tdS + kPieceA[x] * 32 + 8 * k,
-                                          desc_mn_major(sY0(j) + kPieceB[x] * kPieceY, 64, k), idesc_acc, x + k > 0);
-                    tc_commit_warp(smem_u32(&st.acc_full));
-                    tc_commit_warp(smem_u32(&st.y_empty[j & 1]));
+                        for (int k = 0; k < kN / 16; ++k)
+                            tc_mma_f16_ta(tB, tP + kPieceA[x] * kCols + 8 * k,
+                                          desc_mn_major(sY0(j) + (3 + kPieceB[x]) * kPieceY, kN, k), idesc_acc,
+                                          x + k > 0);
                 }
-                __syncwarp();
+                if constexpr (kTake != kTakeP) {
+#pragma unroll
+                    for (int x = 0; x < 6; ++x)
+#pragma unroll
+                        for (int k = 0; k < kN / 16; ++k)
+                            tc_mma_f16_ta(tA, tdS + kPieceA[x] * kCols + 8 * k,
+                                          desc_mn_major(sY0(j) + kPieceB[x] * kPieceY, kN, k), idesc_acc, x + k > 0);
+                }
+                tc_commit_warp(smem_u32(&st.acc_full));
+                tc_commit_warp(smem_u32(&st.y_empty[j & 1]));
             }
         }
         if (!ok) {
@@ -200,22 +216,56 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
         }
     } else {
         // ------------------------------------------------ P and dS
-        const int wg = warp / 4, r = threadIdx.x % 128, col = 32 * wg;    // resident row, first column
+        const int wg = warp / 4, r = threadIdx.x % 128, col = kCols * wg;    // resident row, first column
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;
         const int pos = xpos + r;
         bool ok = true;
         if (n > 0) {
             const int64_t* s = kKeys ? (wg ? p.vs : p.ks) : (wg ? p.dos : p.qs);
             const float* src = (const float*)(kKeys ? (wg ? p.v : p.k) : (wg ? p.dout : p.q)) + b * s[0] + xh * s[1];
-            float4 x[DP / 8][2];
+            if (kXt && wg == 0) {
+                // this thread's row of X0 into its lane of tensor memory, two elements to a column
+                const int row = x0 + r;
+                const bool live = row < xrows && (!docs || doc_at(p, b, row + (kKeys ? 0 : shift)) >= 0);
+#pragma unroll 1
+                for (int c = 0; c < DP; c += 32) {
+                    uint32_t w[3][16];
 #pragma unroll
-            for (int i = 0; i < DP / 8; ++i) {
-                const int row = x0 + r / 8 + 16 * i, e = r % 8;
-                tc32_fetch(x[i], src + row * s[2] + e * 8,
-                           row < xrows && e * 8 < p.D && (!docs || doc_at(p, b, row + (kKeys ? 0 : shift)) >= 0));
+                    for (int e = 0; e < 32; e += 8) {
+                        float4 x[2];
+                        tc32_fetch(x, src + row * s[2] + c + e, live && c + e < p.D);
+                        uint32_t pc[4][3];
+                        split3(x[0].x, x[0].y, pc[0]);
+                        split3(x[0].z, x[0].w, pc[1]);
+                        split3(x[1].x, x[1].y, pc[2]);
+                        split3(x[1].z, x[1].w, pc[3]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int z = 0; z < 3; ++z) w[z][e / 2 + k] = pc[k][z];
+                    }
+#pragma unroll
+                    for (int z = 0; z < 3; ++z) tmem_st_x16(tX + lanes + 64 * z + c / 2, w[z]);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+            } else if (!kXt || kTake != kTakeP) {
+#pragma unroll 1
+                for (int first = 0; first < DP / 8; first += 8) {
+                    float4 x[8][2];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int item = (first + i) * 128 + r, row = x0 + item / (DP / 8), e = item % (DP / 8);
+                        tc32_fetch(x[i], src + row * s[2] + e * 8,
+                                   row < xrows && e * 8 < p.D && (!docs || doc_at(p, b, row + (kKeys ? 0 : shift)) >= 0));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int item = (first + i) * 128 + r;
+                        tc32_put(wg ? sX1 : sX0, 128, kPieceX, item / (DP / 8), item % (DP / 8), x[i]);
+                    }
+                }
             }
-#pragma unroll
-            for (int i = 0; i < DP / 8; ++i) tc32_put(wg ? sX1 : sX0, 128, kPieceX, r / 8 + 16 * i, r % 8, x[i]);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&st.x_full));
@@ -229,9 +279,11 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
             lse2 = -tp.lse2[at];
             delta = -tp.delta[at];
         }
-        // this thread's accumulators: dK (warpgroup 0) or dV (1), or half of dQ
-        constexpr int kAcc = kKeys ? 64 : 32;
-        const uint32_t tAcc = (kKeys ? (wg ? tB : tA) : tA + col) + lanes;
+        // this thread's part of its row's accumulators: dK (warpgroup 0) or dV (1), or half of the only one
+        constexpr int kAcc = kTake == kTakeBoth ? DP : DP / 2;
+        const int ocol = kTake == kTakeBoth ? 0 : kAcc * wg;
+        const bool is_dv = kTake == kTakeP || (kTake == kTakeBoth && wg == 1);
+        const uint32_t tAcc = (is_dv ? tB : tA) + ocol + lanes;
         float o[kAcc];
 #pragma unroll
         for (int i = 0; i < kAcc; ++i) o[i] = 0.f;
@@ -246,7 +298,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
             }
         };
         // this lane's document of a tile's streamed rows, a tile ahead
-        const auto y_of = [&](int i) { return (t0 + (kKeys ? i % tiles : i)) * 64; };
+        const auto y_of = [&](int i) { return (t0 + (kKeys ? i % tiles : i)) * kN; };
         int ydoc[1] = {docs && n > 0 ? doc_at(p, b, y_of(0) + (kKeys ? shift : 0) + col + lane) : -1};
         for (int i = 0; i < n; ++i) {
             const int h = kKeys ? xh * group + i / tiles : xh;
@@ -255,8 +307,8 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
             bool full;
             uint32_t seen[1] = {~0u};
             if (kKeys) full = !p.causal || ypos >= xpos + 127 || xpos + 128 <= prefix;
-            else full = ypos + 64 <= p.Lk && (!p.causal || ypos + 63 <= xpos || ypos + 64 <= prefix);
-            if (docs) full = full && common >= 0 && (!kKeys || y0 + 64 <= p.Lq) && common_doc(dt, ypos, 64, p.Lk) == common;
+            else full = ypos + kN <= p.Lk && (!p.causal || ypos + kN - 1 <= xpos || ypos + kN <= prefix);
+            if (docs) full = full && common >= 0 && (!kKeys || y0 + kN <= p.Lq) && common_doc(dt, ypos, kN, p.Lk) == common;
             if (!full) {
                 if (docs) same_document(rdoc, ydoc, seen);
                 if (!kKeys) seen[0] &= bits_below((!p.causal ? p.Lk : min(p.Lk, max(pos + 1, prefix))) - ypos - col);
@@ -267,9 +319,12 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                                      (!kKeys || tc_wait(smem_u32(&st.y_full[i & 1]), (i >> 1) & 1, failed)));
             if (!ok) break;
             tc_fence_after();
-            float v[32], g[32];
-            tmem_ld_x32(tS + lanes + col, v);
-            tmem_ld_x32(tdP + lanes + col, g);
+            float v[kCols], g[kCols];
+#pragma unroll
+            for (int c0 = 0; c0 < kCols; c0 += 16) {
+                tmem_ld_x16(tS + lanes + col + c0, *reinterpret_cast<float(*)[16]>(v + c0));
+                if (kTake != kTakeP) tmem_ld_x16(tdP + lanes + col + c0, *reinterpret_cast<float(*)[16]>(g + c0));
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&st.s_free));
@@ -283,7 +338,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
             const float far = (float)(pos - ypos - col);
             const uint64_t mul_2 = pack2(mul, mul);
 #pragma unroll
-            for (int c0 = 0; c0 < 32; c0 += 16) {
+            for (int c0 = 0; c0 < kCols; c0 += 16) {
                 float e[16];
 #pragma unroll
                 for (int c = 0; c < 16; c += 4) {
@@ -309,7 +364,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
 #pragma unroll
                     for (int c = 0; c < 16; ++c) e[c] = seen[0] >> (c0 + c) & 1 ? e[c] : 0.f;
                 }
-                if (kKeys) {
+                if (kTake != kTakeDs) {
                     uint32_t w[3][8];
 #pragma unroll
                     for (int c = 0; c < 16; c += 2) {
@@ -319,8 +374,9 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                         for (int k = 0; k < 3; ++k) w[k][c / 2] = pc[k];
                     }
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) tmem_st_x8(tP + lanes + 32 * k + (col + c0) / 2, w[k]);
+                    for (int k = 0; k < 3; ++k) tmem_st_x8(tP + lanes + kCols * k + (col + c0) / 2, w[k]);
                 }
+                if (kTake == kTakeP) continue;
                 // dS = P * curve * (dP - delta)
                 uint32_t w[3][8];
 #pragma unroll
@@ -351,7 +407,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < 3; ++k) tmem_st_x8(tdS + lanes + 32 * k + (col + c0) / 2, w[k]);
+                for (int k = 0; k < 3; ++k) tmem_st_x8(tdS + lanes + kCols * k + (col + c0) / 2, w[k]);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -366,12 +422,11 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
             }
         }
         if (ok && x0 + r < xrows) {
-            const bool is_dv = kKeys && wg == 1;
             const int64_t* os = kKeys ? (is_dv ? p.dvs : p.dks) : p.dqs;
             float* out = (float*)(kKeys ? (is_dv ? p.dv : p.dk) : p.dq) + b * os[0] + xh * os[1] +
-                         (int64_t)(x0 + r) * os[2] + (kKeys ? 0 : col);
+                         (int64_t)(x0 + r) * os[2] + ocol;
             const float f = is_dv ? 1.f : p.scale;
-            const int cols = p.D - (kKeys ? 0 : col);
+            const int cols = p.D - ocol;
 #pragma unroll
             for (int c = 0; c < kAcc; c += 4)
                 if (c < cols)
