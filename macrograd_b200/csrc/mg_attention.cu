@@ -281,18 +281,18 @@ mg_status backward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     MG_TRY(launched(who));
     int* hs = t.head_step;
     int* bs = t.batch_step;
+    // the queries resident: dQ, and delta made exact
+    MG_TRY(tc_map(&t.x0, &hs[0], &bs[0], p.q, p.qs, p.D, p.Lq, p.H, p.B, 128));
+    MG_TRY(tc_map(&t.x1, &hs[3], &bs[3], p.dout, p.dos, p.D, p.Lq, p.H, p.B, 128));
+    MG_TRY(tc_map(&t.y0, &hs[1], &bs[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 64));
+    MG_TRY(tc_map(&t.y1, &hs[2], &bs[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 64));
+    MG_TRY((p.D <= 64 ? launch_tc_backward<64, false>(t, dev, st) : launch_tc_backward<128, false>(t, dev, st)));
     // the keys resident: dK, dV
     MG_TRY(tc_map(&t.x0, &hs[1], &bs[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 128));
     MG_TRY(tc_map(&t.x1, &hs[2], &bs[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 128));
     MG_TRY(tc_map(&t.y0, &hs[0], &bs[0], p.q, p.qs, p.D, p.Lq, p.H, p.B, 64));
     MG_TRY(tc_map(&t.y1, &hs[3], &bs[3], p.dout, p.dos, p.D, p.Lq, p.H, p.B, 64));
-    MG_TRY((p.D <= 64 ? launch_tc_backward<64, true>(t, dev, st) : launch_tc_backward<128, true>(t, dev, st)));
-    // the queries resident: dQ
-    MG_TRY(tc_map(&t.x0, &hs[0], &bs[0], p.q, p.qs, p.D, p.Lq, p.H, p.B, 128));
-    MG_TRY(tc_map(&t.x1, &hs[3], &bs[3], p.dout, p.dos, p.D, p.Lq, p.H, p.B, 128));
-    MG_TRY(tc_map(&t.y0, &hs[1], &bs[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 64));
-    MG_TRY(tc_map(&t.y1, &hs[2], &bs[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 64));
-    return p.D <= 64 ? launch_tc_backward<64, false>(t, dev, st) : launch_tc_backward<128, false>(t, dev, st);
+    return p.D <= 64 ? launch_tc_backward<64, true>(t, dev, st) : launch_tc_backward<128, true>(t, dev, st);
 }
 
 template <int DP, bool kCap, bool kBias>

@@ -9,8 +9,15 @@
 // With the queries resident (X = q, dout; Y = k, v) acc is dQ. With the keys
 // resident (X = k, v; Y = q, dout) S and dP are transposed, acc is dK and acc' is
 // dV, summed over the query heads that share the key-value head. So no gradient
-// is added to by two blocks: no atomics, and the same bits every time, for 7
+// is added to by two blocks: no atomics, and the same bits every time, for 8
 // products instead of the 5 of a single kernel that would add dQ up atomically.
+//
+// delta = rowsum(dout * out) carries the 16-bit rounding of out, which dS = P * (dP -
+// delta) magnifies where a row's weight lies on few keys (errors of dQ and dK of 0.4 %
+// where the rounding of the result itself is 0.17 %). The true delta makes the row's sum of
+// P * (dP - delta) zero, so what that sum is in fp32 is delta's error r: the form with
+// the queries resident, which runs first, adds it to delta for the other one, and
+// corrects its own dQ by r times acc' = sum P * curve * k (the eighth product).
 // P and dS go back to tensor memory over S and dP, as the A operand of the
 // second pair of products: they never pass through shared memory.
 //
@@ -39,7 +46,7 @@ struct TcBwdParams {
     AttnParams a;
     const int2* doc_tiles;
     const float* lse2;                   // [B * H][Lp] lse * log2(e); +inf where no key is seen
-    const float* delta;                  // [B * H][Lp]
+    float* delta;                        // [B * H][Lp]; made exact by the form with the queries resident
     int Lp;                              // q_len rounded up to 128
     int head_step[4], batch_step[4];     // of q, k, v, dout
     uint32_t idesc_s;
@@ -99,7 +106,8 @@ __global__ void attn_tc_stats_kernel(const __grid_constant__ AttnParams p, int L
 
 struct TcBwdState {
     uint64_t x_full, y_full[kTcBwdStages], y_empty[kTcBwdStages];
-    uint64_t s_full[2], dp_full[2], p_full[2], ds_full[2], acc_full, drain;
+    uint64_t s_full[2], dp_full[2], p_full[2], ds_full[2], acc_full, sum_full, drain;
+    float sums[4][128];                  // a quarter of the warps each: the rows' sums of P * (dP - delta)
     uint32_t tmem;
     int failed;
     int loads;                           // stages that were asked for
@@ -169,6 +177,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             mbar_init(smem_u32(&st.ds_full[i]), 8);
         }
         mbar_init(smem_u32(&st.acc_full), 1);
+        mbar_init(smem_u32(&st.sum_full), 16);
         mbar_init(smem_u32(&st.drain), 1);
         mbar_fence_init();
         st.failed = 0;
@@ -184,7 +193,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
     __syncthreads();
     tc_fence_after();
     const int tiles = max(0, t1 - t0), n = kKeys ? tiles * group : tiles;
-    const uint32_t tA = st.tmem + 256, tB = tA + DP;     // accumulators: dS Y0, P Y1
+    const uint32_t tA = st.tmem + 256, tB = tA + DP;     // accumulators: dS Y0, P Y1 (the queries resident: P curve Y0)
     volatile int* failed = &st.failed;
     // columns of step i's S and dP; the 16-bit P and dS of columns [32 h, 32 h + 32) lie in the first 16 of these
     const auto tS = [&](int i) { return st.tmem + 128 * (i & 1); };
@@ -258,11 +267,10 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             ok = __all_sync(~0u, tc_wait(smem_u32(&st.p_full[i & 1]), (i >> 1) & 1, failed));
             if (!ok) break;
             tc_fence_after();
-            if (kKeys) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    tc_mma_f16_ta(tB, tS(i) + 8 * k + 16 * (k / 2), desc_mn_major(sY0(i) + kY, 64, k), idesc_acc, i > 0 || k > 0);
-            }
+            for (int k = 0; k < 4; ++k)
+                tc_mma_f16_ta(tB, tS(i) + 8 * k + 16 * (k / 2), desc_mn_major(sY0(i) + (kKeys ? kY : 0), 64, k), idesc_acc,
+                              i > 0 || k > 0);
             if (i + 2 < n) scores_of(i + 2);
             ok = __all_sync(~0u, ok && tc_wait(smem_u32(&st.ds_full[i & 1]), (i >> 1) & 1, failed));
             if (!ok) break;
@@ -297,6 +305,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             lse2 = tp.lse2[at];
             delta = tp.delta[at];
         }
+        float rsum = 0.f;            // this thread's part of its row's sum of P * (dP - delta)
         bool ok = true;
         // this lane's document of a tile's streamed rows, a tile of the set ahead
         const auto y_of = [&](int i) { return (t0 + (kKeys ? i % tiles : i)) * 64; };
@@ -323,11 +332,6 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             tc_fence_after();
             float v[32];
             tmem_ld_x32(tS(i) + lanes + col, v);
-            if (!kKeys) {                         // S may be overwritten
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&st.p_full[set]));
-            }
             if (kCap) cap_scores(v, tp.curve);      // tanh of the score over the cap
             uint32_t w[16];
             const float far = (float)(pos - ypos - col);
@@ -358,7 +362,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                         if (kCap) v[c + k] = in ? v[c + k] : 0.f;
                     }
                 }
-                if (kKeys) {
+                if (kKeys || !kCap) {
                     w[c / 2] = bf16x2(e[0], e[1]);
                     w[c / 2 + 1] = bf16x2(e[2], e[3]);
                 }
@@ -370,49 +374,85 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                         q = mul2(q, fma2(mul2(t, pack2(-1.f, -1.f)), t, pack2(1.f, 1.f)));
                     }
                     unpack2(q, v[c + k], v[c + k + 1]);
+                    // what the curve takes off P, for the row's sum
+                    if (!kKeys && kCap) w[(c + k) / 2] = bf16x2(e[k] - v[c + k], e[k + 1] - v[c + k + 1]);
                 }
             }
-            if (kKeys) {
+            if (!kKeys && kCap) {
+                // the correction's product takes P * curve
+                uint32_t pc[16];
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) pc[c / 2] = bf16x2(v[c], v[c + 1]);
+                tmem_st_x16(tS(i) + lanes + col, pc);
+            } else {
                 tmem_st_x16(tS(i) + lanes + col, w);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&st.p_full[set]));
             }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&st.p_full[set]));
             ok = __all_sync(~0u, tc_wait(smem_u32(&st.dp_full[set]), (i >> 1) & 1, failed));
             if (!ok) break;
             tc_fence_after();
-            float g[32];
-            tmem_ld_x32(tS(i) + 64 + lanes + col, g);
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-                float nd[4] = {-delta, -delta, -delta, -delta};
-                if (kKeys) {
-                    const float4 x = *reinterpret_cast<const float4*>(&st.delta[s][col + c]);
-                    nd[0] = -x.x, nd[1] = -x.y, nd[2] = -x.z, nd[3] = -x.w;
+            for (int c0 = 0; c0 < 32; c0 += 16) {
+                float g[16];
+                uint32_t ds[8];
+                tmem_ld_x16(tS(i) + 64 + lanes + col + c0, g);
+#pragma unroll
+                for (int c = 0; c < 16; c += 4) {
+                    float nd[4] = {-delta, -delta, -delta, -delta};
+                    if (kKeys) {
+                        const float4 x = *reinterpret_cast<const float4*>(&st.delta[s][col + c0 + c]);
+                        nd[0] = -x.x, nd[1] = -x.y, nd[2] = -x.z, nd[3] = -x.w;
+                    }
+                    float e[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k += 2) {
+                        const int at = c0 + c + k;
+                        const uint64_t d = add2(pack2(g[c + k], g[c + k + 1]), pack2(nd[k], nd[k + 1]));
+                        const uint64_t x = mul2(pack2(v[at], v[at + 1]), d);
+                        unpack2(x, e[k], e[k + 1]);
+                        if (!full) {
+                            e[k] = v[at] == 0.f ? 0.f : e[k];
+                            e[k + 1] = v[at + 1] == 0.f ? 0.f : e[k + 1];
+                        }
+                        if (!kKeys) {
+                            if (kCap) {
+                                float d0, d1;
+                                unpack2(d, d0, d1);
+                                const float p0 = v[at] + __uint_as_float(w[at / 2] << 16);
+                                const float p1 = v[at + 1] + __uint_as_float(w[at / 2] & 0xFFFF0000u);
+                                rsum += (p0 == 0.f ? 0.f : p0 * d0) + (p1 == 0.f ? 0.f : p1 * d1);
+                            } else {
+                                rsum += e[k] + e[k + 1];
+                            }
+                        }
+                    }
+                    ds[c / 2] = bf16x2(e[0], e[1]);
+                    ds[c / 2 + 1] = bf16x2(e[2], e[3]);
                 }
-                float e[4];
-#pragma unroll
-                for (int k = 0; k < 4; k += 2)
-                    unpack2(mul2(pack2(v[c + k], v[c + k + 1]),
-                                 add2(pack2(g[c + k], g[c + k + 1]), pack2(nd[k], nd[k + 1]))),
-                            e[k], e[k + 1]);
-                if (!full) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) e[k] = v[c + k] == 0.f ? 0.f : e[k];
-                }
-                w[c / 2] = bf16x2(e[0], e[1]);
-                w[c / 2 + 1] = bf16x2(e[2], e[3]);
+                tmem_st_x8(tS(i) + 64 + lanes + col + c0 / 2, ds);
             }
-            tmem_st_x16(tS(i) + 64 + lanes + col, w);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&st.ds_full[set]));
         }
-        if (ok && n > 0) ok = __all_sync(~0u, tc_wait(smem_u32(&st.acc_full), 0, failed));
+        if (!kKeys) {
+            st.sums[warp / 4][r] = rsum;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&st.sum_full));
+            ok = ok && tc_wait(smem_u32(&st.sum_full), 0, failed);
+        }
+        if (n > 0) ok = ok && tc_wait(smem_u32(&st.acc_full), 0, failed);
+        ok = __all_sync(~0u, ok);
         if (ok) {
             tc_fence_after();
+            if (!kKeys) {
+                rsum = (st.sums[0][r] + st.sums[1][r]) + (st.sums[2][r] + st.sums[3][r]);
+                if (warp < 4 && x0 + r < xrows) tp.delta[((int64_t)b * p.H + xh) * tp.Lp + x0 + r] = delta + rsum;
+            }
             // with the keys: half of dK or of dV to each four warps; with the queries: a quarter of dQ
             const int quarter = warp / 4;
             const bool is_dv = kKeys && quarter >= 2;
@@ -426,6 +466,12 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                 float o[16];
                 if (n > 0) {
                     tmem_ld_x16((is_dv ? tB : tA) + lanes + c, o);
+                    if (!kKeys) {
+                        float w[16];
+                        tmem_ld_x16(tB + lanes + c, w);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o[k] = fmaf(-rsum, w[k], o[k]);
+                    }
                 } else {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) o[k] = 0.f;
