@@ -369,11 +369,27 @@ mg_status backward_tc32(const mg::AttnParams& p, const Device& dev, void* stream
 
 // ---------------------------------------------------------------- paged
 template <typename T, int DP>
-mg_status launch_paged_kernel(const mg::PagedParams& p, const Device& dev, int blocks, cudaStream_t st)
+mg_status launch_paged_kernel(const mg::PagedParams& p, const Device& dev, int blocks, bool cluster, cudaStream_t st)
 {
     constexpr size_t smem = mg::paged_smem<T, DP>();
-    MG_TRY((allow_smem<mg::paged_kernel<T, DP>>(dev, smem)));
-    mg::paged_kernel<T, DP><<<blocks, mg::kPagedThreads, smem, st>>>(p);
+    if (!cluster) {
+        MG_TRY((allow_smem<mg::paged_kernel<T, DP, false>>(dev, smem)));
+        mg::paged_kernel<T, DP, false><<<blocks, mg::kPagedThreads, smem, st>>>(p);
+        return MG_OK;
+    }
+    MG_TRY((allow_smem<mg::paged_kernel<T, DP, true>>(dev, smem)));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(mg::kPagedThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute size = {};
+    size.id = cudaLaunchAttributeClusterDimension;
+    size.val.clusterDim.x = (unsigned)p.splits;
+    size.val.clusterDim.y = size.val.clusterDim.z = 1;
+    cfg.attrs = &size;
+    cfg.numAttrs = 1;
+    MG_HOST_TRY(cudaLaunchKernelEx(&cfg, mg::paged_kernel<T, DP, true>, p));
     return MG_OK;
 }
 
@@ -400,7 +416,9 @@ mg_status launch_paged(mg::PagedParams& p, int longest, const Device& dev, Scrat
     if (p.page > 0 && (p.page & (p.page - 1)) == 0)
         for (p.page_shift = 0; (1 << p.page_shift) < p.page;) ++p.page_shift;
     if ((int64_t)p.B * p.H >= (1ll << 31) - 1) return fail(MG_ERR_UNSUPPORTED, "%s: batch is too large", who);
-    if (splits > 1) {
+    // few blocks, and no more chunks than a cluster may have: joined there
+    const bool cluster = stream && splits > 1 && splits <= 8 && heads * splits <= dev.sm_count;
+    if (splits > 1 && !cluster) {
         const size_t rows = (size_t)p.B * p.H * splits;
         const size_t part = (rows * p.D * sizeof(float) + 15) / 16 * 16;
         uint8_t* mem = static_cast<uint8_t*>(ws.get(part + rows * sizeof(float2)));
@@ -410,9 +428,10 @@ mg_status launch_paged(mg::PagedParams& p, int longest, const Device& dev, Scrat
     }
     const int blocks = (int)(heads * splits);
     if (!stream) mg::paged_simt_kernel<T><<<blocks, mg::kPagedThreads, 0, st>>>(p);
-    else MG_TRY((p.D <= 64 ? launch_paged_kernel<T, 64>(p, dev, blocks, st) : launch_paged_kernel<T, 128>(p, dev, blocks, st)));
+    else MG_TRY((p.D <= 64 ? launch_paged_kernel<T, 64>(p, dev, blocks, cluster, st)
+                           : launch_paged_kernel<T, 128>(p, dev, blocks, cluster, st)));
     MG_TRY(launched(who));
-    if (splits > 1) {
+    if (splits > 1 && !cluster) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(p.B * p.H));
         cfg.blockDim = dim3(mg::kJoinThreads);

@@ -376,38 +376,39 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
 #pragma unroll
                     for (int k = 0; k < 3; ++k) tmem_st_x8(tP + lanes + kCols * k + (col + c0) / 2, w[k]);
                 }
-                if (kTake == kTakeP) continue;
-                // dS = P * curve * (dP - delta)
-                uint32_t w[3][8];
+                if constexpr (kTake != kTakeP) {
+                    // dS = P * curve * (dP - delta)
+                    uint32_t w[3][8];
 #pragma unroll
-                for (int c = 0; c < 16; c += 4) {
-                    float nd[4] = {delta, delta, delta, delta};
-                    if (kKeys) {
-                        const float4 x = *reinterpret_cast<const float4*>(&st.delta[i & 1][col + c0 + c]);
-                        nd[0] = x.x, nd[1] = x.y, nd[2] = x.z, nd[3] = x.w;
+                    for (int c = 0; c < 16; c += 4) {
+                        float nd[4] = {delta, delta, delta, delta};
+                        if (kKeys) {
+                            const float4 x = *reinterpret_cast<const float4*>(&st.delta[i & 1][col + c0 + c]);
+                            nd[0] = x.x, nd[1] = x.y, nd[2] = x.z, nd[3] = x.w;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; k += 2) {
+                            const int at = c0 + c + k;
+                            uint64_t q = pack2(e[c + k], e[c + k + 1]);
+                            if (kCap) {
+                                const uint64_t t = pack2(v[at], v[at + 1]);
+                                q = mul2(q, fma2(mul2(t, pack2(-1.f, -1.f)), t, pack2(1.f, 1.f)));
+                            }
+                            float x, y;
+                            unpack2(mul2(q, add2(pack2(g[at], g[at + 1]), pack2(nd[k], nd[k + 1]))), x, y);
+                            if (!full) {
+                                x = e[c + k] == 0.f ? 0.f : x;
+                                y = e[c + k + 1] == 0.f ? 0.f : y;
+                            }
+                            uint32_t pc[3];
+                            split3(x, y, pc);
+#pragma unroll
+                            for (int z = 0; z < 3; ++z) w[z][(c + k) / 2] = pc[z];
+                        }
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; k += 2) {
-                        const int at = c0 + c + k;
-                        uint64_t q = pack2(e[c + k], e[c + k + 1]);
-                        if (kCap) {
-                            const uint64_t t = pack2(v[at], v[at + 1]);
-                            q = mul2(q, fma2(mul2(t, pack2(-1.f, -1.f)), t, pack2(1.f, 1.f)));
-                        }
-                        float x, y;
-                        unpack2(mul2(q, add2(pack2(g[at], g[at + 1]), pack2(nd[k], nd[k + 1]))), x, y);
-                        if (!full) {
-                            x = e[c + k] == 0.f ? 0.f : x;
-                            y = e[c + k + 1] == 0.f ? 0.f : y;
-                        }
-                        uint32_t pc[3];
-                        split3(x, y, pc);
-#pragma unroll
-                        for (int z = 0; z < 3; ++z) w[z][(c + k) / 2] = pc[z];
-                    }
+                    for (int k = 0; k < 3; ++k) tmem_st_x8(tdS + lanes + kCols * k + (col + c0) / 2, w[k]);
                 }
-#pragma unroll
-                for (int k = 0; k < 3; ++k) tmem_st_x8(tdS + lanes + kCols * k + (col + c0) / 2, w[k]);
             }
             tmem_wait_st();
             tc_fence_before();

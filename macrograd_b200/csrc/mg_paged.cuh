@@ -238,8 +238,22 @@ template <typename T, int DP>
 constexpr size_t paged_smem()
 {
     const size_t ring = (size_t)kPagedWarps * kPagedStages * 2 * kPagedTile * DP * sizeof(T);
-    const size_t join = (size_t)kPagedWarps * paged_pack<T>() * DP * sizeof(float);
+    const size_t join = (size_t)(kPagedWarps + 1) * paged_pack<T>() * DP * sizeof(float) + paged_pack<T>() * sizeof(float2);
     return ring > join ? ring : join;
+}
+
+// Words of another block's shared memory (shared::cluster addresses).
+__device__ __forceinline__ float remote1(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 remote2(uint32_t addr)
+{
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
 }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live)
@@ -492,7 +506,10 @@ struct PagedAcc<float, DP> {
     }
 };
 
-template <typename T, int DP>
+// kCluster: the chunks of a head are the blocks of one cluster, which join them
+// over distributed shared memory: one launch and no scratch, for calls whose blocks
+// are on the GPU all at once anyway (a block without keys has to stay to the end).
+template <typename T, int DP, bool kCluster>
 __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_constant__ PagedParams p)
 {
     constexpr int kPack = paged_pack<T>(), kPieces = DP * (int)sizeof(T) / 16;
@@ -509,7 +526,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
     const int len = paged_length(p, b);
     if (threadIdx.x == 0 && split == 0 && p.lengths && __ldg(p.lengths + b) != len) paged_report(p, kPagedBadLength);
     const int j0 = split * p.chunk, j1 = min(len, j0 + p.chunk);
-    if (j0 >= j1 && split > 0) return;      // a chunk beyond the request's keys is not joined
+    if (!kCluster && j0 >= j1 && split > 0) return;      // a chunk beyond the request's keys is not joined
     const int h0 = kv * groups + pack * kPack, nh = min(kPack, groups - pack * kPack);
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(paged_dyn) + warp * kPagedStages * 2 * kTileBytes;
@@ -599,6 +616,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __syncthreads();                        // the rings become the join's buffer
     float* so = reinterpret_cast<float*>(paged_dyn);
+    float* block_o = so + kPagedWarps * kPack * DP;        // the block's own result, read by the cluster
+    float2* block_ml = reinterpret_cast<float2*>(block_o + kPack * DP);
     acc.finish(sm_m[warp], sm_l[warp], so + warp * kPack * DP, nh, lane);
     __syncthreads();
     for (int g = warp; g < nh; g += kPagedWarps) {
@@ -611,12 +630,46 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
             f[w] = ex2(sm_m[w][g] - base);
             L = fmaf(f[w], sm_l[w][g], L);
         }
-        paged_store<T>(p, b, h0 + g, split, M * kLn2, L, lane, [&](int d) {
+        const auto joined = [&](int d) {
             float a = 0.f;
 #pragma unroll
             for (int w = 0; w < kPagedWarps; ++w) a = fmaf(f[w], so[(w * kPack + g) * DP + d], a);
             return a;
-        });
+        };
+        if constexpr (kCluster) {
+            for (int d = lane; d < p.D; d += 32) block_o[g * DP + d] = joined(d);
+            if (lane == 0) block_ml[g] = make_float2(M, L);
+        } else {
+            paged_store<T>(p, b, h0 + g, split, M * kLn2, L, lane, joined);
+        }
+    }
+    if constexpr (kCluster) {
+        // head g of the pack is finished by block g % splits
+        cluster_sync_all();
+        for (int g = split + warp * p.splits; g < nh; g += kPagedWarps * p.splits) {
+            float2 x = make_float2(-CUDART_INF_F, 0.f);
+            if (lane < p.splits) x = remote2(cluster_map(smem_u32(&block_ml[g]), lane));
+            float M = x.x;
+#pragma unroll
+            for (int o = 16; o; o /= 2) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
+            const float f = ex2(x.x - (M == -CUDART_INF_F ? 0.f : M));
+            float L = f * x.y;
+#pragma unroll
+            for (int o = 16; o; o /= 2) L += __shfl_xor_sync(~0u, L, o);
+            const float inv = L > 0.f ? 1.f / L : L;       // 0: no key; NaN stays
+            T* out = (T*)p.out + b * p.os[0] + (h0 + g) * p.os[1];
+            for (int d0 = 0; d0 < p.D; d0 += 32) {
+                const int d = d0 + lane;
+                float a = 0.f;
+                for (int s = 0; s < p.splits; ++s) {
+                    const float w = __shfl_sync(~0u, f, s);
+                    if (d < p.D) a = fmaf(w, remote1(cluster_map(smem_u32(&block_o[g * DP + d]), s)), a);
+                }
+                if (d < p.D) out[d] = from_f32<T>(a * inv);
+            }
+            if (lane == 0) p.lse[(int64_t)b * p.H + h0 + g] = L == 0.f ? -CUDART_INF_F : M * kLn2 + logf(L);
+        }
+        cluster_sync_all();                  // nobody leaves while its results are read
     }
 }
 
