@@ -22,10 +22,12 @@ INCLUDE = os.path.join(ROOT, "include")
 # translation unit -> what it includes
 UNITS = {
     "mg_gemm.cu": ["mg_gemm_kernel.cuh", "mg_ptx.cuh", "mg_host.h", "mg_plan.h"],
-    "mg_attention.cu": ["mg_attention_common.cuh", "mg_attention_simt.cuh", "mg_attention_tc.cuh", "mg_attention_tc_bwd.cuh",
-                        "mg_attention_tc32.cuh", "mg_attention_tc32_bwd.cuh",
-                        "mg_tc16.cuh",
-                        "mg_rotary.cuh", "mg_paged.cuh", "mg_ptx.cuh", "mg_host.h"],
+    "mg_attention.cu": ["mg_attention_host.h", "mg_attention_common.cuh", "mg_attention_math.cuh",
+                        "mg_attention_simt.cuh", "mg_attention_tc.cuh",
+                        "mg_attention_tc_bwd.cuh", "mg_attention_tc32.cuh", "mg_attention_tc32_bwd.cuh", "mg_tc16.cuh",
+                        "mg_ptx.cuh", "mg_host.h"],
+    "mg_paged.cu": ["mg_attention_host.h", "mg_attention_common.cuh", "mg_attention_math.cuh", "mg_paged.cuh",
+                    "mg_rotary.cuh", "mg_ptx.cuh", "mg_host.h"],
 }
 SOURCES = [os.path.join(CSRC, u) for u in UNITS]
 HEADERS = [os.path.join(INCLUDE, h) for h in ("mg_gemm.h", "mg_attention.h")]

@@ -12,7 +12,8 @@
 // The bound is the cache's bytes.
 #pragma once
 
-#include "mg_attention_tc.cuh"
+#include "mg_attention_math.cuh"
+#include "mg_ptx.cuh"
 
 namespace mg {
 
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_simt_kernel(const __grid_
 // one to sixteen heads to a key-value head the loads bound the kernel, not the
 // arithmetic, so the warp-level instruction is enough here. fp32: a lane has one key (half of the head
 // each in two lanes) for the scores and D / 32 elements of the output.
-constexpr int kPagedStages = 2;
+constexpr int kPagedStages = 2;          // 3 leave a block less an SM: 102 -> 120 us, 115 -> 141 us (ragged, long)
 constexpr int kPagedTile = 16;
 constexpr int kPagedWarps = kPagedThreads / 32;
 
@@ -676,13 +677,14 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
 // Joins the chunks of one query head: a block per head, D / 4 lanes to a chunk's
 // accumulators. Launched while the chunks are still being read (programmatic
 // dependent launch): it waits for them before it touches their results.
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 512;            // at most
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p)
 {
     __shared__ float weight[kJoinThreads], red[2][kJoinThreads / 32];
     __shared__ float4 acc[kJoinThreads];
+    const int threads = blockDim.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t row = blockIdx.x;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -690,20 +692,19 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     const int n = max(1, (paged_length(p, b) + p.chunk - 1) / p.chunk);
     const float2* st = p.stat + row * p.splits;
     float M = -CUDART_INF_F;
-    for (int s = threadIdx.x; s < n; s += kJoinThreads) M = fmaxf(M, st[s].x);
+    for (int s = threadIdx.x; s < n; s += threads) M = fmaxf(M, st[s].x);
 #pragma unroll
     for (int o = 16; o; o /= 2) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
     if (lane == 0) red[0][warp] = M;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) M = fmaxf(M, red[0][w]);
+    for (int w = 0; w < threads / 32; ++w) M = fmaxf(M, red[0][w]);
     const float base = M == -CUDART_INF_F ? 0.f : M;
     // rows of accumulators are read as pieces of four elements where they allow it
-    const int width = p.D % 4 ? 1 : 4, lanes = (p.D + width - 1) / width, sets = max(1, kJoinThreads / lanes);
+    const int width = p.D % 4 ? 1 : 4, lanes = (p.D + width - 1) / width, sets = max(1, threads / lanes);
     const int set = threadIdx.x / lanes, piece = threadIdx.x % lanes;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     float L = 0.f;
-    for (int s0 = 0; s0 < n; s0 += kJoinThreads) {
+    for (int s0 = 0; s0 < n; s0 += threads) {
         __syncthreads();
         const int s = s0 + threadIdx.x;
         float w = 0.f;
@@ -716,7 +717,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         __syncthreads();
         if (set < sets)
 #pragma unroll 4
-            for (int i = set; i < min(kJoinThreads, n - s0); i += sets) {
+            for (int i = set; i < min(threads, n - s0); i += sets) {
                 const float* src = p.part + (row * p.splits + s0 + i) * p.D + piece * width;
                 const float f = weight[i];
                 if (width == 4) {
@@ -733,8 +734,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     acc[threadIdx.x] = a;
     __syncthreads();
     L = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) L += red[1][w];
+    for (int w = 0; w < threads / 32; ++w) L += red[1][w];
     const float inv = L > 0.f ? 1.f / L : L;           // 0: no key; NaN stays
     if (set == 0) {
         for (int i = 1; i < sets; ++i) {

@@ -18,7 +18,7 @@
 // threads), here 67 us (76 % of the measured copy rate).
 #pragma once
 
-#include "mg_attention_tc.cuh"
+#include "mg_attention_math.cuh"
 
 namespace mg {
 
