@@ -40,7 +40,10 @@ typedef enum mg_dtype { MG_F32 = 0, MG_BF16 = 1 } mg_dtype;
  * used, nor is q or dout of a query of a negative document. Elsewhere v (and in the
  * backward pass k, q, dout) has to be finite also where a mask hides it from
  * some queries.
- * Strides are in elements, for {batch, head, row}; head_dim is contiguous. */
+ * scale lies within +-1e30, cap is 0 or within 1e-30..1e30. Strides are in
+ * elements, for {batch, head, row}; head_dim is contiguous. Outputs must not
+ * overlap k, v or each other. Tensors whose rows start on 16-byte boundaries and hold a
+ * multiple of 8 elements run on the tensor cores, others on the CUDA cores. */
 typedef struct mg_attention_desc {
     int32_t dtype;                       /* mg_dtype of q, k, v, out and the gradients */
     int32_t batch, heads, kv_heads, q_len, k_len, head_dim;

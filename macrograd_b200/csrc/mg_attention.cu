@@ -30,9 +30,7 @@ mg_status check_attention(const mg_attention_desc* d, const char* who)
         return fail(MG_ERR_INVALID, "%s: heads %d is not a multiple of kv_heads %d", who, d->heads, d->kv_heads);
     if (d->head_dim < 1 || d->head_dim > MG_MAX_HEAD_DIM)
         return fail(MG_ERR_UNSUPPORTED, "%s: head_dim %d is outside 1..%d", who, d->head_dim, MG_MAX_HEAD_DIM);
-    if (!std::isfinite(d->scale)) return fail(MG_ERR_INVALID, "%s: scale is not finite", who);
-    if (!(d->cap >= 0.f) || !std::isfinite(d->cap))
-        return fail(MG_ERR_INVALID, "%s: cap must be 0 (none) or a positive number", who);
+    MG_TRY(check_scores(d->scale, d->cap, who));
     if (d->prefix && !d->causal) return fail(MG_ERR_INVALID, "%s: a prefix needs causal", who);
     if ((int64_t)d->q_len + d->k_len >= (1ll << 30)) return fail(MG_ERR_UNSUPPORTED, "%s: rows are too long", who);
     const int64_t rows = (int64_t)d->batch * d->heads * std::max(ceil_div(d->q_len, 32), ceil_div(d->k_len, 32));
@@ -100,7 +98,7 @@ mg_status backward_simt(const mg::AttnParams& p, cudaStream_t st)
 bool tc_serves(const mg_attention_desc* d, const mg::AttnParams& p, std::initializer_list<const void*> rows_q,
                std::initializer_list<const void*> rows_k)
 {
-    if (d->head_dim % 8 || d->scale == 0.f || !std::isfinite(1.f / d->scale)) return false;
+    if (d->head_dim % 8 || std::fabs(d->scale) < 1e-30f) return false;
     const int vec = d->dtype == MG_BF16 ? 8 : 4;
     for (const void* x : rows_q)
         if (reinterpret_cast<uintptr_t>(x) % 16) return false;

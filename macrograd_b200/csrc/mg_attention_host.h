@@ -41,6 +41,17 @@ mg_status allow_smem(const Device& dev, size_t smem)
     return MG_OK;
 }
 
+// Sizes of scale and cap that every kernel's products and powers of two stay in range for.
+constexpr float kMostScale = 1e30f, kLeastCap = 1e-30f;
+
+inline mg_status check_scores(float scale, float cap, const char* who)
+{
+    if (!(std::fabs(scale) <= kMostScale)) return fail(MG_ERR_INVALID, "%s: scale must be a number within +-1e30", who);
+    if (cap != 0.f && !(cap >= kLeastCap && cap <= kMostScale))
+        return fail(MG_ERR_INVALID, "%s: cap must be 0 (none) or within 1e-30..1e30", who);
+    return MG_OK;
+}
+
 // Whether rows at `ptr` with these strides start on multiples of `vec` elements.
 inline bool aligned(const void* ptr, const int64_t* strides, int n, size_t elem, int vec)
 {

@@ -208,9 +208,7 @@ mg_status mg_paged_attention(const mg_paged_desc* d, void* out, float* lse, cons
         return fail(MG_ERR_INVALID, "%s: heads %d is not a multiple of kv_heads %d", who, d->heads, d->kv_heads);
     if (d->head_dim < 1 || d->head_dim > MG_MAX_HEAD_DIM)
         return fail(MG_ERR_UNSUPPORTED, "%s: head_dim %d is outside 1..%d", who, d->head_dim, MG_MAX_HEAD_DIM);
-    if (!std::isfinite(d->scale)) return fail(MG_ERR_INVALID, "%s: scale is not finite", who);
-    if (!(d->cap >= 0.f) || !std::isfinite(d->cap))
-        return fail(MG_ERR_INVALID, "%s: cap must be 0 (none) or a positive number", who);
+    MG_TRY(check_scores(d->scale, d->cap, who));
     if ((k_new == nullptr) != (v_new == nullptr))
         return fail(MG_ERR_INVALID, "%s: k_new and v_new come together", who);
     if (d->batch == 0) return MG_OK;

@@ -120,6 +120,13 @@ def _on(device: torch.device, stream: Optional[torch.cuda.Stream], call):
         return call(stream.cuda_stream)
 
 
+def _cap(cap: float) -> float:
+    cap = _number(cap, "cap")
+    if cap != 0 and not 1e-30 <= cap <= 1e30:
+        _bad("cap must be 0 (none) or within 1e-30..1e30")
+    return cap
+
+
 def _at(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -141,9 +148,7 @@ def _attention_args(q, k, v, scale, causal, cap, slopes, documents, prefix):
     if not 1 <= D <= MAX_HEAD_DIM:
         raise MacrogradError(_lib.MG_ERR_UNSUPPORTED, f"head_dim {D} is outside 1..{MAX_HEAD_DIM}")
     scale = 1.0 / math.sqrt(D) if scale is None else _number(scale, "scale")
-    cap = _number(cap, "cap")
-    if cap < 0:
-        _bad("cap must be 0 (none) or positive")
+    cap = _cap(cap)
     if slopes is not None:
         _plain(slopes, "slopes", (H,), torch.float32, dev)
     if documents is not None:
@@ -170,7 +175,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     A query sees the keys up to its own position (causal) and, besides, the first prefix[b] keys of its row (int32
     [B]); with documents (int32 [B, Lk], the id of each position) only keys of its own document. Ids below 0 mark
     padding: such keys and queries are left out whatever they hold. A query that sees no key gives out = 0,
-    lse = -inf. Everywhere else k, v must be finite also where a mask hides them from some queries.
+    lse = -inf. Everywhere else k, v must be finite also where a mask hides them from some queries. `out` must not
+    share memory with k or v.
 
     Returns (out, laid out as q, lse [B, H, Lq] in float32)."""
     lib = _lib.load()
@@ -352,9 +358,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _plain(block_table, "block_table", (B, width), torch.int32, dev)
     _plain(lengths, "lengths", (B,), torch.int32, dev)
     scale = 1.0 / math.sqrt(D) if scale is None else _number(scale, "scale")
-    cap = _number(cap, "cap")
-    if cap < 0:
-        _bad("cap must be 0 (none) or positive")
+    cap = _cap(cap)
     if slopes is not None:
         _plain(slopes, "slopes", (H,), torch.float32, dev)
     if (k_new is None) != (v_new is None):

@@ -49,6 +49,8 @@ def attention(**kw):
     (dict(scale=float("nan")), INVALID, "scale"),
     (dict(cap=-1.0), INVALID, "cap"),
     (dict(cap=float("inf")), INVALID, "cap"),
+    (dict(cap=1e-31), INVALID, "cap"),
+    (dict(scale=2e30), INVALID, "scale"),
     (dict(causal=0, prefix=PTR), INVALID, "prefix"),
     (dict(Lq=1 << 29, Lk=1 << 29), UNSUPPORTED, "too long"),
     (dict(B=1 << 20, H=1 << 10, Lq=256), UNSUPPORTED, "too large"),

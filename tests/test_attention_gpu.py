@@ -183,6 +183,83 @@ def test_scale_is_the_callers():
     compare(q, k, v, dout, dict(kw, scale=-0.05))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_negative_scale_with_cap_and_slopes(dtype, D):
+    q, k, v, dout, kw = make((1, 2, 1, 150, 150, D), "all", dtype, 12)
+    compare(q, k, v, dout, dict(kw, scale=-0.1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_a_scale_of_zero_and_far_caps(dtype):
+    """Every seen key weighs the same; a cap far above the scores changes nothing, one far below makes them all its own."""
+    q, k, v, dout, kw = make((1, 2, 1, 150, 150, 64), "causal", dtype, 12)
+    compare(q, k, v, dout, dict(kw, scale=0.0))
+    compare(q, k, v, dout, dict(kw, cap=1e6))
+    out, lse = mg.attention(q, k, v, cap=1e-20, **kw)
+    ref = Reference(q, k, v, scale=0.0, **kw)
+    within(out, ref.out, ref.out_tol, "out under a cap of nearly nothing")
+    assert torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 33])
+def test_broadcast_keys_and_values(dtype, D):
+    """k and v expanded over the batch and over heads (stride 0)."""
+    g = torch.Generator(device="cuda").manual_seed(14)
+    q, dout = (torch.randn((3, 4, 140, D), generator=g, device="cuda").to(dtype) for _ in range(2))
+    k = torch.randn((1, 2, 200, D), generator=g, device="cuda").to(dtype).expand(3, 2, 200, D)
+    v = torch.randn((3, 1, 200, D), generator=g, device="cuda").to(dtype).expand(3, 2, 200, D)
+    compare(q, k, v, dout, dict(causal=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("ids", ["each its own", "any sign", "one", "none"])
+def test_kinds_of_documents(dtype, ids):
+    """A document to each position, ids of any 32-bit value, a single document, nothing but padding."""
+    L = 270
+    q, k, v, dout, _ = make((2, 2, 2, L, L, 64), "causal", dtype, 15)
+    docs = {"each its own": torch.arange(L), "any sign": torch.randint(-3, 3, (L,), generator=torch.Generator().manual_seed(1))
+            * (2 ** 30) + torch.arange(L) // 90, "one": torch.full((L,), 2 ** 31 - 1), "none": torch.full((L,), -7)}[ids]
+    kw = dict(documents=docs.int().cuda().expand(2, L).contiguous())
+    compare(q, k, v, dout, dict(kw, causal=True))
+    compare(q, k, v, dout, dict(kw, causal=False))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_prefixes_out_of_range(dtype):
+    q, k, v, dout, _ = make((3, 2, 2, 130, 200, 64), "causal", dtype, 16)
+    compare(q, k, v, dout, dict(prefix=torch.tensor([-5, 0, 2 ** 31 - 1], dtype=torch.int32, device="cuda")))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_few_queries_of_a_long_row(dtype):
+    q, k, v, dout, kw = make((1, 2, 1, 3, 5000, 64), "causal", dtype, 17)
+    compare(q, k, v, dout, kw)
+
+
+def test_two_graphs_at_once():
+    """Two captured graphs, each with scratch of its own, replayed on two streams at the same time."""
+    sets = [make((1, 8, 2, 900, 900, 64), "all", torch.bfloat16, 40 + i) for i in range(2)]
+    want, graphs, got = [], [], []
+    for q, k, v, dout, kw in sets:
+        f = mg.attention(q, k, v, **kw)
+        want.append(f + mg.attention_backward(dout, q, k, v, *f, **kw))
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            f = mg.attention(q, k, v, **kw)
+            got.append(f + mg.attention_backward(dout, q, k, v, *f, **kw))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(4):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_out_and_its_neighbours():
     """out given as a view: its rows are written, what lies around them stays."""
     q, k, v, _, kw = make((2, 3, 3, 150, 150, 64), "causal", torch.bfloat16, 9)
@@ -298,6 +375,8 @@ def test_refusals():
         (lambda: mg.attention(q.transpose(2, 3).contiguous().transpose(2, 3), kv, kv), "contiguous in its last dim"),
         (lambda: mg.attention(t(1, 4, 8, 136), t(1, 2, 8, 136), t(1, 2, 8, 136)), "head_dim"),
         (lambda: mg.attention(q, kv, kv, cap=-1.0), "cap"),
+        (lambda: mg.attention(q, kv, kv, cap=1e31), "cap"),
+        (lambda: mg.attention(q, kv, kv, scale=1e31), "scale"),
         (lambda: mg.attention(q, kv, kv, scale=math.inf), "finite"),
         (lambda: mg.attention(q, kv, kv, slopes=t(2)), "slopes"),
         (lambda: mg.attention(q, kv, kv, documents=t(1, 8)), "documents"),

@@ -161,6 +161,26 @@ def test_captured_and_replayed_while_requests_grow(dtype):
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
 
 
+def test_same_inputs_same_bits():
+    args = make(4, 8, 2, 128, 16, [3000, 7, 129, 4097], torch.bfloat16)
+    q, kp, vp, table, lengths, kn, vn = args
+    first = mg.paged_attention(q, kp, vp, table, lengths, k_new=kn, v_new=vn)
+    for _ in range(3):
+        again = mg.paged_attention(q, kp, vp, table, lengths, k_new=kn, v_new=vn)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("lengths", [[900], [1, 128, 129, 1000], [2000] * 40])
+def test_chunks_joined_in_a_cluster_and_by_a_kernel(lengths):
+    """Few short requests join their chunks in one cluster, many or long ones in a second launch, with a table much wider
+    than the requests too."""
+    for Hkv in (1, 8):
+        args = make(len(lengths), 8, Hkv, 64, 16, lengths, torch.bfloat16, seed=3)
+        compare(args)
+        wide = torch.cat([args[3], torch.zeros((len(lengths), 500), dtype=torch.int32, device="cuda")], 1)
+        compare((*args[:3], wide, *args[4:]))
+
+
 def test_offsets_beyond_32_bits():
     """Pages more than 2^31 elements into the pool."""
     page, Hkv, D = 256, 1, 128
