@@ -215,7 +215,7 @@ mg_status backward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     float* stats = static_cast<float*>(ws.get(2 * rows * sizeof(float)));
     if (!stats) return fail(MG_ERR_ALLOC, "%s: no scratch for the row sums", who);
     t.lse2 = stats, t.delta = stats + rows;
-    mg::attn_tc_stats_kernel<__nv_bfloat16><<<ceil_div(rows, 16), 256, 0, st>>>(p, t.Lp, stats, stats + rows);
+    mg::attn_tc_stats_kernel<__nv_bfloat16><<<ceil_div(rows, 16 * mg::kStatsRows), 256, 0, st>>>(p, t.Lp, stats, stats + rows);
     MG_TRY(launched(who));
     int* hs = t.head_step;
     int* bs = t.batch_step;
@@ -292,7 +292,7 @@ mg_status backward_tc32(const mg::AttnParams& p, const Device& dev, void* stream
     const int64_t rows = (int64_t)p.B * p.H * Lp;
     float* stats = static_cast<float*>(ws.get(2 * rows * sizeof(float)));
     if (!stats) return fail(MG_ERR_ALLOC, "%s: no scratch for the row sums", who);
-    mg::attn_tc_stats_kernel<float><<<ceil_div(rows, 16), 256, 0, st>>>(p, Lp, stats, stats + rows);
+    mg::attn_tc_stats_kernel<float><<<ceil_div(rows, 16 * mg::kStatsRows), 256, 0, st>>>(p, Lp, stats, stats + rows);
     MG_TRY(launched(who));
     mg::Tc32BwdParams t = {p, f.doc_tiles, stats, stats + rows, Lp, 0, f.scale, f.status};
     t.idesc_s = mg::idesc_bf16(128, p.D <= 64 ? 64 : 32, false, false, p.scale < 0.f);

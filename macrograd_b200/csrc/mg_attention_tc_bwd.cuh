@@ -56,7 +56,7 @@ struct TcBwdParams {
 };
 
 // lse2 and delta of each row, padded with rows whose P is 0. 16 lanes to a row of
-// up to 128 elements, 8 each.
+// up to 128 elements, 8 each, and four rows at once: bound by the reads of out and dout.
 __device__ __forceinline__ void load8(const __nv_bfloat16* x, float (&v)[8])
 {
     const uint4 w = *reinterpret_cast<const uint4*>(x);
@@ -73,34 +73,49 @@ __device__ __forceinline__ void load8(const float* x, float (&v)[8])
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
+constexpr int kStatsRows = 4;            // of a group of 16 lanes; divides Lp
+
 template <typename T>
-__global__ void attn_tc_stats_kernel(const __grid_constant__ AttnParams p, int Lp, float* __restrict__ lse2,
-                                     float* __restrict__ delta)
+__global__ void __launch_bounds__(256) attn_tc_stats_kernel(const __grid_constant__ AttnParams p, int Lp,
+                                                            float* __restrict__ lse2, float* __restrict__ delta)
 {
-    const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 16;
-    if (row >= (int64_t)p.B * p.H * Lp) return;      // whole 16-lane groups, and Lp is even: whole warps
-    const int part = threadIdx.x % 16, i = (int)(row % Lp);
-    const int64_t bh = row / Lp;
-    const int h = (int)(bh % p.H), b = (int)(bh / p.H);
-    float s = 0.f, l = CUDART_INF_F;
-    if (i < p.Lq) {
-        const float lse = p.lse[bh * p.Lq + i];
-        if (lse != -CUDART_INF_F) {
-            l = lse * kLog2e;
-            if (part * 8 < p.D) {
-                float o[8], g[8];
-                load8((const T*)p.out + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2] + part * 8, o);
-                load8((const T*)p.dout + b * p.dos[0] + h * p.dos[1] + (int64_t)i * p.dos[2] + part * 8, g);
+    const uint32_t group = (blockIdx.x * blockDim.x + threadIdx.x) / 16, per = (uint32_t)Lp / kStatsRows;
+    if (group >= (uint32_t)p.B * p.H * per) return;     // an even number of groups: whole warps
+    const int part = threadIdx.x % 16;
+    // heads first: their rows lie side by side where heads were split from [batch, length, heads * D]
+    const uint32_t at_h = group / (uint32_t)p.H, h = group - at_h * (uint32_t)p.H, b = at_h / per, bh = b * (uint32_t)p.H + h;
+    const int i0 = (int)(at_h - b * per) * kStatsRows;
+    const T* out = (const T*)p.out + b * p.os[0] + h * p.os[1] + part * 8;
+    const T* dout = (const T*)p.dout + b * p.dos[0] + h * p.dos[1] + part * 8;
+    float o[kStatsRows][8], g[kStatsRows][8], lse[kStatsRows];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) s = fmaf(o[k], g[k], s);
-            }
+    for (int k = 0; k < kStatsRows; ++k) {
+        const int i = i0 + k;
+        lse[k] = i < p.Lq ? __ldg(p.lse + (int64_t)bh * p.Lq + i) : -CUDART_INF_F;
+        if (i < p.Lq && part * 8 < p.D) {
+            load8(out + i * p.os[2], o[k]);
+            load8(dout + i * p.dos[2], g[k]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[k][e] = g[k][e] = 0.f;
         }
     }
+    float sum[kStatsRows];
 #pragma unroll
-    for (int o = 8; o; o /= 2) s += __shfl_xor_sync(~0u, s, o);
+    for (int k = 0; k < kStatsRows; ++k) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(o[k][e], g[k][e], s);
+#pragma unroll
+        for (int w = 8; w; w /= 2) s += __shfl_xor_sync(~0u, s, w);
+        // a row that sees nothing: P = 0 whatever its dout holds
+        sum[k] = lse[k] == -CUDART_INF_F ? 0.f : s;
+        lse[k] = lse[k] == -CUDART_INF_F ? CUDART_INF_F : lse[k] * kLog2e;
+    }
     if (part == 0) {
-        lse2[row] = l;
-        delta[row] = s;
+        const int64_t at = (int64_t)bh * Lp + i0;
+        *reinterpret_cast<float4*>(lse2 + at) = make_float4(lse[0], lse[1], lse[2], lse[3]);
+        *reinterpret_cast<float4*>(delta + at) = make_float4(sum[0], sum[1], sum[2], sum[3]);
     }
 }
 
