@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             lse2 = tp.lse2[at];
             delta = tp.delta[at];
         }
-        float rsum = 0.f;            // this thread's part of its row's sum of P * (dP - delta)
+        uint64_t rsum2 = pack2(0.f, 0.f);   // this thread's part of its row's sum of P * (dP - delta)
         bool ok = true;
         // this lane's document of a tile's streamed rows, a tile of the set ahead
         const auto y_of = [&](int i) { return (t0 + (kKeys ? i % tiles : i)) * 64; };
@@ -426,23 +426,26 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                     for (int k = 0; k < 4; k += 2) {
                         const int at = c0 + c + k;
                         const uint64_t d = add2(pack2(g[c + k], g[c + k + 1]), pack2(nd[k], nd[k + 1]));
-                        const uint64_t x = mul2(pack2(v[at], v[at + 1]), d);
+                        uint64_t x = mul2(pack2(v[at], v[at + 1]), d);
                         unpack2(x, e[k], e[k + 1]);
                         if (!full) {
                             e[k] = v[at] == 0.f ? 0.f : e[k];
                             e[k + 1] = v[at + 1] == 0.f ? 0.f : e[k + 1];
+                            x = pack2(e[k], e[k + 1]);
                         }
-                        if (!kKeys) {
-                            if (kCap) {
-                                float d0, d1;
-                                unpack2(d, d0, d1);
-                                const float p0 = v[at] + __uint_as_float(w[at / 2] << 16);
-                                const float p1 = v[at + 1] + __uint_as_float(w[at / 2] & 0xFFFF0000u);
-                                rsum += (p0 == 0.f ? 0.f : p0 * d0) + (p1 == 0.f ? 0.f : p1 * d1);
+                        if (!kKeys && kCap) {
+                            // P * (dP - delta): what the curve takes off is added again
+                            const uint64_t off = pack2(__uint_as_float(w[at / 2] << 16), __uint_as_float(w[at / 2] & 0xFFFF0000u));
+                            if (full) {
+                                x = fma2(off, d, x);
                             } else {
-                                rsum += e[k] + e[k + 1];
+                                float a, c2, o0, o1;
+                                unpack2(mul2(off, d), a, c2);
+                                unpack2(off, o0, o1);
+                                x = add2(x, pack2(o0 == 0.f ? 0.f : a, o1 == 0.f ? 0.f : c2));
                             }
                         }
+                        if (!kKeys) rsum2 = add2(rsum2, x);
                     }
                     ds[c / 2] = bf16x2(e[0], e[1]);
                     ds[c / 2 + 1] = bf16x2(e[2], e[3]);
@@ -454,8 +457,11 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&st.ds_full[set]));
         }
+        float rsum = 0.f;
         if (!kKeys) {
-            st.sums[warp / 4][r] = rsum;
+            float odd;
+            unpack2(rsum2, rsum, odd);
+            st.sums[warp / 4][r] = rsum + odd;
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&st.sum_full));
             ok = ok && tc_wait(smem_u32(&st.sum_full), 0, failed);
