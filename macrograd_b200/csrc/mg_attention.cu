@@ -149,13 +149,36 @@ mg_status tc_params(mg::TcAttnParams* t, const mg::AttnParams& p, const Device& 
     return MG_OK;
 }
 
+// Parts of a row of keys: where the blocks (of 128 queries of a head) would leave
+// places on the GPU empty, each row is shared by as many as fill them, of no less than 512
+// keys each (the join costs a few microseconds). Scratch for more than one.
+mg_status share_rows(mg::RowParts* r, const mg::AttnParams& p, int places, Scratch& ws)
+{
+    const int64_t blocks = (int64_t)ceil_div(p.Lq, 128) * p.B * p.H;
+    r->parts = (int)std::max<int64_t>(1, std::min<int64_t>(places / blocks, ceil_div(p.Lk, 512)));
+    if (r->parts == 1) return MG_OK;
+    const int64_t rows = (int64_t)r->parts * p.B * p.H * p.Lq;
+    r->out = static_cast<float*>(ws.get(rows * (p.D + 1) * sizeof(float)));
+    if (!r->out) return fail(MG_ERR_ALLOC, "mg_attention: no scratch for %d parts of each row", r->parts);
+    r->lse = r->out + rows * p.D;
+    return MG_OK;
+}
+
+template <typename T>
+mg_status join_rows(const mg::RowParts& r, const mg::AttnParams& p, cudaStream_t st)
+{
+    if (r.parts == 1) return MG_OK;
+    mg::attn_join_kernel<T><<<ceil_div((int64_t)p.B * p.H * p.Lq, 8), 256, 0, st>>>(p, r);
+    return launched("mg_attention");
+}
+
 template <int DP, bool kCap, bool kBias>
 mg_status launch_tc_forward(const mg::TcAttnParams& t, const Device& dev, cudaStream_t st)
 {
     constexpr auto kernel = mg::attn_tc_forward<DP, kCap, kBias>;
     constexpr size_t smem = mg::tc_forward_smem<DP>();
     MG_TRY(allow_smem<kernel>(dev, smem));
-    kernel<<<ceil_div(t.a.Lq, 128) * t.a.B * t.a.H, mg::kTcFwdThreads, smem, st>>>(t);
+    kernel<<<ceil_div(t.a.Lq, 128) * t.a.B * t.a.H * t.rows.parts, mg::kTcFwdThreads, smem, st>>>(t);
     return launched("mg_attention");
 }
 
@@ -176,7 +199,9 @@ mg_status forward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     MG_TRY(tc_map(&t.q, &t.head_step[0], &t.batch_step[0], p.q, p.qs, p.D, p.Lq, p.H, p.B, 128));
     MG_TRY(tc_map(&t.k, &t.head_step[1], &t.batch_step[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 128));
     MG_TRY(tc_map(&t.v, &t.head_step[2], &t.batch_step[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 128));
-    return p.D <= 64 ? launch_tc_forward<64>(t, dev, st) : launch_tc_forward<128>(t, dev, st);
+    MG_TRY(share_rows(&t.rows, p, 2 * dev.sm_count, ws));
+    MG_TRY((p.D <= 64 ? launch_tc_forward<64>(t, dev, st) : launch_tc_forward<128>(t, dev, st)));
+    return join_rows<__nv_bfloat16>(t.rows, p, st);
 }
 
 template <int DP, bool kKeys, bool kCap, bool kBias>
@@ -239,7 +264,7 @@ mg_status launch_tc32_forward(const mg::Tc32Params& t, const Device& dev, cudaSt
     constexpr auto kernel = mg::attn_tc32_forward<DP, kCap, kBias>;
     constexpr size_t smem = mg::tc32_forward_smem<DP>();
     MG_TRY(allow_smem<kernel>(dev, smem));
-    kernel<<<ceil_div(t.a.Lq, 128) * t.a.B * t.a.H, mg::kTc32Threads, smem, st>>>(t);
+    kernel<<<ceil_div(t.a.Lq, 128) * t.a.B * t.a.H * t.rows.parts, mg::kTc32Threads, smem, st>>>(t);
     return launched("mg_attention");
 }
 
@@ -257,8 +282,10 @@ mg_status forward_tc32(const mg::AttnParams& p, const Device& dev, void* stream)
     Scratch ws(dev, stream);
     cudaStream_t st = (cudaStream_t)stream;
     MG_TRY(tc_params(&f, p, dev, ws, st, "mg_attention"));
-    mg::Tc32Params t = {p, f.doc_tiles, mg::idesc_bf16(128, 64, false, false, p.scale < 0.f), f.scale, f.status};
-    return p.D <= 64 ? launch_tc32_forward<64>(t, dev, st) : launch_tc32_forward<128>(t, dev, st);
+    mg::Tc32Params t = {p, f.doc_tiles, mg::idesc_bf16(128, 64, false, false, p.scale < 0.f), f.scale, {}, f.status};
+    MG_TRY(share_rows(&t.rows, p, (p.D <= 64 ? 2 : 1) * dev.sm_count, ws));
+    MG_TRY((p.D <= 64 ? launch_tc32_forward<64>(t, dev, st) : launch_tc32_forward<128>(t, dev, st)));
+    return join_rows<float>(t.rows, p, st);
 }
 
 template <int DP, bool kKeys, int kTake, bool kCap, bool kBias>

@@ -24,6 +24,14 @@ struct AttnParams {
     float* delta;
 };
 
+// A row of keys shared by several blocks of the forward kernels, where there are
+// too few queries to fill the GPU: each leaves its part's out and lse in fp32.
+struct RowParts {
+    int parts;           // 1: the block writes out and lse itself
+    float* out;          // [parts][B * H][Lq][D]
+    float* lse;          // [parts][B * H][Lq]
+};
+
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <typename T>

@@ -4,20 +4,22 @@
 // Forward: one block per 128 queries of one head; two blocks share an SM. Per
 // tile of 128 keys
 //     S = Q K^T        (tcgen05, Q and K in shared memory, S in tensor memory)
-//     P = exp2(S - m)  (four warps; thread i owns query i: no shuffles)
+//     P = exp2(S - m)  (eight warps; warps w and w + 4 have the same 32 queries, a
+//                       thread a query, and half of the keys each: no shuffles)
 //     O += P V         (tcgen05, P from tensor memory, written over S)
 // with the running maximum m of each query in a register. O stays in tensor
 // memory; it is rescaled only when a row's maximum has grown by more than 2^8
 // since it was last used (P is then at most 2^8, exact in bf16's range, and the
 // division by the row sum at the end takes the factor out).
 //
-// Why this shape: the exponentials bound the kernel (16 a clock and SM: 1024
-// clocks a tile, as much as both products together at head_dim 128), so the
-// tensor core has to work on one tile while the exponentials of another are
-// taken. Two blocks an SM with one tile each do that without any hand-off
-// between them; each needs half of the tensor memory (128 columns S, 64 or 128
-// columns O) and one buffer for K and for V, refilled by TMA as soon as its
-// product is done.
+// Why this shape: a tile's exponentials take as long as both of its products at
+// head_dim 128 (16 a clock and SM: 1024 clocks), so the tensor core has to work on one
+// tile while the exponentials of another are taken. Two blocks an SM with one tile
+// each do that without any hand-off between them; each needs half of the tensor memory
+// (128 columns S, 64 or 128 columns O) and one buffer for K and for V, refilled by TMA as
+// soon as its product is done. bf16 [1, 16 over 4, 8192, 128], causal, capped: 0.38 ms,
+// 720 TFLOP/s; the fp32, exponential and integer pipes together are busy all of a tile
+// pair's 4500 clocks, the tensor pipe 38 % of them.
 #pragma once
 
 #include "mg_attention_math.cuh"
@@ -127,6 +129,7 @@ struct TcAttnParams {
     uint32_t idesc_s;            // of S = Q K^T: A negated where the scale is negative
     float scale;                 // |scale|
     CapCurve curve;
+    RowParts rows;
     int* status;
 };
 
@@ -175,6 +178,46 @@ __device__ __forceinline__ void tc_clear_padding(uint32_t tile, int rows, const 
     __syncwarp();
 }
 
+// The block's share of tiles [t0, t1): part of `parts`.
+__device__ __forceinline__ void share_of_row(int part, int parts, int& t0, int& t1)
+{
+    const int each = (max(0, t1 - t0) + parts - 1) / parts;
+    t0 += part * each;
+    t1 = min(t1, t0 + each);
+}
+
+// Joins the parts of each row: out = sum exp(lse_s - lse) out_s, lse = log sum exp(lse_s).
+// One warp to a row, four elements to a lane.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnParams p, RowParts rows)
+{
+    const int64_t all = (int64_t)p.B * p.H * p.Lq, at = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
+    if (at >= all) return;
+    const int lane = threadIdx.x % 32;
+    float top = -CUDART_INF_F;
+    for (int s = 0; s < rows.parts; ++s) top = fmaxf(top, __ldg(rows.lse + s * all + at));
+    const float base = top == -CUDART_INF_F ? 0.f : top;
+    float sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool in = lane * 4 < p.D;
+    for (int s = 0; s < rows.parts; ++s) {
+        const float w = expf(__ldg(rows.lse + s * all + at) - base);
+        sum += w;
+        if (!in || w == 0.f) continue;
+        const float4 x = __ldg(reinterpret_cast<const float4*>(rows.out + (s * all + at) * p.D) + lane);
+        o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum;      // 0: no key; NaN stays
+    const int64_t bh = at / p.Lq;
+    const int row = (int)(at - bh * p.Lq), h = (int)(bh % p.H), b = (int)(bh / p.H);
+    T* out = (T*)p.out + b * p.os[0] + h * p.os[1] + row * p.os[2] + lane * 4;
+    if (in) {
+        out[0] = from_f32<T>(o.x * inv), out[1] = from_f32<T>(o.y * inv);
+        out[2] = from_f32<T>(o.z * inv), out[3] = from_f32<T>(o.w * inv);
+    }
+    if (lane == 0) p.lse[at] = sum == 0.f ? -CUDART_INF_F : base + logf(sum);
+}
+
 constexpr int kTcFwdThreads = 320;       // eight warps of exponentials, loads, products
 
 template <int DP>
@@ -192,7 +235,8 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
 
     // blocks with the most keys first
     const int heads = p.B * p.H, qtiles = (p.Lq + 127) / 128;
-    const int qt = qtiles - 1 - blockIdx.x / heads, bh = blockIdx.x % heads;
+    const int part = blockIdx.x % tp.rows.parts, block = blockIdx.x / tp.rows.parts;
+    const int qt = qtiles - 1 - block / heads, bh = block % heads;
     const int h = bh % p.H, b = bh / p.H, kv = h / (p.H / p.Hkv);
     const int q0 = qt * 128, shift = p.Lk - p.Lq;
     const int32_t* docs = p.docs ? p.docs + (int64_t)b * p.Lk : nullptr;
@@ -223,6 +267,7 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
     int t0 = 0, t1 = (kend + 127) / 128;
     const int2* dt = docs ? tp.doc_tiles + (int64_t)b * ((p.Lk + 127) / 128) : nullptr;
     if (docs) narrow_to_docs(dt, p.Lk, 0, 128, docs_of(dt, q0 + shift, 128, p.Lk), t0, t1);
+    share_of_row(part, tp.rows.parts, t0, t1);
     const int n = max(0, t1 - t0);
     tc_fence_before();
     __syncthreads();
@@ -434,6 +479,15 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
                     for (int i = 0; i < 32; ++i) o[i] = 0.f;
                 }
                 if (!store) continue;
+                if (tp.rows.parts > 1) {
+                    float* to = tp.rows.out + (((int64_t)part * p.B * p.H + bh) * p.Lq + row) * p.D + c;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        if (c + i + 4 <= c1)
+                            *reinterpret_cast<float4*>(to + i) =
+                                make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+                    continue;
+                }
 #pragma unroll
                 for (int i = 0; i < 32; i += 8)
                     if (c + i + 8 <= c1)
@@ -442,7 +496,7 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
                                        bf16x2(o[i + 4] * inv, o[i + 5] * inv), bf16x2(o[i + 6] * inv, o[i + 7] * inv));
             }
             if (store && half == 0)
-                p.lse[((int64_t)b * p.H + h) * p.Lq + row] =
+                (tp.rows.parts > 1 ? tp.rows.lse + (int64_t)part * p.B * p.H * p.Lq : p.lse)[(int64_t)bh * p.Lq + row] =
                     l == 0.f ? -CUDART_INF_F : ((m == -CUDART_INF_F ? 0.f : m * mul) + log2f(l)) * kLn2;
         }
         if (!ok && lane == 0) tc_report(tp.status, 202);

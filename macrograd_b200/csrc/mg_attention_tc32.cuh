@@ -81,6 +81,7 @@ struct Tc32Params {
     const int2* doc_tiles;
     uint32_t idesc_s;            // of S: A negated where the scale is negative
     float scale;                 // |scale|
+    RowParts rows;
     int* status;
 };
 
@@ -109,7 +110,8 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
     constexpr int kLoadWarp = 4, kMmaWarp = 4 + kTc32LoadWarps;
 
     const int heads = p.B * p.H, qtiles = (p.Lq + 127) / 128;
-    const int qt = qtiles - 1 - blockIdx.x / heads, bh = blockIdx.x % heads;
+    const int part = blockIdx.x % tp.rows.parts, block = blockIdx.x / tp.rows.parts;
+    const int qt = qtiles - 1 - block / heads, bh = block % heads;
     const int h = bh % p.H, b = bh / p.H, kv = h / (p.H / p.Hkv);
     const int q0 = qt * 128, shift = p.Lk - p.Lq;
     const int32_t* docs = p.docs ? p.docs + (int64_t)b * p.Lk : nullptr;
@@ -135,6 +137,7 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
     // Tiles of 64 keys [t0, t1) that a query of this block sees something of.
     int t0 = 0, t1 = ((!p.causal ? p.Lk : max(0, min(p.Lk, max(qlast + 1, prefix)))) + 63) / 64;
     if (docs) narrow_to_docs(dt, p.Lk, 0, 64, docs_of(dt, q0 + shift, 128, p.Lk), t0, t1);
+    share_of_row(part, tp.rows.parts, t0, t1);
     const int n = max(0, t1 - t0);
     tc_fence_before();
     __syncthreads();
@@ -370,7 +373,8 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
         if (ok) {
             tc_fence_after();
             const float g = f * (l > 0.f ? 1.f / l : l);   // 0: no key; NaN stays
-            float* out = (float*)p.out + b * p.os[0] + h * p.os[1] + (int64_t)row * p.os[2];
+            float* out = tp.rows.parts > 1 ? tp.rows.out + (((int64_t)part * p.B * p.H + bh) * p.Lq + row) * p.D
+                                           : (float*)p.out + b * p.os[0] + h * p.os[1] + (int64_t)row * p.os[2];
 #pragma unroll
             for (int c0 = 0; c0 < DP; c0 += 32) {
                 float x[32];
@@ -390,7 +394,7 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
                     }
             }
             if (row < p.Lq)
-                p.lse[((int64_t)b * p.H + h) * p.Lq + row] =
+                (tp.rows.parts > 1 ? tp.rows.lse + (int64_t)part * p.B * p.H * p.Lq : p.lse)[(int64_t)bh * p.Lq + row] =
                     l == 0.f ? -CUDART_INF_F : ((m == -CUDART_INF_F ? 0.f : m) + log2f(l)) * kLn2;
         }
         if (!ok && lane == 0) tc_report(tp.status, 222);

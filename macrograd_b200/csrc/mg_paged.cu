@@ -38,7 +38,8 @@ mg_status launch_paged_kernel(const mg::PagedParams& p, const Device& dev, int b
 }
 
 // Splits: 16 blocks an SM, so that requests of uneven lengths even out, but no chunk
-// shorter than 128 keys. Measured with 8 / 16 / 24 / 48: 32 requests of 1..8192 keys
+// shorter than 128 keys, or 512 where there are heads enough for the GPU (a block's
+// start costs what 100 keys do: 113 -> 111 us for the 32 requests). Measured with 8 / 16 / 24 / 48: 32 requests of 1..8192 keys
 // 120 / 102 / 105 / 120 us, two of 100 000 108 / 115 / 120 / 139 us.
 template <typename T>
 mg_status launch_paged(mg::PagedParams& p, int longest, const Device& dev, Scratch& ws, cudaStream_t st,
@@ -52,9 +53,8 @@ mg_status launch_paged(mg::PagedParams& p, int longest, const Device& dev, Scrat
     const int64_t heads = (int64_t)p.B * p.Hkv * packs;
     const int64_t want = std::max<int64_t>(1, (int64_t)dev.sm_count * 16 / heads);
     const int most = std::max(1, ceil_div(longest, 128));
-    int splits = (int)std::min<int64_t>(want, most);
-    p.chunk = std::max(1, ceil_div(longest, splits));
-    p.splits = splits = std::max(1, ceil_div(longest, p.chunk));
+    const int splits = p.splits = (int)std::min<int64_t>(want, most);
+    p.least = heads >= dev.sm_count ? 512 : 128;
     if (heads * splits >= (1ll << 31) - 1) return fail(MG_ERR_UNSUPPORTED, "%s: batch is too large", who);
     p.curve = cap_curve(std::fabs(p.scale), p.cap);
     p.page_shift = -1;

@@ -4,7 +4,7 @@
 // Two forms. paged_kernel streams the cache through shared memory (rows on
 // 16-byte boundaries); paged_simt_kernel takes any strides.
 //
-// One block reads `chunk` keys of one key-value head of one request, once, for
+// One block reads a chunk of the keys of one key-value head of one request, once, for
 // all query heads that share it (in groups of kPagedHeads), and leaves per query
 // head the maximum m, the sum l = sum exp(s - m) and the sum of exp(s - m) v. A
 // request of one chunk is finished there; otherwise a second kernel joins its
@@ -33,7 +33,7 @@ struct PagedParams {
     void* out;
     float* lse;
     int page_shift;              // log2(page), or -1
-    int chunk, splits;           // keys a block reads; blocks along the length
+    int splits, least;           // blocks along the length of a request; fewest keys of one
     CapCurve curve;              // of the cap, with a cap
     float* part;                 // [B * H][splits][D] accumulators
     float2* stat;                // [B * H][splits] (m, l)
@@ -50,6 +50,15 @@ __device__ __forceinline__ int paged_length(const PagedParams& p, int b)
     const int64_t most = (int64_t)p.width * p.page;
     const int n = __ldg(p.lengths + b);
     return n < 0 ? 0 : n > most ? (int)most : n;
+}
+
+// Keys that a block of a request of `len` keys reads: its share, but no less than
+// `least`, in whole rounds of the block's four tiles. By the request's own length:
+// the block table may be much wider.
+__device__ __forceinline__ int paged_chunk(const PagedParams& p, int len)
+{
+    const int share = (len + p.splits - 1) / p.splits;
+    return (max(share, p.least) + 63) / 64 * 64;
 }
 
 __device__ __forceinline__ void paged_report(const PagedParams& p, int code)
@@ -116,7 +125,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_simt_kernel(const __grid_
     const int pack = bh % packs, kv = bh / packs % p.Hkv, b = bh / packs / p.Hkv;
     const int len = paged_length(p, b);
     if (threadIdx.x == 0 && split == 0 && p.lengths && __ldg(p.lengths + b) != len) paged_report(p, kPagedBadLength);
-    const int j0 = split * p.chunk, j1 = min(len, j0 + p.chunk);
+    const int chunk = paged_chunk(p, len);
+    const int j0 = min(len, split * chunk), j1 = min(len, j0 + chunk);
     const int h0 = kv * groups + pack * kPagedHeads, nh = min(kPagedHeads, groups - pack * kPagedHeads);
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     constexpr int kWarps = kPagedThreads / 32, kPer = MG_MAX_HEAD_DIM / 32;
@@ -526,7 +536,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
     const int pack = bh % packs, kv = bh / packs % p.Hkv, b = bh / packs / p.Hkv;
     const int len = paged_length(p, b);
     if (threadIdx.x == 0 && split == 0 && p.lengths && __ldg(p.lengths + b) != len) paged_report(p, kPagedBadLength);
-    const int j0 = split * p.chunk, j1 = min(len, j0 + p.chunk);
+    const int chunk = paged_chunk(p, len);
+    const int j0 = min(len, split * chunk), j1 = min(len, j0 + chunk);
     if (!kCluster && j0 >= j1 && split > 0) return;      // a chunk beyond the request's keys is not joined
     const int h0 = kv * groups + pack * kPack, nh = min(kPack, groups - pack * kPack);
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -689,7 +700,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     const int64_t row = blockIdx.x;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int b = (int)(row / p.H), h = (int)(row % p.H);
-    const int n = max(1, (paged_length(p, b) + p.chunk - 1) / p.chunk);
+    const int len = paged_length(p, b), chunk = paged_chunk(p, len), n = max(1, (len + chunk - 1) / chunk);
     const float2* st = p.stat + row * p.splits;
     float M = -CUDART_INF_F;
     for (int s = threadIdx.x; s < n; s += threads) M = fmaxf(M, st[s].x);

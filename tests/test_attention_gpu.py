@@ -238,6 +238,14 @@ def test_few_queries_of_a_long_row(dtype):
     compare(q, k, v, dout, kw)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("mask", ["full", "all"])
+@pytest.mark.parametrize("D", [64, 96])
+def test_rows_shared_by_several_blocks(dtype, mask, D):
+    """Few heads: each row of keys is read in parts and joined; parts without a key that is seen, and rows without any."""
+    compare(*make((1, 2, 1, 700, 3100, D), mask, dtype, 18))
+
+
 def test_two_graphs_at_once():
     """Two captured graphs, each with scratch of its own, replayed on two streams at the same time."""
     sets = [make((1, 8, 2, 900, 900, 64), "all", torch.bfloat16, 40 + i) for i in range(2)]
