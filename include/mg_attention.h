@@ -9,6 +9,8 @@
  * prefix. The same rules hold: plain C, status codes (mg_last_error() has the
  * message), work enqueued on the caller's stream on the current device, scratch
  * from mg_set_allocator's allocator or the library's own stream-ordered pool.
+ * The library's first call on a device (of any function) sets the device up and
+ * cannot be captured into a graph; every later one can.
  */
 #ifndef MG_ATTENTION_H
 #define MG_ATTENTION_H

@@ -98,7 +98,7 @@ mg_status backward_simt(const mg::AttnParams& p, cudaStream_t st)
 bool tc_serves(const mg_attention_desc* d, const mg::AttnParams& p, std::initializer_list<const void*> rows_q,
                std::initializer_list<const void*> rows_k)
 {
-    if (d->head_dim % 8 || std::fabs(d->scale) < 1e-30f) return false;
+    if (d->head_dim % 8 || std::fabs(d->scale) < 1e-30f || !tame(d->scale, d->cap)) return false;
     const int vec = d->dtype == MG_BF16 ? 8 : 4;
     for (const void* x : rows_q)
         if (reinterpret_cast<uintptr_t>(x) % 16) return false;

@@ -52,6 +52,14 @@ inline mg_status check_scores(float scale, float cap, const char* who)
     return MG_OK;
 }
 
+// Whether scale / cap is in range for the kernels that multiply by it (the others
+// divide their scaled product by the cap).
+inline bool tame(float scale, float cap)
+{
+    const double pre = std::fabs((double)scale / cap);
+    return cap == 0.f || (pre > 1e-30 && pre < 1e30);
+}
+
 // Whether rows at `ptr` with these strides start on multiples of `vec` elements.
 inline bool aligned(const void* ptr, const int64_t* strides, int n, size_t elem, int vec)
 {

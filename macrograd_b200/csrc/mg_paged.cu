@@ -46,7 +46,7 @@ mg_status launch_paged(mg::PagedParams& p, int longest, const Device& dev, Scrat
                        const char* who)
 {
     const int vec = 16 / (int)sizeof(T);
-    bool stream = p.D % vec == 0 && aligned(p.k, p.ks, 3, sizeof(T), vec) && aligned(p.v, p.vs, 3, sizeof(T), vec);
+    bool stream = tame(p.scale, p.cap) && p.D % vec == 0 && aligned(p.k, p.ks, 3, sizeof(T), vec) && aligned(p.v, p.vs, 3, sizeof(T), vec);
     if (p.k_new) stream = stream && aligned(p.k_new, p.kns, 2, sizeof(T), vec) &&
                           aligned(p.v_new, p.vns, 2, sizeof(T), vec);
     const int group = p.H / p.Hkv, packs = ceil_div(group, stream ? mg::paged_pack<T>() : mg::kPagedHeads);

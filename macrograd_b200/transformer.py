@@ -20,7 +20,8 @@ any other strides, float32 or bfloat16, head_dim up to 128; outputs are laid out
 as the tensor they belong to (heads split from [batch, length, heads * head_dim]
 come back ready to be merged). Sums, softmax statistics and angles are kept in
 32 bits or more whatever the type. Calls run on `stream` (default: the current
-one) and are capturable; nothing is kept from one call for the next.
+one) and can be captured into graphs (but for the library's first call on a
+device); nothing is kept from one call for the next.
 """
 from __future__ import annotations
 
@@ -285,6 +286,9 @@ def _rotary(q, k, positions, frequencies, interleaved, inverse, magnitude, out_q
     for x, y, name in ((q, out_q, "out_q"), (k, out_k, "out_k")):
         if x is not None and y is not None and x.data_ptr() == y.data_ptr() and x.stride() != y.stride():
             _bad(f"{name} starts where its input does but has other strides")
+    for y, other, names in ((out_q, k, "out_q and k"), (out_k, q, "out_k and q"), (out_k, out_q, "out_k and out_q")):
+        if y is not None and other is not None and y.numel() and y.data_ptr() == other.data_ptr():
+            _bad(f"{names} are the same memory")
 
     def call(st):
         oq = torch.empty_like(q) if out_q is None else out_q

@@ -196,10 +196,13 @@ def test_a_scale_of_zero_and_far_caps(dtype):
     q, k, v, dout, kw = make((1, 2, 1, 150, 150, 64), "causal", dtype, 12)
     compare(q, k, v, dout, dict(kw, scale=0.0))
     compare(q, k, v, dout, dict(kw, cap=1e6))
-    out, lse = mg.attention(q, k, v, cap=1e-20, **kw)
     ref = Reference(q, k, v, scale=0.0, **kw)
-    within(out, ref.out, ref.out_tol, "out under a cap of nearly nothing")
-    assert torch.isfinite(lse).all()
+    for more in (dict(cap=1e-20), dict(cap=1e-30, scale=1e30)):
+        out, lse = mg.attention(q, k, v, **more, **kw)
+        within(out, ref.out, ref.out_tol, "out under a cap of nearly nothing")
+        assert torch.isfinite(lse).all()
+        one, _ = mg.attention(q[:, :, -1:], k, v, **more, **kw)
+        within(one, ref.out[:, :, -1:], ref.out_tol[:, :, -1:], "one query under it")
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])

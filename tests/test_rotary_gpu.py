@@ -143,6 +143,8 @@ def test_refusals():
             (lambda: mg.rotary(x, x.bfloat16(), pos, f), "as the others"),
             (lambda: mg.rotary(x, None, pos, f, out_k=x), "out_k without k"),
             (lambda: mg.rotary(x, None, pos, f, out_q=x[..., :4]), "out_q"),
+            (lambda: mg.rotary(x, x, pos, f, out_q=x, out_k=x), "same memory"),
+            (lambda: mg.rotary(x, x.clone(), pos, f, out_k=x), "same memory"),
             (lambda: mg.rotary(x, None, pos, f, magnitude=math.nan), "magnitude"),
             (lambda: mg.rotary_frequencies(7), "even"),
             (lambda: mg.rotary_frequencies(8, scaling="other"), "scaling"),
