@@ -127,14 +127,14 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_forward(const __grid_c
         }
     }
     if (q0 + r >= p.Lq) return;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l > 0.f ? 1.f / l : l;             // 0: no key; NaN stays
     T* op = (T*)p.out + b * p.os[0] + h * p.os[1] + (int64_t)(q0 + r) * p.os[2];
 #pragma unroll
     for (int i = 0; i < kSimtMaxD / 8; ++i) {
         const int d = c8 + 8 * i;
         if (d < p.D) op[d] = from_f32<T>(acc[i] * inv);
     }
-    if (c8 == 0) p.lse[((int64_t)b * p.H + h) * p.Lq + q0 + r] = l > 0.f ? m + logf(l) : -CUDART_INF_F;
+    if (c8 == 0) p.lse[((int64_t)b * p.H + h) * p.Lq + q0 + r] = l == 0.f ? -CUDART_INF_F : m + logf(l);
 }
 
 // delta[b][h][i] = sum_d dout * out: one warp per row; 0 for a row that saw nothing.

@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_simt_kernel(const __grid_
             for (int o = 16; o; o /= 2) s += __shfl_xor_sync(~0u, s, o);
             s = score(p.scale * s, p.cap, slope[g], len - 1 - j, bend);
             const float mn = fmaxf(m[g], s);
-            if (mn == -CUDART_INF_F) continue;
+            if (mn == -CUDART_INF_F && s == mn) continue;      // NaN is counted, and stays in l
             const float fix = expf(m[g] - mn), e = expf(s - mn);
             m[g] = mn;
             l[g] = l[g] * fix + e;

@@ -400,3 +400,28 @@ def test_refusals():
     for call, fragment in bad:
         with pytest.raises(mg.MacrogradError, match=fragment):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("size", [(1, 4, 2, 200, 200, 64), (1, 2, 1, 150, 150, 128), (1, 2, 1, 70, 70, 33),
+                                  (1, 2, 2, 3, 3000, 64), (1, 2, 1, 1, 2000, 128), (1, 2, 1, 1, 50, 33)], ids=str)
+@pytest.mark.parametrize("cap", [0.0, 10.0])
+@pytest.mark.parametrize("place", ["q", "k", "v", "dout"])
+def test_nan_that_is_seen_stays(place, cap, size, dtype):
+    """A NaN that a row sees reaches its results, and with them the gradients that the row has a part in."""
+    q, k, v, dout, _ = make(size, "causal", dtype, 3)
+    Lq, Lk = size[3], size[4]
+    row, key = Lq // 2, Lk // 3
+    {"q": q, "dout": dout}.get(place, k if place == "k" else v)[0, 0, row if place in ("q", "dout") else key, 5] = math.nan
+    out, lse = mg.attention(q, k, v, cap=cap)
+    pos = torch.arange(Lq, device="cuda") + Lk - Lq
+    hit = (torch.arange(Lq, device="cuda") == row) if place in ("q", "dout") else pos >= key      # rows it reaches
+    if place != "dout":
+        assert torch.isnan(out[0, 0, hit]).any(-1).all(), "out"
+        assert bool(torch.isnan(lse[0, 0, hit]).all()) == (place != "v"), "lse"
+    dq, dk, dv = mg.attention_backward(dout, q, k, v, out, lse, cap=cap)
+    assert torch.isnan(dq[0, 0, hit]).any(-1).all(), "dq"
+    seen = torch.arange(Lk, device="cuda") <= pos[hit].max()
+    assert torch.isnan(dk[0, 0, seen]).any(-1).all(), "dk"
+    if place != "v":
+        assert torch.isnan(dv[0, 0, seen]).any(-1).all(), "dv"

@@ -251,3 +251,23 @@ def test_refusals():
             (lambda: mg.paged_attention(q, kp, vp, table, lengths, slopes=torch.zeros(3, device="cuda")), "slopes")]:
         with pytest.raises(mg.MacrogradError, match=fragment):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 33])
+@pytest.mark.parametrize("cap", [0.0, 10.0])
+@pytest.mark.parametrize("place", ["q", "k", "v", "new"])
+def test_nan_that_is_seen_stays(place, cap, D, dtype):
+    q, kp, vp, table, lengths, kn, vn = make(3, 4, 2, D, 16, [1, 40, 2500], dtype)
+    for b, n in enumerate(lengths.tolist()):
+        if place == "q":
+            q[b, 0, 5] = float("nan")
+        elif place == "new":
+            kn[b, 0, 5] = float("nan")
+        elif n > 1:
+            (kp if place == "k" else vp)[int(table[b, n // 3 // 16]), n // 3 % 16, 0, 5] = float("nan")
+    out, lse = mg.paged_attention(q, kp, vp, table, lengths, k_new=kn, v_new=vn, cap=cap)
+    hit = lengths > (1 if place in ("k", "v") else 0)
+    assert torch.isnan(out[hit, 0]).any(-1).all()
+    assert bool(torch.isnan(lse[hit, 0]).all()) == (place != "v")
+    assert torch.isfinite(out[:, 2:]).all()          # heads of the other key-value head
