@@ -465,6 +465,7 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
         if (ok) {
             tc_fence_after();
             l = st.top[n & 1][0][r] + st.top[n & 1][1][r];
+            if ((l == 0.f && m != -CUDART_INF_F) || l == CUDART_INF_F) l = CUDART_NAN_F;   // scores too large to resolve
             const float inv = l > 0.f ? 1.f / l : l;       // 0: no key; NaN stays
             const bool store = row < p.Lq;
             __nv_bfloat16* out = (__nv_bfloat16*)p.out + b * p.os[0] + h * p.os[1] + (int64_t)row * p.os[2];

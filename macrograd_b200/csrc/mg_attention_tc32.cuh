@@ -309,8 +309,7 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
             }
             float top;               // the tile's maximum, above the one in use
             uint64_t sum;
-            bool again = __any_sync(~0u, m == -CUDART_INF_F);
-            if (again) {             // no maximum to go by yet
+            if (__any_sync(~0u, m == -CUDART_INF_F)) {       // no maximum to go by yet
                 top = -CUDART_INF_F;
 #pragma unroll
                 for (int c0 = 0; c0 < 64; c0 += 16) {
@@ -320,7 +319,9 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
                 }
                 m = m == -CUDART_INF_F ? top : m;
             }
-            do {
+            // A pass more suffices for a row far above its maximum in use. With powers beyond 2^29 what
+            // rounding leaves of the maximum may itself be above it, whatever is added: hence the limit.
+            for (int pass = 0;; ++pass) {
                 const float base = m == -CUDART_INF_F ? 0.f : m;
                 uint64_t part[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
                 top = -CUDART_INF_F;
@@ -343,17 +344,17 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
                     for (int k = 0; k < 3; ++k) tmem_st_x8(tP + 32 * k + c0 / 2, w[k]);
                 }
                 sum = add2(part[0], part[1]);
-                // far above the maximum in use (or the first keys that the row sees): again with its own
-                const bool high = top > (m == -CUDART_INF_F ? -CUDART_INF_F : 40.f);
-                again = __any_sync(~0u, high);
-                if (again && high) {
-                    const float g = m == -CUDART_INF_F ? 0.f : ex2(-top);
+                // far above the maximum in use: again with its own
+                const bool high = top > 40.f;
+                if (pass == 2 || !__any_sync(~0u, high)) break;
+                if (high) {
+                    const float g = ex2(-top);
                     l *= g;
 #pragma unroll
                     for (int c = 0; c < DP; ++c) o[c] *= g;
                     m = base + top;
                 }
-            } while (again);
+            }
             {
                 float x, y;
                 unpack2(sum, x, y);
@@ -372,6 +373,7 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
         if (ok && n > 0) ok = __all_sync(~0u, tc_wait(smem_u32(&st.o_full), (n - 1) & 1, failed));
         if (ok) {
             tc_fence_after();
+            if ((l == 0.f && m != -CUDART_INF_F) || l == CUDART_INF_F) l = CUDART_NAN_F;   // scores too large to resolve
             const float g = f * (l > 0.f ? 1.f / l : l);   // 0: no key; NaN stays
             float* out = tp.rows.parts > 1 ? tp.rows.out + (((int64_t)part * p.B * p.H + bh) * p.Lq + row) * p.D
                                            : (float*)p.out + b * p.os[0] + h * p.os[1] + (int64_t)row * p.os[2];
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
 #pragma unroll
                 for (int c = 0; c < 32; c += 4)
                     if (c0 + c < p.D) {
-                                                *reinterpret_cast<float4*>(out + c0 + c) =
+                        *reinterpret_cast<float4*>(out + c0 + c) =
                             make_float4((o[c0 + c] + x[c]) * g, (o[c0 + c + 1] + x[c + 1]) * g,
                                         (o[c0 + c + 2] + x[c + 2]) * g, (o[c0 + c + 3] + x[c + 3]) * g);
                     }

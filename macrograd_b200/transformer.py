@@ -176,8 +176,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     A query sees the keys up to its own position (causal) and, besides, the first prefix[b] keys of its row (int32
     [B]); with documents (int32 [B, Lk], the id of each position) only keys of its own document. Ids below 0 mark
     padding: such keys and queries are left out whatever they hold. A query that sees no key gives out = 0,
-    lse = -inf. Everywhere else k, v must be finite also where a mask hides them from some queries. `out` must not
-    share memory with k or v.
+    lse = -inf. Everywhere else k, v must be finite also where a mask hides them from some queries. Scores and
+    biases are resolved up to 2^28 in size; a row with larger ones may come out as NaN. `out` must not share memory with
+    k or v.
 
     Returns (out, laid out as q, lse [B, H, Lq] in float32)."""
     lib = _lib.load()

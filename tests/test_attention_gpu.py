@@ -425,3 +425,31 @@ def test_nan_that_is_seen_stays(place, cap, size, dtype):
     assert torch.isnan(dk[0, 0, seen]).any(-1).all(), "dk"
     if place != "v":
         assert torch.isnan(dv[0, 0, seen]).any(-1).all(), "dv"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 33])
+@pytest.mark.parametrize("power", [20, 26, 40, 100])
+def test_large_scores(power, D, dtype):
+    """Scores of 2^power: the largest takes its row; rows of equal scores take the mean. Beyond 2^28 rows may be NaN."""
+    L, best = 300, 170
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k = (torch.zeros((1, 1, L, D), device="cuda", dtype=dtype) for _ in range(2))
+    v = torch.randn((1, 1, L, D), generator=g, device="cuda").to(dtype)
+    q[..., 0] = 2.0 ** (power // 2)
+    k[..., 0] = 2.0 ** (power // 2 - 1)
+    k[:, :, best, 0] *= 2
+    out, lse = mg.attention(q, k, v, scale=1.0)
+    want = v.double().cumsum(2) / torch.arange(1, L + 1, device="cuda")[:, None]
+    want[:, :, best:] = v[:, :, best].double()
+    # a sum of up to L products whose weights are rounded, then a rounding
+    u = torch.finfo(dtype).eps / 2
+    tol = (2 * u + 8 * 2.0 ** -24 * L ** 0.5) * v.double().abs().cummax(2).values
+    tol[:, :, best:] = tol.max()
+    nan = torch.isnan(out)
+    assert power > 28 or not nan.any()
+    assert ((out.double() - want).abs() <= tol)[~nan].all()
+    mg.attention(q, k, v, scale=1.0, slopes=torch.tensor([3.0e12], device="cuda"))     # ends
+    mg.attention(q, k, v, scale=1.0, causal=False, slopes=torch.tensor([1.0e30], device="cuda"))
+    torch.cuda.synchronize()
+    assert mg.load().mg_device_status(None, 0) == 0
