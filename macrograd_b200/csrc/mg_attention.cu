@@ -366,6 +366,9 @@ mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, 
 {
     Range range("mg_attention_backward");
     MG_TRY(check_attention(d, "mg_attention_backward"));
+    // the row statistics are numbered in 32 bits, four rows of a head (padded to 128) at a time
+    if ((int64_t)d->batch * d->heads * ceil_div(d->q_len, 128) >= (1ll << 27))
+        return fail(MG_ERR_UNSUPPORTED, "mg_attention_backward: batch * heads * rows is too large");
     if (d->batch == 0 || (d->q_len == 0 && d->k_len == 0)) return MG_OK;
     if ((d->q_len > 0 && (!dq || !dout || !q || !out || !lse)) || (d->k_len > 0 && (!dk || !dv || !k || !v)))
         return fail(MG_ERR_INVALID, "mg_attention_backward: a tensor is NULL");

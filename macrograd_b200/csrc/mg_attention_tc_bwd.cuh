@@ -79,7 +79,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) attn_tc_stats_kernel(const __grid_constant__ AttnParams p, int Lp,
                                                             float* __restrict__ lse2, float* __restrict__ delta)
 {
-    const uint32_t group = (blockIdx.x * blockDim.x + threadIdx.x) / 16, per = (uint32_t)Lp / kStatsRows;
+    const uint32_t group = blockIdx.x * (blockDim.x / 16) + threadIdx.x / 16, per = (uint32_t)Lp / kStatsRows;
     if (group >= (uint32_t)p.B * p.H * per) return;     // an even number of groups: whole warps
     const int part = threadIdx.x % 16;
     // heads first: their rows lie side by side where heads were split from [batch, length, heads * D]

@@ -129,3 +129,10 @@ def test_python_refuses_cpu_tensors():
         mg.rotary(x, None, torch.zeros(4, dtype=torch.int32), mg.rotary_frequencies(8, device="cpu"))
     with pytest.raises(mg.MacrogradError, match="CUDA tensor"):
         mg.paged_attention(x[0], x, x, x, x)
+
+
+def test_backward_refuses_more_rows_than_its_statistics_number(lib):
+    d = attention(B=1 << 26, H=2, Lq=2, Lk=2)
+    assert lib.mg_attention_backward(d, *([None] * 10)) == UNSUPPORTED
+    assert "too large" in lib.mg_last_error().decode()
+    assert lib.mg_attention(d, None, None, None, None, None, None) == INVALID     # the forward pass has none
