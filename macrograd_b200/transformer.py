@@ -185,6 +185,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     dev, lead, ptrs = _attention_args(q, k, v, scale, causal, cap, slopes, documents, prefix)
     if out is not None:
         _written(out, "out", q)
+        for t, name in ((k, "k"), (v, "v")):
+            if out.numel() and t.numel() and out.data_ptr() == t.data_ptr():
+                _bad(f"out and {name} are the same memory")
 
     def call(st):
         o = torch.empty_like(q) if out is None else out
@@ -338,9 +341,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     as [pages, Hkv, page_size, D] is passed transposed); block_table int32 [B, width]: the pages of each request in
     order; lengths int32 [B]: its keys, the new token among them. The query stands at position lengths[b] - 1.
     With k_new and v_new [B, Hkv, D] the token's own key and value come from there, and the call also writes them to
-    the cache at that position; requests must not share the page they append to. A length of 0 gives out = 0,
-    lse = -inf and writes nothing. A length beyond the table is cut off there, a page outside the pool is skipped, and
-    mg_device_status() then reports MG_ERR_INVALID.
+    the cache at that position; requests must not share the page they append to, nor keys and values theirs. A length
+    of 0 gives out = 0, lse = -inf and writes nothing. A length beyond the table is cut off there, a page outside the
+    pool is skipped, and mg_device_status() then reports MG_ERR_INVALID.
 
     Returns (out [B, H, D], lse [B, H] in float32)."""
     lib = _lib.load()
@@ -376,6 +379,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if k_new is not None:
         _written(k_pages, "k_pages", k_pages)
         _written(v_pages, "v_pages", v_pages)
+        if k_pages.numel() and k_pages.data_ptr() == v_pages.data_ptr():
+            _bad("k_pages and v_pages are the same memory: nothing can be appended to them")
     if out is not None:
         _written(out, "out", q)
 

@@ -453,3 +453,10 @@ def test_large_scores(power, D, dtype):
     mg.attention(q, k, v, scale=1.0, causal=False, slopes=torch.tensor([1.0e30], device="cuda"))
     torch.cuda.synchronize()
     assert mg.load().mg_device_status(None, 0) == 0
+
+
+def test_out_in_the_place_of_keys_or_values_is_refused():
+    q, k, v = (torch.randn((1, 2, 8, 64), device="cuda") for _ in range(3))
+    for t in (k, v):
+        with pytest.raises(mg.MacrogradError, match="same memory"):
+            mg.attention(q, k, v, out=t)

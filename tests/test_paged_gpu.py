@@ -271,3 +271,10 @@ def test_nan_that_is_seen_stays(place, cap, D, dtype):
     assert torch.isnan(out[hit, 0]).any(-1).all()
     assert bool(torch.isnan(lse[hit, 0]).all()) == (place != "v")
     assert torch.isfinite(out[:, 2:]).all()          # heads of the other key-value head
+
+
+def test_appending_to_one_pool_of_keys_and_values_is_refused():
+    q, kp, vp, table, lengths, kn, vn = make(2, 4, 2, 64, 16, [100, 33], torch.bfloat16)
+    with pytest.raises(mg.MacrogradError, match="same memory"):
+        mg.paged_attention(q, kp, kp, table, lengths, k_new=kn, v_new=vn)
+    compare((q, kp, kp, table, lengths, None, None))      # read alone
