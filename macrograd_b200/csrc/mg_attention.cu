@@ -204,6 +204,59 @@ mg_status forward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     return join_rows<__nv_bfloat16>(t.rows, p, st);
 }
 
+// Parts of a gradient's sum: where blocks (of 128 rows of a head, `steps` streamed tiles of
+// `tile` rows each) would leave SMs empty, as many as fill them, joined in their order. No
+// less than 256 rows to a part, 128 in fp32, whose rows take longer: measured with 256 / 128,
+// fp32 4 heads of 64, 500 rows 54 / 42 us, bf16 16 heads over 1 of 128, 300 rows 55 / 58 us. Whole sums
+// took 99 and 105 us; bf16 8 heads over 2 of 128, 2048 rows 178 -> 99 us, fp32 1024 rows 940 -> 213 us. (The
+// share's arithmetic costs the fp32 kernel 2 % where every SM has its block: 219 -> 223 us.)
+mg_status share_gradient(mg::GradParts* g, int64_t blocks, int64_t steps, int tile, int least, int64_t rows, int D,
+                         bool second, bool sums, const Device& dev, Scratch& ws)
+{
+    *g = {};
+    g->parts = (int)std::max<int64_t>(1, std::min<int64_t>(dev.sm_count / blocks, ceil_div(steps * tile, least)));
+    if (g->parts == 1) return MG_OK;
+    const int64_t each = g->parts * rows * D, all = each * (second ? 2 : 1) + (sums ? g->parts * rows : 0);
+    g->acc = static_cast<float*>(ws.get(all * sizeof(float)));
+    if (!g->acc) return fail(MG_ERR_ALLOC, "mg_attention_backward: no scratch for %d parts of each sum", g->parts);
+    if (second) g->other = g->acc + each;
+    if (sums) g->r = g->acc + 2 * each;
+    return MG_OK;
+}
+
+// dQ's, and dK's and dV's.
+mg_status share_dq(mg::GradParts* g, const mg::AttnParams& p, int tile, int least, bool correct, const Device& dev,
+                   Scratch& ws)
+{
+    return share_gradient(g, (int64_t)ceil_div(p.Lq, 128) * p.B * p.H, ceil_div(p.Lk, tile), tile, least,
+                          (int64_t)p.B * p.H * p.Lq, p.D, correct, correct, dev, ws);
+}
+mg_status share_dkv(mg::GradParts* g, const mg::AttnParams& p, int tile, int least, const Device& dev, Scratch& ws)
+{
+    return share_gradient(g, (int64_t)ceil_div(p.Lk, 128) * p.B * p.Hkv, (int64_t)(p.H / p.Hkv) * ceil_div(p.Lq, tile),
+                          tile, least, (int64_t)p.B * p.Hkv * p.Lk, p.D, true, false, dev, ws);
+}
+
+template <typename T, bool kCorrect>
+mg_status join_dq(const mg::GradParts& g, const mg::AttnParams& p, float* delta, int Lp, cudaStream_t st)
+{
+    if (g.parts == 1) return MG_OK;
+    mg::GradJoin j = {g, p.H, p.Lq, p.D, Lp, (int64_t)p.B * p.H * p.Lq, {p.dq, nullptr}, {}, delta};
+    std::copy(p.dqs, p.dqs + 3, j.os[0]);
+    mg::attn_grad_join_kernel<T, kCorrect><<<ceil_div(j.rows, 8), 256, 0, st>>>(j);
+    return launched("mg_attention_backward");
+}
+template <typename T>
+mg_status join_dkv(const mg::GradParts& g, const mg::AttnParams& p, cudaStream_t st)
+{
+    if (g.parts == 1) return MG_OK;
+    mg::GradJoin j = {g, p.Hkv, p.Lk, p.D, 0, (int64_t)p.B * p.Hkv * p.Lk, {p.dk, p.dv}, {}, nullptr};
+    std::copy(p.dks, p.dks + 3, j.os[0]);
+    std::copy(p.dvs, p.dvs + 3, j.os[1]);
+    mg::attn_grad_join_kernel<T, false><<<dim3(ceil_div(j.rows, 8), 2), 256, 0, st>>>(j);
+    return launched("mg_attention_backward");
+}
+
 template <int DP, bool kKeys, bool kCap, bool kBias>
 mg_status launch_tc_backward(const mg::TcBwdParams& t, const Device& dev, cudaStream_t st)
 {
@@ -211,7 +264,7 @@ mg_status launch_tc_backward(const mg::TcBwdParams& t, const Device& dev, cudaSt
     constexpr size_t smem = mg::tc_backward_smem<DP>();
     MG_TRY(allow_smem<kernel>(dev, smem));
     const int blocks = kKeys ? ceil_div(t.a.Lk, 128) * t.a.B * t.a.Hkv : ceil_div(t.a.Lq, 128) * t.a.B * t.a.H;
-    kernel<<<blocks, mg::kTcBwdThreads, smem, st>>>(t);
+    kernel<<<blocks * t.parts.parts, mg::kTcBwdThreads, smem, st>>>(t);
     return launched("mg_attention_backward");
 }
 
@@ -249,13 +302,17 @@ mg_status backward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     MG_TRY(tc_map(&t.x1, &hs[3], &bs[3], p.dout, p.dos, p.D, p.Lq, p.H, p.B, 128));
     MG_TRY(tc_map(&t.y0, &hs[1], &bs[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 64));
     MG_TRY(tc_map(&t.y1, &hs[2], &bs[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 64));
+    MG_TRY(share_dq(&t.parts, p, 64, 256, true, dev, ws));
     MG_TRY((p.D <= 64 ? launch_tc_backward<64, false>(t, dev, st) : launch_tc_backward<128, false>(t, dev, st)));
+    MG_TRY((join_dq<__nv_bfloat16, true>(t.parts, p, t.delta, t.Lp, st)));
     // the keys resident: dK, dV
     MG_TRY(tc_map(&t.x0, &hs[1], &bs[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 128));
     MG_TRY(tc_map(&t.x1, &hs[2], &bs[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 128));
     MG_TRY(tc_map(&t.y0, &hs[0], &bs[0], p.q, p.qs, p.D, p.Lq, p.H, p.B, 64));
     MG_TRY(tc_map(&t.y1, &hs[3], &bs[3], p.dout, p.dos, p.D, p.Lq, p.H, p.B, 64));
-    return p.D <= 64 ? launch_tc_backward<64, true>(t, dev, st) : launch_tc_backward<128, true>(t, dev, st);
+    MG_TRY(share_dkv(&t.parts, p, 64, 256, dev, ws));
+    MG_TRY((p.D <= 64 ? launch_tc_backward<64, true>(t, dev, st) : launch_tc_backward<128, true>(t, dev, st)));
+    return join_dkv<__nv_bfloat16>(t.parts, p, st);
 }
 
 template <int DP, bool kCap, bool kBias>
@@ -294,7 +351,7 @@ mg_status launch_tc32_backward(const mg::Tc32BwdParams& t, const Device& dev, cu
     constexpr auto kernel = mg::attn_tc32_backward<DP, kKeys, kTake, kCap, kBias>;
     MG_TRY(allow_smem<kernel>(dev, mg::kTc32BwdSmem));
     const int blocks = kKeys ? ceil_div(t.a.Lk, 128) * t.a.B * t.a.Hkv : ceil_div(t.a.Lq, 128) * t.a.B * t.a.H;
-    kernel<<<blocks, mg::kTc32BwdThreads, mg::kTc32BwdSmem, st>>>(t);
+    kernel<<<blocks * t.parts.parts, mg::kTc32BwdThreads, mg::kTc32BwdSmem, st>>>(t);
     return launched("mg_attention_backward");
 }
 
@@ -323,13 +380,19 @@ mg_status backward_tc32(const mg::AttnParams& p, const Device& dev, void* stream
     MG_TRY(launched(who));
     mg::Tc32BwdParams t = {p, f.doc_tiles, stats, stats + rows, Lp, 0, f.scale, f.status};
     t.idesc_s = mg::idesc_bf16(128, p.D <= 64 ? 64 : 32, false, false, p.scale < 0.f);
+    const int tile = p.D <= 64 ? 64 : 32;
+    MG_TRY(share_dkv(&t.parts, p, tile, 128, dev, ws));
     if (p.D <= 64) {
         MG_TRY((launch_tc32_backward<64, true, mg::kTakeBoth>(t, dev, st)));
-        return launch_tc32_backward<64, false, mg::kTakeDs>(t, dev, st);
+    } else {
+        MG_TRY((launch_tc32_backward<128, true, mg::kTakeDs>(t, dev, st)));
+        MG_TRY((launch_tc32_backward<128, true, mg::kTakeP>(t, dev, st)));
     }
-    MG_TRY((launch_tc32_backward<128, true, mg::kTakeDs>(t, dev, st)));
-    MG_TRY((launch_tc32_backward<128, true, mg::kTakeP>(t, dev, st)));
-    return launch_tc32_backward<128, false, mg::kTakeDs>(t, dev, st);
+    MG_TRY(join_dkv<float>(t.parts, p, st));
+    MG_TRY(share_dq(&t.parts, p, tile, 128, false, dev, ws));
+    MG_TRY((p.D <= 64 ? launch_tc32_backward<64, false, mg::kTakeDs>(t, dev, st)
+                      : launch_tc32_backward<128, false, mg::kTakeDs>(t, dev, st)));
+    return join_dq<float, false>(t.parts, p, nullptr, 0, st);
 }
 
 }  // namespace

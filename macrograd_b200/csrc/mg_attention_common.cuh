@@ -32,6 +32,14 @@ struct RowParts {
     float* lse;          // [parts][B * H][Lq]
 };
 
+// A gradient's sum over the streamed rows, shared by several blocks.
+struct GradParts {
+    int parts;           // 1: the block writes the gradient itself
+    float* acc;          // [parts][B * heads][rows][D] of dQ, or of dK
+    float* other;        // as acc: of the correction's product (dQ of 16-bit tensors), or of dV
+    float* r;            // [parts][B * H][Lq] the rows' sums (dQ of 16-bit tensors)
+};
+
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <typename T>

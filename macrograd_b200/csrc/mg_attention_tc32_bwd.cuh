@@ -29,6 +29,7 @@ struct Tc32BwdParams {
     uint32_t idesc_s;
     float scale;                 // |scale|
     int* status;
+    GradParts parts;
 };
 
 // What a launch accumulates: dS Y0 (dQ or dK), P Y1 (dV), or both.
@@ -63,7 +64,8 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;   // uniform: so are the roles
 
     const int nhead = kKeys ? p.Hkv : p.H, xrows = kKeys ? p.Lk : p.Lq, yrows = kKeys ? p.Lq : p.Lk;
-    const int xtiles = (xrows + 127) / 128, bh = blockIdx.x % (p.B * nhead), rank = blockIdx.x / (p.B * nhead);
+    const int xtiles = (xrows + 127) / 128, part = blockIdx.x % tp.parts.parts, block = blockIdx.x / tp.parts.parts;
+    const int bh = block % (p.B * nhead), rank = block / (p.B * nhead);
     const int x0 = (kKeys ? rank : xtiles - 1 - rank) * 128;
     const int xh = bh % nhead, b = bh / nhead, group = p.H / p.Hkv;
     const int shift = p.Lk - p.Lq;
@@ -93,10 +95,13 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
     int t0, t1;
     stream_range<kKeys>(p, docs, dt, prefix, x0, xpos, shift, t0, t1);
     t0 *= 64 / kN, t1 *= 64 / kN;
+    int i0, n;                                       // the block's share of the steps
+    const int tiles = max(0, t1 - t0);
+    share_of_steps(part, tp.parts.parts, kKeys ? tiles * group : tiles, i0, n);
+    if (!kKeys) t0 += i0;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const int tiles = max(0, t1 - t0), n = kKeys ? tiles * group : tiles;
     // columns: X0's pieces, S, dP, the pieces of P and of dS, the accumulators
     const uint32_t tX = st.tmem, tS = tX + (kXt ? 192 : 0), tdP = tS + kN, tP = tdP + kN;
     const uint32_t tdS = tP + (kXt ? 0 : 96), tA = st.tmem + (kXt ? 384 : 320), tB = tA + (kXt ? 0 : 64);
@@ -116,7 +121,8 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
         const int64_t step0 = s0[2], step1 = s1[2];
         bool ok = true;
         for (int i = 0; i < n && ok; ++i) {
-            const int yh = kKeys ? xh * group + i / tiles : xh / group, y0 = (t0 + (kKeys ? i % tiles : i)) * kN;
+            const int yh = kKeys ? xh * group + (i0 + i) / tiles : xh / group;
+            const int y0 = (t0 + (kKeys ? (i0 + i) % tiles : i)) * kN;
             const float* a0 = src0 + yh * s0[1] + (y0 + r0) * step0;
             const float* a1 = src1 + yh * s1[1] + (y0 + r0) * step1;
             float4 x[kItems][2], y[kItems][2];
@@ -298,10 +304,10 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
             }
         };
         // this lane's document of a tile's streamed rows, a tile ahead
-        const auto y_of = [&](int i) { return (t0 + (kKeys ? i % tiles : i)) * kN; };
+        const auto y_of = [&](int i) { return (t0 + (kKeys ? (i0 + i) % tiles : i)) * kN; };
         int ydoc[1] = {docs && n > 0 ? doc_at(p, b, y_of(0) + (kKeys ? shift : 0) + col + lane) : -1};
         for (int i = 0; i < n; ++i) {
-            const int h = kKeys ? xh * group + i / tiles : xh;
+            const int h = kKeys ? xh * group + (i0 + i) / tiles : xh;
             const int y0 = y_of(i), ypos = y0 + (kKeys ? shift : 0);
             const float slope = kBias ? __ldg(p.slopes + h) * kLog2e : 0.f;
             bool full;
@@ -424,8 +430,11 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
         }
         if (ok && x0 + r < xrows) {
             const int64_t* os = kKeys ? (is_dv ? p.dvs : p.dks) : p.dqs;
-            float* out = (float*)(kKeys ? (is_dv ? p.dv : p.dk) : p.dq) + b * os[0] + xh * os[1] +
-                         (int64_t)(x0 + r) * os[2] + ocol;
+            float* out = tp.parts.parts == 1
+                             ? (float*)(kKeys ? (is_dv ? p.dv : p.dk) : p.dq) + b * os[0] + xh * os[1] + (int64_t)(x0 + r) * os[2]
+                             : (is_dv ? tp.parts.other : tp.parts.acc) +
+                                   ((((int64_t)blockIdx.x % tp.parts.parts) * p.B + b) * nhead + xh) * xrows * p.D + (int64_t)(x0 + r) * p.D;
+            out += ocol;
             const float f = is_dv ? 1.f : p.scale;
             const int cols = p.D - ocol;
 #pragma unroll

@@ -11,6 +11,8 @@
 // dV, summed over the query heads that share the key-value head. So no gradient
 // is added to by two blocks: no atomics, and the same bits every time, for 8
 // products instead of the 5 of a single kernel that would add dQ up atomically.
+// Where there are fewer blocks than SMs, several share the streamed tiles of the same
+// resident rows; each leaves its part in scratch, and attn_grad_join_kernel adds them up.
 //
 // delta = rowsum(dout * out) carries the 16-bit rounding of out, which dS = P * (dP -
 // delta) magnifies where a row's weight lies on few keys (errors of dQ and dK of 0.4 %
@@ -53,6 +55,7 @@ struct TcBwdParams {
     float scale;                         // |scale|
     CapCurve curve;
     int* status;
+    GradParts parts;
 };
 
 // lse2 and delta of each row, padded with rows whose P is 0. 16 lanes to a row of
@@ -154,6 +157,58 @@ __device__ __forceinline__ void stream_range(const AttnParams& p, const int32_t*
     if (docs) narrow_to_docs(dt, p.Lk, kKeys ? shift : 0, 64, docs_of(dt, xpos, 128, p.Lk), t0, t1);
 }
 
+// Steps [i0, i0 + n) of `all`: part of `parts`.
+__device__ __forceinline__ void share_of_steps(int part, int parts, int all, int& i0, int& n)
+{
+    const int each = (all + parts - 1) / parts;
+    i0 = min(all, part * each);
+    n = min(all, i0 + each) - i0;
+}
+
+// Adds up the parts of a gradient in their order (blockIdx.y: acc, other). kCorrect: dQ of
+// 16-bit tensors, less the rows' sums r times the other product, and delta made exact.
+// One warp to a row, four elements to a lane.
+struct GradJoin {
+    GradParts parts;
+    int heads, L, D, Lp;
+    int64_t rows;                        // B * heads * L
+    void* out[2];
+    int64_t os[2][3];
+    float* delta;
+};
+
+template <typename T, bool kCorrect>
+__global__ void __launch_bounds__(256) attn_grad_join_kernel(const __grid_constant__ GradJoin j)
+{
+    const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
+    if (row >= j.rows) return;
+    const int d = threadIdx.x % 32 * 4;
+    const bool in = d < j.D;
+    const auto sum_of = [&](const float* src) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (in)
+            for (int s = 0; s < j.parts.parts; ++s) {
+                const float4 x = __ldg(reinterpret_cast<const float4*>(src + (s * j.rows + row) * j.D + d));
+                a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+            }
+        return a;
+    };
+    const int64_t bh = row / j.L;
+    const int i = (int)(row - bh * j.L), h = (int)(bh % j.heads), b = (int)(bh / j.heads);
+    float4 a = sum_of(blockIdx.y ? j.parts.other : j.parts.acc);
+    if (kCorrect) {
+        float r = 0.f;
+        for (int s = 0; s < j.parts.parts; ++s) r += __ldg(j.parts.r + s * j.rows + row);
+        const float4 w = sum_of(j.parts.other);
+        a.x = fmaf(-r, w.x, a.x), a.y = fmaf(-r, w.y, a.y), a.z = fmaf(-r, w.z, a.z), a.w = fmaf(-r, w.w, a.w);
+        if (d == 0) j.delta[bh * j.Lp + i] += r;
+    }
+    if (!in) return;
+    const int64_t* os = j.os[blockIdx.y];
+    T* out = (T*)j.out[blockIdx.y] + b * os[0] + h * os[1] + i * os[2] + d;
+    out[0] = from_f32<T>(a.x), out[1] = from_f32<T>(a.y), out[2] = from_f32<T>(a.z), out[3] = from_f32<T>(a.w);
+}
+
 template <int DP>
 constexpr size_t tc_backward_smem() { return (2 * 128 + kTcBwdStages * 2 * 64) * DP * 2 + 1024; }
 
@@ -170,7 +225,8 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
 
     // blocks with the most tiles first: the first keys, the last queries
     const int nhead = kKeys ? p.Hkv : p.H, xrows = kKeys ? p.Lk : p.Lq;
-    const int xtiles = (xrows + 127) / 128, bh = blockIdx.x % (p.B * nhead), rank = blockIdx.x / (p.B * nhead);
+    const int xtiles = (xrows + 127) / 128, part = blockIdx.x % tp.parts.parts, block = blockIdx.x / tp.parts.parts;
+    const int bh = block % (p.B * nhead), rank = block / (p.B * nhead);
     const int x0 = (kKeys ? rank : xtiles - 1 - rank) * 128;
     const int xh = bh % nhead, b = bh / nhead, group = p.H / p.Hkv;
     const int shift = p.Lk - p.Lq;
@@ -207,7 +263,10 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const int tiles = max(0, t1 - t0), n = kKeys ? tiles * group : tiles;
+    int i0, n;                                           // the block's share of the steps
+    const int tiles = max(0, t1 - t0);
+    share_of_steps(part, tp.parts.parts, kKeys ? tiles * group : tiles, i0, n);
+    if (!kKeys) t0 += i0;
     const uint32_t tA = st.tmem + 256, tB = tA + DP;     // accumulators: dS Y0, P Y1 (the queries resident: P curve Y0)
     volatile int* failed = &st.failed;
     // columns of step i's S and dP; the 16-bit P and dS of columns [32 h, 32 h + 32) lie in the first 16 of these
@@ -227,7 +286,8 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             for (int i = 0; i < n; ++i) {
                 const int s = i % kTcBwdStages;
                 if (i >= kTcBwdStages && !tc_wait(smem_u32(&st.y_empty[s]), (i / kTcBwdStages - 1) & 1, failed)) break;
-                const int yh = kKeys ? xh * group + i / tiles : xh / group, y0 = (t0 + (kKeys ? i % tiles : i)) * 64;
+                const int yh = kKeys ? xh * group + (i0 + i) / tiles : xh / group;
+                const int y0 = (t0 + (kKeys ? (i0 + i) % tiles : i)) * 64;
                 const uint32_t yb = smem_u32(&st.y_full[s]);
                 mbar_arrive_expect_tx(yb, 2 * kY + (kKeys ? 512u : 0u));
                 for (int c = 0; c < DP; c += 64) {
@@ -253,7 +313,7 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             ok = __all_sync(~0u, ok && tc_wait(smem_u32(&st.y_full[s]), (i / kTcBwdStages) & 1, failed));
             if (!ok) return;
             if (docs) {
-                const int y0 = (t0 + (kKeys ? i % tiles : i)) * 64, pos = y0 + (kKeys ? shift : 0);
+                const int y0 = (t0 + (kKeys ? (i0 + i) % tiles : i)) * 64, pos = y0 + (kKeys ? shift : 0);
                 bool pad = pos < 0 || pos + 64 > p.Lk;
                 if (!pad) pad = __ldg(dt + (pos >> 7)).x < 0 || __ldg(dt + ((pos + 63) >> 7)).x < 0;
                 if (pad) {
@@ -323,10 +383,10 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
         uint64_t rsum2 = pack2(0.f, 0.f);   // this thread's part of its row's sum of P * (dP - delta)
         bool ok = true;
         // this lane's document of a tile's streamed rows, a tile of the set ahead
-        const auto y_of = [&](int i) { return (t0 + (kKeys ? i % tiles : i)) * 64; };
+        const auto y_of = [&](int i) { return (t0 + (kKeys ? (i0 + i) % tiles : i)) * 64; };
         int ydoc[1] = {docs && set < n ? doc_at(p, b, y_of(set) + (kKeys ? shift : 0) + col + lane) : -1};
         for (int i = set; i < n; i += 2) {
-            const int h = kKeys ? xh * group + i / tiles : xh;
+            const int h = kKeys ? xh * group + (i0 + i) / tiles : xh;
             const int y0 = y_of(i), ypos = y0 + (kKeys ? shift : 0);
             const int s = i % kTcBwdStages;
             const float slope = kBias ? __ldg(p.slopes + h) * kLog2e : 0.f;
@@ -472,7 +532,10 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
             tc_fence_after();
             if (!kKeys) {
                 rsum = (st.sums[0][r] + st.sums[1][r]) + (st.sums[2][r] + st.sums[3][r]);
-                if (warp < 4 && x0 + r < xrows) tp.delta[((int64_t)b * p.H + xh) * tp.Lp + x0 + r] = delta + rsum;
+                if (warp < 4 && x0 + r < xrows) {
+                    if (tp.parts.parts == 1) tp.delta[(int64_t)bh * tp.Lp + x0 + r] = delta + rsum;
+                    else tp.parts.r[((int64_t)part * p.B * p.H + bh) * p.Lq + x0 + r] = rsum;
+                }
             }
             // with the keys: half of dK or of dV to each four warps; with the queries: a quarter of dQ
             const int quarter = warp / 4;
@@ -482,8 +545,28 @@ __global__ void __launch_bounds__(kTcBwdThreads, 1) attn_tc_backward(const __gri
                                  (int64_t)(x0 + r) * os[2];
             const float f = is_dv ? 1.f : p.scale;
             const int c0 = kKeys ? quarter % 2 * (DP / 2) : quarter * (DP / 4), c1 = min(p.D, c0 + DP / (kKeys ? 2 : 4));
+            if (tp.parts.parts > 1) {
+                const int64_t at = (((int64_t)part * p.B * nhead + bh) * xrows + x0 + r) * p.D;
 #pragma unroll 1
-            for (int c = c0; c < c1; c += 16) {
+                for (int which = 0; which < (kKeys ? 1 : 2); ++which) {
+                    const bool second = kKeys ? is_dv : which == 1;
+                    float* to = (second ? tp.parts.other : tp.parts.acc) + at;
+#pragma unroll 1
+                    for (int c = c0; c < c1; c += 16) {
+                        float o[16];
+                        if (n > 0) tmem_ld_x16((second ? tB : tA) + lanes + c, o);
+                        if (x0 + r >= xrows) continue;
+#pragma unroll
+                        for (int k = 0; k < 16; k += 4)
+                            if (c + k < c1)
+                                *reinterpret_cast<float4*>(to + c + k) =
+                                    n > 0 ? make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f)
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                }
+            }
+#pragma unroll 1
+            for (int c = c0; c < c1 && tp.parts.parts == 1; c += 16) {
                 float o[16];
                 if (n > 0) {
                     tmem_ld_x16((is_dv ? tB : tA) + lanes + c, o);

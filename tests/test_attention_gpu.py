@@ -460,3 +460,41 @@ def test_out_in_the_place_of_keys_or_values_is_refused():
     for t in (k, v):
         with pytest.raises(mg.MacrogradError, match="same memory"):
             mg.attention(q, k, v, out=t)
+
+
+SHARED = [  # B, H, Hkv, Lq, Lk, D: few rows of blocks, so that several share a gradient's sum
+    (1, 8, 2, 700, 700, 128),
+    (1, 2, 1, 1100, 1300, 64),
+    (2, 6, 1, 3, 900, 96),
+    (1, 1, 1, 2000, 130, 72),
+    (1, 16, 1, 150, 150, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("size", SHARED, ids=str)
+def test_gradients_of_shared_sums(size, mask, dtype):
+    compare(*make(size, mask, dtype, 21))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_gradients_of_shared_sums_repeat(dtype):
+    """The same bits every time, and in two captured graphs replayed on two streams."""
+    q, k, v, dout, kw = make((1, 8, 2, 700, 700, 64), "documents", dtype, 22)
+    out, lse = mg.attention(q, k, v, **kw)
+    first = mg.attention_backward(dout, q, k, v, out, lse, **kw)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = mg.attention_backward(dout, q, k, v, out, lse, **kw)
+        graphs.append((g, got, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, _, s in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for _, got, _ in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
