@@ -42,6 +42,8 @@ typedef enum mg_dtype { MG_F32 = 0, MG_BF16 = 1 } mg_dtype;
  * used, nor is q or dout of a query of a negative document. Elsewhere v (and in the
  * backward pass k, q, dout) has to be finite also where a mask hides it from
  * some queries.
+ * The backward pass takes each weight from lse: it carries lse's rounding, a relative
+ * 2^-24 * |lse|.
  * Scores and biases are resolved up to 2^28 in size; a row with larger ones may
  * come out as NaN.
  * scale lies within +-1e30, cap is 0 or within 1e-30..1e30. Strides are in
