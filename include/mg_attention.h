@@ -106,9 +106,11 @@ mg_status mg_rotary(const mg_rotary_desc* d, void* out_q, void* out_k, const voi
  * in mg_attention. With k_new and v_new ([batch, kv_heads, head_dim]) the
  * token's own key and value are taken from there and written to the cache at
  * position lengths[b] - 1. A length of 0 gives out = 0, lse = -inf and writes
- * nothing. A length beyond the table, or a page outside the pool, is cut off
- * or skipped (never read or written) and sets MG_ERR_INVALID in
- * mg_device_status(). Requests must not share the page that they append to. */
+ * nothing. A length beyond the table is cut off there: the call attends to the
+ * keys that the table holds, from the last one's position, and the request
+ * appends nothing. A page outside the pool is skipped (never read or written).
+ * Both set MG_ERR_INVALID in mg_device_status(). Requests must not share the
+ * page that they append to. */
 typedef struct mg_paged_desc {
     int32_t dtype;
     int32_t batch, heads, kv_heads, head_dim, page_size, pages, table_width;

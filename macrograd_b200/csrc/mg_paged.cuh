@@ -43,13 +43,20 @@ struct PagedParams {
 constexpr int kPagedThreads = 128;
 constexpr int kPagedHeads = 8;
 
-// Number of keys of request b; a length beyond the table is cut off there.
+// Number of keys of request b; a length beyond the table is cut off there: what lies
+// beyond, the token to append among it, is neither read nor written.
 __device__ __forceinline__ int paged_length(const PagedParams& p, int b)
 {
     if (p.lengths == nullptr) return p.length;
     const int64_t most = (int64_t)p.width * p.page;
     const int n = __ldg(p.lengths + b);
     return n < 0 ? 0 : n > most ? (int)most : n;
+}
+
+// Place of the token that request b of `len` keys appends, or -1: none, or one that its table has no room for.
+__device__ __forceinline__ int paged_append(const PagedParams& p, int b, int len)
+{
+    return p.k_new != nullptr && len > 0 && __ldg(p.lengths + b) == len ? len - 1 : -1;
 }
 
 // Keys that a block of a request of `len` keys reads: its share, but no less than
@@ -131,6 +138,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_simt_kernel(const __grid_
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     constexpr int kWarps = kPagedThreads / 32, kPer = MG_MAX_HEAD_DIM / 32;
     if (j0 >= j1 && split > 0) return;      // a chunk beyond the request's keys is not joined
+    const int append = paged_append(p, b, len);
 
     float q[kPagedHeads][kPer], acc[kPagedHeads][kPer], m[kPagedHeads], l[kPagedHeads], slope[kPagedHeads];
     const int qdoc = p.docs && len > 0 ? __ldg(p.docs + (int64_t)b * p.length + len - 1) : 0;
@@ -149,7 +157,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_simt_kernel(const __grid_
     for (int j = j0 + warp; j < j1; j += kWarps) {
         int page, row;
         const bool have = paged_row(p, b, j, page, row);
-        const bool fresh = p.k_new != nullptr && j == len - 1;
+        const bool fresh = j == append;
         if (!have) {
             if (lane == 0) paged_report(p, kPagedBadPage);
             continue;
@@ -543,6 +551,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(paged_dyn) + warp * kPagedStages * 2 * kTileBytes;
     const int qdoc = p.docs && len > 0 ? __ldg(p.docs + (int64_t)b * p.length + len - 1) : 0;
+    const int append = paged_append(p, b, len);
 
     // Tile n of this warp: keys j0 + (4 n + warp) * 16 and on. Lanes 0-15 find the
     // rows of a key each and leave them to the others in shared memory.
@@ -568,8 +577,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
         const uint32_t seen = __ballot_sync(~0u, live);
         if (lane == 0) sm_seen[warp][n % kPagedStages] = seen;
         // the token's own key and value go to the cache, and are read from where they came
-        const int last = len - 1 - (j0 + (n * kPagedWarps + warp) * kPagedTile);
-        if (p.k_new != nullptr && last >= 0 && last < kPagedTile && (seen >> last & 1)) {
+        const int last = append - (j0 + (n * kPagedWarps + warp) * kPagedTile);
+        if (last >= 0 && last < kPagedTile && (seen >> last & 1)) {
             __syncwarp();
             const ulonglong2 at = rows[last];
             const bool is_v = lane >= 16;

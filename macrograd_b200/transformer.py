@@ -342,7 +342,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     order; lengths int32 [B]: its keys, the new token among them. The query stands at position lengths[b] - 1.
     With k_new and v_new [B, Hkv, D] the token's own key and value come from there, and the call also writes them to
     the cache at that position; requests must not share the page they append to, nor keys and values theirs. A length
-    of 0 gives out = 0, lse = -inf and writes nothing. A length beyond the table is cut off there, a page outside the
+    of 0 gives out = 0, lse = -inf and writes nothing. A length beyond the table is cut off there (the call attends to
+    the keys that the table holds, from the last one's position, and the request appends nothing), a page outside the
     pool is skipped, and mg_device_status() then reports MG_ERR_INVALID.
 
     Returns (out [B, H, D], lse [B, H] in float32)."""

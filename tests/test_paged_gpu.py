@@ -278,3 +278,27 @@ def test_appending_to_one_pool_of_keys_and_values_is_refused():
     with pytest.raises(mg.MacrogradError, match="same memory"):
         mg.paged_attention(q, kp, kp, table, lengths, k_new=kn, v_new=vn)
     compare((q, kp, kp, table, lengths, None, None))      # read alone
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 33])
+@pytest.mark.parametrize("rows", [16, 176, 6400], ids=["one block", "a cluster", "two launches"])
+def test_a_token_beyond_the_table_is_not_appended(rows, D, dtype):
+    """A request that has outgrown its table by one token: nothing of the cache changes, and the call attends to what the
+    table holds; the requests beside it go on."""
+    q, kp, vp, table, lengths, kn, vn = make(2, 4, 2, D, 16, [rows - 15, rows - 20 if rows > 20 else 3], dtype)
+    table = table[:, :rows // 16].contiguous()
+    slopes = torch.tensor([0.5, 0.25, 0.125, 0.0625], device="cuda")
+    for past in (rows + 1, rows + 17, 2 ** 31 - 1):
+        grown = lengths.clone()
+        grown[0] = past
+        kept = kp.clone(), vp.clone()
+        out, lse = mg.paged_attention(q, kp, vp, table, grown, slopes=slopes, k_new=kn, v_new=vn)
+        assert status()[0] == _lib.MG_ERR_INVALID
+        at = int(table[1, (int(lengths[1]) - 1) // 16]), (int(lengths[1]) - 1) % 16
+        kept[0][at], kept[1][at] = kn[1], vn[1]
+        assert torch.equal(kp, kept[0]) and torch.equal(vp, kept[1])
+        grown[0] = rows
+        want = mg.paged_attention(q, kp, vp, table, grown, slopes=slopes)
+        assert status()[0] == _lib.MG_OK
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
