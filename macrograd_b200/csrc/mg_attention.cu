@@ -58,36 +58,40 @@ mg::AttnParams attention_params(const mg_attention_desc* d)
     return p;
 }
 
-template <typename K>
-mg_status simt_launch(K kernel, int blocks, int rows_in_smem, int tiles33, const mg::AttnParams& p, cudaStream_t st,
-                      const char* what)
+// The shared memory that kernel K may take is the kernel's, not the call's: it is set once, to
+// what the longest heads take, so that calls of several host threads do not lower it for one another.
+template <auto K>
+mg_status simt_launch(int blocks, int rows_in_smem, int tiles33, const mg::AttnParams& p, const Device& dev,
+                      cudaStream_t st, const char* what)
 {
-    const size_t smem = sizeof(float) * ((size_t)rows_in_smem * mg::kSimtTile * (p.D + 1) +
-                                         (size_t)tiles33 * mg::kSimtTile * 33);
-    MG_HOST_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kernel<<<blocks, mg::kSimtThreads, smem, st>>>(p);
+    const auto smem = [&](int D) {
+        return sizeof(float) * ((size_t)rows_in_smem * mg::kSimtTile * (D + 1) + (size_t)tiles33 * mg::kSimtTile * 33);
+    };
+    MG_TRY(allow_smem<K>(dev, smem(mg::kSimtMaxD)));
+    K<<<blocks, mg::kSimtThreads, smem(p.D), st>>>(p);
     return launched(what);
 }
 
 template <typename T>
-mg_status forward_simt(const mg::AttnParams& p, cudaStream_t st)
+mg_status forward_simt(const mg::AttnParams& p, const Device& dev, cudaStream_t st)
 {
-    return simt_launch(mg::attn_simt_forward<T>, p.B * p.H * ceil_div(p.Lq, mg::kSimtTile), 3, 1, p, st,
-                       "mg_attention");
+    return simt_launch<mg::attn_simt_forward<T>>(p.B * p.H * ceil_div(p.Lq, mg::kSimtTile), 3, 1, p, dev, st,
+                                                 "mg_attention");
 }
 
 template <typename T>
-mg_status backward_simt(const mg::AttnParams& p, cudaStream_t st)
+mg_status backward_simt(const mg::AttnParams& p, const Device& dev, cudaStream_t st)
 {
     const char* who = "mg_attention_backward";
     if (p.Lq > 0) {
         mg::attn_delta_kernel<T><<<ceil_div((int64_t)p.B * p.H * p.Lq, 8), 256, 0, st>>>(p);
         MG_TRY(launched(who));
-        MG_TRY(simt_launch(mg::attn_simt_backward_dq<T>, p.B * p.H * ceil_div(p.Lq, mg::kSimtTile), 4, 1, p, st, who));
+        MG_TRY(simt_launch<mg::attn_simt_backward_dq<T>>(p.B * p.H * ceil_div(p.Lq, mg::kSimtTile), 4, 1, p, dev, st,
+                                                         who));
     }
     if (p.Lk > 0)
-        MG_TRY(simt_launch(mg::attn_simt_backward_dkv<T>, p.B * p.Hkv * ceil_div(p.Lk, mg::kSimtTile), 4, 2, p, st,
-                           who));
+        MG_TRY(simt_launch<mg::attn_simt_backward_dkv<T>>(p.B * p.Hkv * ceil_div(p.Lk, mg::kSimtTile), 4, 2, p, dev,
+                                                          st, who));
     return MG_OK;
 }
 
@@ -420,7 +424,7 @@ mg_status mg_attention(const mg_attention_desc* d, void* out, float* lse, const 
     }
     if (p.Lk > 0 && tc_serves(d, p, {q, out}, {k, v}))
         return d->dtype == MG_F32 ? forward_tc32(p, dev, stream) : forward_tc(p, dev, stream);
-    return d->dtype == MG_F32 ? forward_simt<float>(p, st) : forward_simt<__nv_bfloat16>(p, st);
+    return d->dtype == MG_F32 ? forward_simt<float>(p, dev, st) : forward_simt<__nv_bfloat16>(p, dev, st);
 }
 
 mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, void* dv, const void* dout,
@@ -448,7 +452,7 @@ mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, 
         if (!p.delta) return fail(MG_ERR_ALLOC, "mg_attention_backward: no scratch for the row sums");
     }
     cudaStream_t st = (cudaStream_t)stream;
-    return d->dtype == MG_F32 ? backward_simt<float>(p, st) : backward_simt<__nv_bfloat16>(p, st);
+    return d->dtype == MG_F32 ? backward_simt<float>(p, dev, st) : backward_simt<__nv_bfloat16>(p, dev, st);
 }
 
 }  // extern "C"

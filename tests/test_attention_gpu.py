@@ -2,12 +2,15 @@
 shared heads, head sizes, lengths from one token on, strided views, caps, biases,
 documents, prefixes, rows that see nothing, padding that holds NaN; determinism,
 other streams, captured graphs, offsets beyond 32 bits."""
+import ctypes
 import math
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 
 torch = pytest.importorskip("torch")
 import macrograd_b200 as mg  # noqa: E402
+from macrograd_b200 import _lib, transformer  # noqa: E402
 from attention_reference import Reference, within  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -498,3 +501,32 @@ def test_gradients_of_shared_sums_repeat(dtype):
     torch.cuda.synchronize()
     for _, got, _ in graphs:
         assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
+def test_host_threads_with_heads_of_other_sizes():
+    """Two host threads launch the CUDA-core kernels at once, with heads that take different amounts of shared memory:
+    through the C ABI, whose calls follow one another closely enough to meet in the launch."""
+    lib = mg.load()
+    calls = []
+    for D in (33, 127):
+        q, k, v, _, _ = make((1, 1, 1, 2, 2, D), "causal", torch.float32, 50, strided=False)
+        want = mg.attention(q, k, v)
+        out, lse = torch.empty_like(q), torch.empty_like(want[1])
+        desc = transformer._ATTENTION.pack(0, 1, 1, 1, 2, 2, D, 1, 1 / math.sqrt(D), 0.0, *([2 * D, 2 * D, D] * 4),
+                                           *([0] * 12), 0, 0, 0)
+        calls.append((desc, q, k, v, out, lse, want, torch.cuda.Stream().cuda_stream))
+    torch.cuda.synchronize()
+
+    def repeat(desc, q, k, v, out, lse, want, stream):
+        bad = 0
+        for _ in range(20000):
+            bad += lib.mg_attention(desc, out.data_ptr(), lse.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                    ctypes.c_void_p(stream)) != _lib.MG_OK
+        return bad
+
+    with ThreadPoolExecutor(2) as pool:
+        refused = sum(f.result() for f in [pool.submit(repeat, *c) for c in calls])
+    torch.cuda.synchronize()
+    assert refused == 0, f"{refused} of 40000 launches were refused"
+    for _, _, _, _, out, lse, want, _ in calls:
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
