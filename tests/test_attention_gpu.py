@@ -160,7 +160,7 @@ def test_no_queries(dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("cap", [0.0, 30.0])
-def test_large_scores(dtype, cap):
+def test_scores_of_several_hundred(dtype, cap):
     """Scores of several hundred: the running maximum moves far, sums stay finite."""
     g = torch.Generator(device="cuda").manual_seed(2)
     q, k = (torch.randn((1, 2, 400, 64), generator=g, device="cuda").mul(8).to(dtype) for _ in range(2))
