@@ -86,8 +86,8 @@ mg_status backward_simt(const mg::AttnParams& p, const Device& dev, cudaStream_t
     if (p.Lq > 0) {
         mg::attn_delta_kernel<T><<<ceil_div((int64_t)p.B * p.H * p.Lq, 8), 256, 0, st>>>(p);
         MG_TRY(launched(who));
-        MG_TRY(simt_launch<mg::attn_simt_backward_dq<T>>(p.B * p.H * ceil_div(p.Lq, mg::kSimtTile), 4, 1, p, dev, st,
-                                                         who));
+        MG_TRY(simt_launch<mg::attn_simt_backward_dq<T>>(p.B * p.H * ceil_div(p.Lq, mg::kSimtTile), 4,
+                                                         sizeof(T) == 2 ? 2 : 1, p, dev, st, who));
     }
     if (p.Lk > 0)
         MG_TRY(simt_launch<mg::attn_simt_backward_dkv<T>>(p.B * p.Hkv * ceil_div(p.Lk, mg::kSimtTile), 4, 2, p, dev,

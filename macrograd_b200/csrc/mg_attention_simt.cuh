@@ -156,20 +156,27 @@ __global__ void attn_delta_kernel(const __grid_constant__ AttnParams p)
     if (threadIdx.x % 32 == 0) p.delta[row] = s;
 }
 
-// P and dS of pair (query, key) from the two products.
+// P, P * curve and dS of pair (query, key) from the two products.
 __device__ __forceinline__ void simt_grad(const AttnParams& p, bool seen, float qk, float dov, float lse, float delta,
-                                          float slope, int dist, float& P, float& dS)
+                                          float slope, int dist, float& P, float& PC, float& dS)
 {
-    P = dS = 0.f;
+    P = PC = dS = 0.f;
     if (!seen) return;
     float bend;
     const float s = score(p.scale * qk, p.cap, slope, dist, bend);
     P = expf(s - lse);
+    PC = P * (1.f - bend * bend);
     dS = P * (dov - delta) * (1.f - bend * bend) * p.scale;
 }
 
+// dQ. With 16-bit tensors delta carries the rounding of out, which is as large as dP - delta where the
+// values of a row have much in common. The true delta makes the row's sum of P * (dP - delta) zero, so
+// what that sum is is delta's error r: dQ loses r times sum P curve k, and delta becomes exact for dK,
+// which is computed after it. Without, gradients of values that differ in their last bit alone are off by
+// their own size; it costs 6 % (bf16 [4, 8, 512, 33]: gradients 588 -> 624 us). Two blocks an SM: with the
+// 163 registers that it would take, 709 us.
 template <typename T>
-__global__ void __launch_bounds__(kSimtThreads) attn_simt_backward_dq(const __grid_constant__ AttnParams p)
+__global__ void __launch_bounds__(kSimtThreads, 2) attn_simt_backward_dq(const __grid_constant__ AttnParams p)
 {
     extern __shared__ float sm[];
     const int pitch = p.D + 1;
@@ -178,6 +185,8 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_backward_dq(const __gr
     float* K = G + kSimtTile * pitch;
     float* V = K + kSimtTile * pitch;
     float* S = V + kSimtTile * pitch;
+    constexpr bool kCorrect = sizeof(T) == 2;
+    float2* SC = reinterpret_cast<float2*>(S);   // dS and P * curve side by side, where delta is corrected
     __shared__ int kdoc[kSimtTile];
 
     const int tiles = (p.Lq + kSimtTile - 1) / kSimtTile, bh = blockIdx.x / tiles;
@@ -197,9 +206,9 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_backward_dq(const __gr
 
     simt_load(Q, pitch, (const T*)p.q + b * p.qs[0] + h * p.qs[1], p.qs[2], q0, p.Lq, p.D, docs, p.Lk - p.Lq);
     simt_load(G, pitch, (const T*)p.dout + b * p.dos[0] + h * p.dos[1], p.dos[2], q0, p.Lq, p.D, docs, p.Lk - p.Lq);
-    float acc[kSimtMaxD / 8];
+    float acc[kSimtMaxD / 8], off[kSimtMaxD / 8], rest = 0.f;
 #pragma unroll
-    for (int i = 0; i < kSimtMaxD / 8; ++i) acc[i] = 0.f;
+    for (int i = 0; i < kSimtMaxD / 8; ++i) acc[i] = off[i] = 0.f;
     const int jend = key_end(p, query_pos(p, min(q0 + kSimtTile, p.Lq) - 1), prefix);
     for (int j0 = 0; j0 < jend; j0 += kSimtTile) {
         __syncthreads();
@@ -211,27 +220,42 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_backward_dq(const __gr
         for (int i = 0; i < 4; ++i) {
             const int c = c8 + 8 * i, j = j0 + c;
             const bool seen = live && j < p.Lk && sees(p, qpos, qdoc, j, docs ? kdoc[c] : 0, prefix);
-            float P, dS;
-            simt_grad(p, seen, simt_dot(Q + r * pitch, K + c * pitch, p.D), simt_dot(G + r * pitch, V + c * pitch, p.D),
-                      lse, delta, slope, qpos - j, P, dS);
-            S[r * 33 + c] = dS;
+            float P, PC, dS;
+            const float dP = simt_dot(G + r * pitch, V + c * pitch, p.D);
+            simt_grad(p, seen, simt_dot(Q + r * pitch, K + c * pitch, p.D), dP, lse, delta, slope, qpos - j, P, PC, dS);
+            if (kCorrect) {
+                SC[r * 33 + c] = make_float2(dS, PC);
+                if (seen) rest = fmaf(P, dP - delta, rest);
+            } else {
+                S[r * 33 + c] = dS;
+            }
         }
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kSimtMaxD / 8; ++i) {
             const int d = c8 + 8 * i;
             if (d >= p.D) break;
-            float a = acc[i];
-            for (int c = 0; c < kSimtTile; ++c) a = fmaf(S[r * 33 + c], K[c * pitch + d], a);
+            float a = acc[i], o = off[i];
+            for (int c = 0; c < kSimtTile; ++c) {
+                const float2 x = kCorrect ? SC[r * 33 + c] : make_float2(S[r * 33 + c], 0.f);
+                a = fmaf(x.x, K[c * pitch + d], a);
+                if (kCorrect) o = fmaf(x.y, K[c * pitch + d], o);
+            }
             acc[i] = a;
+            off[i] = o;
         }
+    }
+    if (kCorrect) {
+#pragma unroll
+        for (int o = 1; o < 8; o *= 2) rest += __shfl_xor_sync(~0u, rest, o);
+        if (live && c8 == 0) p.delta[row] = delta + rest;
     }
     if (!live) return;
     T* o = (T*)p.dq + b * p.dqs[0] + h * p.dqs[1] + (int64_t)(q0 + r) * p.dqs[2];
 #pragma unroll
     for (int i = 0; i < kSimtMaxD / 8; ++i) {
         const int d = c8 + 8 * i;
-        if (d < p.D) o[d] = from_f32<T>(acc[i]);
+        if (d < p.D) o[d] = from_f32<T>(kCorrect ? fmaf(-rest * p.scale, off[i], acc[i]) : acc[i]);
     }
 }
 
@@ -278,10 +302,10 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_backward_dkv(const __g
                 const int c = c8 + 8 * i, q = q0 + c, qpos = query_pos(p, q);
                 const int64_t row = ((int64_t)b * p.H + h) * p.Lq + q;
                 const bool seen = q < p.Lq && j < p.Lk && sees(p, qpos, docs ? qdoc[c] : 0, j, kdoc, prefix);
-                float P, dS;
+                float P, PC, dS;
                 simt_grad(p, seen, simt_dot(Q + c * pitch, K + r * pitch, p.D),
                           simt_dot(G + c * pitch, V + r * pitch, p.D), seen ? p.lse[row] : 0.f,
-                          seen ? p.delta[row] : 0.f, slope, qpos - j, P, dS);
+                          seen ? p.delta[row] : 0.f, slope, qpos - j, P, PC, dS);
                 PT[r * 33 + c] = P;
                 ST[r * 33 + c] = dS;
             }

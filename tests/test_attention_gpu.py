@@ -11,7 +11,7 @@ import pytest
 torch = pytest.importorskip("torch")
 import macrograd_b200 as mg  # noqa: E402
 from macrograd_b200 import _lib, transformer  # noqa: E402
-from attention_reference import Reference, within  # noqa: E402
+from attention_reference import Reference, half_step, within  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -530,3 +530,45 @@ def test_host_threads_with_heads_of_other_sizes():
     assert refused == 0, f"{refused} of 40000 launches were refused"
     for _, _, _, _, out, lse, want, _ in calls:
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+COMMON = [  # B, H, Hkv, Lq, Lk, D, rows off 16 bytes
+    (1, 4, 2, 300, 300, 64, False),
+    (1, 8, 2, 700, 700, 128, False),         # several blocks share a sum
+    (2, 16, 16, 700, 700, 64, False),        # none does
+    (1, 2, 1, 3, 900, 96, False),
+    (1, 2, 1, 1, 200, 64, False),
+    (1, 2, 1, 150, 150, 33, False),
+    (2, 4, 2, 130, 200, 64, True),
+]
+
+
+@pytest.mark.parametrize("size", COMMON, ids=str)
+@pytest.mark.parametrize("cap", [0.0, 10.0])
+@pytest.mark.parametrize("short", [False, True], ids=["one document", "documents of 7"])
+def test_16_bit_gradients_of_values_with_much_in_common(short, cap, size):
+    """Values that differ in their last bit: dP - delta is as small as the rounding of `out` that delta is computed
+    from, so a gradient that does not make up for it is wrong by about its own size (taken twice or with the wrong sign,
+    by two or three times that).
+
+    Bound, of the norm: half a step (u) each for dS, for the weights of what is made up for (of the size of the
+    gradient itself), for the result, and for everything in fp32 (2^-24 * D * 8 of a sum that 2^-7 of is left: less
+    than u / 4)."""
+    *size, off = size
+    B, H, Hkv, Lq, Lk, D = size
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def heads(n, L, bits=False):
+        x = torch.randn((B, n, L, D + off), generator=g, device="cuda")
+        return (1 + 2.0 ** -7 * (x > 0) if bits else x).bfloat16()[..., off:]
+
+    q, k, v, dout = heads(H, Lq), heads(Hkv, Lk), heads(Hkv, Lk, True), heads(H, Lq)
+    kw = dict(cap=cap)
+    if short:
+        kw["documents"] = (torch.arange(Lk, device="cuda") // 7).int().expand(B, Lk).contiguous()
+    out, lse = mg.attention(q, k, v, **kw)
+    ref = Reference(q, k, v, dout, **kw)
+    dq, dk, dv = mg.attention_backward(dout, q, k, v, out, lse, **kw)
+    for got, want, what in ((dq, ref.dq, "dq"), (dk, ref.dk, "dk"), (dv, ref.dv, "dv")):
+        error = float((got.double() - want).norm() / want.norm())
+        assert error <= 4 * half_step(torch.bfloat16), f"{what}: {error:.3g}"
