@@ -162,9 +162,9 @@ mg_status share_rows(mg::RowParts* r, const mg::AttnParams& p, int places, Scrat
     r->parts = (int)std::max<int64_t>(1, std::min<int64_t>(places / blocks, ceil_div(p.Lk, 512)));
     if (r->parts == 1) return MG_OK;
     const int64_t rows = (int64_t)r->parts * p.B * p.H * p.Lq;
-    r->out = static_cast<float*>(ws.get(rows * (p.D + 1) * sizeof(float)));
+    r->out = static_cast<float*>(ws.get(rows * (p.D + 2) * sizeof(float)));      // p.D is a multiple of 8
     if (!r->out) return fail(MG_ERR_ALLOC, "mg_attention: no scratch for %d parts of each row", r->parts);
-    r->lse = r->out + rows * p.D;
+    r->stat = reinterpret_cast<float2*>(r->out + rows * p.D);
     return MG_OK;
 }
 

@@ -25,11 +25,12 @@ struct AttnParams {
 };
 
 // A row of keys shared by several blocks of the forward kernels, where there are
-// too few queries to fill the GPU: each leaves its part's out and lse in fp32.
+// too few queries to fill the GPU: each leaves its part's out, and the maximum and the sum that
+// it is taken against, in fp32. (From the parts' lse, their weights would carry its rounding, 2^-24 |lse|.)
 struct RowParts {
     int parts;           // 1: the block writes out and lse itself
     float* out;          // [parts][B * H][Lq][D]
-    float* lse;          // [parts][B * H][Lq]
+    float2* stat;        // [parts][B * H][Lq] (m, l): lse = (m + log2 l) ln 2
 };
 
 // A gradient's sum over the streamed rows, shared by several blocks.

@@ -186,7 +186,7 @@ __device__ __forceinline__ void share_of_row(int part, int parts, int& t0, int& 
     t1 = min(t1, t0 + each);
 }
 
-// Joins the parts of each row: out = sum exp(lse_s - lse) out_s, lse = log sum exp(lse_s).
+// Joins the parts of each row: with w_s = 2^(m_s - max m) l_s, out = sum w_s out_s / sum w_s.
 // One warp to a row, four elements to a lane.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnParams p, RowParts rows)
@@ -195,13 +195,14 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     if (at >= all) return;
     const int lane = threadIdx.x % 32;
     float top = -CUDART_INF_F;
-    for (int s = 0; s < rows.parts; ++s) top = fmaxf(top, __ldg(rows.lse + s * all + at));
+    for (int s = 0; s < rows.parts; ++s) top = fmaxf(top, __ldg(rows.stat + s * all + at).x);
     const float base = top == -CUDART_INF_F ? 0.f : top;
     float sum = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     const bool in = lane * 4 < p.D;
     for (int s = 0; s < rows.parts; ++s) {
-        const float w = expf(__ldg(rows.lse + s * all + at) - base);
+        const float2 st = __ldg(rows.stat + s * all + at);
+        const float w = ex2(st.x - base) * st.y;
         sum += w;
         if (!in || w == 0.f) continue;
         const float4 x = __ldg(reinterpret_cast<const float4*>(rows.out + (s * all + at) * p.D) + lane);
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
         out[0] = from_f32<T>(o.x * inv), out[1] = from_f32<T>(o.y * inv);
         out[2] = from_f32<T>(o.z * inv), out[3] = from_f32<T>(o.w * inv);
     }
-    if (lane == 0) p.lse[at] = sum == 0.f ? -CUDART_INF_F : base + logf(sum);
+    if (lane == 0) p.lse[at] = sum == 0.f ? -CUDART_INF_F : (base + log2f(sum)) * kLn2;
 }
 
 constexpr int kTcFwdThreads = 320;       // eight warps of exponentials, loads, products
@@ -496,9 +497,12 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
                             make_uint4(bf16x2(o[i] * inv, o[i + 1] * inv), bf16x2(o[i + 2] * inv, o[i + 3] * inv),
                                        bf16x2(o[i + 4] * inv, o[i + 5] * inv), bf16x2(o[i + 6] * inv, o[i + 7] * inv));
             }
-            if (store && half == 0)
-                (tp.rows.parts > 1 ? tp.rows.lse + (int64_t)part * p.B * p.H * p.Lq : p.lse)[(int64_t)bh * p.Lq + row] =
-                    l == 0.f ? -CUDART_INF_F : ((m == -CUDART_INF_F ? 0.f : m * mul) + log2f(l)) * kLn2;
+            if (store && half == 0) {
+                const float m2 = m == -CUDART_INF_F ? 0.f : m * mul;
+                const int64_t at = (int64_t)bh * p.Lq + row;
+                if (tp.rows.parts == 1) p.lse[at] = l == 0.f ? -CUDART_INF_F : (m2 + log2f(l)) * kLn2;
+                else tp.rows.stat[(int64_t)part * p.B * p.H * p.Lq + at] = make_float2(l == 0.f ? -CUDART_INF_F : m2, l);
+            }
         }
         if (!ok && lane == 0) tc_report(tp.status, 202);
     }

@@ -395,9 +395,12 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
                                         (o[c0 + c + 2] + x[c + 2]) * g, (o[c0 + c + 3] + x[c + 3]) * g);
                     }
             }
-            if (row < p.Lq)
-                (tp.rows.parts > 1 ? tp.rows.lse + (int64_t)part * p.B * p.H * p.Lq : p.lse)[(int64_t)bh * p.Lq + row] =
-                    l == 0.f ? -CUDART_INF_F : ((m == -CUDART_INF_F ? 0.f : m) + log2f(l)) * kLn2;
+            if (row < p.Lq) {
+                const float m2 = m == -CUDART_INF_F ? 0.f : m;
+                const int64_t at = (int64_t)bh * p.Lq + row;
+                if (tp.rows.parts == 1) p.lse[at] = l == 0.f ? -CUDART_INF_F : (m2 + log2f(l)) * kLn2;
+                else tp.rows.stat[(int64_t)part * p.B * p.H * p.Lq + at] = make_float2(l == 0.f ? -CUDART_INF_F : m2, l);
+            }
         }
         if (!ok && lane == 0) tc_report(tp.status, 222);
     }

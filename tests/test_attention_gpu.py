@@ -572,3 +572,26 @@ def test_16_bit_gradients_of_values_with_much_in_common(short, cap, size):
     for got, want, what in ((dq, ref.dq, "dq"), (dk, ref.dk, "dk"), (dv, ref.dv, "dv")):
         error = float((got.double() - want).norm() / want.norm())
         assert error <= 4 * half_step(torch.bfloat16), f"{what}: {error:.3g}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("top", [2 ** 16, 2 ** 18 + 3, 2 ** 20 + 3, 2 ** 20 + 11])
+def test_parts_of_a_row_with_large_scores(top, dtype):
+    """One head whose row is shared by several blocks: one half of the keys scores `top`, the other a quarter less, both
+    exactly. The halves' weights go by that quarter, whatever the rounding of sums as large as `top`.
+
+    Bound: worst rounding of a part's sum of 4096 equal weights by 64 and tile (128 additions), once above and once
+    below the line, two exponentials of 2 ulp each and the logarithm's base in fp32: 300 * 2^-24; 16-bit weights and
+    results half a step each."""
+    Lq, Lk, D = 130, 8192, 16
+    q, k, v = (torch.zeros((1, 1, L, D), device="cuda", dtype=dtype) for L in (Lq, Lk, Lk))
+    hi = float(torch.tensor(float(top)).bfloat16())
+    q[..., :3] = 1
+    k[..., 0], k[..., 1] = hi, top - hi
+    k[:, :, Lk // 2:, 2] = -0.25
+    v[:, :, :Lk // 2, 0], v[:, :, Lk // 2:, 1] = 1, 1
+    out, lse = mg.attention(q, k, v, scale=1.0, causal=False)
+    first = 1 / (1 + math.exp(-0.25))
+    tol = 300 * 2.0 ** -24 + (2 * half_step(dtype) if dtype == torch.bfloat16 else 0.0)
+    for d, want in ((0, first), (1, 1 - first)):
+        assert ((out[..., d].double() - want).abs() <= tol * want).all(), float((out[..., d].double() - want).abs().max() / want)
