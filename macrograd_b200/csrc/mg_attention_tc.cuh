@@ -414,7 +414,8 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
                 const float mn = grown ? top : m;
                 if (j > 0) {
                     tc_fence_after();
-                    const float f = m == -CUDART_INF_F ? 0.f : ex2((m - mn) * mul);
+                    // by the rounded powers of two that P is taken against
+                    const float f = m == -CUDART_INF_F ? 0.f : ex2(__fmul_rn(m, mul) - __fmul_rn(mn, mul));
 #pragma unroll 1
                     for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 16) {
                         float o[16];
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&st.p_full[0]));
             }
-            const float base2 = m == -CUDART_INF_F ? 0.f : m * mul;
+            const float base2 = m == -CUDART_INF_F ? 0.f : __fmul_rn(m, mul);
             const uint64_t mul_2 = pack2(mul, mul), base_2 = pack2(-base2, -base2);
 #pragma unroll
             for (int c = 0; c < 64; c += 32) {
@@ -498,7 +499,7 @@ __global__ void __launch_bounds__(kTcFwdThreads, 2) attn_tc_forward(const __grid
                                        bf16x2(o[i + 4] * inv, o[i + 5] * inv), bf16x2(o[i + 6] * inv, o[i + 7] * inv));
             }
             if (store && half == 0) {
-                const float m2 = m == -CUDART_INF_F ? 0.f : m * mul;
+                const float m2 = m == -CUDART_INF_F ? 0.f : __fmul_rn(m, mul);
                 const int64_t at = (int64_t)bh * p.Lq + row;
                 if (tp.rows.parts == 1) p.lse[at] = l == 0.f ? -CUDART_INF_F : (m2 + log2f(l)) * kLn2;
                 else tp.rows.stat[(int64_t)part * p.B * p.H * p.Lq + at] = make_float2(l == 0.f ? -CUDART_INF_F : m2, l);

@@ -348,11 +348,11 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
                 const bool high = top > 40.f;
                 if (pass == 2 || !__any_sync(~0u, high)) break;
                 if (high) {
-                    const float g = ex2(-top);
+                    m = base + top;
+                    const float g = ex2(base - m);       // not -top: m is rounded
                     l *= g;
 #pragma unroll
                     for (int c = 0; c < DP; ++c) o[c] *= g;
-                    m = base + top;
                 }
             }
             {
@@ -361,9 +361,10 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
                 l += x + y;
             }
             if (top > 8.f) {
-                f = ex2(-top);
+                const float up = m + top;
+                f = ex2(m - up);
                 l *= f;
-                m += top;
+                m = up;
             }
             tmem_wait_st();
             tc_fence_before();

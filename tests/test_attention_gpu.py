@@ -595,3 +595,30 @@ def test_parts_of_a_row_with_large_scores(top, dtype):
     tol = 300 * 2.0 ** -24 + (2 * half_step(dtype) if dtype == torch.bfloat16 else 0.0)
     for d, want in ((0, first), (1, 1 - first)):
         assert ((out[..., d].double() - want).abs() <= tol * want).all(), float((out[..., d].double() - want).abs().max() / want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("heads", [160, 1], ids=["one block", "parts"])
+@pytest.mark.parametrize("top", [2 ** 16, 2 ** 18 + 3, 2 ** 20 + 3, 2 ** 20 + 11])
+def test_a_large_maximum_that_comes_late(top, heads, dtype):
+    """All keys but four near the end score `top` - 8, those `top`, both exactly: what was summed before the maximum
+    moved, and what comes after it, goes by that 8.
+
+    Bound: worst rounding of sums over 4096 keys, 64 additions in a tile and as many tiles, above and below the line,
+    and the exponentials' 2 ulp: 300 * 2^-24; e^-8 itself is taken from 8 log2(e) in fp32, off by 12 * 2^-24 and as much
+    for log2(e); 16-bit weights and results half a step each."""
+    Lq, Lk, D = 128, 4096, 16
+    q = torch.zeros((1, heads, Lq, D), device="cuda", dtype=dtype)
+    k, v = (torch.zeros((1, 1, Lk, D), device="cuda", dtype=dtype) for _ in range(2))
+    hi = float(torch.tensor(float(top)).bfloat16())
+    q[..., :3] = 1
+    k[..., 0], k[..., 1] = hi, top - hi
+    high = slice(Lk - 300, Lk - 296)
+    k[..., 2], v[..., 1] = -8, 1
+    k[:, :, high, 2], v[:, :, high, 1], v[:, :, high, 0] = 0, 0, 1
+    out, lse = mg.attention(q, k, v, scale=1.0, causal=False)
+    late = 4 / (4 + (Lk - 4) * math.exp(-8))
+    tol = 324 * 2.0 ** -24 + (2 * half_step(dtype) if dtype == torch.bfloat16 else 0.0)
+    for d, want in ((0, late), (1, 1 - late)):
+        error = float((out[..., d].double() - want).abs().max() / want)
+        assert error <= tol, error
