@@ -49,6 +49,7 @@ mg_status launch_paged(mg::PagedParams& p, int longest, const Device& dev, Scrat
     bool stream = tame(p.scale, p.cap) && p.D % vec == 0 && aligned(p.k, p.ks, 3, sizeof(T), vec) && aligned(p.v, p.vs, 3, sizeof(T), vec);
     if (p.k_new) stream = stream && aligned(p.k_new, p.kns, 2, sizeof(T), vec) &&
                           aligned(p.v_new, p.vns, 2, sizeof(T), vec);
+    p.powers = stream;
     const int group = p.H / p.Hkv, packs = ceil_div(group, stream ? mg::paged_pack<T>() : mg::kPagedHeads);
     const int64_t heads = (int64_t)p.B * p.Hkv * packs;
     const int64_t want = std::max<int64_t>(1, (int64_t)dev.sm_count * 16 / heads);

@@ -4,11 +4,13 @@
 // Two forms. paged_kernel streams the cache through shared memory (rows on
 // 16-byte boundaries); paged_simt_kernel takes any strides.
 //
-// One block reads a chunk of the keys of one key-value head of one request, once, for
-// all query heads that share it (in groups of kPagedHeads), and leaves per query
-// head the maximum m, the sum l = sum exp(s - m) and the sum of exp(s - m) v. A
-// request of one chunk is finished there; otherwise a second kernel joins its
-// chunks: M = max m, out = sum exp(m - M) acc / sum exp(m - M) l.
+// One block reads a chunk of the keys of one key-value head of one request for the
+// query heads that share it, in packs of kPagedHeads (fp32, and the simple form) or 16
+// (bf16): heads beyond a pack read the cache again. It leaves per query head the
+// maximum m, the sum l = sum exp(s - m) and the sum of exp(s - m) v; in the streaming form
+// scores and m are in powers of two. A call of one chunk a request is finished there;
+// otherwise the chunks are joined, inside a cluster where a call is small and
+// by a second kernel else: M = max m, out = sum exp(m - M) acc / sum exp(m - M) l.
 // The bound is the cache's bytes.
 #pragma once
 
@@ -37,6 +39,7 @@ struct PagedParams {
     CapCurve curve;              // of the cap, with a cap
     float* part;                 // [B * H][splits][D] accumulators
     float2* stat;                // [B * H][splits] (m, l)
+    int powers;                  // m, and the scores, in powers of two (streaming form); else natural
     int* status;
 };
 
@@ -103,8 +106,13 @@ __device__ __forceinline__ float2 lds2(uint32_t addr)
     return v;
 }
 
+__device__ __forceinline__ float paged_lse(const PagedParams& p, float M, float L)
+{
+    return L == 0.f ? -CUDART_INF_F : (p.powers ? M * kLn2 : M) + logf(L);
+}
+
 // What one warp does with a finished chunk of one query head: the result where
-// the request has no other chunk, else its part of the join. M: natural log.
+// the call has one chunk a request, else its part of the join. M: as p.powers says.
 template <typename T, typename F>
 __device__ __forceinline__ void paged_store(const PagedParams& p, int b, int h, int split, float M, float L, int lane,
                                             F&& acc)
@@ -117,7 +125,7 @@ __device__ __forceinline__ void paged_store(const PagedParams& p, int b, int h, 
         else p.part[(row * p.splits + split) * p.D + d] = a;
     }
     if (lane == 0) {
-        if (p.splits == 1) p.lse[row] = L == 0.f ? -CUDART_INF_F : M + logf(L);
+        if (p.splits == 1) p.lse[row] = paged_lse(p, M, L);
         else p.stat[row * p.splits + split] = make_float2(M, L);
     }
 }
@@ -661,7 +669,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
             for (int d = lane; d < p.D; d += 32) block_o[g * DP + d] = joined(d);
             if (lane == 0) block_ml[g] = make_float2(M, L);
         } else {
-            paged_store<T>(p, b, h0 + g, split, M * kLn2, L, lane, joined);
+            paged_store<T>(p, b, h0 + g, split, M, L, lane, joined);
         }
     }
     if constexpr (kCluster) {
@@ -688,7 +696,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
                 }
                 if (d < p.D) out[d] = from_f32<T>(a * inv);
             }
-            if (lane == 0) p.lse[(int64_t)b * p.H + h0 + g] = L == 0.f ? -CUDART_INF_F : M * kLn2 + logf(L);
+            if (lane == 0) p.lse[(int64_t)b * p.H + h0 + g] = paged_lse(p, M, L);
         }
         cluster_sync_all();                  // nobody leaves while its results are read
     }
@@ -730,7 +738,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         float w = 0.f;
         if (s < n) {
             const float2 x = st[s];
-            w = expf(x.x - base);
+            w = p.powers ? ex2(x.x - base) : expf(x.x - base);
             L = fmaf(w, x.y, L);
         }
         weight[threadIdx.x] = w;
@@ -765,7 +773,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         out[0] = from_f32<T>(a.x * inv);
         if (width == 4) out[1] = from_f32<T>(a.y * inv), out[2] = from_f32<T>(a.z * inv), out[3] = from_f32<T>(a.w * inv);
     }
-    if (threadIdx.x == 0) p.lse[row] = L == 0.f ? -CUDART_INF_F : M + logf(L);
+    if (threadIdx.x == 0) p.lse[row] = paged_lse(p, M, L);
 }
 
 }  // namespace mg

@@ -3,13 +3,14 @@ sizes, ragged lengths with 0 and 1, appended tokens, both pool layouts, bad
 pages and lengths; and the chain rotary -> paged cache -> attention as a decoder
 uses it, token by token, against one attention over the whole row."""
 import ctypes
+import math
 
 import pytest
 
 torch = pytest.importorskip("torch")
 import macrograd_b200 as mg  # noqa: E402
 from macrograd_b200 import _lib  # noqa: E402
-from attention_reference import Reference, within  # noqa: E402
+from attention_reference import Reference, half_step, within  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -302,3 +303,32 @@ def test_a_token_beyond_the_table_is_not_appended(rows, D, dtype):
         want = mg.paged_attention(q, kp, vp, table, grown, slopes=slopes)
         assert status()[0] == _lib.MG_OK
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("top", [2 ** 16, 2 ** 18 + 3, 2 ** 20 + 3, 2 ** 20 + 11])
+@pytest.mark.parametrize("keys", [512, 16384], ids=["a cluster", "two launches"])
+def test_chunks_with_large_scores(keys, top, dtype):
+    """One half of the keys scores `top` powers of two, the other a quarter less, both exactly (the scale is ln 2, whose
+    product with log2(e) is 1 in fp32): the halves' weights go by that quarter, whatever the rounding of numbers as
+    large as `top`.
+
+    Bound: the worst rounding of a chunk's sum of up to 256 equal weights (256 additions), once above and once below the
+    line, and of the join (128), exponentials of 2 ulp: 700 * 2^-24; 16-bit weights and results half a step each."""
+    D = 64
+    scale = float(torch.tensor(math.log(2), dtype=torch.float32))
+    q = torch.zeros((1, 2, D), device="cuda", dtype=dtype)
+    kp, vp = (torch.zeros((keys // 16, 16, 1, D), device="cuda", dtype=dtype) for _ in range(2))
+    hi = float(torch.tensor(float(top)).bfloat16())
+    q[..., :3] = 1
+    kp[..., 0], kp[..., 1] = hi, top - hi
+    kp[keys // 32:, ..., 2] = -0.25
+    vp[:keys // 32, ..., 0], vp[keys // 32:, ..., 1] = 1, 1
+    table = torch.arange(keys // 16, device="cuda").int()[None].contiguous()
+    out, lse = mg.paged_attention(q, kp, vp, table, torch.tensor([keys], dtype=torch.int32, device="cuda"), scale=scale)
+    first = 1 / (1 + math.exp(-0.25 * scale))
+    tol = 700 * 2.0 ** -24 + (2 * half_step(dtype) if dtype == torch.bfloat16 else 0.0)
+    for d, want in ((0, first), (1, 1 - first)):
+        error = float((out[..., d].double() - want).abs().max() / want)
+        assert error <= tol, error
+    assert abs(float(lse[0, 0]) - (top * scale + math.log(keys / 2 / first))) <= 2 * 2.0 ** -24 * top
