@@ -48,7 +48,9 @@ typedef enum mg_dtype { MG_F32 = 0, MG_BF16 = 1 } mg_dtype;
  * come out as NaN.
  * scale lies within +-1e30, cap is 0 or within 1e-30..1e30. Strides are in
  * elements, for {batch, head, row}; head_dim is contiguous. Outputs must not
- * overlap k, v or each other. Tensors whose rows start on 16-byte boundaries and hold a
+ * share memory with an input or with each other (MG_ERR_INVALID; views of one buffer
+ * that lie between one another are fine), but `out` may be q itself, with the same
+ * strides. Tensors whose rows start on 16-byte boundaries and hold a
  * multiple of 8 elements run on the tensor cores, others on the CUDA cores. */
 typedef struct mg_attention_desc {
     int32_t dtype;                       /* mg_dtype of q, k, v, out and the gradients */
@@ -83,8 +85,8 @@ mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, 
  * inverse != 0 by the opposite angle (the gradient of the forward call). Pair p
  * is (2p, 2p + 1) if interleaved, else (p, p + pairs). The rest is copied.
  * The angle is reduced in 64-bit fixed point: exact for any int32 position.
- * Outputs may be the inputs themselves (same strides) but not overlap them
- * otherwise. */
+ * Outputs may be the inputs themselves (same strides) but not share memory with
+ * them, the other input or each other otherwise (MG_ERR_INVALID). */
 typedef struct mg_rotary_desc {
     int32_t dtype;
     int32_t batch, heads, kv_heads, len, head_dim, pairs;
@@ -110,7 +112,9 @@ mg_status mg_rotary(const mg_rotary_desc* d, void* out_q, void* out_k, const voi
  * keys that the table holds, from the last one's position, and the request
  * appends nothing. A page outside the pool is skipped (never read or written).
  * Both set MG_ERR_INVALID in mg_device_status(). Requests must not share the
- * page that they append to. */
+ * page that they append to, nor keys and values theirs; k_new and v_new may lie in
+ * the cache, but not where the call appends. Outputs must not share memory with an
+ * input or with each other, but `out` may be q itself, with the same strides. */
 typedef struct mg_paged_desc {
     int32_t dtype;
     int32_t batch, heads, kv_heads, head_dim, page_size, pages, table_width;

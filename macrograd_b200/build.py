@@ -25,9 +25,9 @@ UNITS = {
     "mg_attention.cu": ["mg_attention_host.h", "mg_attention_common.cuh", "mg_attention_math.cuh",
                         "mg_attention_simt.cuh", "mg_attention_tc.cuh",
                         "mg_attention_tc_bwd.cuh", "mg_attention_tc32.cuh", "mg_attention_tc32_bwd.cuh", "mg_tc16.cuh",
-                        "mg_ptx.cuh", "mg_host.h"],
+                        "mg_ptx.cuh", "mg_host.h", "mg_overlap.h"],
     "mg_paged.cu": ["mg_attention_host.h", "mg_attention_common.cuh", "mg_attention_math.cuh", "mg_paged.cuh",
-                    "mg_rotary.cuh", "mg_ptx.cuh", "mg_host.h"],
+                    "mg_rotary.cuh", "mg_ptx.cuh", "mg_host.h", "mg_overlap.h"],
 }
 SOURCES = [os.path.join(CSRC, u) for u in UNITS]
 HEADERS = [os.path.join(INCLUDE, h) for h in ("mg_gemm.h", "mg_attention.h")]

@@ -38,6 +38,44 @@ mg_status check_attention(const mg_attention_desc* d, const char* who)
     return MG_OK;
 }
 
+// Blocks store their results while others still read the inputs.
+mg_status check_places(const mg_attention_desc* d, const void* out, const float* lse, const void* q, const void* k,
+                       const void* v, const char* who)
+{
+    const auto arg = [&](const char* name, const void* at, const int64_t* s, int heads, int rows) {
+        return heads_arg(name, at, d->dtype, s, d->batch, heads, rows, d->head_dim);
+    };
+    const Arg o = arg("out", out, d->out_stride, d->heads, d->q_len), l = lse_arg(lse, (int64_t)d->batch * d->heads * d->q_len);
+    const Arg in[3] = {arg("q", q, d->q_stride, d->heads, d->q_len), arg("k", k, d->k_stride, d->kv_heads, d->k_len),
+                       arg("v", v, d->v_stride, d->kv_heads, d->k_len)};
+    for (int i = 0; i < 3; ++i) {
+        MG_TRY(apart(o, in[i], who, i == 0));       // a block of queries is read before its results take its place
+        MG_TRY(apart(l, in[i], who));
+    }
+    return apart(l, o, who);
+}
+
+// dQ is written before dK and dV are computed, in fp32 after them.
+mg_status check_gradient_places(const mg_attention_desc* d, const void* dq, const void* dk, const void* dv,
+                                const void* dout, const void* q, const void* k, const void* v, const void* out,
+                                const float* lse, const char* who)
+{
+    const auto arg = [&](const char* name, const void* at, const int64_t* s, bool key) {
+        return heads_arg(name, at, d->dtype, s, d->batch, key ? d->kv_heads : d->heads, key ? d->k_len : d->q_len,
+                         d->head_dim);
+    };
+    const Arg grad[3] = {arg("dq", dq, d->dq_stride, false), arg("dk", dk, d->dk_stride, true),
+                         arg("dv", dv, d->dv_stride, true)};
+    const Arg in[6] = {arg("q", q, d->q_stride, false),       arg("k", k, d->k_stride, true),
+                       arg("v", v, d->v_stride, true),        arg("dout", dout, d->dout_stride, false),
+                       arg("out", out, d->out_stride, false), lse_arg(lse, (int64_t)d->batch * d->heads * d->q_len)};
+    for (int i = 0; i < 3; ++i) {
+        for (const Arg& x : in) MG_TRY(apart(grad[i], x, who));
+        for (int j = i + 1; j < 3; ++j) MG_TRY(apart(grad[i], grad[j], who));
+    }
+    return MG_OK;
+}
+
 mg::AttnParams attention_params(const mg_attention_desc* d)
 {
     mg::AttnParams p = {};
@@ -411,6 +449,7 @@ mg_status mg_attention(const mg_attention_desc* d, void* out, float* lse, const 
     if (d->batch == 0 || d->q_len == 0) return MG_OK;
     if (!out || !lse || !q || (d->k_len > 0 && (!k || !v)))
         return fail(MG_ERR_INVALID, "mg_attention: a tensor is NULL");
+    MG_TRY(check_places(d, out, lse, q, k, v, "mg_attention"));
     Device dev;
     MG_TRY(mg::host::device(&dev));
     mg::AttnParams p = attention_params(d);
@@ -439,6 +478,7 @@ mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, 
     if (d->batch == 0 || (d->q_len == 0 && d->k_len == 0)) return MG_OK;
     if ((d->q_len > 0 && (!dq || !dout || !q || !out || !lse)) || (d->k_len > 0 && (!dk || !dv || !k || !v)))
         return fail(MG_ERR_INVALID, "mg_attention_backward: a tensor is NULL");
+    MG_TRY(check_gradient_places(d, dq, dk, dv, dout, q, k, v, out, lse, "mg_attention_backward"));
     Device dev;
     MG_TRY(mg::host::device(&dev));
     mg::AttnParams p = attention_params(d);

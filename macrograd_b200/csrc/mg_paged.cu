@@ -113,6 +113,45 @@ mg_status launch_rotary(mg::RotaryParams& p, const Device& dev, cudaStream_t st)
     return launched("mg_rotary");
 }
 
+// A thread reads its own elements before it writes them, and none of another's.
+mg_status check_rotary_places(const mg_rotary_desc* d, int kv_heads, const void* out_q, const void* out_k, const void* q,
+                              const void* k)
+{
+    const char* who = "mg_rotary";
+    const auto arg = [&](const char* name, const void* at, const int64_t* s, int heads) {
+        return heads_arg(name, at, d->dtype, s, d->batch, heads, d->len, d->head_dim);
+    };
+    const Arg oq = arg("out_q", out_q, d->out_q_stride, d->heads), ok = arg("out_k", out_k, d->out_k_stride, kv_heads);
+    const Arg iq = arg("q", q, d->q_stride, d->heads), ik = arg("k", k, d->k_stride, kv_heads);
+    MG_TRY(apart(oq, iq, who, true));
+    MG_TRY(apart(ok, ik, who, true));
+    MG_TRY(apart(oq, ik, who));
+    MG_TRY(apart(ok, iq, who));
+    return apart(oq, ok, who);
+}
+
+mg_status check_paged_places(const mg_paged_desc* d, const void* out, const float* lse, const void* q,
+                             const void* k_pages, const void* v_pages, const void* k_new, const void* v_new,
+                             const char* who)
+{
+    const auto pool = [&](const char* name, const void* at, const int64_t* s) {
+        return heads_arg(name, at, d->dtype, s, d->pages, d->page_size, d->kv_heads, d->head_dim);
+    };
+    const auto rows = [&](const char* name, const void* at, const int64_t* s, int heads) {
+        return rows_arg(name, at, d->dtype, s, at ? d->batch : 0, heads, d->head_dim);
+    };
+    const Arg o = rows("out", out, d->out_stride, d->heads), l = lse_arg(lse, (int64_t)d->batch * d->heads);
+    const Arg in[5] = {rows("q", q, d->q_stride, d->heads), pool("k_pages", k_pages, d->k_stride),
+                       pool("v_pages", v_pages, d->v_stride), rows("k_new", k_new, d->k_new_stride, d->kv_heads),
+                       rows("v_new", v_new, d->v_new_stride, d->kv_heads)};
+    for (int i = 0; i < 5; ++i) {
+        MG_TRY(apart(o, in[i], who, i == 0));
+        MG_TRY(apart(l, in[i], who));
+    }
+    MG_TRY(apart(l, o, who));
+    return k_new ? apart(in[1], in[2], who) : MG_OK;
+}
+
 }  // namespace
 
 namespace mg {
@@ -159,6 +198,7 @@ mg_status mg_rotary(const mg_rotary_desc* d, void* out_q, void* out_k, const voi
         return fail(MG_ERR_INVALID, "mg_rotary: a tensor is NULL");
     if (d->pairs > 0 && (!d->positions || !d->frequencies))
         return fail(MG_ERR_INVALID, "mg_rotary: positions and frequencies are needed");
+    MG_TRY(check_rotary_places(d, kvh, out_q, out_k, q, k));
     Device dev;
     MG_TRY(mg::host::device(&dev));
     mg::RotaryParams p = {};
@@ -217,6 +257,7 @@ mg_status mg_paged_attention(const mg_paged_desc* d, void* out, float* lse, cons
     if (longest >= (1ll << 30)) return fail(MG_ERR_UNSUPPORTED, "%s: the block table is too wide", who);
     if (!out || !lse || !q || !d->lengths || (longest > 0 && (!k_pages || !v_pages || !d->block_table)))
         return fail(MG_ERR_INVALID, "%s: a tensor is NULL", who);
+    MG_TRY(check_paged_places(d, out, lse, q, k_pages, v_pages, k_new, v_new, who));
     Device dev;
     MG_TRY(mg::host::device(&dev));
     mg::PagedParams p = {};

@@ -177,15 +177,15 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     [B]); with documents (int32 [B, Lk], the id of each position) only keys of its own document. Ids below 0 mark
     padding: such keys and queries are left out whatever they hold. A query that sees no key gives out = 0,
     lse = -inf. Everywhere else k, v must be finite also where a mask hides them from some queries. Scores and
-    biases are resolved up to 2^28 in size; a row with larger ones may come out as NaN. `out` must not share memory with
-    k or v.
+    biases are resolved up to 2^28 in size; a row with larger ones may come out as NaN. `out` may be q itself, but must not
+    share memory with q in another way, nor with k or v.
 
     Returns (out, laid out as q, lse [B, H, Lq] in float32)."""
     lib = _lib.load()
     dev, lead, ptrs = _attention_args(q, k, v, scale, causal, cap, slopes, documents, prefix)
     if out is not None:
         _written(out, "out", q)
-        for t, name in ((k, "k"), (v, "v")):
+        for t, name in ((k, "k"), (v, "v")):           # other overlaps are the library's to refuse
             if out.numel() and t.numel() and out.data_ptr() == t.data_ptr():
                 _bad(f"out and {name} are the same memory")
 
@@ -341,7 +341,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     as [pages, Hkv, page_size, D] is passed transposed); block_table int32 [B, width]: the pages of each request in
     order; lengths int32 [B]: its keys, the new token among them. The query stands at position lengths[b] - 1.
     With k_new and v_new [B, Hkv, D] the token's own key and value come from there, and the call also writes them to
-    the cache at that position; requests must not share the page they append to, nor keys and values theirs. A length
+    the cache at that position; requests must not share the page they append to, nor keys and values theirs, and k_new
+    and v_new must not lie there. `out` may be q itself, but shares memory with no input otherwise. A length
     of 0 gives out = 0, lse = -inf and writes nothing. A length beyond the table is cut off there (the call attends to
     the keys that the table holds, from the last one's position, and the request appends nothing), a page outside the
     pool is skipped, and mg_device_status() then reports MG_ERR_INVALID.

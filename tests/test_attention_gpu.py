@@ -622,3 +622,38 @@ def test_a_large_maximum_that_comes_late(top, heads, dtype):
     for d, want in ((0, late), (1, 1 - late)):
         error = float((out[..., d].double() - want).abs().max() / want)
         assert error <= tol, error
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("size", [(1, 3, 3, 150, 150, 64), (1, 2, 2, 140, 1500, 128), (2, 2, 2, 70, 70, 33),
+                                  (1, 4, 4, 1, 600, 64)], ids=str)
+def test_out_in_the_place_of_q(size, dtype):
+    """Inside a packed projection too, whose keys and values lie between its queries."""
+    B, H, _, Lq, Lk, D = size
+    q, k, v, _, kw = make(size, "causal", dtype, 60)
+    want = mg.attention(q, k, v, **kw)
+    got = mg.attention(q, k, v, out=q, **kw)
+    assert got[0] is q and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    if Lq != Lk:
+        return
+    qkv = torch.randn((B, Lq, 3, H, D), device="cuda").to(dtype)
+    q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
+    kept = qkv.clone()
+    want = mg.attention(q, k, v, **kw)
+    got = mg.attention(q, k, v, out=q, **kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(qkv[:, :, 1:], kept[:, :, 1:])
+
+
+def test_out_that_overlaps_an_input_is_refused():
+    """Where the views start elsewhere, or are laid out in another way."""
+    qkv = torch.randn((2, 8, 3, 4, 64), device="cuda")
+    q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
+    flat = qkv.flatten(2)
+    for out, name in [(flat[:, :, 320:576].unflatten(2, (4, 64)).transpose(1, 2), "k"),
+                      (flat[:, :, 500:756].unflatten(2, (4, 64)).transpose(1, 2), "k"),
+                      (flat[:, :, 512 + 64:].unflatten(2, (3, 64)).transpose(1, 2), "v"),
+                      (flat[:, :, 64:256].unflatten(2, (3, 64)).transpose(1, 2), "q"),
+                      (qkv.flatten()[:2 * 4 * 8 * 64].view(2, 4, 8, 64), "q")]:
+        n = out.shape[1]
+        with pytest.raises(mg.MacrogradError, match=f"out overlaps {name}"):
+            mg.attention(q[:, :n], k[:, :n], v[:, :n], out=out)

@@ -332,3 +332,17 @@ def test_chunks_with_large_scores(keys, top, dtype):
         error = float((out[..., d].double() - want).abs().max() / want)
         assert error <= tol, error
     assert abs(float(lse[0, 0]) - (top * scale + math.log(keys / 2 / first))) <= 2 * 2.0 ** -24 * top
+
+
+def test_pools_and_outputs_that_overlap_are_refused():
+    q, kp, vp, table, lengths, kn, vn = make(2, 4, 2, 64, 16, [100, 33], torch.bfloat16)
+    room = torch.zeros((*kp.shape[:3], 128), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(mg.MacrogradError, match="k_pages overlaps v_pages"):
+        mg.paged_attention(q, room[..., :64], room[..., 32:96], table, lengths, k_new=kn, v_new=vn)
+    compare((q, room[..., :64], room[..., 32:96], table, lengths, None, None))          # read alone
+    compare((q, room[..., :64], room[..., 64:], table, lengths, kn, vn))
+    with pytest.raises(mg.MacrogradError, match="out overlaps v_pages"):
+        mg.paged_attention(q, kp, vp, table, lengths, out=vp[3, 4:8, :, :].flatten()[:512].view(2, 4, 64))
+    want = mg.paged_attention(q, kp, vp, table, lengths)
+    got = mg.paged_attention(q, kp, vp, table, lengths, out=q)
+    assert got[0] is q and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -152,3 +152,15 @@ def test_refusals():
             (lambda: mg.rotary_frequencies(8, theta=-1.0), "positive")]:
         with pytest.raises(mg.MacrogradError, match=fragment):
             call()
+
+
+def test_outputs_that_overlap_the_inputs_otherwise_are_refused():
+    buf = torch.randn((2, 40, 3, 4, 64), device="cuda")
+    q, k = buf[:, :, 0].transpose(1, 2), buf[:, :, 1].transpose(1, 2)
+    pos, f = torch.arange(40, device="cuda").int(), mg.rotary_frequencies(64)
+    flat = buf.flatten(2)
+    between = flat[:, :, 64:320].unflatten(2, (4, 64)).transpose(1, 2)          # queries 1 to 3 and the first key
+    for kw, fragment in [(dict(out_q=between), "out_q overlaps q"), (dict(out_k=between), "out_k overlaps k"),
+                         (dict(out_q=flat[:, :, 320:576].unflatten(2, (4, 64)).transpose(1, 2)), "out_q overlaps k")]:
+        with pytest.raises(mg.MacrogradError, match=fragment):
+            mg.rotary(q, k, pos, f, **kw)
