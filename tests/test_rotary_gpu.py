@@ -164,3 +164,16 @@ def test_outputs_that_overlap_the_inputs_otherwise_are_refused():
                          (dict(out_q=flat[:, :, 320:576].unflatten(2, (4, 64)).transpose(1, 2)), "out_q overlaps k")]:
         with pytest.raises(mg.MacrogradError, match=fragment):
             mg.rotary(q, k, pos, f, **kw)
+
+
+def test_one_token_in_place_through_another_view():
+    """The stride of a dim of one element says nothing: a token's heads viewed in two ways are the same elements."""
+    x = torch.randn((3, 4, 64), device="cuda")
+    a, b = x.view(3, 1, 4, 64).transpose(1, 2), x.view(3, 4, 1, 64)
+    assert a.stride() != b.stride()
+    pos, f = torch.tensor([[5], [6], [1000]], dtype=torch.int32, device="cuda"), mg.rotary_frequencies(64)
+    want, _ = mg.rotary(a, None, pos, f)
+    got, _ = mg.rotary(a, None, pos, f, out_q=b)
+    assert got is b and torch.equal(x.view(3, 4, 1, 64), want)
+    with pytest.raises(mg.MacrogradError, match="out_q overlaps q"):
+        mg.rotary(x.view(1, 3, 4, 64), None, pos.new_zeros((4,)), f, out_q=x.view(1, 4, 3, 64).transpose(1, 2))
