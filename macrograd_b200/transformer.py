@@ -21,7 +21,9 @@ as the tensor they belong to (heads split from [batch, length, heads * head_dim]
 come back ready to be merged). Sums, softmax statistics and angles are kept in
 32 bits or more whatever the type. Calls run on `stream` (default: the current
 one) and can be captured into graphs (but for the library's first call on a
-device); nothing is kept from one call for the next.
+device); nothing is kept from one call for the next. A `stream` that is given has
+to be ordered behind whatever writes the operands, as by stream.wait_stream(), and
+what comes back belongs to it; the operands may be let go right after the call.
 """
 from __future__ import annotations
 
@@ -107,9 +109,10 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 _device = torch.cuda.current_device
 
 
-def _on(device: torch.device, stream: Optional[torch.cuda.Stream], call):
+def _on(device: torch.device, stream: Optional[torch.cuda.Stream], call, *used: Optional[torch.Tensor]):
     """call(stream handle) on `stream` (its device current, its allocations the stream's own), by default on the
-    current stream of the operands' device."""
+    current stream of the operands' device. The memory of the tensors `used` is not given to others before a `stream`
+    that is given is done with them."""
     if stream is None:
         if _device() == device.index:
             return call(_raw_stream(device.index))
@@ -118,7 +121,11 @@ def _on(device: torch.device, stream: Optional[torch.cuda.Stream], call):
     if torch.device(stream.device) != device:
         _bad(f"operands (and stream) are on different devices: {device}, {stream.device}")
     with torch.cuda.stream(stream):
-        return call(stream.cuda_stream)
+        results = call(stream.cuda_stream)
+    for t in used:
+        if t is not None:
+            t.record_stream(stream)
+    return results
 
 
 def _cap(cap: float) -> float:
@@ -198,7 +205,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
         check(lib.mg_attention(desc, o.data_ptr(), lse.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), st))
         return o, lse
 
-    return _on(dev, stream, call)
+    return _on(dev, stream, call, q, k, v, slopes, documents, prefix, out)
 
 
 def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
@@ -226,7 +233,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                                         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), st))
         return dq, dk, dv
 
-    return _on(dev, stream, call)
+    return _on(dev, stream, call, dout, q, k, v, out, lse, slopes, documents, prefix)
 
 
 # ------------------------------------------------------------------ rotary positions
@@ -302,7 +309,7 @@ def _rotary(q, k, positions, frequencies, interleaved, inverse, magnitude, out_q
         check(lib.mg_rotary(desc, oq.data_ptr(), _at(ok), q.data_ptr(), _at(k), st))
         return oq, ok
 
-    return _on(dev, stream, call)
+    return _on(dev, stream, call, q, k, positions, frequencies, out_q, out_k)
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor,
@@ -395,4 +402,4 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                                      v_pages.data_ptr(), _at(k_new), _at(v_new), st))
         return o, lse
 
-    return _on(dev, stream, call)
+    return _on(dev, stream, call, q, k_pages, v_pages, block_table, lengths, slopes, k_new, v_new, out)

@@ -657,3 +657,62 @@ def test_out_that_overlaps_an_input_is_refused():
         n = out.shape[1]
         with pytest.raises(mg.MacrogradError, match=f"out overlaps {name}"):
             mg.attention(q[:, :n], k[:, :n], v[:, :n], out=out)
+
+
+@pytest.mark.parametrize("op", ["attention", "attention_backward", "rotary", "rotary_backward", "paged_attention"])
+def test_operands_let_go_after_a_call_on_another_stream(op):
+    """Their memory is not given away while the other stream may still be reading it."""
+    dev, dt = "cuda", torch.bfloat16
+    heads = lambda n: torch.randn((1, n, 96, 64), device=dev, dtype=dt)  # noqa: E731
+    if op.startswith("attention"):
+        used = dict(q=heads(4), k=heads(2), v=heads(2), slopes=torch.rand(4, device=dev),
+                    documents=torch.zeros((1, 96), dtype=torch.int32, device=dev))
+        if op == "attention_backward":
+            out, lse = mg.attention(**used)
+            used.update(out=out, lse=lse, dout=heads(4))
+            del out, lse
+        else:
+            used["out"] = heads(4)
+    elif op.startswith("rotary"):
+        names = ("dq", "dk") if op == "rotary_backward" else ("q", "k")
+        used = {names[0]: heads(4), names[1]: heads(2), "positions": torch.arange(96, device=dev).int(),
+                "frequencies": mg.rotary_frequencies(64)}
+    else:
+        used = dict(q=heads(4)[:, :, 0], k_pages=torch.randn((6, 16, 2, 64), device=dev, dtype=dt),
+                    v_pages=torch.randn((6, 16, 2, 64), device=dev, dtype=dt),
+                    block_table=torch.arange(6, device=dev).int()[None].contiguous(),
+                    lengths=torch.tensor([90], device=dev).int(), k_new=heads(2)[:, :, 0], v_new=heads(2)[:, :, 0])
+    getattr(mg, op)(**used)                  # loads what the call needs, which may wait for the device
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(400_000_000)       # about a fifth of a second
+    results = getattr(mg, op)(stream=stream, **used)
+    held = {n: (t.untyped_storage().data_ptr(), t.untyped_storage().nbytes()) for n, t in used.items()}
+    used.clear()
+    fresh = [torch.empty(size, dtype=torch.uint8, device=dev) for _, size in held.values() for _ in range(3)]
+    assert not stream.query(), "the stream was done too early for the test to tell"
+    places = {t.untyped_storage().data_ptr() for t in fresh}
+    assert not [n for n, (at, _) in held.items() if at in places]
+    torch.cuda.synchronize()
+    assert all(torch.isfinite(t).all() for t in results)
+
+
+def test_captured_on_another_stream_than_the_graphs():
+    """A call on a stream that is forked from the captured one and joined to it, with operands of the graph's own."""
+    q, k, v, dout, kw = make((1, 4, 2, 200, 200, 64), "all", torch.bfloat16, 61)
+    want = mg.attention(q, k, v, **kw)
+    want = want + mg.attention_backward(dout, q, k, v, *want, **kw)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        own = q.clone()
+        side.wait_stream(torch.cuda.current_stream())
+        got = mg.attention(own, k, v, stream=side, **kw)
+        got = got + mg.attention_backward(dout, own, k, v, *got, stream=side, **kw)
+        del own
+        torch.cuda.current_stream().wait_stream(side)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
