@@ -64,18 +64,13 @@ __device__ __forceinline__ bool sees(const AttnParams& p, int qpos, int qdoc, in
     return (!p.causal || j <= qpos || j < prefix) && (p.docs == nullptr || (qdoc >= 0 && qdoc == kdoc));
 }
 
-// tanh(x) = 1 - 2 / (1 + exp(2x)), from both ends right for any x; the
-// absolute error is that of one fp32 rounding near 1, which is what a score
-// of up to `cap` can hold anyway. Used by the 32-bit kernels.
-__device__ __forceinline__ float tanh_full(float x) { return tanhf(x); }
-
 // The score of one pair from the scaled product t: capped and biased. `bend`
 // receives tanh(t / cap) (0 without a cap).
 __device__ __forceinline__ float score(float t, float cap, float slope, int dist, float& bend)
 {
     bend = 0.f;
     if (cap > 0.f) {
-        bend = tanh_full(t / cap);
+        bend = tanhf(t / cap);
         t = cap * bend;
     }
     return t - slope * (float)(dist < 0 ? -dist : dist);

@@ -122,10 +122,10 @@ __device__ __forceinline__ void same_document(int mine, const int (&theirs)[W], 
 
 // ---------------------------------------------------------------- parameters
 struct TcAttnParams {
-    CUtensorMap q, k, v, dout;   // {D, rows, heads, batch}, boxes of 64 x 128 rows
+    CUtensorMap q, k, v;         // {D, rows, heads, batch}, boxes of 64 x 128 rows
     AttnParams a;
     const int2* doc_tiles;       // [B][ceil(Lk / 128)], with documents
-    int head_step[4], batch_step[4];   // of q, k, v, dout: 0 where the dim is broadcast (stride 0)
+    int head_step[3], batch_step[3];   // of q, k, v: 0 where the dim is broadcast (stride 0)
     uint32_t idesc_s;            // of S = Q K^T: A negated where the scale is negative
     float scale;                 // |scale|
     CapCurve curve;

@@ -70,10 +70,10 @@ __device__ __forceinline__ void tc32_put(uint32_t tile, int rows, uint32_t piece
 
 // As cap_scores, at fp32 accuracy for every size of score.
 template <int N>
-__device__ __forceinline__ void cap_scores32(float (&s)[N], float pre, float cap2)
+__device__ __forceinline__ void cap_scores32(float (&s)[N], float pre)
 {
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = cap2 * tanh_fast(s[i] * pre);
+    for (int i = 0; i < N; ++i) s[i] = tanh_fast(s[i] * pre);
 }
 
 struct Tc32Params {
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kTc32Threads, DP == 64 ? 2 : 1) attn_tc32_forw
             // columns [c0, c0 + 16): the powers of two less `base`, -inf where masked
             const auto powers = [&](int c0, float base, float (&s)[16]) {
                 tmem_ld_x16(tS + c0, s);
-                if (kCap) cap_scores32(s, pre, 1.f);
+                if (kCap) cap_scores32(s, pre);
 #pragma unroll
                 for (int c = 0; c < 16; c += 2) {
                     float b0 = -base, b1 = -base;

@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                 tc_fence_after();
                 add_up();
             }
-            if (kCap) cap_scores32(v, pre, 1.f);
+            if (kCap) cap_scores32(v, pre);
             const float far = (float)(pos - ypos - col);
             const uint64_t mul_2 = pack2(mul, mul);
 #pragma unroll
