@@ -74,22 +74,30 @@ inline bool aligned(const void* ptr, const int64_t* strides, int n, size_t elem,
 struct Arg {
     const char* name;
     View view;
+    Span span;
 };
 
 inline Arg heads_arg(const char* name, const void* at, int dtype, const int64_t* stride, int64_t n0, int64_t n1, int64_t n2,
                      int head_dim)
 {
-    return {name, {at, (int)elem_size(dtype), {n0, n1, n2, head_dim}, {stride[0], stride[1], stride[2], 1}}};
+    const View v = {at, (int)elem_size(dtype), {n0, n1, n2, head_dim}, {stride[0], stride[1], stride[2], 1}};
+    return {name, v, span_of(v)};
 }
 inline Arg rows_arg(const char* name, const void* at, int dtype, const int64_t* stride, int64_t n0, int64_t n1, int head_dim)
 {
-    return {name, {at, (int)elem_size(dtype), {n0, n1, 1, head_dim}, {stride[0], stride[1], 0, 1}}};
+    const View v = {at, (int)elem_size(dtype), {n0, n1, 1, head_dim}, {stride[0], stride[1], 0, 1}};
+    return {name, v, span_of(v)};
 }
-inline Arg lse_arg(const void* at, int64_t n) { return {"lse", {at, 4, {n, 1, 1, 1}, {1, 0, 0, 0}}}; }
+inline Arg lse_arg(const void* at, int64_t n)
+{
+    const View v = {at, 4, {n, 1, 1, 1}, {1, 0, 0, 0}};
+    return {"lse", v, span_of(v)};
+}
 
 // Refuses an output that shares memory with `other`; `itself`: it may be the same elements in the same places.
 inline mg_status apart(const Arg& out, const Arg& other, const char* who, bool itself = false)
 {
+    if (out.span.lo >= other.span.hi || other.span.lo >= out.span.hi) return MG_OK;
     if (!views_meet(out.view, other.view) || (itself && same_view(out.view, other.view))) return MG_OK;
     return fail(MG_ERR_INVALID, "%s: %s overlaps %s", who, out.name, other.name);
 }

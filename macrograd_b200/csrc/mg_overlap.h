@@ -45,6 +45,22 @@ inline bool within(Terms& t, int k, wide lo, wide hi)
 
 }  // namespace overlap
 
+// The bytes [lo, hi) that a view spans; none where it has no element.
+struct Span {
+    overlap::wide lo, hi;
+};
+
+inline Span span_of(const View& v)
+{
+    Span s = {(overlap::wide)(intptr_t)v.at, (overlap::wide)(intptr_t)v.at + v.elem};
+    for (int i = 0; i < 4; ++i) {
+        if (v.n[i] <= 0) return {0, 0};
+        const overlap::wide far = (overlap::wide)v.stride[i] * v.elem * (v.n[i] - 1);
+        (far < 0 ? s.lo : s.hi) += far;
+    }
+    return s;
+}
+
 inline bool views_meet(const View& a, const View& b)
 {
     using overlap::wide;

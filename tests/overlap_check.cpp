@@ -49,6 +49,11 @@ int main()
         bool want = false;
         for (int64_t x : a) want = want || b.count(x);
         met += want;
+        const mg::Span s = mg::span_of(v[0]);
+        if (!a.empty() && (s.lo != *a.begin() || s.hi != *a.rbegin() + 1)) {
+            std::printf("FAIL span, round %d\n", round);
+            return 1;
+        }
         if (mg::views_meet(v[0], v[1]) != want || mg::views_meet(v[1], v[0]) != want) {
             std::printf("FAIL round %d, want %d\n", round, want);
             return 1;
