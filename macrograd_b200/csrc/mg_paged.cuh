@@ -369,11 +369,8 @@ struct PagedAcc {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = 8 * n + 2 * t + (i & 1);
-                float x = s[n][i] * mul;
-                x = fmaf(-slope[i >> 1], (float)(back - key), x);
-                x = (seen >> key) & 1 ? x : -CUDART_INF_F;
-                s[n][i] = x;
-                top[i >> 1] = fmaxf(top[i >> 1], x);
+                const float x = fmaf(s[n][i], mul, -slope[i >> 1] * (float)(back - key));
+                top[i >> 1] = fmaxf(top[i >> 1], (seen >> key) & 1 ? x : -CUDART_INF_F);
             }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -395,8 +392,15 @@ struct PagedAcc {
         uint32_t a[4];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const float e0 = ex2(s[n][0] - b0), e1 = ex2(s[n][1] - b0);
-            const float e2 = ex2(s[n][2] - b1), e3 = ex2(s[n][3] - b1);
+            // score and maximum in one rounding: the scores' own, 2^-24 of their size, would stay in the weights
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = 8 * n + 2 * t + (i & 1);
+                const float x = fmaf(s[n][i], mul, fmaf(-slope[i >> 1], (float)(back - key), i < 2 ? -b0 : -b1));
+                e[i] = ex2((seen >> key) & 1 ? x : -CUDART_INF_F);
+            }
+            const float e0 = e[0], e1 = e[1], e2 = e[2], e3 = e[3];
             l[0] += e0 + e1;
             l[1] += e2 + e3;
             const __nv_bfloat162 x = __floats2bfloat162_rn(e0, e1), y = __floats2bfloat162_rn(e2, e3);
@@ -470,15 +474,14 @@ struct PagedAcc<float, DP> {
                 s[g] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[g]))));
             }
         }
-        const float mul = p.scale * kLog2e;
+        const float mul = (p.cap > 0.f ? p.cap : p.scale) * kLog2e, far = (float)(back - key);
+        const bool in = (seen >> key) & 1;
 #pragma unroll
         for (int g = 0; g < kPagedHeads; ++g) {
             if (g >= nh) break;
             float x = s[g] + __shfl_xor_sync(~0u, s[g], 16);
-            x = p.cap > 0.f ? p.cap * kLog2e * tanhf(x * p.scale / p.cap) : x * mul;
-            x = fmaf(-slope[g], (float)(back - key), x);
-            x = (seen >> key) & 1 ? x : -CUDART_INF_F;
-            float top = x;
+            if (p.cap > 0.f) x = tanhf(x * p.scale / p.cap);
+            float top = in ? fmaf(x, mul, -slope[g] * far) : -CUDART_INF_F;
 #pragma unroll
             for (int w = 8; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
             if (m[g] == -CUDART_INF_F ? top > m[g] : top - m[g] > 8.f) {     // the same for the whole warp
@@ -488,7 +491,8 @@ struct PagedAcc<float, DP> {
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) o[g][i].x *= f, o[g][i].y *= f, o[g][i].z *= f, o[g][i].w *= f;
             }
-            s[g] = ex2(x - (m[g] == -CUDART_INF_F ? 0.f : m[g]));
+            // score and maximum in one rounding
+            s[g] = ex2(in ? fmaf(x, mul, fmaf(-slope[g], far, m[g] == -CUDART_INF_F ? 0.f : -m[g])) : -CUDART_INF_F);
             l[g] += half ? 0.f : s[g];
         }
 #pragma unroll

@@ -346,3 +346,30 @@ def test_pools_and_outputs_that_overlap_are_refused():
     want = mg.paged_attention(q, kp, vp, table, lengths)
     got = mg.paged_attention(q, kp, vp, table, lengths, out=q)
     assert got[0] is q and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("top", [2 ** 16, 2 ** 18 + 3, 2 ** 20 + 3, 2 ** 20 + 11])
+@pytest.mark.parametrize("keys", [64, 512, 16384], ids=["one block", "a cluster", "two launches"])
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.75])
+def test_scores_are_not_rounded_before_the_maximum_is_off_them(scale, keys, top, dtype):
+    """As above with scales that leave no score a whole number of powers of two; the two kinds of keys alternate, and a
+    single query over a contiguous row is the same call. Bound as above."""
+    D = 64
+    q = torch.zeros((1, 2, D), device="cuda", dtype=dtype)
+    kp, vp = (torch.zeros((keys // 16, 16, 1, D), device="cuda", dtype=dtype) for _ in range(2))
+    hi = float(torch.tensor(float(top)).bfloat16())
+    q[..., :3] = 1 if scale > 0 else -1
+    kp[..., 0], kp[..., 1] = hi, top - hi
+    kp[:, 1::2, :, 2] = -0.25
+    vp[:, 0::2, :, 0], vp[:, 1::2, :, 1] = 1, 1
+    table = torch.arange(keys // 16, device="cuda").int()[None].contiguous()
+    out, _ = mg.paged_attention(q, kp, vp, table, torch.tensor([keys], dtype=torch.int32, device="cuda"), scale=scale)
+    first = 1 / (1 + math.exp(-0.25 * abs(scale)))
+    tol = 700 * 2.0 ** -24 + (2 * half_step(dtype) if dtype == torch.bfloat16 else 0.0)
+    k, v = (x.view(1, keys, 1, D).transpose(1, 2) for x in (kp, vp))
+    row, _ = mg.attention(q[:, :, None], k, v, scale=scale)
+    for got in (out, row[:, :, 0]):
+        for d, want in ((0, first), (1, 1 - first)):
+            error = float((got[..., d].double() - want).abs().max() / want)
+            assert error <= tol, error
