@@ -55,7 +55,7 @@ mg_status check_places(const mg_attention_desc* d, const void* out, const float*
     return apart(l, o, who);
 }
 
-// dQ is written before dK and dV are computed, in fp32 after them.
+// dQ is written before dK and dV are computed.
 mg_status check_gradient_places(const mg_attention_desc* d, const void* dq, const void* dk, const void* dv,
                                 const void* dout, const void* q, const void* k, const void* v, const void* out,
                                 const float* lse, const char* who)
@@ -258,11 +258,11 @@ mg_status share_gradient(mg::GradParts* g, int64_t blocks, int64_t steps, int ti
     *g = {};
     g->parts = (int)std::max<int64_t>(1, std::min<int64_t>(dev.sm_count / blocks, ceil_div(steps * tile, least)));
     if (g->parts == 1) return MG_OK;
-    const int64_t each = g->parts * rows * D, all = each * (second ? 2 : 1) + (sums ? g->parts * rows : 0);
+    const int64_t each = g->parts * rows * D, accs = each * (second ? 2 : 1), all = accs + (sums ? g->parts * rows : 0);
     g->acc = static_cast<float*>(ws.get(all * sizeof(float)));
     if (!g->acc) return fail(MG_ERR_ALLOC, "mg_attention_backward: no scratch for %d parts of each sum", g->parts);
     if (second) g->other = g->acc + each;
-    if (sums) g->r = g->acc + 2 * each;
+    if (sums) g->r = g->acc + accs;
     return MG_OK;
 }
 
@@ -271,7 +271,7 @@ mg_status share_dq(mg::GradParts* g, const mg::AttnParams& p, int tile, int leas
                    Scratch& ws)
 {
     return share_gradient(g, (int64_t)ceil_div(p.Lq, 128) * p.B * p.H, ceil_div(p.Lk, tile), tile, least,
-                          (int64_t)p.B * p.H * p.Lq, p.D, correct, correct, dev, ws);
+                          (int64_t)p.B * p.H * p.Lq, p.D, correct, true, dev, ws);
 }
 mg_status share_dkv(mg::GradParts* g, const mg::AttnParams& p, int tile, int least, const Device& dev, Scratch& ws)
 {
@@ -279,23 +279,23 @@ mg_status share_dkv(mg::GradParts* g, const mg::AttnParams& p, int tile, int lea
                           tile, least, (int64_t)p.B * p.Hkv * p.Lk, p.D, true, false, dev, ws);
 }
 
-template <typename T, bool kCorrect>
-mg_status join_dq(const mg::GradParts& g, const mg::AttnParams& p, float* delta, int Lp, cudaStream_t st)
+template <typename T, int kForm>
+mg_status join_dq(const mg::GradParts& g, const mg::AttnParams& p, float* delta, float* fine, int Lp, cudaStream_t st)
 {
     if (g.parts == 1) return MG_OK;
-    mg::GradJoin j = {g, p.H, p.Lq, p.D, Lp, (int64_t)p.B * p.H * p.Lq, {p.dq, nullptr}, {}, delta};
+    mg::GradJoin j = {g, p.H, p.Lq, p.D, Lp, (int64_t)p.B * p.H * p.Lq, {p.dq, nullptr}, {}, delta, fine};
     std::copy(p.dqs, p.dqs + 3, j.os[0]);
-    mg::attn_grad_join_kernel<T, kCorrect><<<ceil_div(j.rows, 8), 256, 0, st>>>(j);
+    mg::attn_grad_join_kernel<T, kForm><<<ceil_div(j.rows, 8), 256, 0, st>>>(j);
     return launched("mg_attention_backward");
 }
 template <typename T>
 mg_status join_dkv(const mg::GradParts& g, const mg::AttnParams& p, cudaStream_t st)
 {
     if (g.parts == 1) return MG_OK;
-    mg::GradJoin j = {g, p.Hkv, p.Lk, p.D, 0, (int64_t)p.B * p.Hkv * p.Lk, {p.dk, p.dv}, {}, nullptr};
+    mg::GradJoin j = {g, p.Hkv, p.Lk, p.D, 0, (int64_t)p.B * p.Hkv * p.Lk, {p.dk, p.dv}, {}, nullptr, nullptr};
     std::copy(p.dks, p.dks + 3, j.os[0]);
     std::copy(p.dvs, p.dvs + 3, j.os[1]);
-    mg::attn_grad_join_kernel<T, false><<<dim3(ceil_div(j.rows, 8), 2), 256, 0, st>>>(j);
+    mg::attn_grad_join_kernel<T, mg::kJoinPlain><<<dim3(ceil_div(j.rows, 8), 2), 256, 0, st>>>(j);
     return launched("mg_attention_backward");
 }
 
@@ -346,7 +346,7 @@ mg_status backward_tc(const mg::AttnParams& p, const Device& dev, void* stream)
     MG_TRY(tc_map(&t.y1, &hs[2], &bs[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 64));
     MG_TRY(share_dq(&t.parts, p, 64, 256, true, dev, ws));
     MG_TRY((p.D <= 64 ? launch_tc_backward<64, false>(t, dev, st) : launch_tc_backward<128, false>(t, dev, st)));
-    MG_TRY((join_dq<__nv_bfloat16, true>(t.parts, p, t.delta, t.Lp, st)));
+    MG_TRY((join_dq<__nv_bfloat16, mg::kJoinCorrect>(t.parts, p, t.delta, nullptr, t.Lp, st)));
     // the keys resident: dK, dV
     MG_TRY(tc_map(&t.x0, &hs[1], &bs[1], p.k, p.ks, p.D, p.Lk, p.Hkv, p.B, 128));
     MG_TRY(tc_map(&t.x1, &hs[2], &bs[2], p.v, p.vs, p.D, p.Lk, p.Hkv, p.B, 128));
@@ -416,13 +416,18 @@ mg_status backward_tc32(const mg::AttnParams& p, const Device& dev, void* stream
     MG_TRY(tc_params(&f, p, dev, ws, st, who));
     const int Lp = ceil_div(p.Lq, 128) * 128;
     const int64_t rows = (int64_t)p.B * p.H * Lp;
-    float* stats = static_cast<float*>(ws.get(2 * rows * sizeof(float)));
+    float* stats = static_cast<float*>(ws.get(3 * rows * sizeof(float)));
     if (!stats) return fail(MG_ERR_ALLOC, "%s: no scratch for the row sums", who);
     mg::attn_tc_stats_kernel<float><<<ceil_div(rows, 16 * mg::kStatsRows), 256, 0, st>>>(p, Lp, stats, stats + rows);
     MG_TRY(launched(who));
-    mg::Tc32BwdParams t = {p, f.doc_tiles, stats, stats + rows, Lp, 0, f.scale, f.status};
+    mg::Tc32BwdParams t = {p, f.doc_tiles, stats, stats + rows, stats + 2 * rows, Lp, 0, f.scale, f.status};
     t.idesc_s = mg::idesc_bf16(128, p.D <= 64 ? 64 : 32, false, false, p.scale < 0.f);
     const int tile = p.D <= 64 ? 64 : 32;
+    // dQ, and what the rows' lse are short of
+    MG_TRY(share_dq(&t.parts, p, tile, 128, false, dev, ws));
+    MG_TRY((p.D <= 64 ? launch_tc32_backward<64, false, mg::kTakeDs>(t, dev, st)
+                      : launch_tc32_backward<128, false, mg::kTakeDs>(t, dev, st)));
+    MG_TRY((join_dq<float, mg::kJoinWeights>(t.parts, p, nullptr, t.fine, Lp, st)));
     MG_TRY(share_dkv(&t.parts, p, tile, 128, dev, ws));
     if (p.D <= 64) {
         MG_TRY((launch_tc32_backward<64, true, mg::kTakeBoth>(t, dev, st)));
@@ -430,11 +435,7 @@ mg_status backward_tc32(const mg::AttnParams& p, const Device& dev, void* stream
         MG_TRY((launch_tc32_backward<128, true, mg::kTakeDs>(t, dev, st)));
         MG_TRY((launch_tc32_backward<128, true, mg::kTakeP>(t, dev, st)));
     }
-    MG_TRY(join_dkv<float>(t.parts, p, st));
-    MG_TRY(share_dq(&t.parts, p, tile, 128, false, dev, ws));
-    MG_TRY((p.D <= 64 ? launch_tc32_backward<64, false, mg::kTakeDs>(t, dev, st)
-                      : launch_tc32_backward<128, false, mg::kTakeDs>(t, dev, st)));
-    return join_dq<float, false>(t.parts, p, nullptr, 0, st);
+    return join_dkv<float>(t.parts, p, st);
 }
 
 }  // namespace
@@ -488,8 +489,10 @@ mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, 
         return d->dtype == MG_BF16 ? backward_tc(p, dev, stream) : backward_tc32(p, dev, stream);
     Scratch ws(dev, stream);
     if (d->q_len > 0) {
-        p.delta = static_cast<float*>(ws.get(sizeof(float) * d->batch * d->heads * (size_t)d->q_len));
+        const size_t rows = d->batch * d->heads * (size_t)d->q_len;
+        p.delta = static_cast<float*>(ws.get(2 * rows * sizeof(float)));
         if (!p.delta) return fail(MG_ERR_ALLOC, "mg_attention_backward: no scratch for the row sums");
+        p.fine = p.delta + rows;
     }
     cudaStream_t st = (cudaStream_t)stream;
     return d->dtype == MG_F32 ? backward_simt<float>(p, dev, st) : backward_simt<__nv_bfloat16>(p, dev, st);

@@ -22,6 +22,7 @@ struct AttnParams {
     void *out, *dq, *dk, *dv;
     float* lse;
     float* delta;
+    float* fine;                                 // log of each row's sum of exp(s - lse): what lse is short of
 };
 
 // A row of keys shared by several blocks of the forward kernels, where there are
@@ -38,7 +39,7 @@ struct GradParts {
     int parts;           // 1: the block writes the gradient itself
     float* acc;          // [parts][B * heads][rows][D] of dQ, or of dK
     float* other;        // as acc: of the correction's product (dQ of 16-bit tensors), or of dV
-    float* r;            // [parts][B * H][Lq] the rows' sums (dQ of 16-bit tensors)
+    float* r;            // [parts][B * H][Lq] the rows' sums (dQ): of P * (dP - delta) of 16-bit tensors, of P of fp32
 };
 
 __device__ __forceinline__ float to_f32(float x) { return x; }

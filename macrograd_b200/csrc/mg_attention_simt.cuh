@@ -156,15 +156,15 @@ __global__ void attn_delta_kernel(const __grid_constant__ AttnParams p)
     if (threadIdx.x % 32 == 0) p.delta[row] = s;
 }
 
-// P, P * curve and dS of pair (query, key) from the two products.
-__device__ __forceinline__ void simt_grad(const AttnParams& p, bool seen, float qk, float dov, float lse, float delta,
-                                          float slope, int dist, float& P, float& PC, float& dS)
+// P, P * curve and dS of pair (query, key) from the two products. fine: what lse is short of (dQ's kernel finds it).
+__device__ __forceinline__ void simt_grad(const AttnParams& p, bool seen, float qk, float dov, float lse, float fine,
+                                          float delta, float slope, int dist, float& P, float& PC, float& dS)
 {
     P = PC = dS = 0.f;
     if (!seen) return;
     float bend;
     const float s = score(p.scale * qk, p.cap, slope, dist, bend);
-    P = expf(s - lse);
+    P = expf((s - lse) - fine);
     PC = P * (1.f - bend * bend);
     dS = P * (dov - delta) * (1.f - bend * bend) * p.scale;
 }
@@ -172,7 +172,8 @@ __device__ __forceinline__ void simt_grad(const AttnParams& p, bool seen, float 
 // dQ. With 16-bit tensors delta carries the rounding of out, which is as large as dP - delta where the
 // values of a row have much in common. The true delta makes the row's sum of P * (dP - delta) zero, so
 // what that sum is is delta's error r: dQ loses r times sum P curve k, and delta becomes exact for dK,
-// which is computed after it. Without, gradients of values that differ in their last bit alone are off by
+// which is computed after it. The row's sum of P, 1 but for the rounding of the fp32 lse, divides dQ, and its
+// logarithm goes to dK and dV in the same way. Without the first, gradients of values that differ in their last bit alone are off by
 // their own size; it costs 6 % (bf16 [4, 8, 512, 33]: gradients 588 -> 624 us). Two blocks an SM: with the
 // 163 registers that it would take, 709 us.
 template <typename T>
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) attn_simt_backward_dq(const _
 
     simt_load(Q, pitch, (const T*)p.q + b * p.qs[0] + h * p.qs[1], p.qs[2], q0, p.Lq, p.D, docs, p.Lk - p.Lq);
     simt_load(G, pitch, (const T*)p.dout + b * p.dos[0] + h * p.dos[1], p.dos[2], q0, p.Lq, p.D, docs, p.Lk - p.Lq);
-    float acc[kSimtMaxD / 8], off[kSimtMaxD / 8], rest = 0.f;
+    float acc[kSimtMaxD / 8], off[kSimtMaxD / 8], rest = 0.f, total = 0.f;
 #pragma unroll
     for (int i = 0; i < kSimtMaxD / 8; ++i) acc[i] = off[i] = 0.f;
     const int jend = key_end(p, query_pos(p, min(q0 + kSimtTile, p.Lq) - 1), prefix);
@@ -222,7 +223,8 @@ __global__ void __launch_bounds__(kSimtThreads, 2) attn_simt_backward_dq(const _
             const bool seen = live && j < p.Lk && sees(p, qpos, qdoc, j, docs ? kdoc[c] : 0, prefix);
             float P, PC, dS;
             const float dP = simt_dot(G + r * pitch, V + c * pitch, p.D);
-            simt_grad(p, seen, simt_dot(Q + r * pitch, K + c * pitch, p.D), dP, lse, delta, slope, qpos - j, P, PC, dS);
+            simt_grad(p, seen, simt_dot(Q + r * pitch, K + c * pitch, p.D), dP, lse, 0.f, delta, slope, qpos - j, P, PC, dS);
+            total += P;
             if (kCorrect) {
                 SC[r * 33 + c] = make_float2(dS, PC);
                 if (seen) rest = fmaf(P, dP - delta, rest);
@@ -245,17 +247,23 @@ __global__ void __launch_bounds__(kSimtThreads, 2) attn_simt_backward_dq(const _
             off[i] = o;
         }
     }
-    if (kCorrect) {
 #pragma unroll
-        for (int o = 1; o < 8; o *= 2) rest += __shfl_xor_sync(~0u, rest, o);
-        if (live && c8 == 0) p.delta[row] = delta + rest;
+    for (int o = 1; o < 8; o *= 2) {
+        total += __shfl_xor_sync(~0u, total, o);
+        rest += __shfl_xor_sync(~0u, rest, o);
     }
     if (!live) return;
+    const float inv = total == 0.f ? 1.f : 1.f / total;
+    rest *= inv;
+    if (c8 == 0) {
+        p.fine[row] = total == 0.f ? 0.f : logf(total);
+        if (kCorrect) p.delta[row] = delta + rest;
+    }
     T* o = (T*)p.dq + b * p.dqs[0] + h * p.dqs[1] + (int64_t)(q0 + r) * p.dqs[2];
 #pragma unroll
     for (int i = 0; i < kSimtMaxD / 8; ++i) {
         const int d = c8 + 8 * i;
-        if (d < p.D) o[d] = from_f32<T>(kCorrect ? fmaf(-rest * p.scale, off[i], acc[i]) : acc[i]);
+        if (d < p.D) o[d] = from_f32<T>((kCorrect ? fmaf(-rest * p.scale, off[i], acc[i]) : acc[i]) * inv);
     }
 }
 
@@ -305,7 +313,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_backward_dkv(const __g
                 float P, PC, dS;
                 simt_grad(p, seen, simt_dot(Q + c * pitch, K + r * pitch, p.D),
                           simt_dot(G + c * pitch, V + r * pitch, p.D), seen ? p.lse[row] : 0.f,
-                          seen ? p.delta[row] : 0.f, slope, qpos - j, P, PC, dS);
+                          seen ? p.fine[row] : 0.f, seen ? p.delta[row] : 0.f, slope, qpos - j, P, PC, dS);
                 PT[r * 33 + c] = P;
                 ST[r * 33 + c] = dS;
             }

@@ -8,6 +8,11 @@
 // share of each tile's accumulators up in registers. The tensor core runs S and dP of
 // the next tile while the exponentials of this one are taken.
 //
+// P = exp2(S - lse) carries the rounding of the fp32 lse, 2^-24 |lse|, and that of lse log2(e)
+// (gradients off by 1e-6 to 2.7e-6 with |lse| of 25 to 50). Both are the same for a whole row: the
+// form with the queries resident, which runs first, adds up each row's P, divides dQ by the sum, and
+// leaves its logarithm for the other form to take off the exponents.
+//
 // Heads of up to 64: the pieces of 128 resident rows and of two stages of kN = 64
 // streamed rows of two tensors fill the shared memory (96 + 96 KB).
 // Heads of up to 128: X0's pieces lie in tensor memory (3 x 64 columns, the A operand
@@ -25,6 +30,7 @@ struct Tc32BwdParams {
     const int2* doc_tiles;
     const float* lse2;           // as TcBwdParams
     const float* delta;
+    float* fine;                 // [B * H][Lp] log2 of the row's sum of exp2(S - lse2), from the form with the queries resident
     int Lp;
     uint32_t idesc_s;
     float scale;                 // |scale|
@@ -36,16 +42,19 @@ struct Tc32BwdParams {
 enum : int { kTakeBoth = 0, kTakeDs = 1, kTakeP = 2 };
 
 struct Tc32BwdState {
-    uint64_t x_full, y_full[2], y_empty[2], s_full, s_free, p_full, acc_full, drain;
+    uint64_t x_full, y_full[2], y_empty[2], s_full, s_free, p_full, acc_full, sum_full, drain;
     uint32_t tmem;
     int failed;
     alignas(16) float lse2[2][64];       // negated
     alignas(16) float delta[2][64];      // negated
+    alignas(16) float fine[2][64];       // negated
 };
 
 constexpr int kTc32BwdThreads = 384;     // two warpgroups, three warps that load, one that issues
 constexpr size_t kTc32BwdSmem = (size_t)(2 * 128 + 2 * 2 * 64) * 64 * 6 + 1024;
 static_assert(kTc32BwdSmem == (size_t)(128 + 2 * 2 * 32) * 128 * 6 + 1024, "both head sizes take the same");
+// With a KB of the system's own: beyond 196 KB the SM gives shared memory 228, and L1 half of what it had (dQ 84 -> 90 us).
+static_assert(kTc32BwdSmem + sizeof(Tc32BwdState) + 1024 <= 196 * 1024, "the L1's share");
 
 template <int DP, bool kKeys, int kTake, bool kCap, bool kBias>
 __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const __grid_constant__ Tc32BwdParams tp)
@@ -84,6 +93,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
         mbar_init(smem_u32(&st.s_free), 8);
         mbar_init(smem_u32(&st.p_full), 8);
         mbar_init(smem_u32(&st.acc_full), 1);
+        mbar_init(smem_u32(&st.sum_full), 8);
         mbar_init(smem_u32(&st.drain), 1);
         mbar_fence_init();
         st.failed = 0;
@@ -134,10 +144,12 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                 tc32_fetch(x[k], a0 + k * kRows * step0, live);
                 tc32_fetch(y[k], a1 + k * kRows * step1, live);
             }
-            float lse2 = 0.f, delta = 0.f;
+            float lse2 = 0.f, delta = 0.f, fine = 0.f;
             if (kKeys && tid < kN) {
-                lse2 = tp.lse2[((int64_t)b * p.H + yh) * tp.Lp + y0 + tid];
-                delta = tp.delta[((int64_t)b * p.H + yh) * tp.Lp + y0 + tid];
+                const int64_t at = ((int64_t)b * p.H + yh) * tp.Lp + y0 + tid;
+                lse2 = tp.lse2[at];
+                delta = tp.delta[at];
+                if (y0 + tid < p.Lq) fine = tp.fine[at];
             }
             if (i >= 2) ok = __all_sync(~0u, tc_wait(smem_u32(&st.y_empty[i & 1]), (i / 2 - 1) & 1, failed));
             if (!ok) break;
@@ -150,6 +162,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
             if (kKeys && tid < kN) {
                 st.lse2[i & 1][tid] = -lse2;
                 st.delta[i & 1][tid] = -delta;
+                st.fine[i & 1][tid] = -fine;
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -293,6 +306,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
         float o[kAcc];
 #pragma unroll
         for (int i = 0; i < kAcc; ++i) o[i] = 0.f;
+        uint64_t psum = pack2(0.f, 0.f);                // this thread's part of its row's sum of P
         const auto add_up = [&]() {
 #pragma unroll
             for (int c = 0; c < kAcc; c += 32) {
@@ -359,8 +373,9 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                     }
 #pragma unroll
                     for (int k = 0; k < 4; k += 2) {
-                        unpack2(fma2(pack2(v[c0 + c + k], v[c0 + c + k + 1]), mul_2, pack2(nl[k], nl[k + 1])), e[c + k],
-                                e[c + k + 1]);
+                        uint64_t x = fma2(pack2(v[c0 + c + k], v[c0 + c + k + 1]), mul_2, pack2(nl[k], nl[k + 1]));
+                        if (kKeys) x = add2(x, *reinterpret_cast<const uint64_t*>(&st.fine[i & 1][col + c0 + c + k]));
+                        unpack2(x, e[c + k], e[c + k + 1]);
                         e[c + k] = ex2(e[c + k]);
                         e[c + k + 1] = ex2(e[c + k + 1]);
                     }
@@ -369,6 +384,10 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                     // a pair that is not seen: P = 0, and its dP does not count
 #pragma unroll
                     for (int c = 0; c < 16; ++c) e[c] = seen[0] >> (c0 + c) & 1 ? e[c] : 0.f;
+                }
+                if (!kKeys) {
+#pragma unroll
+                    for (int c = 0; c < 16; c += 2) psum = add2(psum, pack2(e[c], e[c + 1]));
                 }
                 if (kTake != kTakeDs) {
                     uint32_t w[3][8];
@@ -428,14 +447,30 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                 add_up();
             }
         }
+        float total = 0.f;                              // of the row's P, in this block's share of the keys
+        if (!kKeys) {
+            float odd;
+            unpack2(psum, total, odd);
+            // in the place of the streamed rows, which nobody reads any more
+            float* sums = reinterpret_cast<float*>(dyn + (sY - smem_u32(dyn)));
+            sums[128 * wg + r] = total + odd;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&st.sum_full));
+            ok = __all_sync(~0u, ok && tc_wait(smem_u32(&st.sum_full), 0, failed));
+            total = sums[r] + sums[128 + r];
+        }
         if (ok && x0 + r < xrows) {
+            if (!kKeys && wg == 0) {
+                if (tp.parts.parts == 1) tp.fine[((int64_t)b * p.H + xh) * tp.Lp + x0 + r] = total == 0.f ? 0.f : log2f(total);
+                else tp.parts.r[((int64_t)part * p.B * p.H + bh) * p.Lq + x0 + r] = total;
+            }
             const int64_t* os = kKeys ? (is_dv ? p.dvs : p.dks) : p.dqs;
             float* out = tp.parts.parts == 1
                              ? (float*)(kKeys ? (is_dv ? p.dv : p.dk) : p.dq) + b * os[0] + xh * os[1] + (int64_t)(x0 + r) * os[2]
                              : (is_dv ? tp.parts.other : tp.parts.acc) +
                                    ((((int64_t)blockIdx.x % tp.parts.parts) * p.B + b) * nhead + xh) * xrows * p.D + (int64_t)(x0 + r) * p.D;
             out += ocol;
-            const float f = is_dv ? 1.f : p.scale;
+            const float f = is_dv ? 1.f : !kKeys && tp.parts.parts == 1 && total != 0.f ? p.scale / total : p.scale;
             const int cols = p.D - ocol;
 #pragma unroll
             for (int c = 0; c < kAcc; c += 4)

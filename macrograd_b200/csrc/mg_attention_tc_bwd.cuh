@@ -165,9 +165,11 @@ __device__ __forceinline__ void share_of_steps(int part, int parts, int all, int
     n = min(all, i0 + each) - i0;
 }
 
-// Adds up the parts of a gradient in their order (blockIdx.y: acc, other). kCorrect: dQ of
-// 16-bit tensors, less the rows' sums r times the other product, and delta made exact.
-// One warp to a row, four elements to a lane.
+// Adds up the parts of a gradient in their order (blockIdx.y: acc, other). One warp to a row,
+// four elements to a lane. kJoinCorrect: dQ of 16-bit tensors, less the rows' sums r times the
+// other product, and delta made exact. kJoinWeights: dQ of fp32 tensors, divided by the rows'
+// sums of P, whose logarithm is kept.
+enum : int { kJoinPlain = 0, kJoinCorrect = 1, kJoinWeights = 2 };
 struct GradJoin {
     GradParts parts;
     int heads, L, D, Lp;
@@ -175,9 +177,10 @@ struct GradJoin {
     void* out[2];
     int64_t os[2][3];
     float* delta;
+    float* fine;                         // log2 of the sums of P
 };
 
-template <typename T, bool kCorrect>
+template <typename T, int kForm>
 __global__ void __launch_bounds__(256) attn_grad_join_kernel(const __grid_constant__ GradJoin j)
 {
     const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
@@ -196,9 +199,15 @@ __global__ void __launch_bounds__(256) attn_grad_join_kernel(const __grid_consta
     const int64_t bh = row / j.L;
     const int i = (int)(row - bh * j.L), h = (int)(bh % j.heads), b = (int)(bh / j.heads);
     float4 a = sum_of(blockIdx.y ? j.parts.other : j.parts.acc);
-    if (kCorrect) {
-        float r = 0.f;
+    float r = 0.f;
+    if (kForm != kJoinPlain)
         for (int s = 0; s < j.parts.parts; ++s) r += __ldg(j.parts.r + s * j.rows + row);
+    if (kForm == kJoinWeights) {
+        const float inv = r == 0.f ? 1.f : 1.f / r;
+        a.x *= inv, a.y *= inv, a.z *= inv, a.w *= inv;
+        if (d == 0) j.fine[bh * j.Lp + i] = r == 0.f ? 0.f : log2f(r);
+    }
+    if (kForm == kJoinCorrect) {
         const float4 w = sum_of(j.parts.other);
         a.x = fmaf(-r, w.x, a.x), a.y = fmaf(-r, w.y, a.y), a.z = fmaf(-r, w.z, a.z), a.w = fmaf(-r, w.w, a.w);
         if (d == 0) j.delta[bh * j.Lp + i] += r;

@@ -716,3 +716,27 @@ def test_captured_on_another_stream_than_the_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("size", [(64, 6, 6, 130, 200, 64), (1, 4, 2, 700, 700, 64), (1, 8, 2, 300, 300, 128),
+                                  (40, 8, 8, 130, 130, 96), (2, 4, 2, 150, 150, 33), (1, 4, 1, 1, 500, 64)], ids=str)
+@pytest.mark.parametrize("top", [2 ** 12 + 3, 2 ** 14 + 7])
+def test_fp32_gradients_of_large_scores(top, size):
+    """Scores of `top` less 0 to 3, exactly: the weights go by the small part, whatever the rounding of lse, which is some
+    2^-24 * top. Of dq and dk the elements that k and q do not hold `top` or its share in, whose own products cancel.
+
+    Bound, of the norm, in steps of 2^-24: exponents of up to 16 powers of two, rounded once (16), exponentials of 2 ulp
+    (4), products of 3 pieces (2) and their sums over up to 128 elements and 64 keys truncated at the worst (128), lse's
+    part that is taken off (4): below 2^8."""
+    B, H, Hkv, Lq, Lk, D = size
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v, dout = (torch.randn((B, n, L, D), generator=g, device="cuda") for n, L in ((H, Lq), (Hkv, Lk), (Hkv, Lk), (H, Lq)))
+    q[..., :3] = 1
+    k[..., 0], k[..., 1], k[..., 3:] = 2 ** 12, top - 2 ** 12, 0
+    k[..., 2] = -torch.randint(0, 25, (B, Hkv, Lk), generator=g, device="cuda") / 8
+    out, lse = mg.attention(q, k, v, scale=1.0)
+    ref = Reference(q, k, v, dout, scale=1.0)
+    dq, dk, dv = mg.attention_backward(dout, q, k, v, out, lse, scale=1.0)
+    for got, want, what in ((dq[..., 2:3], ref.dq[..., 2:3], "dq"), (dk, ref.dk, "dk"), (dv, ref.dv, "dv")):
+        error = float((got.double() - want).norm() / want.norm())
+        assert error <= 2.0 ** -16, f"{what}: {error:.3g}"
