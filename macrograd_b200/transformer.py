@@ -47,6 +47,7 @@ _ATTENTION = struct.Struct("@8i2f24q3P")
 _ROTARY = struct.Struct("@9if13q2P")
 _PAGED = struct.Struct("@8i2f15q3P")
 _ZERO3 = (0, 0, 0)
+_LARGEST = (2 - 2.0 ** -23) * 2.0 ** 127      # of fp32
 
 
 # ------------------------------------------------------------------ checks
@@ -96,9 +97,10 @@ def _written(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
 
 
 def _number(x: float, name: str) -> float:
+    """A finite number that stays one in the descriptors' fp32."""
     x = float(x)
-    if not math.isfinite(x):
-        _bad(f"{name} must be finite")
+    if not abs(x) <= _LARGEST:
+        _bad(f"{name} must be finite in fp32, found {x}")
     return x
 
 
@@ -249,9 +251,9 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str = "
         _bad(f"rotary_dim must be even, found {rotary_dim}")
     if scaling not in ("none", "linear", "ntk", "parts"):
         _bad(f"scaling must be 'none', 'linear', 'ntk' or 'parts', found {scaling!r}")
-    theta, factor = _number(theta, "theta"), _number(factor, "factor")
-    if theta <= 0 or factor <= 0:
-        _bad("theta and factor must be positive")
+    theta, factor = float(theta), float(factor)
+    if not (0 < theta < math.inf and 0 < factor < math.inf):
+        _bad("theta and factor must be positive and finite")
     if scaling == "parts" and (trained < 1 or not low < high):
         _bad("scaling 'parts' needs trained > 0 and low < high")
     if scaling == "ntk" and rotary_dim > 2:

@@ -136,3 +136,18 @@ def test_backward_refuses_more_rows_than_its_statistics_number(lib):
     assert lib.mg_attention_backward(d, *([None] * 10)) == UNSUPPORTED
     assert "too large" in lib.mg_last_error().decode()
     assert lib.mg_attention(d, None, None, None, None, None, None) == INVALID     # the forward pass has none
+
+
+@pytest.mark.parametrize("x", [1e39, -1e39, float("inf"), float("nan")])
+def test_numbers_beyond_fp32_are_refused_as_arguments(x):
+    with pytest.raises(mg.MacrogradError, match="scale must be finite"):
+        T._number(x, "scale")
+    largest = (2 - 2.0 ** -23) * 2.0 ** 127
+    assert T._number(largest, "scale") == largest
+    assert len(T._ATTENTION.pack(0, 1, 1, 1, 1, 1, 8, 1, largest, 0.0, *([0] * 27))) == T._ATTENTION.size
+
+
+@pytest.mark.parametrize("kw", [dict(theta=0.0), dict(theta=float("inf")), dict(factor=-1.0), dict(factor=float("nan"))])
+def test_rotary_frequencies_refuse_what_is_not_positive_and_finite(kw):
+    with pytest.raises(mg.MacrogradError, match="positive"):
+        mg.rotary_frequencies(8, device="cpu", **kw)
