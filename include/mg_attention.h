@@ -42,8 +42,11 @@ typedef enum mg_dtype { MG_F32 = 0, MG_BF16 = 1 } mg_dtype;
  * used, nor is q or dout of a query of a negative document. Elsewhere v (and in the
  * backward pass k, q, dout) has to be finite also where a mask hides it from
  * some queries.
- * The backward pass takes each weight from lse: it carries lse's rounding, a relative
- * 2^-24 * |lse|.
+ * The backward pass takes each weight from the forward's lse of the same call, exp(s - lse).
+ * fp32 tensors, and those that run on the CUDA cores, have a row's weights divided by their
+ * sum; 16-bit ones on the tensor cores keep lse's rounding, a relative 2^-24 * |lse|. In 16-bit
+ * calls the weights, and dS, are rounded to 16 bits for their products; sums, softmax
+ * statistics and delta are kept in 32.
  * Scores and biases are resolved up to 2^28 in size; a row with larger ones may
  * come out as NaN.
  * scale lies within +-1e30, cap is 0 or within 1e-30..1e30. Strides are in
@@ -70,7 +73,7 @@ mg_status mg_attention(const mg_attention_desc* d, void* out, float* lse, const 
 
 /* Gradients of sum(dout * out) with respect to q, k and v, from the forward's
  * out and lse:
- *   P = exp(s - lse), dV = P^T dout, delta = rowsum(dout * out),
+ *   P = exp(s - lse), its rows summing to one, dV = P^T dout, delta = rowsum(dout * out),
  *   dS = P * (dout V^T - delta) * scale * (1 - tanh^2), dQ = dS K, dK = dS^T Q,
  * dK and dV summed over the query heads that share a key-value head.
  * Deterministic: no atomics. The slopes are constants. */

@@ -8,7 +8,10 @@
 // = (tid / 8, tid % 8) owns query r and the elements c8, c8 + 8, ... of the head,
 // so the eight threads of a query share its statistics by shuffles and the
 // score of the query against keys c8, c8 + 8, ... is a dot product of two
-// shared-memory rows (pitch D + 1: no bank conflicts).
+// shared-memory rows (pitch D + 1: no bank conflicts where D is even; at D = 127 all rows
+// begin in one bank). It is the form that takes any call, and it is slow: causal [1, 16 over 4,
+// 2048, D], D = 100: 2.6 ms forward, 11.7 ms gradients; D = 127: 8.7 and 45.9 ms; the tensor-core
+// kernels at D = 128: 41 and 146 us in bf16, 176 and 1137 us in fp32; 32-bit torch operations 1.3 and 2.8 ms.
 // Backward: the same tiles seen from the keys (dK, dV: one block per 32 keys of a
 // key-value head, walking the queries of all its query heads in order, so that
 // no atomics are needed) and from the queries (dQ).

@@ -2,10 +2,12 @@
 // cores at fp32 accuracy.
 //
 // Each fp32 operand x is the sum of three bf16 numbers, x = x0 + x1 + x2: its 24 bits
-// cut into three times 8 (exactly), and a product is the six of their products that
-// reach 2^-24 of it: x0 y2 + x2 y0 + x1 y1 + x0 y1 + x1 y0 + x0 y0, issued
-// smallest first into one fp32 accumulator, so that its truncating additions
-// lose no more than those of x0 y0 alone. Six products of 16-bit operands cost as
+// cut into three times 8 (exactly), and a product is the six largest of their nine
+// products: x0 y2 + x2 y0 + x1 y1 + x0 y1 + x1 y0 + x0 y0, issued smallest first
+// into one fp32 accumulator, so that its truncating additions lose no more than
+// those of x0 y0 alone. (The pieces are cut, not rounded, and carry x's sign: what is
+// dropped, x1 y2 + x2 y1 + x2 y2, is some 2^-23 of the product, below 2^-21, and
+// always taken from its size.) Six products of 16-bit operands cost as
 // much as the three of 3xTF32, take 6 bytes of shared memory an element instead
 // of 8, and keep fp32's range. An accumulator in tensor memory holds one tile;
 // the sum over the tiles is kept in registers (with one accumulator over a long

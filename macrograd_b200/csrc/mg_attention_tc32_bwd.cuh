@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
 
     if (warp >= 8 && warp < 11) {
         // ------------------------------------------------ loads and splits of the streamed rows
-        // item k of a thread: 8 elements of row r0 + 12 k of both tensors, always the same columns
+        // item k of a thread: 8 elements of row r0 + k * kRows of both tensors, always the same columns
         constexpr int kRows = kTc32LoadWarps * 32 / (DP / 8), kItems = (kN + kRows - 1) / kRows;
         const int tid = threadIdx.x - 256, r0 = tid / (DP / 8), c = tid % (DP / 8);
         const bool in = c * 8 < p.D;

@@ -16,7 +16,8 @@
 //
 // delta = rowsum(dout * out) carries the 16-bit rounding of out, which dS = P * (dP -
 // delta) magnifies where a row's weight lies on few keys (errors of dQ and dK of 0.4 %
-// where the rounding of the result itself is 0.17 %). The true delta makes the row's sum of
+// where the rounding of the result itself is 0.17 %) and where its values have much in
+// common (errors as large as dQ and dK). The true delta makes the row's sum of
 // P * (dP - delta) zero, so what that sum is in fp32 is delta's error r: the form with
 // the queries resident, which runs first, adds it to delta for the other one, and
 // corrects its own dQ by r times acc' = sum P * curve * k (the eighth product).

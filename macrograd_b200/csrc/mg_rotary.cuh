@@ -5,7 +5,7 @@
 // fp32, so it is kept in turns as a 64-bit fixed-point fraction: frequency / 2 pi
 // as an unsigned 0.64 number, times the position modulo 2^64 -- the integer
 // product drops whole turns exactly. Its upper 32 bits, read as a signed number,
-// are the angle in (-1/2, 1/2] turns, and sincospi needs no further reduction.
+// are the angle in [-1/2, 1/2) turns, and sincospi needs no further reduction.
 // Frequencies below one turn a position are exact to 2^-53 of themselves, so the
 // angle at position 2^31 is off by less than 2^-22 turns from the double's own.
 //
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kRotaryThreads, 4) rotary_kernel(const __grid_
         f -= rint(f);
         const int64_t fixed = f >= 0.5 ? INT64_MIN : (int64_t)(f * 18446744073709551616.0);
         const uint64_t angle = (uint64_t)fixed * (uint64_t)pos;
-        // the nearest 32-bit fraction: half turns of (-1, 1]
+        // the nearest 32-bit fraction: half turns of [-1, 1)
         const int32_t top = (int32_t)(uint32_t)((angle + 0x80000000ull) >> 32);
         float s, c;
         sincospif((float)top * 4.656612873077393e-10f, &s, &c);   // 2^-31

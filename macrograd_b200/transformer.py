@@ -19,7 +19,8 @@ Heads are views [batch, heads, length, head_dim] with a contiguous last dim and
 any other strides, float32 or bfloat16, head_dim up to 128; outputs are laid out
 as the tensor they belong to (heads split from [batch, length, heads * head_dim]
 come back ready to be merged). Sums, softmax statistics and angles are kept in
-32 bits or more whatever the type. Calls run on `stream` (default: the current
+32 bits or more whatever the type; with bfloat16 tensors the weights P and, in the
+gradients, dS are rounded to 16 bits for their products, as the tensors are. Calls run on `stream` (default: the current
 one) and can be captured into graphs (but for the library's first call on a
 device); nothing is kept from one call for the next. A `stream` that is given has
 to be ordered behind whatever writes the operands, as by stream.wait_stream(), and
@@ -218,7 +219,8 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     """Gradients (dq, dk, dv) of sum(dout * out) for attention() called with the same arguments; `out` and `lse`
     are what it returned. Gradients of shared key-value heads are summed over their query heads, in a fixed order:
     the same inputs give the same bits. The slopes are constants (no gradient). Besides k and v, q and dout must be
-    finite everywhere but at padding."""
+    finite everywhere but at padding. The weights are exp(s - lse), made to sum to one in each row (but for bfloat16 on
+    the tensor cores, where lse's rounding, 2^-24 of its size, is below that of the weights)."""
     lib = _lib.load()
     dev, lead, ptrs = _attention_args(q, k, v, scale, causal, cap, slopes, documents, prefix)
     for t, name in ((dout, "dout"), (out, "out")):
