@@ -489,7 +489,7 @@ mg_status mg_attention_backward(const mg_attention_desc* d, void* dq, void* dk, 
         return d->dtype == MG_BF16 ? backward_tc(p, dev, stream) : backward_tc32(p, dev, stream);
     Scratch ws(dev, stream);
     if (d->q_len > 0) {
-        const size_t rows = d->batch * d->heads * (size_t)d->q_len;
+        const size_t rows = (size_t)d->batch * d->heads * d->q_len;
         p.delta = static_cast<float*>(ws.get(2 * rows * sizeof(float)));
         if (!p.delta) return fail(MG_ERR_ALLOC, "mg_attention_backward: no scratch for the row sums");
         p.fine = p.delta + rows;

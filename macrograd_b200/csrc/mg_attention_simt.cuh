@@ -176,9 +176,9 @@ __device__ __forceinline__ void simt_grad(const AttnParams& p, bool seen, float 
 // values of a row have much in common. The true delta makes the row's sum of P * (dP - delta) zero, so
 // what that sum is is delta's error r: dQ loses r times sum P curve k, and delta becomes exact for dK,
 // which is computed after it. The row's sum of P, 1 but for the rounding of the fp32 lse, divides dQ, and its
-// logarithm goes to dK and dV in the same way. Without the first, gradients of values that differ in their last bit alone are off by
-// their own size; it costs 6 % (bf16 [4, 8, 512, 33]: gradients 588 -> 624 us). Two blocks an SM: with the
-// 163 registers that it would take, 709 us.
+// logarithm goes to dK and dV in the same way. Without the first, gradients of values that differ in their last
+// bit alone are off by their own size; it costs 6 % (bf16 [4, 8, 512, 33]: gradients 588 -> 624 us). Two blocks
+// an SM: with the 163 registers that it would take, 709 us.
 template <typename T>
 __global__ void __launch_bounds__(kSimtThreads, 2) attn_simt_backward_dq(const __grid_constant__ AttnParams p)
 {
@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) attn_simt_backward_dq(const _
         simt_load(V, pitch, vp, p.vs[2], j0, p.Lk, p.D, docs, 0);
         if (docs && threadIdx.x < kSimtTile) kdoc[threadIdx.x] = doc_at(p, b, j0 + threadIdx.x);
         __syncthreads();
+        float part = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int c = c8 + 8 * i, j = j0 + c;
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) attn_simt_backward_dq(const _
             float P, PC, dS;
             const float dP = simt_dot(G + r * pitch, V + c * pitch, p.D);
             simt_grad(p, seen, simt_dot(Q + r * pitch, K + c * pitch, p.D), dP, lse, 0.f, delta, slope, qpos - j, P, PC, dS);
-            total += P;
+            part += P;
             if (kCorrect) {
                 SC[r * 33 + c] = make_float2(dS, PC);
                 if (seen) rest = fmaf(P, dP - delta, rest);
@@ -235,6 +236,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) attn_simt_backward_dq(const _
                 S[r * 33 + c] = dS;
             }
         }
+        total += part;
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kSimtMaxD / 8; ++i) {

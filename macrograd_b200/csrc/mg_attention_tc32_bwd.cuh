@@ -357,6 +357,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
             if (kCap) cap_scores32(v, pre);
             const float far = (float)(pos - ypos - col);
             const uint64_t mul_2 = pack2(mul, mul);
+            uint64_t tsum = pack2(0.f, 0.f);            // of this tile: long rows add up tiles, not pairs
 #pragma unroll
             for (int c0 = 0; c0 < kCols; c0 += 16) {
                 float e[16];
@@ -387,7 +388,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                 }
                 if (!kKeys) {
 #pragma unroll
-                    for (int c = 0; c < 16; c += 2) psum = add2(psum, pack2(e[c], e[c + 1]));
+                    for (int c = 0; c < 16; c += 2) tsum = add2(tsum, pack2(e[c], e[c + 1]));
                 }
                 if (kTake != kTakeDs) {
                     uint32_t w[3][8];
@@ -435,6 +436,7 @@ __global__ void __launch_bounds__(kTc32BwdThreads, 1) attn_tc32_backward(const _
                     for (int k = 0; k < 3; ++k) tmem_st_x8(tdS + lanes + kCols * k + (col + c0) / 2, w[k]);
                 }
             }
+            if (!kKeys) psum = add2(psum, tsum);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
