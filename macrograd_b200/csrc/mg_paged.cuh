@@ -363,14 +363,33 @@ struct PagedAcc {
             for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = x[i];
             mul = p.cap * kLog2e;
         }
+        uint32_t a[4];
+        if (p.slopes != nullptr) weights<true, false>(s, mul, seen, back, t, a);
+        else if (seen != 0xFFFFu) weights<false, false>(s, mul, seen, back, t, a);
+        else weights<false, true>(s, mul, seen, back, t, a);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            // matrices: keys 0-7 and 8-15 of 8 elements, then of the next 8
+            const int row = lane & 15, piece = 2 * k + (lane >> 4);
+            uint32_t b[4];
+            ldmatrix4_trans(b, sv + row * (DP * 2) + ((piece ^ (row & 7)) << 4));
+            mma16816(o[2 * k], a, b[0], b[1]);
+            mma16816(o[2 * k + 1], a, b[2], b[3]);
+        }
+    }
+    // Weights of a tile's scores (their powers of two are s * mul - slope * distance) as the A operand of the second
+    // product; m, l and o follow a new maximum. kAll: every key is seen, the usual tile.
+    template <bool kBias, bool kAll>
+    __device__ __forceinline__ void weights(const float (&s)[2][4], float mul, uint32_t seen, int back, int t, uint32_t (&a)[4])
+    {
         float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = 8 * n + 2 * t + (i & 1);
-                const float x = fmaf(s[n][i], mul, -slope[i >> 1] * (float)(back - key));
-                top[i >> 1] = fmaxf(top[i >> 1], (seen >> key) & 1 ? x : -CUDART_INF_F);
+                const float x = kBias ? fmaf(s[n][i], mul, -slope[i >> 1] * (float)(back - key)) : s[n][i] * mul;
+                top[i >> 1] = fmaxf(top[i >> 1], kAll || (seen >> key & 1) ? x : -CUDART_INF_F);
             }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -388,8 +407,7 @@ struct PagedAcc {
 #pragma unroll
             for (int i = 0; i < DP / 8; ++i) o[i][0] *= f0, o[i][1] *= f0, o[i][2] *= f1, o[i][3] *= f1;
         }
-        const float b0 = m[0] == -CUDART_INF_F ? 0.f : m[0], b1 = m[1] == -CUDART_INF_F ? 0.f : m[1];
-        uint32_t a[4];
+        const float b[2] = {m[0] == -CUDART_INF_F ? 0.f : -m[0], m[1] == -CUDART_INF_F ? 0.f : -m[1]};
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             // score and maximum in one rounding: the scores' own, 2^-24 of their size, would stay in the weights
@@ -397,8 +415,8 @@ struct PagedAcc {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = 8 * n + 2 * t + (i & 1);
-                const float x = fmaf(s[n][i], mul, fmaf(-slope[i >> 1], (float)(back - key), i < 2 ? -b0 : -b1));
-                e[i] = ex2((seen >> key) & 1 ? x : -CUDART_INF_F);
+                const float x = fmaf(s[n][i], mul, kBias ? fmaf(-slope[i >> 1], (float)(back - key), b[i >> 1]) : b[i >> 1]);
+                e[i] = ex2(kAll || (seen >> key & 1) ? x : -CUDART_INF_F);
             }
             const float e0 = e[0], e1 = e[1], e2 = e[2], e3 = e[3];
             l[0] += e0 + e1;
@@ -406,15 +424,6 @@ struct PagedAcc {
             const __nv_bfloat162 x = __floats2bfloat162_rn(e0, e1), y = __floats2bfloat162_rn(e2, e3);
             a[2 * n] = *reinterpret_cast<const uint32_t*>(&x);
             a[2 * n + 1] = *reinterpret_cast<const uint32_t*>(&y);
-        }
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-            // matrices: keys 0-7 and 8-15 of 8 elements, then of the next 8
-            const int row = lane & 15, piece = 2 * k + (lane >> 4);
-            uint32_t b[4];
-            ldmatrix4_trans(b, sv + row * (DP * 2) + ((piece ^ (row & 7)) << 4));
-            mma16816(o[2 * k], a, b[0], b[1]);
-            mma16816(o[2 * k + 1], a, b[2], b[3]);
         }
     }
     __device__ __forceinline__ void finish(float* sm_m, float* sm_l, float* sm_o, int nh, int lane)
